@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define OW_ABI_VERSION 5
+#define OW_ABI_VERSION 6
 
 #if defined(__GNUC__)
 #define OW_API __attribute__((visibility("default")))
@@ -366,6 +366,78 @@ typedef struct ow_pool_head_t {
  * unsupported): 256, plus room for the converted weight when weight is f32. */
 OW_API size_t ow_pool_head_workspace_size(const ow_pool_head_t* args);
 OW_API int ow_pool_head_fwd(const ow_pool_head_t* args, void* stream);
+
+/*
+ * AdamW over many tensors at once, the optimizer of the reference's training
+ * engine (``torch.optim.AdamW`` at omniweave/training/engine.py:411, with the
+ * clipping and the finite checks of :229-251), moments in 32 or in 8 bits:
+ *
+ *   g  = clip * grad
+ *   m <- b1 m + (1 - b1) g          v <- b2 v + (1 - b2) g^2
+ *   p <- p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ *
+ * in f32, rounded once to the parameter's dtype.  All tensors of a call share
+ * a dtype (f32, bf16 or f16; the gradient has the parameter's) and the
+ * hyperparameters; every tensor counts its own steps t.
+ *
+ * State is flat: tensor i owns the slots [slots[i], slots[i + 1]), of which the
+ * first numel[i] are used; slots are multiples of OW_ADAMW_BLOCK.  With
+ * state_bits == 32 the moments are f32.  With 8 they are e4m3 codes, with one
+ * f32 scale (largest magnitude / 448) for each block of OW_ADAMW_BLOCK slots;
+ * they are rounded stochastically by a hash of (slot, step), so a run is
+ * reproducible bit for bit, and a positive second moment is never held as 0.
+ *
+ * ``params``, ``grads`` and ``slots`` are host arrays, read during the call
+ * (a captured graph keeps the pointers it was captured with).  A NULL
+ * gradient leaves its tensor, its state and its step count as they are.
+ * Neither function allocates or synchronises.
+ */
+#define OW_ADAMW_BLOCK 256
+#define OW_ADAMW_CONTROL_BYTES 64
+typedef struct ow_adamw_t {
+  int32_t tensors;
+  int32_t dtype;
+  void* const* params;              /* host [tensors] */
+  const void* const* grads;         /* host [tensors] */
+  const int64_t* slots;             /* host [tensors + 1] */
+  const int64_t* dev_slots;         /* device [tensors + 1], the same values */
+  const int64_t* dev_numel;         /* device [tensors] */
+  const int32_t* dev_block_tensor;  /* device [slots[tensors] / OW_ADAMW_BLOCK]: each block's tensor */
+  void* control;                    /* device, OW_ADAMW_CONTROL_BYTES, zero before its first use, this
+                                     * optimizer's own: calls that overlap must not share it */
+  int32_t state_bits;               /* 32 or 8 */
+  void* exp_avg;                    /* flat m */
+  void* exp_avg_sq;                 /* flat v */
+  float* exp_avg_scale;             /* 8 bits: one a block */
+  float* exp_avg_sq_scale;
+  float* dev_steps;                 /* device [tensors]: steps done, counted up by the call */
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_ptr;              /* device learning rate in the place of ``lr``, or NULL */
+  const float* found;               /* device flag, or NULL: nonzero calls the step off */
+  int32_t use_norm;                 /* 1: apply what ow_grad_norm left in ``control`` */
+} ow_adamw_t;
+
+/*
+ * Norm of all gradients (the tensors of several calls when only the last has
+ * ``finish`` set: each adds ow_grad_norm_partials() sums from ``first`` on).
+ * The last call leaves in ``control`` the clip coefficient
+ * min(1, max_norm / (norm + 1e-6)) (1 when max_norm <= 0) and, with
+ * skip_nonfinite, whether a gradient is inf or NaN, which ``found`` gets as
+ * well.  The squares are added in f64 in a fixed order.
+ */
+typedef struct ow_grad_norm_t {
+  double* partials;       /* device */
+  int32_t first, capacity;
+  int32_t finish;
+  float max_norm;
+  int32_t skip_nonfinite;
+  float* norm;            /* device, or NULL */
+  float* found;           /* device, or NULL: set to 1 when a gradient is not finite */
+} ow_grad_norm_t;
+
+OW_API int32_t ow_grad_norm_partials(const ow_adamw_t* args);
+OW_API int ow_grad_norm(const ow_adamw_t* args, const ow_grad_norm_t* options, void* stream);
+OW_API int ow_adamw_step(const ow_adamw_t* args, void* stream);
 
 #ifdef __cplusplus
 }

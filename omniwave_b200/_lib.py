@@ -16,7 +16,7 @@ import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libomniwave_b200.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_CODE = {
     torch.float32: 0,
@@ -29,6 +29,7 @@ OW_OK = 0
 _ERR_NAMES = {1: "invalid argument", 2: "unsupported", 3: "CUDA error", 4: "workspace too small"}
 
 _c_i32 = ctypes.c_int32
+_c_f64 = ctypes.c_double
 _vp = ctypes.c_void_p
 
 
@@ -97,6 +98,29 @@ class PoolHead(ctypes.Structure):
     ]
 
 
+class AdamW(ctypes.Structure):
+    _fields_ = [
+        ("tensors", _c_i32), ("dtype", _c_i32),
+        ("params", _vp), ("grads", _vp), ("slots", _vp),
+        ("dev_slots", _vp), ("dev_numel", _vp), ("dev_block_tensor", _vp), ("control", _vp),
+        ("state_bits", _c_i32),
+        ("exp_avg", _vp), ("exp_avg_sq", _vp), ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp),
+        ("dev_steps", _vp),
+        ("lr", _c_f64), ("beta1", _c_f64), ("beta2", _c_f64), ("eps", _c_f64), ("weight_decay", _c_f64),
+        ("lr_ptr", _vp), ("found", _vp), ("use_norm", _c_i32),
+    ]
+
+
+class GradNorm(ctypes.Structure):
+    _fields_ = [
+        ("partials", _vp), ("first", _c_i32), ("capacity", _c_i32), ("finish", _c_i32),
+        ("max_norm", ctypes.c_float), ("skip_nonfinite", _c_i32), ("norm", _vp), ("found", _vp),
+    ]
+
+
+ADAMW_BLOCK = 256
+ADAMW_CONTROL_BYTES = 64
+
 LAYOUT_NHWC = 0
 LAYOUT_NCHW = 1
 
@@ -108,6 +132,7 @@ EXPORTS = (
     "ow_s2d_linear_workspace_size", "ow_s2d_linear_fwd",
     "ow_pool_head_workspace_size", "ow_pool_head_fwd",
     "ow_d2s_linear_workspace_size", "ow_d2s_linear_fwd",
+    "ow_grad_norm_partials", "ow_grad_norm", "ow_adamw_step",
 )
 
 _lock = threading.Lock()
@@ -166,6 +191,12 @@ def load() -> ctypes.CDLL:
         lib.ow_d2s_linear_workspace_size.restype = ctypes.c_size_t
         lib.ow_d2s_linear_fwd.argtypes = [ctypes.POINTER(D2sLinear), _vp]
         lib.ow_d2s_linear_fwd.restype = ctypes.c_int
+        lib.ow_grad_norm_partials.argtypes = [ctypes.POINTER(AdamW)]
+        lib.ow_grad_norm_partials.restype = _c_i32
+        lib.ow_grad_norm.argtypes = [ctypes.POINTER(AdamW), ctypes.POINTER(GradNorm), _vp]
+        lib.ow_grad_norm.restype = ctypes.c_int
+        lib.ow_adamw_step.argtypes = [ctypes.POINTER(AdamW), _vp]
+        lib.ow_adamw_step.restype = ctypes.c_int
         v = lib.ow_abi_version()
         if v != ABI_VERSION:
             raise NativeLibraryError(f"ABI version mismatch: library {v}, binding {ABI_VERSION}")

@@ -1,0 +1,488 @@
+// AdamW over many tensors in one launch, the moments held in 32 or in 8 bits,
+// and the global gradient norm that clips a step or calls it off.
+//
+// With g the gradient times the clip coefficient, t the tensor's step count
+// and every value taken in f32:
+//   m <- b1 m + (1 - b1) g             v <- b2 v + (1 - b2) g^2
+//   p <- p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Layout.  Every tensor's state starts on a multiple of 256 slots of one flat
+// array, so a block of 256 slots belongs to one tensor and one warp does one
+// block: 8 elements a lane in two groups of four, each array read and written
+// with whole 128-byte lines.  A table of one int per block names the tensor;
+// the parameters' and gradients' pointers travel in the launch itself, so
+// gradients that move from step to step cost no copy.
+//
+// 8-bit moments.  A block holds 256 e4m3 codes and one f32 scale = max / 448.
+// They are rounded stochastically, by a hash of (slot, step): with b2 = 0.999
+// a step moves v by 0.1% or less, far under half a step of a 3-bit mantissa
+// (3 to 6%), so rounding to nearest would hold v where it is for good, while
+// this keeps its expectation.  The update itself uses the unrounded moments.
+// A positive v is never held as 0: an element with v = 0 and m != 0 would
+// next move by m / eps.
+//
+// Bound: HBM.  An f32 parameter costs 28 bytes (p, m, v read and written, g
+// read), with 8-bit moments 16.
+#include <math.h>
+
+#include <algorithm>
+
+#include <cuda_fp8.h>
+
+#include "ow_common.cuh"
+#include "ow_internal.h"
+
+namespace ow {
+namespace {
+
+constexpr int BLK = OW_ADAMW_BLOCK;  // slots a warp works on, and that share a scale
+constexpr int WARPS = 8;
+constexpr float TINY = 7.888609052210118e-31f;  // 2^-100: a block below it is held as zeros
+
+template <int MAXT>
+struct Ptrs {
+  void* p[MAXT];
+  const void* g[MAXT];
+};
+
+struct Tables {
+  const int64_t* slot;     // [tensors + 1] first slot of each tensor
+  const int64_t* numel;    // [tensors]
+  const int32_t* tensor;   // [blocks] tensor of each block
+  int t0;                  // first tensor of this launch
+  int64_t blk0, nblk;      // its blocks
+};
+
+// Scalars the norm leaves for the update.
+struct Ctl {
+  float coef;   // clip coefficient
+  float found;  // 1: a gradient was not finite
+  unsigned ticket_norm, ticket_step;
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float (&o)[4]) {
+  if (vec && i + 4 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + i);
+      const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = Elem<T>::to_f(h[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = i + k < n ? Elem<T>::to_f(p[i + k]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float (&v)[4]) {
+  if (vec && i + 4 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint2 o;
+      T* h = reinterpret_cast<T*>(&o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) h[k] = Elem<T>::from(v[k]);
+      *reinterpret_cast<uint2*>(p + i) = o;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k < n) p[i + k] = Elem<T>::from(v[k]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool aligned4(const void* p) {
+  return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Two 16-bit numbers from (slot, step), as the 20 bits below an e4m3 mantissa
+// see them: 16 random bits and half of the last one.
+__device__ __forceinline__ void random20(int64_t slot, uint32_t step, uint32_t& r1, uint32_t& r2) {
+  uint32_t h = (uint32_t)slot * 0x9E3779B1u + (uint32_t)((uint64_t)slot >> 32) * 0x85EBCA6Bu + step * 0xC2B2AE35u;
+  h = (h ^ (h >> 16)) * 0x7FEB352Du;
+  h = (h ^ (h >> 15)) * 0x846CA68Bu;
+  h ^= h >> 16;
+  r1 = ((h & 0xFFFFu) << 4) | 8u;
+  r2 = ((h >> 16) << 4) | 8u;
+}
+
+// |x| inv, at most 448, as an e4m3 magnitude.  Times 2^-120 the exponents of
+// e4m3 (subnormals included) are those of f32, so the code is the top bits and
+// adding a random number below them rounds.  A NaN keeps being one.
+__device__ __forceinline__ uint32_t hold8(float x, float inv, uint32_t r20) {
+  const float y = __fmul_rn(fabsf(x), inv);
+  const uint32_t q = (__float_as_uint(y * 7.52316384526264e-37f) + r20) >> 20;  // 2^-120
+  return y != y ? 127u : min(q, 126u);
+}
+
+__device__ __forceinline__ void unhold4(uint32_t codes, float scale, float (&o)[4]) {
+  const __half2 a(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), __NV_E4M3));
+  const __half2 b(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3));
+  const float2 fa = __half22float2(a), fb = __half22float2(b);
+  o[0] = fa.x * scale; o[1] = fa.y * scale; o[2] = fb.x * scale; o[3] = fb.y * scale;
+}
+
+struct StepArgs {
+  Tables tab;
+  void* m;             // flat: f32, or e4m3 codes
+  void* v;
+  float* ms;           // [blocks] scales of the 8-bit states
+  float* vs;
+  float* steps;        // [tensors] steps done
+  const float* lr_ptr; // device learning rate, or NULL
+  const float* found_in;
+  Ctl* ctl;            // also the clip coefficient when ``use_ctl``
+  int use_ctl;
+  float lr, b1c, b2c, b1, b2, ln_b1, ln_b2, eps, wd;
+  int ntensors;
+};
+
+template <typename T, bool EIGHT, int MAXT>
+__global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const StepArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // A step that was called off leaves everything as it is.
+  if (a.found_in && *a.found_in != 0.f) return;
+  float coef = 1.f;
+  if (a.use_ctl) {
+    if (a.ctl->found != 0.f) return;
+    coef = a.ctl->coef;
+  }
+  const float lr = a.lr_ptr ? *a.lr_ptr : a.lr;
+  const float decay = 1.f - lr * a.wd;
+  float t_have = -1.f, alpha = 0.f, rc2 = 0.f;
+  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.tab.nblk; b += (int64_t)gridDim.x * WARPS) {
+    const int64_t blk = a.tab.blk0 + b;
+    const int ti = a.tab.tensor[blk];
+    const T* g = reinterpret_cast<const T*>(ptr.g[ti - a.tab.t0]);
+    if (!g) continue;  // no gradient: this tensor takes no step
+    T* p = reinterpret_cast<T*>(ptr.p[ti - a.tab.t0]);
+    const int64_t slot = blk * BLK;
+    const int64_t n = a.tab.numel[ti], base = slot - a.tab.slot[ti];
+    const float t = a.steps[ti] + 1.f;
+    const bool vec = aligned4<T>(p) && aligned4<T>(g);
+    float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
+    uint32_t mc[2], vc[2];
+    float msc = 0.f, vsc = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int e = j * 128 + lane * 4;
+      load4(p, base + e, n, vec, pv[j]);
+      load4(g, base + e, n, vec, gv[j]);
+      if constexpr (EIGHT) {
+        mc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.m + slot + e);
+        vc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.v + slot + e);
+      } else {
+        load4((const float*)a.m, slot + e, slot + BLK, true, mv[j]);
+        load4((const float*)a.v, slot + e, slot + BLK, true, vv[j]);
+      }
+    }
+    if constexpr (EIGHT) {
+      msc = a.ms[blk];
+      vsc = a.vs[blk];
+    }
+    if (t != t_have) {  // most often all tensors are at the same step
+      t_have = t;
+      alpha = lr / -expm1f(t * a.ln_b1);
+      rc2 = rsqrtf(-expm1f(t * a.ln_b2));
+    }
+    float mmax = 0.f, vmax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (EIGHT) {
+        unhold4(mc[j], msc, mv[j]);
+        unhold4(vc[j], vsc, vv[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // Every product and sum of the moments is rounded on its own (no fused
+        // multiply-add), so they, and with them the codes, are those of the
+        // formula taken operation by operation in f32, on any machine.
+        const float gg = __fmul_rn(gv[j][k], coef);
+        const float m = __fadd_rn(__fmul_rn(a.b1, mv[j][k]), __fmul_rn(a.b1c, gg));
+        const float v = __fadd_rn(__fmul_rn(a.b2, vv[j][k]), __fmul_rn(__fmul_rn(a.b2c, gg), gg));
+        pv[j][k] = pv[j][k] * decay - alpha * (m / (sqrtf(v) * rc2 + a.eps));
+        mv[j][k] = m;
+        vv[j][k] = v;
+        if constexpr (EIGHT) {
+          mmax = fmaxf(mmax, fabsf(m));
+          vmax = fmaxf(vmax, v);
+        }
+      }
+      store4(p, base + j * 128 + lane * 4, n, vec, pv[j]);
+      if constexpr (!EIGHT) {
+        store4((float*)a.m, slot + j * 128 + lane * 4, slot + BLK, true, mv[j]);
+        store4((float*)a.v, slot + j * 128 + lane * 4, slot + BLK, true, vv[j]);
+      }
+    }
+    if constexpr (EIGHT) {
+      mmax = warp_max(mmax);
+      vmax = warp_max(vmax);
+      const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t om = 0, ov = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t r1, r2;
+          random20(slot + j * 128 + lane * 4 + k, (uint32_t)t, r1, r2);
+          const uint32_t qm = hold8(mv[j][k], minv, r1) | (mv[j][k] < 0.f ? 128u : 0u);
+          uint32_t qv = hold8(vv[j][k], vinv, r2);
+          if (qv == 0 && vv[j][k] > 0.f && vinv > 0.f) qv = 1;
+          om |= qm << (8 * k);
+          ov |= qv << (8 * k);
+        }
+        *reinterpret_cast<uint32_t*>((unsigned char*)a.m + slot + j * 128 + lane * 4) = om;
+        *reinterpret_cast<uint32_t*>((unsigned char*)a.v + slot + j * 128 + lane * 4) = ov;
+      }
+      if (lane == 0) {
+        a.ms[blk] = mmax > TINY ? __fmul_rn(mmax, 1.f / 448.f) : 0.f;
+        a.vs[blk] = vmax > TINY ? __fmul_rn(vmax, 1.f / 448.f) : 0.f;
+      }
+    }
+  }
+  // The last block counts the step: every block has read the counts by then.
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(&a.ctl->ticket_step, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (last) {
+    for (int i = threadIdx.x; i < a.ntensors; i += blockDim.x)
+      if (ptr.g[i]) a.steps[a.tab.t0 + i] += 1.f;
+    if (threadIdx.x == 0) a.ctl->ticket_step = 0;
+  }
+}
+
+struct NormArgs {
+  Tables tab;
+  double* part;     // one sum of squares a block of every launch
+  int part0;        // this launch's first
+  int finish;       // the last launch: add up part[0 .. part0 + gridDim.x)
+  float max_norm;   // <= 0: no clipping
+  int skip;         // a norm that is not finite calls the step off
+  float* norm;      // the norm, written when not NULL
+  float* found;     // set to 1 as well when the step is called off, when not NULL
+  Ctl* ctl;
+};
+
+// Sum of squares of every gradient.  The squares are added in f64: a finite
+// gradient never overflows the sum, so the sum is finite exactly when every
+// gradient is, and one pass serves the clipping and the finite check.  The
+// order of the additions is fixed by the grid.
+template <typename T, int MAXT>
+__global__ void __launch_bounds__(WARPS * 32) grad_norm_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const NormArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double s = 0.0;
+  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.tab.nblk; b += (int64_t)gridDim.x * WARPS) {
+    const int64_t blk = a.tab.blk0 + b;
+    const int ti = a.tab.tensor[blk];
+    const T* g = reinterpret_cast<const T*>(ptr.g[ti - a.tab.t0]);
+    if (!g) continue;
+    const int64_t n = a.tab.numel[ti], base = blk * BLK - a.tab.slot[ti];
+    const bool vec = aligned4<T>(g);
+    float v[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) load4(g, base + j * 128 + lane * 4, n, vec, v[j]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += (double)v[j][k] * (double)v[j][k];
+  }
+  __shared__ double sh[WARPS];
+  __shared__ bool last;
+  auto block_sum = [&](double x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    __syncthreads();
+    if (lane == 0) sh[warp] = x;
+    __syncthreads();
+    double r = 0.0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) r += sh[i];
+    return r;
+  };
+  s = block_sum(s);
+  if (threadIdx.x == 0) {
+    a.part[a.part0 + blockIdx.x] = s;
+    __threadfence();
+    last = a.finish && atomicAdd(&a.ctl->ticket_norm, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double tot = 0.0;
+  const int np = a.part0 + (int)gridDim.x;
+  for (int i = threadIdx.x; i < np; i += blockDim.x) tot += __ldcg(a.part + i);
+  tot = block_sum(tot);
+  if (threadIdx.x == 0) {
+    const float norm = (float)sqrt(tot);
+    const bool bad = !isfinite(tot);
+    float c = 1.f;
+    if (a.max_norm > 0.f) {
+      const float r = (float)((double)a.max_norm / (sqrt(tot) + 1e-6));
+      c = r >= 1.f ? 1.f : r;  // a NaN stays one
+    }
+    a.ctl->coef = c;
+    a.ctl->found = a.skip && bad ? 1.f : 0.f;
+    if (a.skip && bad && a.found) *a.found = 1.f;
+    if (a.norm) *a.norm = norm;
+    a.ctl->ticket_norm = 0;
+  }
+}
+
+constexpr int MAX_FEW = 32, MAX_MANY = 512;  // tensors of one launch (their pointers are its arguments)
+
+int grid_for(int64_t nblk, int per_sm) {
+  return (int)std::min<int64_t>((nblk + WARPS - 1) / WARPS, (int64_t)device_sm_count() * per_sm);
+}
+
+int check(const ow_adamw_t* a) {
+  OW_CHECK_ARG(a != nullptr, "ow_adamw: args is NULL");
+  OW_CHECK_ARG(a->tensors > 0, "ow_adamw: tensors must be positive (got %d)", a->tensors);
+  OW_CHECK_ARG(a->params && a->grads && a->slots, "ow_adamw: params, grads or slots is NULL");
+  OW_CHECK_ARG(a->dev_slots && a->dev_numel && a->dev_block_tensor && a->control, "ow_adamw: a device table is NULL");
+  if (a->dtype != OW_DTYPE_F32 && a->dtype != OW_DTYPE_BF16 && a->dtype != OW_DTYPE_F16) {
+    set_error("ow_adamw: parameters must be float32, bfloat16 or float16 (dtype code %d)", a->dtype);
+    return OW_ERR_UNSUPPORTED;
+  }
+  for (int i = 0; i < a->tensors; ++i)
+    OW_CHECK_ARG(a->slots[i] >= 0 && a->slots[i] % BLK == 0 && a->slots[i + 1] % BLK == 0 && a->slots[i] < a->slots[i + 1],
+                 "ow_adamw: slots of tensor %d must be a rising multiple of %d", i, BLK);
+  return OW_OK;
+}
+
+// Calls f(pointers, tables, tensors of the launch) for each launch of the call.
+template <class F>
+int each_launch(const ow_adamw_t* a, F&& f) {
+  for (int t0 = 0; t0 < a->tensors; t0 += MAX_MANY) {
+    const int n = std::min(MAX_MANY, a->tensors - t0);
+    Tables tab{a->dev_slots, a->dev_numel, a->dev_block_tensor, t0, a->slots[t0] / BLK,
+               (a->slots[t0 + n] - a->slots[t0]) / BLK};
+    const bool end = t0 + n == a->tensors;
+    auto fill = [&](auto& ptr) {
+      for (int i = 0; i < n; ++i) {
+        ptr.g[i] = a->grads[t0 + i];
+        ptr.p[i] = a->params[t0 + i];
+      }
+    };
+    if (n <= MAX_FEW) {  // a launch with few pointers starts sooner than one with 8 KB of them
+      Ptrs<MAX_FEW> ptr{};
+      fill(ptr);
+      OW_RETURN_IF(f(ptr, tab, n, end));
+    } else {
+      Ptrs<MAX_MANY> ptr{};
+      fill(ptr);
+      OW_RETURN_IF(f(ptr, tab, n, end));
+    }
+  }
+  return OW_OK;
+}
+
+template <class F>
+int by_type(int dtype, F&& f) {
+  if (dtype == OW_DTYPE_F32) return f((float*)nullptr);
+  if (dtype == OW_DTYPE_BF16) return f((__nv_bfloat16*)nullptr);
+  return f((__half*)nullptr);
+}
+
+constexpr int NORM_PER_SM = 6, STEP_PER_SM = 8;
+
+}  // namespace
+}  // namespace ow
+
+using namespace ow;
+
+extern "C" {
+
+int32_t ow_grad_norm_partials(const ow_adamw_t* a) {
+  clear_error();
+  if (!a || a->tensors <= 0 || !a->slots) {
+    set_error("ow_grad_norm_partials: no tensors");
+    return 0;
+  }
+  int32_t n = 0;
+  for (int t0 = 0; t0 < a->tensors; t0 += MAX_MANY) {
+    const int c = std::min(MAX_MANY, a->tensors - t0);
+    n += grid_for((a->slots[t0 + c] - a->slots[t0]) / BLK, NORM_PER_SM);
+  }
+  return n;
+}
+
+int ow_grad_norm(const ow_adamw_t* a, const ow_grad_norm_t* o, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  OW_CHECK_ARG(o && o->partials, "ow_grad_norm: options or partials is NULL");
+  OW_CHECK_ARG(o->first >= 0 && o->capacity >= o->first + ow_grad_norm_partials(a),
+               "ow_grad_norm: room for %d partial sums from %d on is needed, got %d", ow_grad_norm_partials(a), o->first,
+               o->capacity);
+  int at = o->first;
+  return by_type(a->dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return each_launch(a, [&](auto& ptr, const Tables& tab, int, bool end) -> int {
+      NormArgs k{tab, o->partials, at, o->finish && end, o->max_norm, o->skip_nonfinite, o->norm, o->found, (Ctl*)a->control};
+      const int grid = grid_for(tab.nblk, NORM_PER_SM);
+      at += grid;
+      using P = std::remove_reference_t<decltype(ptr)>;
+      launch(grad_norm_kernel<T, sizeof(ptr.p) / sizeof(void*)>, grid, WARPS * 32, 0, (cudaStream_t)stream, (const P&)ptr, k);
+      OW_CHECK_LAUNCH("grad_norm_kernel");
+      return OW_OK;
+    });
+  });
+}
+
+int ow_adamw_step(const ow_adamw_t* a, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  OW_CHECK_ARG(a->state_bits == 32 || a->state_bits == 8, "ow_adamw_step: state_bits must be 32 or 8 (got %d)", a->state_bits);
+  OW_CHECK_ARG(a->exp_avg && a->exp_avg_sq && a->dev_steps, "ow_adamw_step: a state pointer is NULL");
+  OW_CHECK_ARG(a->state_bits == 32 || (a->exp_avg_scale && a->exp_avg_sq_scale), "ow_adamw_step: 8-bit states need their scales");
+  OW_CHECK_ARG(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "ow_adamw_step: betas must be in [0, 1)");
+  for (int i = 0; i < a->tensors; ++i)
+    OW_CHECK_ARG(a->params[i] || !a->grads[i], "ow_adamw_step: parameter %d is NULL", i);
+  StepArgs k{};
+  k.m = a->exp_avg; k.v = a->exp_avg_sq;
+  k.ms = a->exp_avg_scale; k.vs = a->exp_avg_sq_scale;
+  k.steps = a->dev_steps;
+  k.lr_ptr = a->lr_ptr;
+  k.found_in = a->found;
+  k.ctl = (Ctl*)a->control;
+  k.use_ctl = a->use_norm;
+  k.lr = (float)a->lr;
+  k.b1 = (float)a->beta1; k.b2 = (float)a->beta2;
+  k.b1c = (float)(1.0 - a->beta1); k.b2c = (float)(1.0 - a->beta2);
+  k.ln_b1 = (float)log(a->beta1); k.ln_b2 = (float)log(a->beta2);  // -inf for 0: the correction is then 1
+  k.eps = (float)a->eps; k.wd = (float)a->weight_decay;
+  return by_type(a->dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return each_launch(a, [&](auto& ptr, const Tables& tab, int n, bool) -> int {
+      k.tab = tab;
+      k.ntensors = n;
+      const int grid = grid_for(tab.nblk, STEP_PER_SM);
+      using P = std::remove_reference_t<decltype(ptr)>;
+      constexpr int MAXT = sizeof(ptr.p) / sizeof(void*);
+      if (a->state_bits == 8)
+        launch(adamw_kernel<T, true, MAXT>, grid, WARPS * 32, 0, (cudaStream_t)stream, (const P&)ptr, k);
+      else
+        launch(adamw_kernel<T, false, MAXT>, grid, WARPS * 32, 0, (cudaStream_t)stream, (const P&)ptr, k);
+      OW_CHECK_LAUNCH("adamw_kernel");
+      return OW_OK;
+    });
+  });
+}
+
+}  // extern "C"

@@ -32,6 +32,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from omniwave_b200.optim import AdamW
+
 __all__ = ["DistInfo", "EMA", "init_distributed", "broadcast_parameters", "shard_range", "TrainStep"]
 
 
@@ -133,6 +135,11 @@ class TrainStep:
     raises ``FloatingPointError`` afterwards, as the reference raises at
     the step itself.
 
+    ``optimizer="fused"`` (CUDA only) takes the step with
+    ``omniwave_b200.optim.AdamW`` in the place of torch's: finite check, norm
+    and clipping in one pass over the gradients, the update in another, the
+    moments in ``state_bits`` bits (32, or 8).
+
     ``cuda_graph=True`` (single process only) captures the whole step --
     forward, backward, finite check, optimizer and EMA -- into one CUDA
     graph after ``graph_warmup`` eager steps; later steps copy the batch
@@ -152,7 +159,13 @@ class TrainStep:
         ema_decay: float | None = None,
         cuda_graph: bool = False,
         graph_warmup: int = 3,
+        optimizer: str = "torch",
+        state_bits: int = 32,
     ) -> None:
+        if optimizer not in ("torch", "fused"):
+            raise ValueError(f"optimizer must be 'torch' or 'fused', got {optimizer!r}")
+        if state_bits != 32 and optimizer != "fused":
+            raise ValueError("state_bits other than 32 needs optimizer='fused'")
         self.device = next(model.parameters()).device
         distributed = dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
         if distributed and broadcast:
@@ -171,9 +184,15 @@ class TrainStep:
         else:
             self.model = model
         on_cuda = self.device.type == "cuda"
-        self.optimizer = torch.optim.AdamW(
-            model.parameters(), lr=lr, weight_decay=weight_decay, fused=on_cuda,
-            capturable=cuda_graph)
+        self._fused = optimizer == "fused"
+        if self._fused:
+            self.optimizer: torch.optim.Optimizer = AdamW(
+                model.parameters(), lr=lr, weight_decay=weight_decay, state_bits=state_bits,
+                max_norm=clip_norm, skip_nonfinite=True)
+        else:
+            self.optimizer = torch.optim.AdamW(
+                model.parameters(), lr=lr, weight_decay=weight_decay, fused=on_cuda,
+                capturable=cuda_graph)
         self.amp_dtype = amp_dtype if on_cuda else None
         self.clip_norm = clip_norm
         self.ema = EMA(model, ema_decay) if ema_decay is not None else None
@@ -199,6 +218,17 @@ class TrainStep:
         loss.backward()
         loss = loss.detach()
         self._found.copy_((~torch.isfinite(loss)).to(torch.float32))
+        if self._fused:
+            self.optimizer.step(found_inf=self._found)  # also sets it for a non-finite gradient
+        else:
+            self._torch_update()
+        if self.ema is not None:
+            self.ema.update(self.module, skip=self._found)
+        self._bad |= self._found.bool()
+        return loss
+
+    def _torch_update(self) -> None:
+        """Finite check of the gradients, clipping and the update with torch's AdamW."""
         grads = [p.grad for p in self._params if p.grad is not None]
         if self.device.type == "cuda":
             # One multi-tensor pass: sets _found when any gradient is inf/nan.
@@ -218,10 +248,6 @@ class TrainStep:
                 keep = self._found.bool()
                 for p, old in zip(self._params, snapshot):
                     p.copy_(torch.where(keep, old, p))
-        if self.ema is not None:
-            self.ema.update(self.module, skip=self._found)
-        self._bad |= self._found.bool()
-        return loss
 
     def step(self, images: Tensor, labels: Tensor) -> Tensor:
         """Forward, backward (gradients all-reduced by DDP), optimizer step.
