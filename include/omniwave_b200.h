@@ -439,6 +439,67 @@ OW_API int32_t ow_grad_norm_partials(const ow_adamw_t* args);
 OW_API int ow_grad_norm(const ow_adamw_t* args, const ow_grad_norm_t* options, void* stream);
 OW_API int ow_adamw_step(const ow_adamw_t* args, void* stream);
 
+/*
+ * RMSNorm before and after a block, fused with the block's gate, the
+ * per-sample residual scale and the residual add (the norm, LayerScale and
+ * drop-path of omniweave/models/block.py:80-108 around an operator that is
+ * normalised on both sides).  x, delta, h and n are [samples, tokens,
+ * channels]; rms(v) = v rsqrt(mean(v^2) + eps) over the channels:
+ *
+ *   h = x + sample_scale[b] * gate[c] * rms(delta) * post_w[c]
+ *   n = rms(h) * next_w[c]
+ *
+ * in f32, each output rounded once; n is taken from the f32 h.  delta NULL:
+ * h is x, only n is written (the plain RMSNorm).  next_w NULL: only h is.
+ * gate_rows: 0 no gate, 1 a gate [channels], samples a gate [samples,
+ * channels].  dtypes are f32, bf16 or f16, each array its own; h has x's.
+ * rstd_delta and rstd_h [samples * tokens] are written by the forward when
+ * not NULL and read by the backward.
+ *
+ * The backward takes dh (x's dtype, NULL for zero) and dn (n's dtype, needed
+ * with next_w) and writes dx, ddelta and, where not NULL, the weights'
+ * gradients in their dtypes; these are added in f32 in a fixed order.
+ */
+typedef struct ow_norm_t {
+  int64_t samples, tokens;
+  int32_t channels;
+  const void* x;
+  int32_t x_dtype;
+  const void* delta;
+  int32_t delta_dtype;
+  const void* post_w;
+  int32_t post_dtype;
+  const void* gate;
+  int32_t gate_dtype;
+  int64_t gate_rows;
+  const float* sample_scale;   /* [samples] or NULL */
+  const void* next_w;
+  int32_t next_dtype;
+  double eps;
+  void* h;                     /* forward only */
+  void* n;                     /* forward only */
+  int32_t n_dtype;
+  float* rstd_delta;
+  float* rstd_h;
+  void* workspace;             /* backward only: ow_norm_bwd_workspace_size() bytes */
+  size_t workspace_bytes;
+} ow_norm_t;
+
+typedef struct ow_norm_grads_t {
+  const void* dh;
+  const void* dn;
+  void* dx;
+  void* ddelta;
+  void* dpost;
+  void* dgate;
+  void* dnext;
+} ow_norm_grads_t;
+
+/* Workspace bytes of ow_norm_bwd (0 if the arguments are invalid). */
+OW_API size_t ow_norm_bwd_workspace_size(const ow_norm_t* args);
+OW_API int ow_norm_fwd(const ow_norm_t* args, void* stream);
+OW_API int ow_norm_bwd(const ow_norm_t* args, const ow_norm_grads_t* grads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

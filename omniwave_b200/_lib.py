@@ -118,6 +118,22 @@ class GradNorm(ctypes.Structure):
     ]
 
 
+class Norm(ctypes.Structure):
+    _fields_ = [
+        ("samples", ctypes.c_int64), ("tokens", ctypes.c_int64), ("channels", _c_i32),
+        ("x", _vp), ("x_dtype", _c_i32), ("delta", _vp), ("delta_dtype", _c_i32),
+        ("post_w", _vp), ("post_dtype", _c_i32), ("gate", _vp), ("gate_dtype", _c_i32),
+        ("gate_rows", ctypes.c_int64), ("sample_scale", _vp), ("next_w", _vp), ("next_dtype", _c_i32),
+        ("eps", _c_f64), ("h", _vp), ("n", _vp), ("n_dtype", _c_i32),
+        ("rstd_delta", _vp), ("rstd_h", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class NormGrads(ctypes.Structure):
+    _fields_ = [(k, _vp) for k in ("dh", "dn", "dx", "ddelta", "dpost", "dgate", "dnext")]
+
+
 ADAMW_BLOCK = 256
 ADAMW_CONTROL_BYTES = 64
 
@@ -133,6 +149,7 @@ EXPORTS = (
     "ow_pool_head_workspace_size", "ow_pool_head_fwd",
     "ow_d2s_linear_workspace_size", "ow_d2s_linear_fwd",
     "ow_grad_norm_partials", "ow_grad_norm", "ow_adamw_step",
+    "ow_norm_bwd_workspace_size", "ow_norm_fwd", "ow_norm_bwd",
 )
 
 _lock = threading.Lock()
@@ -197,6 +214,12 @@ def load() -> ctypes.CDLL:
         lib.ow_grad_norm.restype = ctypes.c_int
         lib.ow_adamw_step.argtypes = [ctypes.POINTER(AdamW), _vp]
         lib.ow_adamw_step.restype = ctypes.c_int
+        lib.ow_norm_bwd_workspace_size.argtypes = [ctypes.POINTER(Norm)]
+        lib.ow_norm_bwd_workspace_size.restype = ctypes.c_size_t
+        lib.ow_norm_fwd.argtypes = [ctypes.POINTER(Norm), _vp]
+        lib.ow_norm_fwd.restype = ctypes.c_int
+        lib.ow_norm_bwd.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(NormGrads), _vp]
+        lib.ow_norm_bwd.restype = ctypes.c_int
         v = lib.ow_abi_version()
         if v != ABI_VERSION:
             raise NativeLibraryError(f"ABI version mismatch: library {v}, binding {ABI_VERSION}")

@@ -1,0 +1,719 @@
+// RMSNorm before and after a block, fused with the block's gate, the
+// per-sample residual scale and the residual add.
+//
+// A row is one token's C channels; sample b owns ``tokens`` rows.  With
+// rms(v) = v rsqrt(mean(v^2) + eps), everything in f32:
+//   d^ = rms(delta);  h = x + s_b q (d^ wp)          (post-norm, gate q, scale s)
+//   h^ = rms(h);      n = h^ wn                      (the next block's pre-norm)
+// Without delta h is x and only n is written.  Backward, from dh and dn:
+//   u = dn wn;        D = dh + r_h (u - h^ mean(u h^))                dx = D
+//   e = s q wp D;     ddelta = r_d (e - d^ mean(e d^))
+//   dwn = sum dn h^;  dwp = sum s q D d^;  dq = sum s D d^ wp
+// h is recomputed from x and delta, so the f32 sums see the f32 h and not the
+// rounded one, and nothing but x, delta and two floats a row is kept.
+//
+// Split.  G threads share a row, each with NV vectors of V channels in
+// registers, so a row is read once; rows of up to 32 lanes need only shuffles.
+// The backward needs three sums a row, taken in one exchange: with
+// A = sum e' (dh + r_h u), B = sum e' h^, S = sum u h^ (e' = s q wp d^),
+// mean(e d^) = (A - B r_h S / C) / C.  Each thread keeps its channels' share of
+// the weight gradients in registers over all its rows; a block leaves one
+// partial row and a second kernel adds these in a fixed order.
+//
+// Bound: HBM.
+#include <algorithm>
+
+#include "ow_common.cuh"
+#include "ow_internal.h"
+
+namespace ow {
+namespace {
+
+struct Args {
+  int64_t rows, tokens;
+  int C;
+  const void* x;
+  const void* delta;
+  const void* dh;
+  const void* dn;
+  const void* wp;
+  const void* q;
+  const void* wn;
+  int wp_dt, q_dt, wn_dt, n_dt;
+  int x_dt, d_dt;
+  int q_rows;            // 0: no gate, 1: one for all, else one for each sample
+  const float* scale;    // [samples] or NULL
+  float eps, inv_c;
+  void* h;
+  void* n;
+  float* rd;             // [rows] 1 / rms(delta)
+  float* rh;             // [rows] 1 / rms(h)
+  void* dx;
+  void* ddelta;
+  float* part;           // [parts][arrays][C] partial weight gradients
+  int arrays;            // 3: dwn, dwp, dq; 1: dwn
+  int64_t groups;        // gate rows whose gradients are kept apart (1 or samples)
+  int per_group;         // blocks that share a group's rows
+  int64_t group_rows;
+};
+
+// V channels from p (an array of dtype dt) as floats.
+template <int V>
+__device__ __forceinline__ void ldv(const void* p, int dt, int64_t i, float (&o)[V]) {
+  if (dt == OW_DTYPE_F32) {
+    const float* f = (const float*)p + i;
+    if constexpr (V == 8) {
+      const float4 a = *reinterpret_cast<const float4*>(f), b = *reinterpret_cast<const float4*>(f + 4);
+      o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+    } else {
+      o[0] = f[0];
+    }
+  } else if constexpr (V == 8) {
+    const uint4 r = *reinterpret_cast<const uint4*>((const uint16_t*)p + i);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float2 f;
+      if (dt == OW_DTYPE_BF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+      else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      o[2 * k] = f.x;
+      o[2 * k + 1] = f.y;
+    }
+  } else {
+    o[0] = dt == OW_DTYPE_BF16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : __half2float(((const __half*)p)[i]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void stv(void* p, int dt, int64_t i, const float (&v)[V]) {
+  if (dt == OW_DTYPE_F32) {
+    float* f = (float*)p + i;
+    if constexpr (V == 8) {
+      *reinterpret_cast<float4*>(f) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(f + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      f[0] = v[0];
+    }
+  } else if constexpr (V == 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (dt == OW_DTYPE_BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&t);
+      } else {
+        const __half2 t = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+    }
+    *reinterpret_cast<uint4*>((uint16_t*)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if (dt == OW_DTYPE_BF16) {
+    ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v[0]);
+  } else {
+    ((__half*)p)[i] = __float2half_rn(v[0]);
+  }
+}
+
+__device__ __forceinline__ float ld1(const void* p, int dt, int64_t i) {
+  float o[1];
+  ldv<1>(p, dt, i, o);
+  return o[0];
+}
+
+// Sum of K values over the G threads of a row; every thread gets it.  Rows of
+// more than a warp meet in shared memory (``sh``: [2][K][32] floats a block,
+// used in turn, so one barrier an exchange is enough).
+template <int G, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int& turn) {
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (G > 32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w0 = threadIdx.x / G * (G / 32);
+    float* s = sh + turn * K * 32;
+    turn ^= 1;
+    if (lane == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k * 32 + warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < G / 32; ++i) t += s[k * 32 + w0 + i];
+      v[k] = t;
+    }
+  }
+}
+
+// One block does ``blockDim / G`` rows at a time and strides over all rows.
+template <int V, int G, int NV, bool DELTA, bool NEXT>
+__global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args a) {
+  constexpr int T = G > 256 ? G : 256, RB = T / G;
+  __shared__ float sh[G > 32 ? 2 * 32 : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.rows; r0 += (int64_t)gridDim.x * RB) {
+    const int64_t row = r0 + sub;
+    const bool live = row < a.rows;
+    const int64_t at = row * a.C;
+    float x[NV][V], d[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+      const bool on = live && c < a.C;
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = 0.f;
+      if (on) {
+        ldv<V>(a.x, a.x_dt, at + c, x[j]);
+        if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
+      }
+    }
+    if constexpr (DELTA) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[0] += d[j][k] * d[j][k];
+      row_sum<G>(s, sh, turn);
+      const float rd = rsqrtf(s[0] * a.inv_c + a.eps);
+      if (live && lane == 0 && a.rd) a.rd[row] = rd;
+      const int64_t b = live ? row / a.tokens : 0;
+      const float sc = rd * (a.scale ? a.scale[b] : 1.f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + lane) * V;
+        if (!live || c >= a.C) continue;
+        float w[V], q[V];
+        ldv<V>(a.wp, a.wp_dt, c, w);
+        if (a.q_rows) {
+          ldv<V>(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c, q);
+#pragma unroll
+          for (int k = 0; k < V; ++k) w[k] *= q[k];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[j][k] += sc * d[j][k] * w[k];
+        stv<V>(a.h, a.x_dt, at + c, x[j]);
+      }
+    }
+    if constexpr (NEXT) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[0] += x[j][k] * x[j][k];
+      row_sum<G>(s, sh, turn);
+      const float rh = rsqrtf(s[0] * a.inv_c + a.eps);
+      if (live && lane == 0 && a.rh) a.rh[row] = rh;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + lane) * V;
+        if (!live || c >= a.C) continue;
+        float w[V];
+        ldv<V>(a.wn, a.wn_dt, c, w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[k] *= x[j][k] * rh;
+        stv<V>(a.n, a.n_dt, at + c, w);
+      }
+    }
+  }
+}
+
+// Block (group, part) strides over its group's rows; ``part`` gets its sums.
+template <int V, int G, int NV, bool DELTA, bool NEXT>
+__global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args a) {
+  constexpr int T = G > 256 ? G : 256, RB = T / G;
+  extern __shared__ float dyn[];  // the block's sums over its row groups (RB > 1)
+  __shared__ float sh[G > 32 ? 2 * 3 * 32 : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int64_t group = blockIdx.x / a.per_group;
+  const int part = blockIdx.x % a.per_group;
+  const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
+  float an[NV][V], ap[NV][V], aq[NV][V];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int k = 0; k < V; ++k) an[j][k] = ap[j][k] = aq[j][k] = 0.f;
+
+  for (int64_t r0 = group * a.group_rows + (int64_t)part * RB; r0 < row_end; r0 += (int64_t)a.per_group * RB) {
+    const int64_t row = r0 + sub;
+    const bool live = row < row_end;
+    const int64_t at = row * a.C;
+    const int64_t b = live ? row / a.tokens : 0;
+    float x[NV][V], d[NV][V], gh[NV][V], gn[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+      const bool on = live && c < a.C;
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = gh[j][k] = gn[j][k] = 0.f;
+      if (on) {
+        if constexpr (NEXT) {
+          ldv<V>(a.x, a.x_dt, at + c, x[j]);
+          ldv<V>(a.dn, a.n_dt, at + c, gn[j]);
+        }
+        if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
+        if (a.dh) ldv<V>(a.dh, a.x_dt, at + c, gh[j]);
+      }
+    }
+    const float rd = DELTA && live ? a.rd[row] : 0.f, rh = NEXT && live ? a.rh[row] : 0.f;
+    const float sc = DELTA && a.scale ? a.scale[b] : 1.f;
+    float wp[NV][V], q[NV][V], wn[NV][V];
+    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+#pragma unroll
+      for (int k = 0; k < V; ++k) { wp[j][k] = wn[j][k] = 0.f; q[j][k] = 1.f; }
+      if (live && c < a.C) {
+        if constexpr (DELTA) {
+          ldv<V>(a.wp, a.wp_dt, c, wp[j]);
+          if (a.q_rows) ldv<V>(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c, q[j]);
+        }
+        if constexpr (NEXT) ldv<V>(a.wn, a.wn_dt, c, wn[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float e = 0.f;
+        if constexpr (DELTA) {
+          d[j][k] *= rd;                                // d^
+          e = sc * q[j][k] * wp[j][k] * d[j][k];        // h - x
+        }
+        if constexpr (NEXT) {
+          x[j][k] = (x[j][k] + e) * rh;                 // h^
+          const float u = gn[j][k] * wn[j][k];
+          an[j][k] += gn[j][k] * x[j][k];
+          s[0] += u * x[j][k];
+          if constexpr (DELTA) s[2] += e * x[j][k];
+          gh[j][k] += rh * u;
+        }
+        if constexpr (DELTA) s[1] += e * gh[j][k];
+      }
+    }
+    row_sum<G>(s, sh, turn);
+    const float mu = s[0] * a.inv_c * rh;              // r_h mean(u h^)
+    const float me = (s[1] - s[2] * mu) * a.inv_c;     // mean(e d^)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+      if (!live || c >= a.C) continue;
+      float o[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float D = NEXT ? gh[j][k] - x[j][k] * mu : gh[j][k];
+        gh[j][k] = D;
+        if constexpr (DELTA) {
+          const float f = sc * D * d[j][k];
+          ap[j][k] += f * q[j][k];
+          aq[j][k] += f * wp[j][k];
+          o[k] = rd * (sc * q[j][k] * wp[j][k] * D - d[j][k] * me);
+        }
+      }
+      stv<V>(a.dx, a.x_dt, at + c, gh[j]);
+      if constexpr (DELTA) stv<V>(a.ddelta, a.d_dt, at + c, o);
+    }
+  }
+
+  float* out = a.part + (int64_t)blockIdx.x * a.arrays * a.C;
+  auto leave = [&](float (&v)[NV][V], int which) {
+    float* to = out + (int64_t)which * a.C;
+    if constexpr (RB > 1) {  // add the block's row groups in order
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const int c = (j * G + lane) * V + k;
+          if (c < a.C) dyn[sub * a.C + c] = v[j][k];
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.C; c += T) {
+        float t = 0.f;
+        for (int i = 0; i < RB; ++i) t += dyn[i * a.C + c];
+        to[c] = t;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const int c = (j * G + lane) * V + k;
+          if (c < a.C) to[c] = v[j][k];
+        }
+    }
+  };
+  int which = 0;
+  if constexpr (NEXT) leave(an, which++);
+  if constexpr (DELTA) {
+    leave(ap, which++);
+    leave(aq, which++);
+  }
+}
+
+// Rows longer than the kernels above hold: one block a row, read again for
+// each pass.  part is added by the same second kernel.
+template <bool DELTA, bool NEXT>
+__global__ void __launch_bounds__(256) norm_long_fwd_kernel(const Args a) {
+  __shared__ float sh[2 * 32];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t at = row * a.C, b = row / a.tokens;
+    float rd = 0.f;
+    if constexpr (DELTA) {
+      float s[1] = {0.f};
+      for (int c = threadIdx.x; c < a.C; c += 256) {
+        const float d = ld1(a.delta, a.d_dt, at + c);
+        s[0] += d * d;
+      }
+      row_sum<256>(s, sh, turn);
+      rd = rsqrtf(s[0] * a.inv_c + a.eps);
+      if (threadIdx.x == 0 && a.rd) a.rd[row] = rd;
+    }
+    const float sc = DELTA ? rd * (a.scale ? a.scale[b] : 1.f) : 0.f;
+    auto hval = [&](int c) {
+      float h = ld1(a.x, a.x_dt, at + c);
+      if constexpr (DELTA) {
+        float w = ld1(a.wp, a.wp_dt, c);
+        if (a.q_rows) w *= ld1(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c);
+        h += sc * ld1(a.delta, a.d_dt, at + c) * w;
+      }
+      return h;
+    };
+    float s[1] = {0.f};
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const float h[1] = {hval(c)};
+      s[0] += h[0] * h[0];
+      if constexpr (DELTA) stv<1>(a.h, a.x_dt, at + c, h);
+    }
+    if constexpr (NEXT) {
+      row_sum<256>(s, sh, turn);
+      const float rh = rsqrtf(s[0] * a.inv_c + a.eps);
+      if (threadIdx.x == 0 && a.rh) a.rh[row] = rh;
+      for (int c = threadIdx.x; c < a.C; c += 256) {
+        const float o[1] = {hval(c) * rh * ld1(a.wn, a.wn_dt, c)};
+        stv<1>(a.n, a.n_dt, at + c, o);
+      }
+    }
+  }
+}
+
+template <bool DELTA, bool NEXT>
+__global__ void __launch_bounds__(256) norm_long_bwd_kernel(const Args a) {
+  __shared__ float sh[2 * 3 * 32];
+  int turn = 0;
+  const int64_t group = blockIdx.x / a.per_group;
+  const int part = blockIdx.x % a.per_group;
+  const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
+  float* out = a.part + (int64_t)blockIdx.x * a.arrays * a.C;
+  for (int c = threadIdx.x; c < a.C; c += 256)
+    for (int i = 0; i < a.arrays; ++i) out[(int64_t)i * a.C + c] = 0.f;  // each thread adds to its own channels only
+  for (int64_t row = group * a.group_rows + part; row < row_end; row += a.per_group) {
+    const int64_t at = row * a.C, b = row / a.tokens;
+    const float rd = DELTA ? a.rd[row] : 0.f, rh = NEXT ? a.rh[row] : 0.f;
+    const float sc = DELTA && a.scale ? a.scale[b] : 1.f;
+    struct El { float d, e, q, wp, hh, g, gn; };
+    auto el = [&](int c) {
+      El r{};
+      r.q = 1.f;
+      if constexpr (DELTA) {
+        r.d = ld1(a.delta, a.d_dt, at + c) * rd;
+        r.wp = ld1(a.wp, a.wp_dt, c);
+        if (a.q_rows) r.q = ld1(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c);
+        r.e = sc * r.q * r.wp * r.d;
+      }
+      r.g = a.dh ? ld1(a.dh, a.x_dt, at + c) : 0.f;
+      if constexpr (NEXT) {
+        r.hh = (ld1(a.x, a.x_dt, at + c) + r.e) * rh;
+        r.gn = ld1(a.dn, a.n_dt, at + c);
+      }
+      return r;
+    };
+    float s[3] = {0.f, 0.f, 0.f};
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      El r = el(c);
+      if constexpr (NEXT) {
+        const float u = r.gn * ld1(a.wn, a.wn_dt, c);
+        s[0] += u * r.hh;
+        s[2] += r.e * r.hh;
+        r.g += rh * u;
+      }
+      s[1] += r.e * r.g;
+    }
+    row_sum<256>(s, sh, turn);
+    const float mu = s[0] * a.inv_c * rh, me = (s[1] - s[2] * mu) * a.inv_c;
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const El r = el(c);
+      float D[1] = {r.g};
+      int which = 0;
+      if constexpr (NEXT) {
+        D[0] += rh * r.gn * ld1(a.wn, a.wn_dt, c) - r.hh * mu;
+        out[c] += r.gn * r.hh;
+        which = 1;
+      }
+      stv<1>(a.dx, a.x_dt, at + c, D);
+      if constexpr (DELTA) {
+        const float f = sc * D[0] * r.d;
+        out[(int64_t)which * a.C + c] += f * r.q;
+        out[(int64_t)(which + 1) * a.C + c] += f * r.wp;
+        const float o[1] = {rd * (sc * r.q * r.wp * D[0] - r.d * me)};
+        stv<1>(a.ddelta, a.d_dt, at + c, o);
+      }
+    }
+  }
+}
+
+// Column sums of the partial rows: 32 channels a block, 8 threads a channel,
+// added in the order of the parts.  ``apart``: array ``q_at`` is summed for
+// each group of its own.
+struct SumArgs {
+  const float* part;
+  int C, arrays, per_group;
+  int64_t groups;
+  void* out[3];
+  int dt[3];
+  int q_at;        // the array that is summed group by group (-1: none)
+};
+
+__global__ void __launch_bounds__(256) norm_sum_kernel(const SumArgs a) {
+  __shared__ float sh[8][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
+  // blockIdx.y: the arrays summed over all groups first, then (q_at, group)
+  int which = 0;
+  int64_t p0 = 0, p1 = a.groups * a.per_group, orow = 0;
+  const int whole = a.arrays - (a.q_at >= 0 ? 1 : 0);
+  for (int64_t y = blockIdx.y; y < whole + (a.q_at >= 0 ? a.groups : 0); y += gridDim.y) {
+    if (y < whole) {
+      which = (int)y;
+      p0 = 0;
+      p1 = a.groups * a.per_group;
+      orow = 0;
+    } else {
+      which = a.q_at;
+      orow = y - whole;
+      p0 = orow * a.per_group;
+      p1 = p0 + a.per_group;
+    }
+    float t = 0.f;
+    if (c < a.C && a.out[which])
+      for (int64_t p = p0 + ry; p < p1; p += 8) t += a.part[(p * a.arrays + which) * a.C + c];
+    sh[ry][cx] = t;
+    __syncthreads();
+    if (ry == 0 && c < a.C && a.out[which]) {
+      float v[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[0] += sh[i][cx];
+      stv<1>(a.out[which], a.dt[which], orow * a.C + c, v);
+    }
+    __syncthreads();
+  }
+}
+
+bool float_type(int dt) { return dt == OW_DTYPE_F32 || dt == OW_DTYPE_BF16 || dt == OW_DTYPE_F16; }
+
+int check(const ow_norm_t* a) {
+  OW_CHECK_ARG(a != nullptr, "ow_norm: args is NULL");
+  OW_CHECK_ARG(a->samples >= 0 && a->tokens >= 0 && a->channels > 0, "ow_norm: bad shape [%lld, %lld, %d]",
+               (long long)a->samples, (long long)a->tokens, a->channels);
+  OW_CHECK_ARG(a->samples < (1LL << 31) && a->tokens < (1LL << 31) && a->samples * a->tokens < (1LL << 40), "ow_norm: too many rows");
+  const bool d = a->delta != nullptr;
+  OW_CHECK_ARG(a->x && (!d || a->post_w) && (d || a->next_w), "ow_norm: an input pointer is NULL");
+  OW_CHECK_ARG(a->gate_rows == 0 || (d && a->gate && (a->gate_rows == 1 || a->gate_rows == a->samples)),
+               "ow_norm: the gate must have 1 row or one for each sample (got %lld)", (long long)a->gate_rows);
+  OW_CHECK_ARG(d || !a->sample_scale, "ow_norm: a residual scale needs delta");
+  if (!float_type(a->x_dtype) || (d && (!float_type(a->delta_dtype) || !float_type(a->post_dtype))) ||
+      (a->gate_rows && !float_type(a->gate_dtype)) || (a->next_w && (!float_type(a->next_dtype) || !float_type(a->n_dtype)))) {
+    set_error("ow_norm: dtypes must be float32, bfloat16 or float16");
+    return OW_ERR_UNSUPPORTED;
+  }
+  OW_CHECK_ARG(a->eps >= 0.0, "ow_norm: eps must not be negative");
+  return OW_OK;
+}
+
+Args base(const ow_norm_t* a) {
+  Args k{};
+  k.rows = a->samples * a->tokens;
+  k.tokens = a->tokens;
+  k.C = a->channels;
+  k.x = a->x; k.delta = a->delta;
+  k.wp = a->post_w; k.q = a->gate; k.wn = a->next_w;
+  k.x_dt = a->x_dtype; k.d_dt = a->delta_dtype;
+  k.wp_dt = a->post_dtype; k.q_dt = a->gate_dtype; k.wn_dt = a->next_dtype; k.n_dt = a->n_dtype;
+  k.q_rows = a->gate_rows > 1 ? 2 : (int)a->gate_rows;
+  k.scale = a->sample_scale;
+  k.eps = (float)a->eps;
+  k.inv_c = 1.f / (float)a->channels;
+  k.rd = a->rstd_delta; k.rh = a->rstd_h;
+  return k;
+}
+
+// 16-byte vectors of 8 channels need every array on 16 bytes and rows of a
+// multiple of 8 channels.
+bool vectors(const Args& k, const void* const* more, int n) {
+  if (k.C % 8) return false;
+  const void* all[] = {k.x, k.delta, k.wp, k.q, k.wn};
+  for (const void* p : all)
+    if ((uintptr_t)p % 16) return false;
+  for (int i = 0; i < n; ++i)
+    if ((uintptr_t)more[i] % 16) return false;
+  return true;
+}
+
+constexpr int LONG_V = 8192, LONG_1 = 1024;  // channels a row may have in the register kernels
+
+// Calls f<V, G, NV> with the split of a row of C channels.
+template <class F>
+int split_fwd(int C, bool vec, F&& f) {
+#define OW_SPLIT(V, G, NV) return f(std::integral_constant<int, V>(), std::integral_constant<int, G>(), std::integral_constant<int, NV>())
+  if (vec) {
+    if (C <= 64) OW_SPLIT(8, 8, 1);
+    if (C <= 128) OW_SPLIT(8, 16, 1);
+    if (C <= 256) OW_SPLIT(8, 32, 1);
+    if (C <= 512) OW_SPLIT(8, 32, 2);
+    if (C <= 1024) OW_SPLIT(8, 128, 1);
+    if (C <= 2048) OW_SPLIT(8, 256, 1);
+    if (C <= 4096) OW_SPLIT(8, 256, 2);
+    OW_SPLIT(8, 256, 4);
+  }
+  if (C <= 128) OW_SPLIT(1, 32, 4);
+  if (C <= 512) OW_SPLIT(1, 128, 4);
+  OW_SPLIT(1, 256, 4);
+}
+
+template <class F>
+int split_bwd(int C, bool vec, F&& f) {
+  if (vec) {
+    if (C <= 64) OW_SPLIT(8, 8, 1);
+    if (C <= 128) OW_SPLIT(8, 16, 1);
+    if (C <= 256) OW_SPLIT(8, 32, 1);
+    if (C <= 512) OW_SPLIT(8, 64, 1);
+    if (C <= 1024) OW_SPLIT(8, 128, 1);
+    if (C <= 2048) OW_SPLIT(8, 256, 1);
+    if (C <= 4096) OW_SPLIT(8, 512, 1);
+    OW_SPLIT(8, 1024, 1);
+  }
+  if (C <= 128) OW_SPLIT(1, 32, 4);
+  if (C <= 512) OW_SPLIT(1, 128, 4);
+  OW_SPLIT(1, 256, 4);
+#undef OW_SPLIT
+}
+
+bool too_long(int C, bool vec) { return C > (vec ? LONG_V : LONG_1); }
+
+template <class F>
+int modes(bool delta, bool next, F&& f) {
+  if (delta) return next ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
+  return f(std::false_type(), std::true_type());
+}
+
+// Blocks of the backward: a few waves of the device, no more than there are
+// rows, shared out over the groups.
+void parts(const ow_norm_t* a, Args* k) {
+  k->groups = a->gate_rows > 1 ? a->samples : 1;
+  k->group_rows = k->rows / std::max<int64_t>(k->groups, 1);
+  const int64_t want = (int64_t)device_sm_count() * 4;
+  const int64_t per = std::max<int64_t>(1, want / std::max<int64_t>(k->groups, 1));
+  k->per_group = (int)std::max<int64_t>(1, std::min<int64_t>(per, k->group_rows));
+  k->arrays = (a->next_w ? 1 : 0) + (a->delta ? 2 : 0);
+}
+
+}  // namespace
+}  // namespace ow
+
+using namespace ow;
+
+extern "C" {
+
+size_t ow_norm_bwd_workspace_size(const ow_norm_t* a) {
+  clear_error();
+  if (check(a) != OW_OK) return 0;
+  Args k = base(a);
+  parts(a, &k);
+  return (size_t)k.groups * k.per_group * k.arrays * k.C * sizeof(float) + 256;
+}
+
+int ow_norm_fwd(const ow_norm_t* a, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  Args k = base(a);
+  if (k.rows == 0) return OW_OK;
+  const bool delta = a->delta, next = a->next_w;
+  OW_CHECK_ARG((!delta || a->h) && (!next || a->n), "ow_norm_fwd: an output pointer is NULL");
+  k.h = a->h;
+  k.n = a->n;
+  const void* outs[] = {k.h, k.n};
+  const bool vec = vectors(k, outs, 2);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int sms = device_sm_count();
+  return modes(delta, next, [&](auto D, auto N) -> int {
+    if (too_long(k.C, vec)) {
+      launch(norm_long_fwd_kernel<D.value, N.value>, (int)std::min<int64_t>(k.rows, sms * 8), 256, 0, st, k);
+    } else {
+      OW_RETURN_IF(split_fwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
+        constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
+        const int grid = (int)std::min<int64_t>((k.rows + RB - 1) / RB, sms * 8);
+        launch(norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value>, grid, T, 0, st, k);
+        return OW_OK;
+      }));
+    }
+    OW_CHECK_LAUNCH("norm_fwd_kernel");
+    return OW_OK;
+  });
+}
+
+int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  const bool delta = a->delta, next = a->next_w;
+  OW_CHECK_ARG(g != nullptr, "ow_norm_bwd: grads is NULL");
+  Args k = base(a);
+  OW_CHECK_ARG(k.rows == 0 || (g->dx && (!next || g->dn) && (!delta || g->ddelta) && (g->dh || next) &&
+                               (!delta || k.rd) && (!next || k.rh)),
+               "ow_norm_bwd: a pointer is NULL");
+  parts(a, &k);
+  const size_t need = ow_norm_bwd_workspace_size(a);
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("ow_norm_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
+    return OW_ERR_WORKSPACE;
+  }
+  k.dh = g->dh; k.dn = g->dn; k.dx = g->dx; k.ddelta = g->ddelta;
+  k.part = (float*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255);
+  const void* more[] = {k.dh, k.dn, k.dx, k.ddelta};
+  const bool vec = vectors(k, more, 4);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int64_t grid = k.groups * k.per_group;
+  OW_CHECK_ARG(grid < (1LL << 31), "ow_norm_bwd: too many samples");
+  if (grid > 0) OW_RETURN_IF(modes(delta, next, [&](auto D, auto N) -> int {
+    if (too_long(k.C, vec)) {
+      launch(norm_long_bwd_kernel<D.value, N.value>, (int)grid, 256, 0, st, k);
+    } else {
+      OW_RETURN_IF(split_bwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
+        constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
+        const size_t smem = RB > 1 ? (size_t)RB * k.C * sizeof(float) : 0;
+        launch(norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value>, (int)grid, T, smem, st, k);
+        return OW_OK;
+      }));
+    }
+    OW_CHECK_LAUNCH("norm_bwd_kernel");
+    return OW_OK;
+  }));
+  SumArgs s{};
+  s.part = k.part; s.C = k.C; s.arrays = k.arrays; s.per_group = k.per_group; s.groups = k.groups;
+  int which = 0;
+  if (next) { s.out[which] = g->dnext; s.dt[which++] = a->next_dtype; }
+  s.q_at = -1;
+  if (delta) {
+    s.out[which] = g->dpost; s.dt[which++] = a->post_dtype;
+    s.out[which] = a->gate_rows ? g->dgate : nullptr; s.dt[which] = a->gate_dtype;
+    if (a->gate_rows > 1) s.q_at = which;
+    ++which;
+  }
+  const int64_t ys = s.arrays - (s.q_at >= 0 ? 1 : 0) + (s.q_at >= 0 ? s.groups : 0);
+  launch(norm_sum_kernel, dim3((k.C + 31) / 32, (unsigned)std::min<int64_t>(ys, 32768)), 256, 0, st, s);
+  OW_CHECK_LAUNCH("norm_sum_kernel");
+  return OW_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,93 @@
+"""Norms with gate and residual (host side, no GPU): argument checks of the functions and of the C entry points."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from omniwave_b200 import _lib, norm
+from omniwave_b200.block import OmniWeaveBlock
+
+
+def test_refuses_host_tensors():
+    x, w = torch.zeros(2, 3, 8), torch.ones(8)
+    assert norm.norm_supported(x, w) == (False, "CUDA is unavailable")
+    with pytest.raises(RuntimeError, match="CUDA is unavailable"):
+        norm.rms_norm(x, w)
+    with pytest.raises(RuntimeError, match="CUDA is unavailable"):
+        norm.norm_residual(x, x, w)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda x, w: norm.rms_norm(x, torch.ones(7)), r"weight must be \[8\]"),
+    (lambda x, w: norm.rms_norm(torch.zeros(3, 0), torch.ones(0)), r"x must be"),
+    (lambda x, w: norm.rms_norm(x, w, eps=-1.0), "eps"),
+    (lambda x, w: norm.norm_residual(x[0, 0], x[0, 0], w), r"x must be \[B"),
+    (lambda x, w: norm.norm_residual(x, x[:1], w), "delta must be"),
+    (lambda x, w: norm.norm_residual(x, x, w[:5]), "weight must be"),
+    (lambda x, w: norm.norm_residual(x, x, w, w[:1]), "gate must be"),
+    (lambda x, w: norm.norm_residual(x, x, w, torch.ones(3, 8)), "gate must be"),
+    (lambda x, w: norm.norm_residual(x, x, w, next_weight=torch.ones(2, 8)), "next_weight must be"),
+])
+def test_refuses_shapes(call, match):
+    with pytest.raises(ValueError, match=match):
+        call(torch.zeros(2, 3, 8), torch.ones(8))
+
+
+def _args(**over):
+    a = _lib.Norm(4, 49, 70, 16, 0, 16, 2, 16, 0, 16, 0, 1, None, 16, 0, 1e-6, 16, 16, 0, 16, 16, None, 0)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("over,status,msg", [
+    (dict(channels=0), 1, "bad shape"),
+    (dict(tokens=-1), 1, "bad shape"),
+    (dict(samples=1 << 31), 1, "too many rows"),
+    (dict(x=None), 1, "input pointer"),
+    (dict(post_w=None), 1, "input pointer"),
+    (dict(gate_rows=3), 1, "gate must have"),
+    (dict(gate=None), 1, "gate must have"),
+    (dict(delta=None, gate_rows=0, sample_scale=16), 1, "needs delta"),
+    (dict(delta=None, gate_rows=0, next_w=None), 1, "input pointer"),
+    (dict(x_dtype=1), 2, "float32, bfloat16 or float16"),
+    (dict(gate_dtype=7), 2, "float32, bfloat16 or float16"),
+    (dict(eps=-1.0), 1, "eps"),
+    (dict(h=None), 1, "output pointer"),
+    (dict(n=None), 1, "output pointer"),
+])
+def test_c_forward_refuses_before_any_cuda_call(over, status, msg):
+    lib = _lib.load()
+    assert lib.ow_norm_fwd(ctypes.byref(_args(**over)), None) == status
+    assert msg in lib.ow_last_error().decode()
+
+
+def test_c_backward_refuses_before_any_cuda_call():
+    lib = _lib.load()
+    g = _lib.NormGrads(16, 16, 16, 16, 16, 16, 16)
+    assert lib.ow_norm_bwd(ctypes.byref(_args()), ctypes.byref(g), None) == 4  # no workspace
+    assert "workspace" in lib.ow_last_error().decode()
+    for k in ("dx", "ddelta", "dn"):
+        g2 = _lib.NormGrads(16, 16, 16, 16, 16, 16, 16)
+        setattr(g2, k, None)
+        assert lib.ow_norm_bwd(ctypes.byref(_args()), ctypes.byref(g2), None) == 1, k
+    assert lib.ow_norm_bwd(ctypes.byref(_args(rstd_h=None)), ctypes.byref(g), None) == 1
+    assert lib.ow_norm_bwd(ctypes.byref(_args()), None, None) == 1
+    assert lib.ow_norm_bwd_workspace_size(ctypes.byref(_args(channels=0))) == 0
+    # three arrays of partial sums, at least one row of 70 channels each
+    assert lib.ow_norm_bwd_workspace_size(ctypes.byref(_args())) >= 3 * 70 * 4
+
+
+def test_post_norm_block_parameters():
+    torch.manual_seed(0)
+    plain = OmniWeaveBlock(4, 4, 64, 64, "local", 0)
+    torch.manual_seed(0)
+    post = OmniWeaveBlock(4, 4, 64, 64, "local", 0, post_norm=True)
+    assert set(post.state_dict()) - set(plain.state_dict()) == {"post_norm_weight"}
+    for k, v in plain.state_dict().items():
+        assert torch.equal(v, post.state_dict()[k])
+    with pytest.raises(RuntimeError, match="CUDA is unavailable"):
+        post(torch.zeros(1, 4, 4, 64))
