@@ -500,6 +500,60 @@ OW_API size_t ow_norm_bwd_workspace_size(const ow_norm_t* args);
 OW_API int ow_norm_fwd(const ow_norm_t* args, void* stream);
 OW_API int ow_norm_bwd(const ow_norm_t* args, const ow_norm_grads_t* grads, void* stream);
 
+/*
+ * Linear layer with its epilogue, for the 16-bit compute types:
+ *
+ *   z = x W^T + bias;   out = act(z) + residual
+ *
+ * x [rows, in_features] with row stride ldx, weight [out_features,
+ * in_features] with row stride ldw, residual [rows, out_features] with row
+ * stride ldr, all of ``dtype`` (bf16 or f16) with unit column stride; bias
+ * [out_features] f32, bf16 or f16, or NULL; out [rows, out_features]
+ * contiguous.  The sums and the activation are f32, out is rounded once.
+ * ``z`` (NULL, or [rows, ldz] with ldz = out_features rounded up to 8) gets z
+ * rounded to ``dtype`` for the backward of an activation.
+ *
+ * Backward: dz = dout act'(z); dx = dz W; dweight = dz^T x; dbias = column
+ * sums of dz (in bias_dtype).  The residual's gradient is dout itself.  dz is
+ * rounded to ``dtype`` when there is an activation.  NULL outputs are not
+ * computed.  All sums are taken in a fixed order.
+ */
+#define OW_ACT_NONE 0
+#define OW_ACT_RELU 1
+#define OW_ACT_SILU 2
+#define OW_ACT_GELU 3 /* z Phi(z), by erf */
+typedef struct ow_linear_t {
+  int64_t rows;
+  int32_t in_features, out_features;
+  int32_t dtype, activation;
+  const void* x;
+  int64_t ldx;
+  const void* weight;
+  int64_t ldw;
+  const void* bias;
+  int32_t bias_dtype;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  void* z;
+  void* workspace;             /* ow_linear_workspace_size() bytes */
+  size_t workspace_bytes;
+} ow_linear_t;
+
+typedef struct ow_linear_grads_t {
+  const void* dout;            /* [rows, out_features] contiguous */
+  void* dx;                    /* [rows, in_features] contiguous, or NULL */
+  void* dweight;               /* [out_features, in_features] contiguous, or NULL */
+  int32_t dweight_dtype;       /* dtype, or f32 */
+  void* dbias;                 /* or NULL */
+} ow_linear_grads_t;
+
+/* Workspace bytes of the forward (grads NULL) or of the backward; reads the
+ * shapes, dtypes, strides and pointers (their alignment).  0: invalid. */
+OW_API size_t ow_linear_workspace_size(const ow_linear_t* args, const ow_linear_grads_t* grads);
+OW_API int ow_linear_fwd(const ow_linear_t* args, void* stream);
+OW_API int ow_linear_bwd(const ow_linear_t* args, const ow_linear_grads_t* grads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,24 @@ class NormGrads(ctypes.Structure):
     _fields_ = [(k, _vp) for k in ("dh", "dn", "dx", "ddelta", "dpost", "dgate", "dnext")]
 
 
+class Linear(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("in_features", _c_i32), ("out_features", _c_i32),
+        ("dtype", _c_i32), ("activation", _c_i32),
+        ("x", _vp), ("ldx", ctypes.c_int64), ("weight", _vp), ("ldw", ctypes.c_int64),
+        ("bias", _vp), ("bias_dtype", _c_i32), ("residual", _vp), ("ldr", ctypes.c_int64),
+        ("out", _vp), ("z", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LinearGrads(ctypes.Structure):
+    _fields_ = [
+        ("dout", _vp), ("dx", _vp), ("dweight", _vp), ("dweight_dtype", _c_i32), ("dbias", _vp),
+    ]
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 ADAMW_BLOCK = 256
 ADAMW_CONTROL_BYTES = 64
 
@@ -150,6 +168,7 @@ EXPORTS = (
     "ow_d2s_linear_workspace_size", "ow_d2s_linear_fwd",
     "ow_grad_norm_partials", "ow_grad_norm", "ow_adamw_step",
     "ow_norm_bwd_workspace_size", "ow_norm_fwd", "ow_norm_bwd",
+    "ow_linear_workspace_size", "ow_linear_fwd", "ow_linear_bwd",
 )
 
 _lock = threading.Lock()
@@ -220,6 +239,12 @@ def load() -> ctypes.CDLL:
         lib.ow_norm_fwd.restype = ctypes.c_int
         lib.ow_norm_bwd.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(NormGrads), _vp]
         lib.ow_norm_bwd.restype = ctypes.c_int
+        lib.ow_linear_workspace_size.argtypes = [ctypes.POINTER(Linear), ctypes.POINTER(LinearGrads)]
+        lib.ow_linear_workspace_size.restype = ctypes.c_size_t
+        lib.ow_linear_fwd.argtypes = [ctypes.POINTER(Linear), _vp]
+        lib.ow_linear_fwd.restype = ctypes.c_int
+        lib.ow_linear_bwd.argtypes = [ctypes.POINTER(Linear), ctypes.POINTER(LinearGrads), _vp]
+        lib.ow_linear_bwd.restype = ctypes.c_int
         v = lib.ow_abi_version()
         if v != ABI_VERSION:
             raise NativeLibraryError(f"ABI version mismatch: library {v}, binding {ABI_VERSION}")

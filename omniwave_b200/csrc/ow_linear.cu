@@ -1,0 +1,977 @@
+// Linear layer with bias, activation and residual in its epilogue, forward
+// and backward, on the tensor cores (sm_100a):
+//
+//   z = x W^T + b;  y = act(z) + r;    dz = dy act'(z);  dx = dz W;  dW = dz^T x
+//
+// One GEMM kernel, D[m, n] = sum_k A[m, k] B[n, k], serves all three products.
+// An operand is read where it lies, by TMA boxes of 64 elements (128 bytes)
+// with the 128-byte swizzle: K-major when its rows run along k (x and W in
+// the forward, dz in dx), MN-major when they run across (W in dx, dz and x in
+// dW), so nothing is transposed in memory.
+//
+// Persistent, one CTA per SM, 320 threads: 8 epilogue warps, one thread that
+// issues the copies and one that issues the tcgen05.mma (M = 128, N = 64, 128
+// or 256).  A ring of 64-wide k blocks feeds the MMA; the accumulator is
+// double-buffered in TMEM, so a tile's epilogue runs under the next tile's
+// products.  Tiles are walked in patches of 12 row blocks, so that the SMs at
+// work share A and B blocks in L2.
+//
+// Where the tiles are few and k is long (dW: k is all tokens) the k blocks
+// are split over CTAs; each leaves an f32 partial, and a second kernel adds
+// them in a fixed order and does the epilogue.
+//
+// A few rows (serving) are a matter of reading W once: a CUDA-core kernel, a
+// warp (or several, for few features) a feature.
+#include <cuda.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "ow_common.cuh"
+#include "ow_internal.h"
+#include "ow_sm100.cuh"
+
+namespace ow {
+namespace {
+
+using namespace sm100;
+
+constexpr int TM = 128, KE = 64;
+constexpr int EPI_WARPS = 8, PROD_W = 8, MMA_W = 9, THREADS = 320;
+constexpr int A_ST = TM * 128;
+constexpr int STG_W = 4096;  // a warp's staging: 2 KB for the residual, 2 KB for what it stores
+constexpr int PATCH = 12;
+
+template <int BN>
+struct GC {
+  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int B_ST = BN * 128;
+  static constexpr int OFF_B = STAGES * A_ST;
+  static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
+  static constexpr int OFF_BAR = OFF_STG + EPI_WARPS * STG_W;
+  static constexpr int NBAR = 2 * STAGES + 4 + 1;  // full, empty, tfull[2], tfree[2], probe
+  static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+// What happens to a block of D on its way out.
+struct Epi {
+  const void* bias;
+  int bias_dt;
+  int act;
+  int bf16;          // 16-bit type of z, residual and out
+  void* z;
+  int64_t ldz;
+  const void* res;
+  int64_t ldr;
+  void* out;         // 16-bit, or f32 (partials, an f32 weight gradient)
+  int64_t ldo;
+  int out32;
+  int vz, vr, vo;    // rows take 16-byte accesses
+};
+
+struct GemmArgs {
+  int64_t M;
+  int N;
+  int kblocks;       // 64-wide blocks of k
+  int mtiles, ntiles;
+  int splits;        // of the k blocks; with more than one, out is the partials
+  int64_t part_stride;
+  Epi e;
+  int* fault;
+  uint32_t probe_ns;
+};
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Descriptor of an SW128 operand read MN-major: 64-element MN atoms ``lbo``
+// bytes apart, 8-line K groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// ---------------------------------------------------------------- activations
+__device__ __forceinline__ float act_fwd(float z, int act) {
+  if (act == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (act == OW_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
+  if (act == OW_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  return z;
+}
+
+// act'(z)
+__device__ __forceinline__ float act_slope(float z, int act) {
+  if (act == OW_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
+  if (act == OW_ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  if (act == OW_ACT_GELU)
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  return 1.f;
+}
+
+// z as it is kept for the backward: a finite value stays finite in f16 (an
+// infinite one would make silu' and gelu' NaN).
+__device__ __forceinline__ float keep_z(float z, int bf16) {
+  return bf16 ? z : z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z;
+}
+
+__device__ __forceinline__ float ld16(const void* p, int64_t i, int bf16) {
+  return bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : __half2float(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void st16(void* p, int64_t i, int bf16, float v) {
+  if (bf16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
+  else ((__half*)p)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ float ld_any(const void* p, int dt, int64_t i) {
+  return dt == OW_DTYPE_F32 ? ((const float*)p)[i] : ld16(p, i, dt == OW_DTYPE_BF16);
+}
+__device__ __forceinline__ uint32_t pk(float a, float b, int bf16) { return bf16 ? pack2<true>(a, b) : pack2<false>(a, b); }
+__device__ __forceinline__ float2 upk(uint32_t v, int bf16) { return bf16 ? unpack2<true>(v) : unpack2<false>(v); }
+
+// ---------------------------------------------------------------- epilogue
+// A warp's 32 rows x 32 columns, a row a lane, through 2 KB of staging
+// (16-byte units rotated by the row pair: conflict free both ways) to or from
+// 64-byte row segments.
+__device__ __forceinline__ uint32_t stg_at(int row, int u) { return row * 64 + ((u ^ ((row >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ void store_block16(unsigned char* stg, const float (&v)[32], int bf16, void* out, int64_t ld,
+                                              int64_t m0, int64_t M, int n0, int N, bool vec) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4*>(stg + stg_at(lane, u)) =
+        make_uint4(pk(v[8 * u], v[8 * u + 1], bf16), pk(v[8 * u + 2], v[8 * u + 3], bf16),
+                   pk(v[8 * u + 4], v[8 * u + 5], bf16), pk(v[8 * u + 6], v[8 * u + 7], bf16));
+  __syncwarp();
+  uint16_t* o = reinterpret_cast<uint16_t*>(out);
+  if (vec && n0 + 32 <= N) {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int row = it * 8 + (lane >> 2), u = lane & 3;
+      const uint4 w = *reinterpret_cast<const uint4*>(stg + stg_at(row, u));
+      if (m0 + row < M) *reinterpret_cast<uint4*>(o + (m0 + row) * ld + n0 + 8 * u) = w;
+    }
+  } else {
+    for (int row = 0; row < 32 && m0 + row < M; ++row)
+      if (n0 + lane < N)
+        o[(m0 + row) * ld + n0 + lane] =
+            *reinterpret_cast<const uint16_t*>(stg + stg_at(row, lane >> 3) + (lane & 7) * 2);
+  }
+}
+
+__device__ __forceinline__ void store_block32(unsigned char* stg, const float (&v)[32], float* out, int64_t ld, int64_t m0,
+                                              int64_t M, int n0, int N, bool vec) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<float4*>(stg + stg_at(lane, u)) =
+          make_float4(v[16 * h + 4 * u], v[16 * h + 4 * u + 1], v[16 * h + 4 * u + 2], v[16 * h + 4 * u + 3]);
+    __syncwarp();
+    const int nb = n0 + 16 * h;
+    if (vec && nb + 16 <= N) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int row = it * 8 + (lane >> 2), u = lane & 3;
+        const float4 w = *reinterpret_cast<const float4*>(stg + stg_at(row, u));
+        if (m0 + row < M) *reinterpret_cast<float4*>(out + (m0 + row) * ld + nb + 4 * u) = w;
+      }
+    } else {
+      for (int row = lane >> 4; row < 32 && m0 + row < M; row += 2) {
+        const int c = lane & 15;
+        if (nb + c < N) out[(m0 + row) * ld + nb + c] = *reinterpret_cast<const float*>(stg + stg_at(row, c >> 2) + (c & 3) * 4);
+      }
+    }
+  }
+}
+
+// The residual's 64-byte row segments of a block, as the coalesced loads of
+// the warp (kept in registers until the block is due).
+struct ResBlock {
+  uint4 w[4];
+};
+__device__ __forceinline__ void fetch_res(ResBlock& r, const Epi& e, int64_t m0, int64_t M, int n0, int N) {
+  const int lane = threadIdx.x & 31;
+  if (!e.res || !e.vr || n0 + 32 > N) return;
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(e.res);
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int row = it * 8 + (lane >> 2), u = lane & 3;
+    r.w[it] = m0 + row < M ? *reinterpret_cast<const uint4*>(p + (m0 + row) * e.ldr + n0 + 8 * u) : make_uint4(0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void add_res(float (&v)[32], const ResBlock& r, unsigned char* stg, const Epi& e, int64_t m0,
+                                        int64_t M, int n0, int N) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  if (e.vr && n0 + 32 <= N) {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) *reinterpret_cast<uint4*>(stg + stg_at(it * 8 + (lane >> 2), lane & 3)) = r.w[it];
+  } else {
+    for (int row = 0; row < 32; ++row)
+      *reinterpret_cast<uint16_t*>(stg + stg_at(row, lane >> 3) + (lane & 7) * 2) =
+          m0 + row < M && n0 + lane < N ? reinterpret_cast<const uint16_t*>(e.res)[(m0 + row) * e.ldr + n0 + lane] : 0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint4 w = *reinterpret_cast<const uint4*>(stg + stg_at(lane, u));
+    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = upk(q[k], e.bf16);
+      v[8 * u + 2 * k] += f.x;
+      v[8 * u + 2 * k + 1] += f.y;
+    }
+  }
+}
+
+__device__ __forceinline__ void add_bias(float (&v)[32], const Epi& e, int n0, int N) {
+  if (n0 + 32 <= N && e.bias_dt == OW_DTYPE_F32 && ((uintptr_t)e.bias & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>((const float*)e.bias + n0) + i);
+      v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
+    }
+  } else if (n0 + 32 <= N && e.bias_dt != OW_DTYPE_F32 && ((uintptr_t)e.bias & 15) == 0) {
+    const int bf = e.bias_dt == OW_DTYPE_BF16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)e.bias + n0) + i);
+      const uint32_t q[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = upk(q[k], bf);
+        v[8 * i + 2 * k] += f.x;
+        v[8 * i + 2 * k + 1] += f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (n0 + i < N) v[i] += ld_any(e.bias, e.bias_dt, n0 + i);
+  }
+}
+
+__device__ __forceinline__ void finish_block(float (&v)[32], const ResBlock& r, unsigned char* stg, const Epi& e, int64_t m0,
+                                             int64_t M, int n0, int N) {
+  if (e.bias) add_bias(v, e, n0, N);
+  if (e.z) {
+    float z[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i] = keep_z(v[i], e.bf16);
+    store_block16(stg + 2048, z, e.bf16, e.z, e.ldz, m0, M, n0, N, e.vz);
+  }
+  if (e.act == OW_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_RELU);
+  } else if (e.act == OW_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_SILU);
+  } else if (e.act == OW_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_GELU);
+  }
+  if (e.res) add_res(v, r, stg, e, m0, M, n0, N);
+  if (e.out32) store_block32(stg + 2048, v, (float*)e.out, e.ldo, m0, M, n0, N, e.vo);
+  else store_block16(stg + 2048, v, e.bf16, e.out, e.ldo, m0, M, n0, N, e.vo);
+}
+
+// ---------------------------------------------------------------- GEMM
+struct Unit {
+  int mt, nt, split, kb0, kb1;
+};
+
+// Unit u: the splits outermost (CTAs at work then read the same k range),
+// tiles in patches of PATCH row blocks.
+__device__ __forceinline__ Unit unit_of(const GemmArgs& a, int u) {
+  const int tiles = a.mtiles * a.ntiles;
+  Unit r;
+  r.split = u / tiles;
+  const int t = u - r.split * tiles;
+  const int per = PATCH * a.ntiles, p = t / per, q = t - p * per;
+  const int rows = min(PATCH, a.mtiles - p * PATCH);
+  r.nt = q / rows;
+  r.mt = p * PATCH + (q - r.nt * rows);
+  r.kb0 = (int)((int64_t)a.kblocks * r.split / a.splits);
+  r.kb1 = (int)((int64_t)a.kblocks * (r.split + 1) / a.splits);
+  return r;
+}
+
+template <int BN, bool AMN, bool BMN, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const GemmArgs a) {
+  using C = GC<BN>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tfree = tfull + 2;
+  uint64_t* probe = tfree + 2;
+  uint32_t* tmem = reinterpret_cast<uint32_t*>(full + C::NBAR);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = a.mtiles * a.ntiles * a.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tfull + i, 1);
+      mbar_init(tfree + i, EPI_WARPS);
+    }
+    mbar_init(probe, 1);
+    *abort = 0;
+    fence_mbar_init();
+    wait_probe(probe, abort, a.probe_ns);
+  }
+  if (warp == MMA_W) tmem_alloc(tmem, C::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem;
+
+  if (*abort) {
+    // the wait-timeout self-check ran out: nothing is issued
+  } else if (warp == PROD_W) {
+    if (lane == 0) {
+      int g = 0;
+      for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x) {
+        const Unit t = unit_of(a, u);
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
+          const int s = g % C::STAGES;
+          if (g >= C::STAGES && !mbar_wait(empty + s, ((g / C::STAGES) - 1) & 1, abort)) break;
+          mbar_arrive_expect_tx(full + s, A_ST + C::B_ST);
+          unsigned char* sa = sm + s * A_ST;
+          unsigned char* sb = sm + C::OFF_B + s * C::B_ST;
+          if constexpr (AMN) {
+#pragma unroll
+            for (int i = 0; i < TM / 64; ++i) tma_load_2d(sa + i * 8192, &amap, t.mt * TM + i * 64, kb * KE, full + s);
+          } else {
+            tma_load_2d(sa, &amap, kb * KE, t.mt * TM, full + s);
+          }
+          if constexpr (BMN) {
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i) tma_load_2d(sb + i * 8192, &bmap, t.nt * BN + i * 64, kb * KE, full + s);
+          } else {
+            tma_load_2d(sb, &bmap, kb * KE, t.nt * BN, full + s);
+          }
+        }
+      }
+    }
+  } else if (warp == MMA_W) {
+    if (lane == 0) {
+      constexpr uint32_t ID = idesc_f16(TM, BN, BF16) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
+      const uint32_t s0 = smem_u32(sm);
+      int g = 0, tl = 0;
+      for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x, ++tl) {
+        const Unit t = unit_of(a, u);
+        const int acc = tl & 1;
+        if (tl >= 2 && !mbar_wait(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
+        tc_fence_after();
+        const uint32_t tacc = tbase + acc * BN;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
+          const int s = g % C::STAGES;
+          if (!mbar_wait(full + s, (g / C::STAGES) & 1, abort)) break;
+          tc_fence_after();
+          const uint32_t aA = s0 + s * A_ST, aB = s0 + C::OFF_B + s * C::B_ST;
+#pragma unroll
+          for (int kk = 0; kk < KE / 16; ++kk) {
+            const uint64_t da = AMN ? sdesc_mn(aA + kk * 2048, 8192) : sdesc_sw128(aA + kk * 32);
+            const uint64_t db = BMN ? sdesc_mn(aB + kk * 2048, 8192) : sdesc_sw128(aB + kk * 32);
+            umma_f16(tacc, da, db, ID, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(empty + s);
+        }
+        umma_commit(tfull + acc);
+      }
+    }
+  } else {
+    unsigned char* stg = sm + C::OFF_STG + warp * STG_W;
+    const int q = warp & 3, half = warp >> 2;
+    constexpr int NCH = BN / 64;  // 32-column blocks of a warp
+    int tl = 0;
+    for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x, ++tl) {
+      const Unit t = unit_of(a, u);
+      const int acc = tl & 1;
+      const int64_t m0 = (int64_t)t.mt * TM + q * 32;
+      const int nb = t.nt * BN + half * (BN / 2);
+      Epi e = a.e;
+      if (a.splits > 1) e.out = (float*)a.e.out + (int64_t)t.split * a.part_stride;
+      ResBlock r;
+      fetch_res(r, e, m0, a.M, nb, a.N);
+      if (!mbar_wait(tfull + acc, (tl >> 1) & 1, abort)) break;
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll 1
+      for (int cb = 0; cb < NCH; ++cb) {
+        const int n0 = nb + cb * 32;
+        if (n0 >= a.N) break;
+        uint32_t w[32];
+        tmem_ld32(tbase + acc * BN + half * (BN / 2) + cb * 32 + ((uint32_t)(q * 32) << 16), w);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
+        if (m0 < a.M) {
+          finish_block(v, r, stg, e, m0, a.M, n0, a.N);
+          if (cb + 1 < NCH) fetch_res(r, e, m0, a.M, n0 + 32, a.N);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tfree + acc);
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  report_abort(abort, a.fault);
+  if (*abort) {
+    // A wait gave up: give in-flight copies and MMAs time to land before the
+    // shared memory and TMEM they target are released.
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  }
+  if (warp == MMA_W) {
+    tc_fence_after();
+    tmem_dealloc(tbase, C::TMEM_COLS);
+  }
+}
+
+// Adds the split-k partials of [M, N] (row stride ld) in order and finishes.
+__global__ void __launch_bounds__(256) gemm_sum_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t ld,
+                                                       int64_t M, int N, const Epi e) {
+  const int64_t nv = (N + 3) / 4, total = M * nv;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t m = i / nv;
+    const int n = (int)(i - m * nv) * 4;
+    float4 s = *reinterpret_cast<const float4*>(part + m * ld + n);  // ld is a multiple of 4
+    for (int p = 1; p < splits; ++p) {
+      const float4 t = *reinterpret_cast<const float4*>(part + p * stride + m * ld + n);
+      s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+    }
+    float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (n + k >= N) break;
+      float z = v[k];
+      if (e.bias) z += ld_any(e.bias, e.bias_dt, n + k);
+      if (e.z) st16(e.z, m * e.ldz + n + k, e.bf16, keep_z(z, e.bf16));
+      z = act_fwd(z, e.act);
+      if (e.res) z += ld16(e.res, m * e.ldr + n + k, e.bf16);
+      if (e.out32) ((float*)e.out)[m * e.ldo + n + k] = z;
+      else st16(e.out, m * e.ldo + n + k, e.bf16, z);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- a few rows
+struct RowsArgs {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  int M, N, K;
+  int vec;
+  Epi e;
+};
+
+// P warps share a feature (its k range dealt out in 256-element turns); a
+// block of 8 warps does 8 / P features.  MR rows are taken at a time.
+template <int MR, int P>
+__global__ void __launch_bounds__(256) linear_rows_kernel(const RowsArgs a) {
+  __shared__ float sh[8][MR];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % P;
+  const int n = blockIdx.x * (8 / P) + warp / P;
+  const int bf = a.e.bf16;
+  for (int m0 = 0; m0 < a.M; m0 += MR) {
+    float s[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) s[r] = 0.f;
+    if (n < a.N) {
+      const uint16_t* w = reinterpret_cast<const uint16_t*>(a.w) + n * a.ldw;
+      const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
+      if (a.vec) {
+#pragma unroll 4
+        for (int k = part * 256 + lane * 8; k < a.K; k += P * 256) {
+          const uint4 wv = __ldg(reinterpret_cast<const uint4*>(w + k));
+          const uint32_t wq[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+          for (int r = 0; r < MR; ++r) {
+            if (m0 + r >= a.M) break;
+            const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + (m0 + r) * a.ldx + k));
+            const uint32_t xq[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 p = upk(wq[i], bf), q = upk(xq[i], bf);
+              s[r] = fmaf(p.x, q.x, s[r]);
+              s[r] = fmaf(p.y, q.y, s[r]);
+            }
+          }
+        }
+      } else {
+        for (int k = part * 32 + lane; k < a.K; k += P * 32) {
+          const float wk = ld16(w, k, bf);
+#pragma unroll
+          for (int r = 0; r < MR; ++r)
+            if (m0 + r < a.M) s[r] = fmaf(wk, ld16(x, (m0 + r) * a.ldx + k, bf), s[r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+    float mine = 0.f;  // row ``lane``'s sum
+    if constexpr (P == 1) {
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+        if (lane == r) mine = s[r];
+    } else {
+      if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < MR; ++r) sh[warp][r] = s[r];
+      __syncthreads();
+      if (lane < MR)
+#pragma unroll
+        for (int i = 0; i < P; ++i) mine += sh[warp - part + i][lane];
+      __syncthreads();
+    }
+    if (part == 0 && lane < MR && m0 + lane < a.M && n < a.N) {
+      const int64_t m = m0 + lane;
+      if (a.e.bias) mine += ld_any(a.e.bias, a.e.bias_dt, n);
+      if (a.e.z) st16(a.e.z, m * a.e.ldz + n, bf, keep_z(mine, bf));
+      mine = act_fwd(mine, a.e.act);
+      if (a.e.res) mine += ld16(a.e.res, m * a.e.ldr + n, bf);
+      st16(a.e.out, m * a.e.ldo + n, bf, mine);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- backward of the epilogue
+struct DzArgs {
+  const void* dy;    // [M, N] contiguous
+  const void* z;     // [M, ldz] or NULL
+  void* dz;          // [M, ldz] or NULL (only the sums are wanted)
+  float* part;       // [chunks][N] column sums, or NULL
+  int64_t M, ldz, chunk;
+  int N, act, bf16, vec;
+};
+
+// dz = dy act'(z), rounded to the 16-bit type (the GEMMs take it so), and its
+// f32 column sums for the bias.  A block does 256 columns of a chunk of rows.
+__global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
+  __shared__ float sh[8][264];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = blockIdx.x * 256 + tx * 8;
+  const int64_t m1 = min(a.M, (blockIdx.y + 1) * a.chunk);
+  float s[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[k] = 0.f;
+  for (int64_t m = blockIdx.y * a.chunk + ty; m < m1; m += 8) {
+    if (n >= a.N) continue;
+    float g[8], z[8];
+    if (a.vec && n + 8 <= a.N) {
+      const uint4 gv = *reinterpret_cast<const uint4*>((const uint16_t*)a.dy + m * a.N + n);
+      uint4 zv = make_uint4(0, 0, 0, 0);
+      if (a.z) zv = *reinterpret_cast<const uint4*>((const uint16_t*)a.z + m * a.ldz + n);
+      const uint32_t gq[4] = {gv.x, gv.y, gv.z, gv.w}, zq[4] = {zv.x, zv.y, zv.z, zv.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = upk(gq[k], a.bf16), h = upk(zq[k], a.bf16);
+        g[2 * k] = f.x; g[2 * k + 1] = f.y;
+        z[2 * k] = h.x; z[2 * k + 1] = h.y;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        g[k] = n + k < a.N ? ld16(a.dy, m * a.N + n + k, a.bf16) : 0.f;
+        z[k] = a.z && n + k < a.N ? ld16(a.z, m * a.ldz + n + k, a.bf16) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      g[k] *= act_slope(z[k], a.act);
+      s[k] += g[k];
+    }
+    if (a.dz)  // rows of dz start on 16 bytes and have room for whole vectors
+      *reinterpret_cast<uint4*>((uint16_t*)a.dz + m * a.ldz + n) =
+          make_uint4(pk(g[0], g[1], a.bf16), pk(g[2], g[3], a.bf16), pk(g[4], g[5], a.bf16), pk(g[6], g[7], a.bf16));
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sh[ty][tx * 8 + k] = s[k];
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (blockIdx.x * 256 + c < a.N) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += sh[i][c];
+    a.part[(int64_t)blockIdx.y * a.N + blockIdx.x * 256 + c] = t;
+  }
+}
+
+__global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ part, int chunks, int N, void* out, int dt) {
+  __shared__ float sh[8][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
+  float t = 0.f;
+  if (c < N)
+    for (int p = ry; p < chunks; p += 8) t += part[(int64_t)p * N + c];
+  sh[ry][cx] = t;
+  __syncthreads();
+  if (ry == 0 && c < N) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sh[i][cx];
+    if (dt == OW_DTYPE_F32) ((float*)out)[c] = v;
+    else st16(out, c, dt == OW_DTYPE_BF16, v);
+  }
+}
+
+// Rows of ``cols`` 16-bit elements copied to rows of ``ldd`` (a multiple of 8),
+// for an operand whose rows TMA cannot read in place.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t lds, uint16_t* __restrict__ dst,
+                                                       int64_t ldd, int64_t rows, int cols) {
+  const int64_t total = rows * cols;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t r = i / cols;
+    const int c = (int)(i - r * cols);
+    dst[r * ldd + c] = src[r * lds + c];
+  }
+}
+
+// ---------------------------------------------------------------- host
+int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+
+bool tma_rows(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+
+// An operand as the GEMM reads it: rows x cols 16-bit elements, row stride ld.
+struct Mat {
+  const void* p;
+  int64_t rows;
+  int cols;
+  int64_t ld;
+};
+
+// Shape of one GEMM: the tile's width and the k splits that a simple model
+// finds fastest.  A 64-wide k block of a 128 x BN tile takes BN / 32 units of
+// time but no less than what its copies take (A's 128 rows count as well); a
+// tile's epilogue 10 + BN / 8 units; a split costs writing and reading its
+// f32 partial.
+struct Plan {
+  int bn, splits;
+};
+Plan plan_gemm(int64_t M, int N, int kblocks) {
+  const int sms = device_sm_count();
+  Plan best{128, 1};
+  double least = 1e300;
+  const int64_t mt = (M + TM - 1) / TM;
+  for (int bn : {64, 128, 256}) {
+    const int64_t tiles = mt * ((N + bn - 1) / bn);
+    // more splits than fill the SMs twice gain nothing
+    const int smax = (int)std::min<int64_t>(std::min(kblocks, 64), 1 + 2 * sms / tiles);
+    for (int s = 1; s <= smax; ++s) {
+      const int64_t waves = (tiles * s + sms - 1) / sms;
+      const int kb = (kblocks + s - 1) / s;
+      const double block = std::max(bn / 32.0, (128 + bn) / 64.0);
+      double t = (double)waves * (kb * block + 10.0 + bn / 8.0);
+      // f32 partials written and read: 8 bytes each at about 3.4 KB a unit (0.5 us), and a launch
+      if (s > 1) t += 40.0 + (double)s * M * N * 8.0 / 400e3;
+      if (t < least) {
+        least = t;
+        best = Plan{bn, s};
+      }
+    }
+  }
+  return best;
+}
+
+// Workspace of one GEMM: padded copies of operands TMA cannot read, partials.
+struct GemmWs {
+  void* a;
+  void* b;
+  float* part;
+  int64_t part_ld;
+};
+
+GemmWs gemm_take(const Mat& A, const Mat& B, int64_t M, int N, const Plan& p, Carver& ws) {
+  GemmWs w{};
+  if (!tma_rows(A.p, A.ld)) w.a = ws.take((size_t)A.rows * up8(A.cols) * 2);
+  if (!tma_rows(B.p, B.ld)) w.b = ws.take((size_t)B.rows * up8(B.cols) * 2);
+  w.part_ld = (N + 3) / 4 * 4;
+  if (p.splits > 1) w.part = (float*)ws.take((size_t)p.splits * M * w.part_ld * 4);
+  return w;
+}
+
+int pad_rows(Mat& m, void* to, cudaStream_t st) {
+  const int64_t ld = up8(m.cols), total = m.rows * m.cols;
+  const int grid = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);
+  launch(pad_rows_kernel, grid, 256, 0, st, (const uint16_t*)m.p, m.ld, (uint16_t*)to, ld, m.rows, m.cols);
+  OW_CHECK_LAUNCH("pad_rows_kernel");
+  m.p = to;
+  m.ld = ld;
+  return OW_OK;
+}
+
+int map_of(CUtensorMap* map, const Mat& m, bool bf16, uint32_t box_rows) {
+  const uint64_t dims[2] = {(uint64_t)m.cols, (uint64_t)m.rows};
+  const uint64_t strides[1] = {(uint64_t)m.ld * 2};
+  const uint32_t box[2] = {(uint32_t)KE, box_rows};
+  return encode_tiled_map(map, bf16, 2, m.p, dims, strides, box, "ow_linear");
+}
+
+template <int BN, bool AMN, bool BMN, bool BF16>
+int run_gemm(const CUtensorMap& am, const CUtensorMap& bm, const GemmArgs& k, int grid, cudaStream_t st) {
+  auto kern = gemm_kernel<BN, AMN, BMN, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC<BN>::SMEM);
+  if (e != cudaSuccess) {
+    set_error("ow_linear: cannot reserve %d bytes of shared memory: %s", GC<BN>::SMEM, cudaGetErrorString(e));
+    return OW_ERR_CUDA;
+  }
+  launch(kern, grid, THREADS, GC<BN>::SMEM, st, am, bm, k);
+  OW_CHECK_LAUNCH("gemm_kernel");
+  return OW_OK;
+}
+
+// D[M, N] = sum_k A B with the epilogue ``e``.  AMN/BMN: the operand's rows
+// run along M or N and its row index is k.
+template <bool AMN, bool BMN>
+int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs& w, const Epi& e, bool bf16, cudaStream_t st) {
+  if (w.a) OW_RETURN_IF(pad_rows(A, w.a, st));
+  if (w.b) OW_RETURN_IF(pad_rows(B, w.b, st));
+  CUtensorMap am, bm;
+  OW_RETURN_IF(map_of(&am, A, bf16, AMN ? KE : TM));
+  OW_RETURN_IF(map_of(&bm, B, bf16, BMN ? KE : p.bn));
+  GemmArgs k{};
+  k.M = M;
+  k.N = N;
+  k.kblocks = (int)((K + KE - 1) / KE);
+  k.mtiles = (int)((M + TM - 1) / TM);
+  k.ntiles = (N + p.bn - 1) / p.bn;
+  k.splits = p.splits;
+  k.e = e;
+  if (p.splits > 1) {
+    k.e = Epi{};
+    k.e.bf16 = e.bf16;
+    k.e.out = w.part;
+    k.e.ldo = w.part_ld;
+    k.e.out32 = 1;
+    k.e.vo = 1;
+    k.part_stride = M * w.part_ld;
+  }
+  OW_RETURN_IF(fault_word(&k.fault));
+  k.probe_ns = wait_probe_ns();
+  const int64_t units = (int64_t)k.mtiles * k.ntiles * k.splits;
+  OW_CHECK_ARG(units < (1LL << 31) - 1024, "ow_linear: too many tiles");
+  const int grid = (int)std::min<int64_t>(units, device_sm_count());
+  auto go = [&](auto bn) -> int {
+    constexpr int BN = decltype(bn)::value;
+    return bf16 ? run_gemm<BN, AMN, BMN, true>(am, bm, k, grid, st) : run_gemm<BN, AMN, BMN, false>(am, bm, k, grid, st);
+  };
+  if (p.bn == 64) OW_RETURN_IF(go(std::integral_constant<int, 64>()));
+  else if (p.bn == 128) OW_RETURN_IF(go(std::integral_constant<int, 128>()));
+  else OW_RETURN_IF(go(std::integral_constant<int, 256>()));
+  if (p.splits > 1) {
+    const int64_t total = M * ((N + 3) / 4);
+    const int g2 = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);
+    launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, k.part_stride, w.part_ld, M, N, e);
+    OW_CHECK_LAUNCH("gemm_sum_kernel");
+  }
+  return OW_OK;
+}
+
+bool is16(int dt) { return dt == OW_DTYPE_BF16 || dt == OW_DTYPE_F16; }
+
+int check(const ow_linear_t* a) {
+  OW_CHECK_ARG(a != nullptr, "ow_linear: args is NULL");
+  OW_CHECK_ARG(a->rows >= 0 && a->in_features > 0 && a->out_features > 0, "ow_linear: bad shape [%lld, %d] x [%d]",
+               (long long)a->rows, a->in_features, a->out_features);
+  OW_CHECK_ARG(a->rows < (1LL << 31) - 256 && a->in_features < (1 << 30) && a->out_features < (1 << 30), "ow_linear: too large");
+  if (!is16(a->dtype)) {
+    set_error("ow_linear: dtype must be bfloat16 or float16 (code %d)", a->dtype);
+    return OW_ERR_UNSUPPORTED;
+  }
+  OW_CHECK_ARG(a->activation >= OW_ACT_NONE && a->activation <= OW_ACT_GELU, "ow_linear: unknown activation %d", a->activation);
+  OW_CHECK_ARG(a->ldx >= a->in_features && a->ldw >= a->in_features && (!a->residual || a->ldr >= a->out_features),
+               "ow_linear: a row stride is shorter than its row");
+  OW_CHECK_ARG(!a->bias || is16(a->bias_dtype) || a->bias_dtype == OW_DTYPE_F32, "ow_linear: bias must be float32, bfloat16 or float16");
+  return OW_OK;
+}
+
+// Up to this many rows the kernel that reads W once from CUDA cores is used.
+constexpr int FEW_ROWS = 8;
+
+Mat mat_x(const ow_linear_t* a) { return Mat{a->x, a->rows, a->in_features, a->ldx}; }
+Mat mat_w(const ow_linear_t* a) { return Mat{a->weight, a->out_features, a->in_features, a->ldw}; }
+int blocks_of(int64_t k) { return (int)((k + KE - 1) / KE); }
+
+// Everything a backward call needs, carved from its workspace.
+struct BwdWs {
+  void* dz;        // [rows, up8(N)], or NULL: dout serves as it is
+  float* bias;     // [chunks][N]
+  int chunks;
+  int64_t chunk;
+  Plan px, pw;
+  GemmWs x, w;
+};
+
+BwdWs bwd_take(const ow_linear_t* a, const ow_linear_grads_t* g, Carver& ws) {
+  BwdWs b{};
+  const int N = a->out_features, K = a->in_features;
+  const int64_t M = a->rows;
+  if ((g->dx || g->dweight) && (a->activation != OW_ACT_NONE || !tma_rows(g->dout, N)))
+    b.dz = ws.take((size_t)M * up8(N) * 2);
+  // chunks of rows: a few blocks an SM, at least 8 rows each
+  const int64_t col_blocks = (N + 255) / 256;
+  b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
+  b.chunk = (M + b.chunks - 1) / b.chunks;
+  b.chunks = (int)((M + b.chunk - 1) / b.chunk);
+  if (g->dbias) b.bias = (float*)ws.take((size_t)b.chunks * N * 4);
+  const Mat dz = b.dz ? Mat{nullptr, M, N, up8(N)} : Mat{g->dout, M, N, N};
+  if (g->dx) {
+    b.px = plan_gemm(M, K, blocks_of(N));
+    b.x = gemm_take(dz, mat_w(a), M, K, b.px, ws);
+  }
+  if (g->dweight) {
+    b.pw = plan_gemm(N, K, blocks_of(M));
+    b.w = gemm_take(dz, mat_x(a), N, K, b.pw, ws);
+  }
+  return b;
+}
+
+}  // namespace
+}  // namespace ow
+
+using namespace ow;
+
+extern "C" {
+
+size_t ow_linear_workspace_size(const ow_linear_t* a, const ow_linear_grads_t* g) {
+  clear_error();
+  if (check(a) != OW_OK) return 0;
+  Carver c(nullptr);
+  if (a->rows > 0) {
+    if (g) {
+      bwd_take(a, g, c);
+    } else if (a->rows > FEW_ROWS) {
+      gemm_take(mat_x(a), mat_w(a), a->rows, a->out_features, plan_gemm(a->rows, a->out_features, blocks_of(a->in_features)), c);
+    }
+  }
+  return c.used + 256;
+}
+
+int ow_linear_fwd(const ow_linear_t* a, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  if (a->rows == 0) return OW_OK;
+  OW_CHECK_ARG(a->x && a->weight && a->out, "ow_linear_fwd: a pointer is NULL");
+  OW_CHECK_ARG(((uintptr_t)a->x | (uintptr_t)a->weight | (uintptr_t)a->out | (uintptr_t)a->residual) % 2 == 0 &&
+                   (uintptr_t)a->z % 16 == 0,
+               "ow_linear_fwd: a tensor is not aligned");
+  const size_t need = ow_linear_workspace_size(a, nullptr);
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("ow_linear_fwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
+    return OW_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool bf = a->dtype == OW_DTYPE_BF16;
+  const int N = a->out_features, K = a->in_features;
+  Epi e{};
+  e.bias = a->bias; e.bias_dt = a->bias_dtype; e.act = a->activation; e.bf16 = bf;
+  e.z = a->z; e.ldz = up8(N); e.vz = 1;
+  e.res = a->residual; e.ldr = a->ldr; e.vr = tma_rows(a->residual, a->ldr);
+  e.out = a->out; e.ldo = N; e.vo = tma_rows(a->out, N);
+  if (a->rows <= FEW_ROWS) {
+    RowsArgs k{a->x, a->ldx, a->weight, a->ldw, (int)a->rows, N, K,
+               K % 8 == 0 && tma_rows(a->x, a->ldx) && tma_rows(a->weight, a->ldw), e};
+    // warps for a feature: enough that few features still fill the SMs
+    const int want = device_sm_count() * 16;
+    auto go = [&](auto p) -> int {
+      constexpr int P = decltype(p)::value, F = 8 / P;
+      const int grid = (N + F - 1) / F;
+      if (a->rows == 1) launch(linear_rows_kernel<1, P>, grid, 256, 0, st, k);
+      else if (a->rows == 2) launch(linear_rows_kernel<2, P>, grid, 256, 0, st, k);
+      else if (a->rows <= 4) launch(linear_rows_kernel<4, P>, grid, 256, 0, st, k);
+      else launch(linear_rows_kernel<8, P>, grid, 256, 0, st, k);
+      OW_CHECK_LAUNCH("linear_rows_kernel");
+      return OW_OK;
+    };
+    const int turns = (K + 255) / 256;
+    if (turns >= 8 && N * 8 <= want) return go(std::integral_constant<int, 8>());
+    if (turns >= 4 && N * 4 <= want) return go(std::integral_constant<int, 4>());
+    if (turns >= 2 && N * 2 <= want) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, 1>());
+  }
+  Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
+  const Plan p = plan_gemm(a->rows, N, blocks_of(K));
+  const GemmWs w = gemm_take(mat_x(a), mat_w(a), a->rows, N, p, ws);
+  return gemm<false, false>(mat_x(a), mat_w(a), a->rows, N, K, p, w, e, bf, st);
+}
+
+int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  OW_CHECK_ARG(g != nullptr, "ow_linear_bwd: grads is NULL");
+  OW_CHECK_ARG(!g->dbias || is16(a->bias_dtype) || a->bias_dtype == OW_DTYPE_F32, "ow_linear_bwd: bias_dtype is not set");
+  if (g->dweight && g->dweight_dtype != a->dtype && g->dweight_dtype != OW_DTYPE_F32) {
+    set_error("ow_linear_bwd: dweight must be of dtype or float32 (code %d)", g->dweight_dtype);
+    return OW_ERR_UNSUPPORTED;
+  }
+  OW_CHECK_ARG(a->rows > 0, "ow_linear_bwd: no rows");
+  OW_CHECK_ARG(g->dout && (!g->dx || a->weight) && (!g->dweight || a->x) && (a->activation == OW_ACT_NONE || a->z),
+               "ow_linear_bwd: a pointer is NULL");
+  const size_t need = ow_linear_workspace_size(a, g);
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("ow_linear_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
+    return OW_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool bf = a->dtype == OW_DTYPE_BF16;
+  const int N = a->out_features, K = a->in_features;
+  const int64_t M = a->rows;
+  Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
+  const BwdWs b = bwd_take(a, g, ws);
+  if (b.dz || g->dbias) {
+    DzArgs k{g->dout, a->activation == OW_ACT_NONE ? nullptr : a->z, b.dz, b.bias, M, up8(N), b.chunk, N, a->activation, bf,
+             tma_rows(g->dout, N)};
+    launch(dz_kernel, dim3((N + 255) / 256, b.chunks), 256, 0, st, k);
+    OW_CHECK_LAUNCH("dz_kernel");
+    if (g->dbias) {
+      launch(dbias_kernel, (N + 31) / 32, 256, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype);
+      OW_CHECK_LAUNCH("dbias_kernel");
+    }
+  }
+  const Mat dz = b.dz ? Mat{b.dz, M, N, up8(N)} : Mat{g->dout, M, N, N};
+  if (g->dx) {
+    Epi e{};
+    e.bf16 = bf;
+    e.out = g->dx; e.ldo = K; e.vo = tma_rows(g->dx, K);
+    OW_RETURN_IF((gemm<false, true>(dz, mat_w(a), M, K, N, b.px, b.x, e, bf, st)));
+  }
+  if (g->dweight) {
+    Epi e{};
+    e.bf16 = bf;
+    e.out = g->dweight; e.ldo = K;
+    e.out32 = g->dweight_dtype == OW_DTYPE_F32;
+    e.vo = (uintptr_t)g->dweight % 16 == 0 && K % (e.out32 ? 4 : 8) == 0;
+    OW_RETURN_IF((gemm<true, true>(dz, mat_x(a), N, K, M, b.pw, b.w, e, bf, st)));
+  }
+  return OW_OK;
+}
+
+}  // extern "C"

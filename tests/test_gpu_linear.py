@@ -1,0 +1,345 @@
+"""Linear with its epilogue on the GPU against float64.
+
+Operands are 16-bit values; products of two are exact in f32.  The tensor
+core and the CUDA cores add K of them, in any order, to within (K + 8) u of the
+sum of their magnitudes (u = 2^-24; an f32 sum of n terms is off by at most
+n - 1 roundings of its partial sums).  Bias and residual add one rounding each.
+The activations are within 8 u (|z| + 1) of theirs (fast exponential and
+division, a few steps each) and pass z's own error on with a slope of at most
+1.13.  An output is rounded by half(t) of itself.
+The backward holds z in 16 bits, off by half(t) |z| plus z's error; the slopes
+change by at most 1.13 |dz| (silu'' <= 0.5, gelu'' <= 0.8; relu' jumps at 0, so
+relu is tested on values whose sums are exact).  dz is rounded to 16 bits, half(t) of itself, when there is an
+activation, and then summed.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from omniwave_b200 import _lib, linear
+from omniwave_b200.optim import AdamW
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, BF, HF = torch.float32, torch.bfloat16, torch.float16
+
+
+def _half(t):
+    return U if t == F32 else torch.finfo(t).eps / 2
+
+
+def _act(z, act):
+    if act == "none":
+        return z, torch.ones_like(z)
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    cdf = 0.5 * (1 + torch.erf(z / 2 ** 0.5))
+    return z * cdf, cdf + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+
+
+def _define(x, w, b, r, dy, act, t):
+    """Outputs, gradients and the bounds of their errors, in float64."""
+    x, w, dy = x.double(), w.double(), dy.double()
+    m, k = x.shape
+    n = w.shape[0]
+    h = _half(t)
+    z = x @ w.t()
+    zm = x.abs() @ w.abs().t()
+    if b is not None:
+        z, zm = z + b.double(), zm + b.double().abs()
+    ez = (k + 10) * U * zm if act != "relu" else torch.zeros_like(zm)  # relu's inputs add up exactly
+    y, slope = _act(z, act)
+    ey = 1.13 * ez + (8 * U * (z.abs() + 1) if act != "none" else 0.0)
+    if r is not None:
+        y = y + r.double()
+        ey = ey + 2 * U * (y.abs() + r.double().abs())
+    tiny = 2.0 ** -25 if t == HF else 0.0
+    out, tol = {"y": y}, {"y": ey + h * 1.01 * (y.abs() + ey) + tiny}
+    if act == "none":
+        dz, edz = dy, torch.zeros_like(dy)
+    else:
+        eslope = 1.13 * (ez + h * 1.01 * z.abs() + tiny) + 8 * U * (z.abs() + 1)
+        if act == "relu":
+            assert ((z.abs() > ez + tiny) | (z == 0)).all()
+            eslope = torch.zeros_like(z)
+        dz = dy * slope
+        edz = dy.abs() * eslope
+    # as it is summed for the bias, and as the products take it
+    edb = edz + (U * dz.abs())
+    ez16 = edz + (h * 1.01 * (dz.abs() + edz) + tiny if act != "none" else 0.0)
+    for name, a, ea, c, terms in (("dx", dz, ez16, w, n), ("dw", dz.t(), ez16.t(), x, m)):
+        out[name] = a @ c
+        e = ea @ c.abs() + (terms + 8) * U * ((a.abs() + ea) @ c.abs())
+        tol[name] = (e, out[name])
+    out["db"] = dz.sum(0)
+    tol["db"] = (edb.sum(0) + (m + 8) * U * (dz.abs() + edb).sum(0), out["db"])
+    return out, tol
+
+
+def _ok(got, want, tol, where):
+    if isinstance(tol, tuple):
+        e, v = tol
+        tol = e + _half(got.dtype) * 1.01 * (v.abs() + e) + (2.0 ** -25 if got.dtype == HF else 0.0)
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), f"{where}: worst {(err / tol.clamp(min=1e-300)).max().item():.2f} of the bound"
+
+
+def _inputs(dev, m, k, n, t, seed=0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=g, device=dev)
+
+    return (r(m, k).to(t), (r(n, k) * k ** -0.5).to(t), (r(n) * 0.3).to(t), r(m, n).to(t), r(m, n).to(t))
+
+
+def _both(x, w, b, r, dy, act, where):
+    want, tol = _define(x, w, b, r, dy, act, x.dtype)
+    with torch.no_grad():
+        plain = linear.linear(x, w, b, activation=act, residual=r)
+    assert plain.dtype == x.dtype and plain.shape == want["y"].shape
+    _ok(plain, want["y"], tol["y"], f"{where} y")
+    leaves = [None if t is None else t.detach().requires_grad_() for t in (x, w, b, r)]
+    y = linear.linear(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3])
+    assert torch.equal(y, plain)
+    grads = torch.autograd.grad(y, [t for t in leaves if t is not None], dy)
+    for name, g, leaf in zip(["dx", "dw"] + ["db"] * (b is not None) + ["dr"] * (r is not None), grads,
+                             [t for t in leaves if t is not None]):
+        assert g.dtype == leaf.dtype and g.shape == leaf.shape
+        if name == "dr":
+            assert torch.equal(g, dy)
+        else:
+            _ok(g, want[name], tol[name], f"{where} {name}")
+    return grads
+
+
+SHAPES = [(1, 8, 1), (1, 1024, 2048), (2, 64, 7), (3, 70, 33), (5, 2048, 16), (8, 300, 129), (9, 64, 64), (17, 8, 8),
+          (100, 63, 45), (128, 64, 64), (129, 65, 257), (200, 1000, 24), (256, 512, 1024), (300, 129, 130),
+          (1000, 48, 128), (333, 2048, 300), (2500, 72, 40)]
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES, ids=["x".join(map(str, s)) for s in SHAPES])
+@pytest.mark.parametrize("t", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("act,bias,res", [("none", False, False), ("gelu", True, True), ("silu", True, False),
+                                          ("none", True, True), ("relu", False, True)])
+def test_forward_and_gradients(cuda_device, m, k, n, t, act, bias, res):
+    x, w, b, r, dy = _inputs(cuda_device, m, k, n, t)
+    if act == "relu":  # eighths: products are 64ths, and sums of up to 2^18 are exact in f32, so z's sign is
+        x, w = (x.float() * 8).round().clamp(-8, 8).div(8).to(t), (w.float() * 64).round().clamp(-8, 8).div(8).to(t)
+    _both(x, w, b if bias else None, r if res else None, dy, act, f"{m}x{k}x{n}")
+
+
+@pytest.mark.parametrize("m,k,n,act", [(25088, 512, 1024, "gelu"), (12544, 2048, 1024, "none"), (4096, 256, 2048, "silu"),
+                                       (50_000, 64, 64, "none"), (777, 4096, 136, "silu")])
+def test_larger(cuda_device, m, k, n, act):
+    x, w, b, r, dy = _inputs(cuda_device, m, k, n, BF, seed=1)
+    a = _both(x, w, b, r, dy, act, f"{m}x{k}x{n}")
+    c = _both(x, w, b, r, dy, act, f"{m}x{k}x{n}")
+    assert all(torch.equal(p, q) for p, q in zip(a, c))  # bit for bit
+
+
+def test_strides_offsets_and_shapes(cuda_device):
+    """Views with long rows, odd offsets and odd strides, batched shapes, broadcast inputs."""
+    x, w, b, r, dy = _inputs(cuda_device, 60, 96, 40, BF, seed=2)
+    want = linear.linear(x, w, b, activation="silu", residual=r)
+    wide = torch.zeros(60, 200, dtype=BF, device=cuda_device)
+    for off in (0, 8, 3):
+        wide[:, off:off + 96] = x
+        assert torch.equal(linear.linear(wide[:, off:off + 96], w, b, activation="silu", residual=r), want)
+    flat = torch.zeros(60 * 96 + 1, dtype=BF, device=cuda_device)
+    xo = flat[1:].view(60, 96).copy_(x)
+    ww = torch.zeros(40, 97, dtype=BF, device=cuda_device)
+    ww[:, :96] = w
+    rr = torch.zeros(60, 41, dtype=BF, device=cuda_device)
+    rr[:, 1:] = r
+    assert torch.equal(linear.linear(xo, ww[:, :96], b, activation="silu", residual=rr[:, 1:]), want)
+    assert torch.equal(linear.linear(x.view(3, 4, 5, 96), w, b, activation="silu", residual=r.view(3, 4, 5, 40)).view(60, 40),
+                       want)
+    xt = x.t().contiguous().t()
+    assert torch.equal(linear.linear(xt, w, b, activation="silu", residual=r), want)
+    assert linear.linear(x[0], w, b).shape == (40,)
+    xe = x[:1].expand(60, 96)
+    assert torch.equal(linear.linear(xe, w), linear.linear(xe.contiguous(), w))
+    one = torch.randn(1, 96, device=cuda_device).to(BF).requires_grad_()
+    y = linear.linear(one.expand(60, 96), w)
+    (g,) = torch.autograd.grad(y, one, torch.ones_like(y))  # the broadcast row gets the sum
+    exact = 60 * w.double().sum(0)
+    # each of 60 rows rounded to 16 bits, their sum once more
+    assert ((g.double() - exact).abs() <= 3 * _half(BF) * 60 * w.double().abs().sum(0)).all()
+
+
+def test_autocast_with_f32_parameters(cuda_device):
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(72, 48).to(cuda_device)
+    x = torch.randn(500, 72, device=cuda_device, requires_grad=True)
+    dy = torch.randn(500, 48, device=cuda_device).to(BF)
+    with torch.autocast("cuda", dtype=BF):
+        y = linear.linear(x, lin.weight, lin.bias, activation="gelu")
+        assert y.dtype == BF
+    grads = torch.autograd.grad(y, [x, lin.weight, lin.bias], dy)
+    want, tol = _define(x.detach().to(BF), lin.weight.detach().to(BF), lin.bias.detach(), None, dy, "gelu", BF)
+    _ok(y.detach(), want["y"], tol["y"], "y")
+    for g, k in zip(grads, ("dx", "dw", "db")):
+        assert g.dtype == F32
+        e, v = tol[k]
+        # dx is rounded to 16 bits before it is cast up; dw and db stay f32
+        bound = e + (_half(BF) * 1.01 * (v.abs() + e) if k == "dx" else U * v.abs())
+        assert ((g.double() - want[k]).abs() <= bound).all(), k
+
+
+def test_gradients_against_differences(cuda_device):
+    """gelu and silu: the loss along a random direction changes as the gradients say (differences in float64)."""
+    for act in ("gelu", "silu"):
+        x, w, b, r, dy = _inputs(cuda_device, 40, 24, 32, HF, seed=4)
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        grads = torch.autograd.grad(linear.linear(leaves[0], leaves[1], leaves[2], activation=act, residual=leaves[3]),
+                                    leaves, dy)
+        g = torch.Generator(device=cuda_device).manual_seed(1)
+        way = [torch.randn(t.shape, generator=g, device=cuda_device).double() for t in leaves]
+
+        def loss(s):
+            a, c, d, e = [t.double() + s * v for t, v in zip((x, w, b, r), way)]
+            return ((_act(a @ c.t() + d, act)[0] + e) * dy.double()).sum()
+
+        want = float((loss(1e-5) - loss(-1e-5)) / 2e-5)
+        got = float(sum((p.double() * v).sum() for p, v in zip(grads, way)))
+        size = float(sum((p.double() * v).abs().sum() for p, v in zip(grads, way)))
+        assert abs(got - want) <= 4 * _half(HF) * size  # z, dz and each gradient rounded to f16
+
+
+def test_special_values(cuda_device):
+    x = torch.zeros(4, 16, dtype=BF, device=cuda_device)
+    x[1, 0], x[2, 0], x[3, 0] = float("inf"), float("nan"), -3e4
+    w = torch.ones(8, 16, dtype=BF, device=cuda_device)
+    for act in ("none", "relu", "silu", "gelu"):
+        for rows in (x, x.repeat(40, 1)):  # both kernels
+            y = linear.linear(rows, w, activation=act)
+            assert (y[0] == 0).all() and (y[1] == float("inf")).all() and torch.isnan(y[2]).all()
+            assert (y[3] == (-29952.0 if act == "none" else 0.0)).all()
+    big = torch.full((10, 16), -300.0, dtype=HF, device=cuda_device, requires_grad=True)  # z = -1.4e6: beyond f16
+    w = torch.full((8, 16), 300.0, dtype=HF, device=cuda_device)
+    for act in ("relu", "silu", "gelu"):
+        y = linear.linear(big, w, activation=act)
+        (g,) = torch.autograd.grad(y, big, torch.ones_like(y))
+        assert (y == 0).all() and (g == 0).all()
+
+
+def test_empty_and_partial_gradients(cuda_device):
+    x, w, b, r, dy = _inputs(cuda_device, 20, 24, 16, BF)
+    wl, bl = w.detach().requires_grad_(), b.detach().requires_grad_()
+    e = torch.zeros(0, 24, dtype=BF, device=cuda_device, requires_grad=True)
+    y = linear.linear(e, wl, bl, activation="gelu")
+    ge = torch.autograd.grad(y.sum(), [e, wl, bl])
+    assert y.shape == (0, 16) and ge[0].shape == (0, 24) and (ge[1] == 0).all() and (ge[2] == 0).all()
+    full = torch.autograd.grad(linear.linear(x.requires_grad_(), wl, bl, activation="silu"), [x, wl, bl], dy)
+    x = x.detach()
+    (only_w,) = torch.autograd.grad(linear.linear(x, wl, b, activation="silu"), [wl], dy)
+    (only_b,) = torch.autograd.grad(linear.linear(x, w, bl, activation="silu"), [bl], dy)
+    (only_x,) = torch.autograd.grad(linear.linear(x.requires_grad_(), w, b, activation="silu"), [x], dy)
+    assert torch.equal(only_x, full[0]) and torch.equal(only_w, full[1]) and torch.equal(only_b, full[2])
+    rl = r.detach().requires_grad_()
+    (only_r,) = torch.autograd.grad(linear.linear(x.detach(), w, residual=rl), [rl], dy)
+    assert torch.equal(only_r, dy)
+
+
+def test_refusals(cuda_device):
+    x, w = torch.zeros(4, 16, device=cuda_device), torch.zeros(8, 16, device=cuda_device)
+    with pytest.raises(RuntimeError, match="not 16-bit"):
+        linear.linear(x, w)
+    with pytest.raises(RuntimeError, match="without autocast"):
+        linear.linear(x.to(BF), w)
+    with pytest.raises(RuntimeError, match="without autocast"):
+        linear.linear(x.to(BF), w.to(BF), residual=torch.zeros(4, 8, device=cuda_device))
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        linear.linear(x.to(BF), w.to(BF), torch.zeros(8, dtype=torch.float64, device=cuda_device))
+    with pytest.raises(RuntimeError, match="tensors on"):
+        linear.linear(x.to(BF), w.to(BF).cpu())
+
+
+def test_captured_and_on_another_stream(cuda_device):
+    x, w, b, r, dy = _inputs(cuda_device, 300, 128, 96, BF, seed=6)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+
+    def once():
+        y = linear.linear(*leaves, activation="silu", residual=r)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = once()
+    torch.cuda.current_stream().wait_stream(side)
+    here = once()
+    assert all(torch.equal(p, q) for p, q in zip(there, here))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = once()
+    with torch.no_grad():
+        leaves[0].mul_(-0.5)
+    graph.replay()
+    want = once()
+    assert all(torch.equal(p, q) for p, q in zip(outs, want))
+
+
+def test_wait_that_runs_out_is_reported(cuda_device):
+    """The GEMM's bounded waits report to the library's fault word, as every pipelined kernel's do."""
+    x, w, *_ = _inputs(cuda_device, 200, 64, 64, BF)
+    want = linear.linear(x, w)
+    lib = _lib.load()
+    assert lib.ow_debug_wait_probe(1_000_000) == 0
+    try:
+        linear.linear(x, w)
+    finally:
+        lib.ow_debug_wait_probe(0)
+    assert _lib.device_fault(cuda_device.index or 0, reset=True) == 1
+    assert torch.equal(linear.linear(x, w), want)
+
+
+def test_run_of_the_operators_together(cuda_device):
+    """Norms, two linears with their epilogues and the optimizer as a residual network uses them, against float64
+    autograd; 16-bit roundings of a chain of six operators are at most 16 half steps relative to the largest value."""
+    from omniwave_b200 import norm
+
+    torch.manual_seed(0)
+    c, hid = 128, 256
+    names = ["w1", "b1", "w2", "b2", "pre", "post", "gate"]
+    make = {"w1": torch.randn(hid, c) * c ** -0.5, "b1": torch.randn(hid) * 0.1, "w2": torch.randn(c, hid) * hid ** -0.5,
+            "b2": torch.randn(c) * 0.1, "pre": 1 + 0.1 * torch.randn(c), "post": 1 + 0.1 * torch.randn(c),
+            "gate": 0.5 + 0.1 * torch.randn(c)}
+    ps = {k: torch.nn.Parameter(v.to(cuda_device).to(BF)) for k, v in make.items()}
+    x = torch.randn(4, 50, c, device=cuda_device).to(BF)
+    dy = torch.randn(4, 50, c, device=cuda_device).to(BF)
+
+    def net(p, x):
+        n = norm.rms_norm(x, p["pre"])
+        d = linear.linear(linear.linear(n, p["w1"], p["b1"], activation="silu"), p["w2"], p["b2"], residual=n)
+        return norm.norm_residual(x, d, p["post"], p["gate"])
+
+    def net64(p, x):
+        rms = lambda v: v * (v.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt()  # noqa: E731
+        n = rms(x) * p["pre"]
+        d = torch.nn.functional.silu(n @ p["w1"].t() + p["b1"]) @ p["w2"].t() + p["b2"] + n
+        return x + p["gate"] * rms(d) * p["post"]
+
+    p64 = {k: v.detach().double().requires_grad_() for k, v in ps.items()}
+    y64 = net64(p64, x.double())
+    g64 = torch.autograd.grad(y64, [p64[k] for k in names], dy.double())
+    opt = AdamW(list(ps.values()), lr=1e-2, weight_decay=0.0, max_norm=1e6, skip_nonfinite=True)
+    y = net(ps, x)
+    y.backward(dy)
+    tol = 16 * _half(BF)
+    assert (y.double() - y64).abs().max() <= tol * y64.abs().max()
+    for k, g in zip(names, g64):
+        assert (ps[k].grad.double() - g).abs().max() <= tol * g.abs().max(), k
+    before = {k: v.detach().clone() for k, v in ps.items()}
+    opt.step()
+    for k, g in zip(names, g64):
+        step = ps[k].detach().double() - before[k].double()
+        sure = g.abs() > tol * g.abs().max()  # a first step is lr against the gradient's sign
+        assert ((step + 1e-2 * torch.sign(g)).abs()[sure] <= 1e-4 + _half(BF) * 1.01 * ps[k].double().abs()[sure]).all(), k
