@@ -173,6 +173,7 @@ EXPORTS = (
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_host = None
 
 
 class NativeLibraryError(RuntimeError):
@@ -250,6 +251,22 @@ def load() -> ctypes.CDLL:
             raise NativeLibraryError(f"ABI version mismatch: library {v}, binding {ABI_VERSION}")
         _lib = lib
         return lib
+
+
+def host():
+    """The module ``omniwave_b200._host`` (checks, autograd and calls over torch tensors)."""
+    global _host
+    if _host is None:
+        load()  # a missing or mismatched library is reported as such
+        try:
+            from omniwave_b200 import _host as mod
+        except ImportError as exc:
+            raise NativeLibraryError(f"omniwave_b200/_host.so cannot be loaded ({exc}); build it with "
+                                     f"`python -m omniwave_b200.build`") from exc
+        if mod.abi_version != ABI_VERSION:
+            raise NativeLibraryError(f"ABI version mismatch: _host.so {mod.abi_version}, binding {ABI_VERSION}")
+        _host = mod
+    return _host
 
 
 def check(status: int, what: str) -> None:

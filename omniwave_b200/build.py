@@ -4,6 +4,8 @@ Every ``csrc/*.cu`` file is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) and linked into
 ``omniwave_b200/libomniwave_b200.so``.  Objects go to ``omniwave_b200/_build``;
 files whose sources and headers are older than their object are not rebuilt.
+``csrc/host/ow_host.cpp``, the host side of the norms, the linear layer and
+AdamW over torch tensors, becomes the Python module ``omniwave_b200/_host.so``.
 
 Usage: ``python -m omniwave_b200.build [--force] [--verbose]``.
 """
@@ -23,6 +25,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libomniwave_b200.so")
+HOST_SRC = os.path.join(CSRC, "host", "ow_host.cpp")
+HOST = os.path.join(PKG, "_host.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = [
@@ -50,6 +54,34 @@ def _stale(target: str, deps: list[str]) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _build_host(force: bool, verbose: bool) -> None:
+    """Compile and link the Python module against torch and the library beside it."""
+    if not (force or _stale(HOST, [HOST_SRC, os.path.join(INCLUDE, "omniwave_b200.h")])):
+        return
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include"), INCLUDE]
+    # The system's compiler, as nvcc takes it, and not $CXX: a toolchain that links its own C++ runtime
+    # statically cannot share strings and exceptions with torch.
+    cxx = shutil.which("g++") or "c++"
+    tmp = HOST + ".tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_host",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-I{i}" for i in inc], HOST_SRC, "-o", tmp, f"-L{os.path.join(root, 'lib')}", f"-L{PKG}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-l:libomniwave_b200.so", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cxx} failed for {HOST_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST)
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
@@ -81,6 +113,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if force or jobs or _stale(LIB, objects):
         cmd = [nvcc, *ARCH, "-shared", "-o", LIB, *objects, "-lcudart"]
         run(cmd)
+    _build_host(force, verbose)
     return LIB
 
 

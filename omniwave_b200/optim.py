@@ -33,7 +33,6 @@ __all__ = ["AdamW", "adamw_supported"]
 
 BLOCK = _lib.ADAMW_BLOCK
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_dtype, _is_sparse = Tensor.dtype.__get__, Tensor.is_sparse.__get__
 
 
 def _dense(p: Tensor) -> bool:
@@ -70,8 +69,7 @@ class _Bucket:
         self.group, self.params, self.bits = group, params, bits
         dev = self.device = params[0].device
         self.dtype = params[0].dtype
-        self.strides = [p.stride() for p in params]
-        self.numel = [p.numel() for p in params]
+        self._gather = _lib.host().Gather(params)
         slots, total = [0], 0
         for p in params:
             total += -(-p.numel() // BLOCK) * BLOCK
@@ -79,7 +77,7 @@ class _Bucket:
         self.slots = slots
         blocks = total // BLOCK
         self._slots = (ctypes.c_int64 * len(slots))(*slots)
-        numel = torch.tensor(self.numel, dtype=torch.int64)
+        numel = torch.tensor([p.numel() for p in params], dtype=torch.int64)
         counts = (torch.tensor(slots[1:]) - torch.tensor(slots[:-1])) // BLOCK
         self.dev_slots = torch.tensor(slots, dtype=torch.int64, device=dev)
         self.dev_numel = numel.to(dev)
@@ -117,38 +115,8 @@ class _Bucket:
         return out
 
     def gather(self) -> list[Tensor]:
-        """Write down this step's pointers; returns the gradients that had to be copied.
-
-        The checks run list by list: an eager step over many small tensors is
-        bound by the host, and a loop over all of them costs twice as much.
-        """
-        ps = self.params
-        gs = [p.grad for p in ps]
-        self.some = True
-        copied: list[Tensor] = []
-        missing = [i for i, g in enumerate(gs) if g is None]
-        if missing:
-            self.some = len(missing) < len(gs)
-            for i in missing:
-                gs[i] = ps[i]  # stands in for the checks
-        if any(map(_is_sparse, gs)):
-            raise RuntimeError("AdamW does not support sparse gradients")
-        dtype, index = {self.dtype}, {self.device.index}
-        if set(map(_dtype, ps)) != dtype or set(map(Tensor.get_device, ps)) != index \
-                or list(map(Tensor.stride, ps)) != self.strides or list(map(Tensor.numel, ps)) != self.numel:
-            raise RuntimeError("a parameter moved to another device, dtype or layout since it was added to AdamW")
-        if set(map(_dtype, gs)) != dtype or set(map(Tensor.get_device, gs)) != index \
-                or list(map(Tensor.numel, gs)) != self.numel:
-            raise RuntimeError("a gradient has another dtype, device or size than its parameter")
-        if list(map(Tensor.stride, gs)) != self.strides:
-            for i, g in enumerate(gs):
-                if g.stride() != self.strides[i] and g.numel() > 1:
-                    gs[i] = torch.empty_like(ps[i]).copy_(g)  # dense in the parameter's own order
-                    copied.append(gs[i])
-        self._p[:] = list(map(Tensor.data_ptr, ps))
-        self._g[:] = list(map(Tensor.data_ptr, gs))
-        for i in missing:
-            self._g[i] = None
+        """Write down this step's pointers; returns the gradients that had to be copied."""
+        self.some, copied = self._gather.gather(ctypes.addressof(self._p), ctypes.addressof(self._g))
         return copied
 
 

@@ -248,6 +248,13 @@ def test_empty_and_partial_gradients(cuda_device):
     assert torch.equal(only_r, dy)
 
 
+def test_second_derivative_is_refused(cuda_device):
+    x, w, *_ = _inputs(cuda_device, 20, 16, 8, BF)
+    y = linear.linear(x.requires_grad_(), w, activation="silu")
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_refusals(cuda_device):
     x, w = torch.zeros(4, 16, device=cuda_device), torch.zeros(8, 16, device=cuda_device)
     with pytest.raises(RuntimeError, match="not 16-bit"):

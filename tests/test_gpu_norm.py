@@ -232,6 +232,13 @@ def test_empty(cuda_device):
     assert (w.grad == 0).all() and x.grad.shape == (0, 5, 16)
 
 
+def test_second_derivative_is_refused(cuda_device):
+    x = torch.randn(2, 3, 8, device=cuda_device, requires_grad=True)
+    y = norm.rms_norm(x, torch.ones(8, device=cuda_device))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_refusals(cuda_device):
     x, w = torch.zeros(2, 3, 8, device=cuda_device), torch.ones(8, device=cuda_device)
     with pytest.raises(RuntimeError, match="dtype"):
