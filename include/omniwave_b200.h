@@ -380,8 +380,8 @@ OW_API int ow_pool_head_fwd(const ow_pool_head_t* args, void* stream);
  * a dtype (f32, bf16 or f16; the gradient has the parameter's) and the
  * hyperparameters; every tensor counts its own steps t.
  *
- * State is flat: tensor i owns the slots [slots[i], slots[i + 1]), of which the
- * first numel[i] are used; slots are multiples of OW_ADAMW_BLOCK.  With
+ * State is flat: tensor i owns the slots [slots[i], slots[i + 1]), multiples of
+ * OW_ADAMW_BLOCK, of which its first elements are used.  With
  * state_bits == 32 the moments are f32.  With 8 they are e4m3 codes, with one
  * f32 scale (largest magnitude / 448) for each block of OW_ADAMW_BLOCK slots;
  * they are rounded stochastically by a hash of (slot, step), so a run is
@@ -400,9 +400,9 @@ typedef struct ow_adamw_t {
   void* const* params;              /* host [tensors] */
   const void* const* grads;         /* host [tensors] */
   const int64_t* slots;             /* host [tensors + 1] */
-  const int64_t* dev_slots;         /* device [tensors + 1], the same values */
-  const int64_t* dev_numel;         /* device [tensors] */
-  const int32_t* dev_block_tensor;  /* device [slots[tensors] / OW_ADAMW_BLOCK]: each block's tensor */
+  const int32_t* dev_blocks;        /* device, 16-byte aligned: four ints for each block of OW_ADAMW_BLOCK
+                                     * slots: its tensor, the how manieth block of that tensor it is, the
+                                     * number of its slots in use (1 to OW_ADAMW_BLOCK), 0 */
   void* control;                    /* device, OW_ADAMW_CONTROL_BYTES, zero before its first use, this
                                      * optimizer's own: calls that overlap must not share it */
   int32_t state_bits;               /* 32 or 8 */

@@ -102,7 +102,7 @@ class AdamW(ctypes.Structure):
     _fields_ = [
         ("tensors", _c_i32), ("dtype", _c_i32),
         ("params", _vp), ("grads", _vp), ("slots", _vp),
-        ("dev_slots", _vp), ("dev_numel", _vp), ("dev_block_tensor", _vp), ("control", _vp),
+        ("dev_blocks", _vp), ("control", _vp),
         ("state_bits", _c_i32),
         ("exp_avg", _vp), ("exp_avg_sq", _vp), ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp),
         ("dev_steps", _vp),

@@ -16,6 +16,13 @@
 // products.  Tiles are walked in patches of 12 row blocks, so that the SMs at
 // work share A and B blocks in L2.
 //
+// A 128 x 256 tile of one SM takes in 48 KB for every 512 cycles of products,
+// more than an SM's 64 bytes a cycle.  So large products run on pairs of SMs
+// (a cluster of two, cta_group::2): a 256 x 256 tile, each SM holding 128 rows
+// of A and 128 of B and accumulating 128 rows of the tile, 32 KB for the same
+// products.  The even CTA issues the MMAs of the pair; both load their own
+// halves, counted on the even CTA's barriers.
+//
 // Where the tiles are few and k is long (dW: k is all tokens) the k blocks
 // are split over CTAs; each leaves an f32 partial, and a second kernel adds
 // them in a fixed order and does the epilogue.
@@ -42,10 +49,12 @@ constexpr int A_ST = TM * 128;
 constexpr int STG_W = 4096;  // a warp's staging: 2 KB for the residual, 2 KB for what it stores
 constexpr int PATCH = 12;
 
-template <int BN>
+// BN columns of a tile; CG CTAs share it (2: 256 rows, BN / 2 rows of B each).
+template <int BN, int CG>
 struct GC {
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int B_ST = BN * 128;
+  static constexpr int B_ROWS = BN / CG;
+  static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
+  static constexpr int B_ST = B_ROWS * 128;
   static constexpr int OFF_B = STAGES * A_ST;
   static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
   static constexpr int OFF_BAR = OFF_STG + EPI_WARPS * STG_W;
@@ -91,6 +100,74 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// ---------------------------------------------------------------- CTA pairs
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of ``p`` in CTA ``rank`` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_in(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A load into this CTA that completes on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  if constexpr (CG == 1) {
+    umma_f16(d, a, b, id, acc);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+  }
+}
+// Arrive on ``bar`` (of both CTAs of a pair) once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    umma_commit(bar);
+  } else {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_take(uint32_t* holder, uint32_t ncols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(holder, ncols);
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_give(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 1) tmem_dealloc(taddr, ncols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
 // Descriptor of an SW128 operand read MN-major: 64-element MN atoms ``lbo``
 // bytes apart, 8-line K groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t lbo) {
@@ -99,10 +176,27 @@ __device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t lbo) {
 }
 
 // ---------------------------------------------------------------- activations
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and exp(-z^2 / 2): one exponential serves
+// the function and its slope.  erfc by Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2),
+// t = 1 / (1 + p x), off by 1.5e-7 at most; a value that is rounded to 16 bits
+// next.  About 16 instructions where erff and expf take 40, which bound the
+// epilogue (25088 x 512 x 1024 forward 88 us) and the backward's first pass.
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+  bell = __expf(-0.5f * z * z);
+  const float tail = 0.5f * bell * t * fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+  return z > 0.f ? 1.f - tail : tail;
+}
+
 __device__ __forceinline__ float act_fwd(float z, int act) {
   if (act == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
   if (act == OW_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
-  if (act == OW_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == OW_ACT_GELU) {
+    float bell;
+    return z * normal_cdf(z, bell);
+  }
   return z;
 }
 
@@ -113,8 +207,11 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     const float s = __fdividef(1.f, 1.f + __expf(-z));
     return s * (1.f + z * (1.f - s));
   }
-  if (act == OW_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  if (act == OW_ACT_GELU) {
+    float bell;
+    const float cdf = normal_cdf(z, bell);
+    return fmaf(z * 0.39894228040143268f, bell, cdf);
+  }
   return 1.f;
 }
 
@@ -310,10 +407,10 @@ __device__ __forceinline__ Unit unit_of(const GemmArgs& a, int u) {
   return r;
 }
 
-template <int BN, bool AMN, bool BMN, bool BF16>
+template <int BN, int CG, bool AMN, bool BMN, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const GemmArgs a) {
-  using C = GC<BN>;
+  using C = GC<BN, CG>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
@@ -325,6 +422,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* abort = reinterpret_cast<volatile int*>(tmem + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = a.mtiles * a.ntiles * a.splits;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -333,16 +432,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + i, 1);
-      mbar_init(tfree + i, EPI_WARPS);
+      mbar_init(tfree + i, EPI_WARPS * CG);
     }
     mbar_init(probe, 1);
     *abort = 0;
     fence_mbar_init();
     wait_probe(probe, abort, a.probe_ns);
   }
-  if (warp == MMA_W) tmem_alloc(tmem, C::TMEM_COLS);
+  if (warp == MMA_W) tmem_take<CG>(tmem, C::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the pair's barriers are set up
   tc_fence_after();
   const uint32_t tbase = *tmem;
 
@@ -351,35 +451,40 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == PROD_W) {
     if (lane == 0) {
       int g = 0;
-      for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x) {
+      for (int u = first; u < units && !*abort; u += step) {
         const Unit t = unit_of(a, u);
+        const int am0 = (t.mt * CG + (int)rank) * TM, bn0 = t.nt * BN + (int)rank * C::B_ROWS;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
           const int s = g % C::STAGES;
           if (g >= C::STAGES && !mbar_wait(empty + s, ((g / C::STAGES) - 1) & 1, abort)) break;
-          mbar_arrive_expect_tx(full + s, A_ST + C::B_ST);
+          if (rank == 0) mbar_arrive_expect_tx(full + s, CG * (A_ST + C::B_ST));
           unsigned char* sa = sm + s * A_ST;
           unsigned char* sb = sm + C::OFF_B + s * C::B_ST;
+          auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1) {
+            if constexpr (CG == 1) tma_load_2d(dst, map, c0, c1, full + s);
+            else tma_load_2d_pair(dst, map, c0, c1, in_cta(full + s, 0));
+          };
           if constexpr (AMN) {
 #pragma unroll
-            for (int i = 0; i < TM / 64; ++i) tma_load_2d(sa + i * 8192, &amap, t.mt * TM + i * 64, kb * KE, full + s);
+            for (int i = 0; i < TM / 64; ++i) load(sa + i * 8192, &amap, am0 + i * 64, kb * KE);
           } else {
-            tma_load_2d(sa, &amap, kb * KE, t.mt * TM, full + s);
+            load(sa, &amap, kb * KE, am0);
           }
           if constexpr (BMN) {
 #pragma unroll
-            for (int i = 0; i < BN / 64; ++i) tma_load_2d(sb + i * 8192, &bmap, t.nt * BN + i * 64, kb * KE, full + s);
+            for (int i = 0; i < C::B_ROWS / 64; ++i) load(sb + i * 8192, &bmap, bn0 + i * 64, kb * KE);
           } else {
-            tma_load_2d(sb, &bmap, kb * KE, t.nt * BN, full + s);
+            load(sb, &bmap, kb * KE, bn0);
           }
         }
       }
     }
   } else if (warp == MMA_W) {
-    if (lane == 0) {
-      constexpr uint32_t ID = idesc_f16(TM, BN, BF16) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t ID = idesc_f16(TM * CG, BN, BF16) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
       const uint32_t s0 = smem_u32(sm);
       int g = 0, tl = 0;
-      for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x, ++tl) {
+      for (int u = first; u < units && !*abort; u += step, ++tl) {
         const Unit t = unit_of(a, u);
         const int acc = tl & 1;
         if (tl >= 2 && !mbar_wait(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
@@ -394,11 +499,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int kk = 0; kk < KE / 16; ++kk) {
             const uint64_t da = AMN ? sdesc_mn(aA + kk * 2048, 8192) : sdesc_sw128(aA + kk * 32);
             const uint64_t db = BMN ? sdesc_mn(aB + kk * 2048, 8192) : sdesc_sw128(aB + kk * 32);
-            umma_f16(tacc, da, db, ID, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+            umma<CG>(tacc, da, db, ID, (kb > t.kb0 || kk > 0) ? 1u : 0u);
           }
-          umma_commit(empty + s);
+          commit<CG>(empty + s);
         }
-        umma_commit(tfull + acc);
+        commit<CG>(tfull + acc);
       }
     }
   } else {
@@ -406,10 +511,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int q = warp & 3, half = warp >> 2;
     constexpr int NCH = BN / 64;  // 32-column blocks of a warp
     int tl = 0;
-    for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x, ++tl) {
+    for (int u = first; u < units && !*abort; u += step, ++tl) {
       const Unit t = unit_of(a, u);
       const int acc = tl & 1;
-      const int64_t m0 = (int64_t)t.mt * TM + q * 32;
+      const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
       const int nb = t.nt * BN + half * (BN / 2);
       Epi e = a.e;
       if (a.splits > 1) e.out = (float*)a.e.out + (int64_t)t.split * a.part_stride;
@@ -435,7 +540,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tfree + acc);
+      if (lane == 0) {
+        if constexpr (CG == 1) mbar_arrive(tfree + acc);
+        else arrive_in(in_cta(tfree + acc, 0));
+      }
     }
   }
 
@@ -447,9 +555,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     // shared memory and TMEM they target are released.
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   }
+  // Neither CTA of a pair leaves while the other may still count on its barriers.
+  if constexpr (CG == 2) cluster_sync();
   if (warp == MMA_W) {
     tc_fence_after();
-    tmem_dealloc(tbase, C::TMEM_COLS);
+    tmem_give<CG>(tbase, C::TMEM_COLS);
   }
 }
 
@@ -668,33 +778,35 @@ struct Mat {
   int64_t ld;
 };
 
-// Shape of one GEMM: the tile's width and the k splits that a simple model
-// finds fastest.  A 64-wide k block of a 128 x BN tile takes BN / 32 units of
-// time but no less than what its copies take (A's 128 rows count as well); a
-// tile's epilogue 10 + BN / 8 units; a split costs writing and reading its
-// f32 partial.
+// Shape of one GEMM: the tile's width, whether pairs of SMs share it, and the
+// k splits that a simple model finds fastest, in cycles.  A 64-wide k block
+// takes its products (BN * 2 cycles on an SM) or its copies at 64 bytes a
+// cycle, whichever is longer: 384 cycles for 128 x 64, 512 for 128 x 128, 768
+// for 128 x 256, and 512 for the pair's 256 x 256.  A tile adds its start and
+// the last one its epilogue (20 cycles a column and 2000); splits write and
+// read f32 partials at about 3 KB a cycle and start one more kernel (6000).
 struct Plan {
-  int bn, splits;
+  int bn, cg, splits;
 };
 Plan plan_gemm(int64_t M, int N, int kblocks) {
   const int sms = device_sm_count();
-  Plan best{128, 1};
+  Plan best{128, 1, 1};
   double least = 1e300;
-  const int64_t mt = (M + TM - 1) / TM;
-  for (int bn : {64, 128, 256}) {
-    const int64_t tiles = mt * ((N + bn - 1) / bn);
+  struct Tile { int bn, cg, block; };
+  for (const Tile t : {Tile{64, 1, 384}, Tile{128, 1, 512}, Tile{256, 1, 768}, Tile{256, 2, 512}}) {
+    const int64_t tiles = (M + TM * t.cg - 1) / (TM * t.cg) * ((N + t.bn - 1) / t.bn);
+    const int slots = sms / t.cg;
     // more splits than fill the SMs twice gain nothing
-    const int smax = (int)std::min<int64_t>(std::min(kblocks, 64), 1 + 2 * sms / tiles);
+    const int smax = (int)std::min<int64_t>(std::min(kblocks, 64), 1 + 2 * slots / tiles);
     for (int s = 1; s <= smax; ++s) {
-      const int64_t waves = (tiles * s + sms - 1) / sms;
+      const int64_t waves = (tiles * s + slots - 1) / slots;
       const int kb = (kblocks + s - 1) / s;
-      const double block = std::max(bn / 32.0, (128 + bn) / 64.0);
-      double t = (double)waves * (kb * block + 10.0 + bn / 8.0);
-      // f32 partials written and read: 8 bytes each at about 3.4 KB a unit (0.5 us), and a launch
-      if (s > 1) t += 40.0 + (double)s * M * N * 8.0 / 400e3;
-      if (t < least) {
-        least = t;
-        best = Plan{bn, s};
+      const double main = std::max<double>((double)kb * t.block, t.bn * 20.0);  // an epilogue runs under the next tile
+      double c = waves * main + t.bn * 20.0 + 2000.0;
+      if (s > 1) c += 6000.0 + (double)s * M * N * 8.0 / 3000.0;
+      if (c < least) {
+        least = c;
+        best = Plan{t.bn, t.cg, s};
       }
     }
   }
@@ -735,15 +847,37 @@ int map_of(CUtensorMap* map, const Mat& m, bool bf16, uint32_t box_rows) {
   return encode_tiled_map(map, bf16, 2, m.p, dims, strides, box, "ow_linear");
 }
 
-template <int BN, bool AMN, bool BMN, bool BF16>
+template <int BN, int CG, bool AMN, bool BMN, bool BF16>
 int run_gemm(const CUtensorMap& am, const CUtensorMap& bm, const GemmArgs& k, int grid, cudaStream_t st) {
-  auto kern = gemm_kernel<BN, AMN, BMN, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GC<BN>::SMEM);
+  using C = GC<BN, CG>;
+  auto kern = gemm_kernel<BN, CG, AMN, BMN, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) {
-    set_error("ow_linear: cannot reserve %d bytes of shared memory: %s", GC<BN>::SMEM, cudaGetErrorString(e));
+    set_error("ow_linear: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e));
     return OW_ERR_CUDA;
   }
-  launch(kern, grid, THREADS, GC<BN>::SMEM, st, am, bm, k);
+  if constexpr (CG == 1) {
+    launch(kern, grid, THREADS, C::SMEM, st, am, bm, k);
+  } else {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = CG;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    count_launches(1);
+    e = cudaLaunchKernelEx(&cfg, kern, am, bm, k);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      set_error("gemm_kernel: launch failed: %s", cudaGetErrorString(e));
+      return OW_ERR_CUDA;
+    }
+  }
   OW_CHECK_LAUNCH("gemm_kernel");
   return OW_OK;
 }
@@ -756,12 +890,12 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   if (w.b) OW_RETURN_IF(pad_rows(B, w.b, st));
   CUtensorMap am, bm;
   OW_RETURN_IF(map_of(&am, A, bf16, AMN ? KE : TM));
-  OW_RETURN_IF(map_of(&bm, B, bf16, BMN ? KE : p.bn));
+  OW_RETURN_IF(map_of(&bm, B, bf16, BMN ? KE : p.bn / p.cg));
   GemmArgs k{};
   k.M = M;
   k.N = N;
   k.kblocks = (int)((K + KE - 1) / KE);
-  k.mtiles = (int)((M + TM - 1) / TM);
+  k.mtiles = (int)((M + TM * p.cg - 1) / (TM * p.cg));
   k.ntiles = (N + p.bn - 1) / p.bn;
   k.splits = p.splits;
   k.e = e;
@@ -778,14 +912,16 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   k.probe_ns = wait_probe_ns();
   const int64_t units = (int64_t)k.mtiles * k.ntiles * k.splits;
   OW_CHECK_ARG(units < (1LL << 31) - 1024, "ow_linear: too many tiles");
-  const int grid = (int)std::min<int64_t>(units, device_sm_count());
-  auto go = [&](auto bn) -> int {
-    constexpr int BN = decltype(bn)::value;
-    return bf16 ? run_gemm<BN, AMN, BMN, true>(am, bm, k, grid, st) : run_gemm<BN, AMN, BMN, false>(am, bm, k, grid, st);
+  const int grid = (int)std::min<int64_t>(units, device_sm_count() / p.cg) * p.cg;
+  auto go = [&](auto bn, auto cg) -> int {
+    constexpr int BN = decltype(bn)::value, CG = decltype(cg)::value;
+    return bf16 ? run_gemm<BN, CG, AMN, BMN, true>(am, bm, k, grid, st) : run_gemm<BN, CG, AMN, BMN, false>(am, bm, k, grid, st);
   };
-  if (p.bn == 64) OW_RETURN_IF(go(std::integral_constant<int, 64>()));
-  else if (p.bn == 128) OW_RETURN_IF(go(std::integral_constant<int, 128>()));
-  else OW_RETURN_IF(go(std::integral_constant<int, 256>()));
+  using I1 = std::integral_constant<int, 1>;
+  if (p.cg == 2) OW_RETURN_IF(go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>()));
+  else if (p.bn == 64) OW_RETURN_IF(go(std::integral_constant<int, 64>(), I1()));
+  else if (p.bn == 128) OW_RETURN_IF(go(std::integral_constant<int, 128>(), I1()));
+  else OW_RETURN_IF(go(std::integral_constant<int, 256>(), I1()));
   if (p.splits > 1) {
     const int64_t total = M * ((N + 3) / 4);
     const int g2 = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);

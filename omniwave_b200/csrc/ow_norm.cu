@@ -14,11 +14,15 @@
 //
 // Split.  G threads share a row, each with NV vectors of V channels in
 // registers, so a row is read once; rows of up to 32 lanes need only shuffles.
+// A block stays within the rows that share a gate (all of them, or one
+// sample's), so it keeps the channels' factors q wp and wn in shared memory
+// instead of reading 8 to 12 bytes of weights an element again and again.
 // The backward needs three sums a row, taken in one exchange: with
 // A = sum e' (dh + r_h u), B = sum e' h^, S = sum u h^ (e' = s q wp d^),
-// mean(e d^) = (A - B r_h S / C) / C.  Each thread keeps its channels' share of
-// the weight gradients in registers over all its rows; a block leaves one
-// partial row and a second kernel adds these in a fixed order.
+// mean(e d^) = (A - B r_h S / C) / C.  Both of the post-norm's gradients follow
+// from one sum, t = sum s D d^: dwp = q t and dq = wp t.  Each thread adds its
+// channels' shares in registers over all its rows; a block leaves one partial
+// row and a second kernel adds these in a fixed order.
 //
 // Bound: HBM.
 #include <algorithm>
@@ -50,8 +54,8 @@ struct Args {
   float* rh;             // [rows] 1 / rms(h)
   void* dx;
   void* ddelta;
-  float* part;           // [parts][arrays][C] partial weight gradients
-  int arrays;            // 3: dwn, dwp, dq; 1: dwn
+  float* part;           // [parts][arrays][C] partial sums: of dn h^ (with a next norm), of s D d^ (with delta)
+  int arrays;
   int64_t groups;        // gate rows whose gradients are kept apart (1 or samples)
   int per_group;         // blocks that share a group's rows
   int64_t group_rows;
@@ -147,25 +151,65 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* sh, int& turn) {
   }
 }
 
-// One block does ``blockDim / G`` rows at a time and strides over all rows.
+// A block's channel factors in shared memory: C floats of q wp (with delta),
+// C of wn (with a next norm).  Vectors of 8 are kept as two planes of 4, so a
+// warp's 16-byte reads do not conflict.
+template <int V>
+__device__ __forceinline__ int plane(int c, int C) {
+  if constexpr (V == 8) return (c & 4) * (C >> 3) + (c >> 3) * 4 + (c & 3);
+  else return c;
+}
+template <int V>
+__device__ __forceinline__ void factors(const float* w, int c, int C, float (&o)[V]) {
+  if constexpr (V == 8) {
+    const float4 a = *reinterpret_cast<const float4*>(w + (c >> 1)), b = *reinterpret_cast<const float4*>(w + (C >> 1) + (c >> 1));
+    o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+  } else {
+    o[0] = w[c];
+  }
+}
+template <int V, bool DELTA, bool NEXT>
+__device__ __forceinline__ void load_factors(const Args& a, int64_t group, float* kq, float* wn) {
+  for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
+    if constexpr (DELTA) {
+      float w = ld1(a.wp, a.wp_dt, c);
+      if (a.q_rows) w *= ld1(a.q, a.q_dt, (a.q_rows > 1 ? group * a.C : 0) + c);
+      kq[plane<V>(c, a.C)] = w;
+    }
+    if constexpr (NEXT) wn[plane<V>(c, a.C)] = ld1(a.wn, a.wn_dt, c);
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ int64_t sample_of(const Args& a, int64_t row) {
+  return a.rows < (1LL << 32) ? (int64_t)((uint32_t)row / (uint32_t)a.tokens) : row / a.tokens;
+}
+
+// Block (group, part) strides over its group's rows, ``blockDim / G`` at a time.
 template <int V, int G, int NV, bool DELTA, bool NEXT>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args a) {
   constexpr int T = G > 256 ? G : 256, RB = T / G;
+  extern __shared__ float4 dyn4[];
+  float* kq = reinterpret_cast<float*>(dyn4);
+  float* wn = kq + (DELTA ? a.C : 0);
   __shared__ float sh[G > 32 ? 2 * 32 : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.rows; r0 += (int64_t)gridDim.x * RB) {
+  const int64_t group = blockIdx.x / a.per_group;
+  const int part = blockIdx.x % a.per_group;
+  const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
+  load_factors<V, DELTA, NEXT>(a, group, kq, wn);
+  for (int64_t r0 = group * a.group_rows + (int64_t)part * RB; r0 < row_end; r0 += (int64_t)a.per_group * RB) {
     const int64_t row = r0 + sub;
-    const bool live = row < a.rows;
+    const bool live = row < row_end;
     const int64_t at = row * a.C;
     float x[NV][V], d[NV][V];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * V;
-      const bool on = live && c < a.C;
 #pragma unroll
       for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = 0.f;
-      if (on) {
+      if (live && c < a.C) {
         ldv<V>(a.x, a.x_dt, at + c, x[j]);
         if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
       }
@@ -179,19 +223,13 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args 
       row_sum<G>(s, sh, turn);
       const float rd = rsqrtf(s[0] * a.inv_c + a.eps);
       if (live && lane == 0 && a.rd) a.rd[row] = rd;
-      const int64_t b = live ? row / a.tokens : 0;
-      const float sc = rd * (a.scale ? a.scale[b] : 1.f);
+      const float sc = rd * (a.scale && live ? a.scale[sample_of(a, row)] : 1.f);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = (j * G + lane) * V;
         if (!live || c >= a.C) continue;
-        float w[V], q[V];
-        ldv<V>(a.wp, a.wp_dt, c, w);
-        if (a.q_rows) {
-          ldv<V>(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c, q);
-#pragma unroll
-          for (int k = 0; k < V; ++k) w[k] *= q[k];
-        }
+        float w[V];
+        factors<V>(kq, c, a.C, w);
 #pragma unroll
         for (int k = 0; k < V; ++k) x[j][k] += sc * d[j][k] * w[k];
         stv<V>(a.h, a.x_dt, at + c, x[j]);
@@ -211,7 +249,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args 
         const int c = (j * G + lane) * V;
         if (!live || c >= a.C) continue;
         float w[V];
-        ldv<V>(a.wn, a.wn_dt, c, w);
+        factors<V>(wn, c, a.C, w);
 #pragma unroll
         for (int k = 0; k < V; ++k) w[k] *= x[j][k] * rh;
         stv<V>(a.n, a.n_dt, at + c, w);
@@ -224,66 +262,61 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args 
 template <int V, int G, int NV, bool DELTA, bool NEXT>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args a) {
   constexpr int T = G > 256 ? G : 256, RB = T / G;
-  extern __shared__ float dyn[];  // the block's sums over its row groups (RB > 1)
+  extern __shared__ float4 dyn4[];  // the channel factors, later the sums of the block's row groups
+  float* kq = reinterpret_cast<float*>(dyn4);
+  float* wn = kq + (DELTA ? a.C : 0);
   __shared__ float sh[G > 32 ? 2 * 3 * 32 : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, sub = threadIdx.x / G;
   const int64_t group = blockIdx.x / a.per_group;
   const int part = blockIdx.x % a.per_group;
   const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
-  float an[NV][V], ap[NV][V], aq[NV][V];
+  load_factors<V, DELTA, NEXT>(a, group, kq, wn);
+  float an[NV][V], at_[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int k = 0; k < V; ++k) an[j][k] = ap[j][k] = aq[j][k] = 0.f;
+    for (int k = 0; k < V; ++k) an[j][k] = at_[j][k] = 0.f;
 
   for (int64_t r0 = group * a.group_rows + (int64_t)part * RB; r0 < row_end; r0 += (int64_t)a.per_group * RB) {
     const int64_t row = r0 + sub;
     const bool live = row < row_end;
     const int64_t at = row * a.C;
-    const int64_t b = live ? row / a.tokens : 0;
     float x[NV][V], d[NV][V], gh[NV][V], gn[NV][V];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * V;
-      const bool on = live && c < a.C;
 #pragma unroll
       for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = gh[j][k] = gn[j][k] = 0.f;
-      if (on) {
+      if (live && c < a.C) {
         if constexpr (NEXT) {
           ldv<V>(a.x, a.x_dt, at + c, x[j]);
           ldv<V>(a.dn, a.n_dt, at + c, gn[j]);
         }
         if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
-        if (a.dh) ldv<V>(a.dh, a.x_dt, at + c, gh[j]);
+        if (DELTA && a.dh) ldv<V>(a.dh, a.x_dt, at + c, gh[j]);
       }
     }
     const float rd = DELTA && live ? a.rd[row] : 0.f, rh = NEXT && live ? a.rh[row] : 0.f;
-    const float sc = DELTA && a.scale ? a.scale[b] : 1.f;
-    float wp[NV][V], q[NV][V], wn[NV][V];
+    const float sc = DELTA && a.scale && live ? a.scale[sample_of(a, row)] : 1.f;
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * V;
-#pragma unroll
-      for (int k = 0; k < V; ++k) { wp[j][k] = wn[j][k] = 0.f; q[j][k] = 1.f; }
-      if (live && c < a.C) {
-        if constexpr (DELTA) {
-          ldv<V>(a.wp, a.wp_dt, c, wp[j]);
-          if (a.q_rows) ldv<V>(a.q, a.q_dt, (a.q_rows > 1 ? b * a.C : 0) + c, q[j]);
-        }
-        if constexpr (NEXT) ldv<V>(a.wn, a.wn_dt, c, wn[j]);
-      }
+      if (!live || c >= a.C) continue;
+      float wp[V], w[V];
+      if constexpr (DELTA) factors<V>(kq, c, a.C, wp);
+      if constexpr (NEXT) factors<V>(wn, c, a.C, w);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         float e = 0.f;
         if constexpr (DELTA) {
-          d[j][k] *= rd;                                // d^
-          e = sc * q[j][k] * wp[j][k] * d[j][k];        // h - x
+          d[j][k] *= rd;                 // d^
+          e = sc * wp[k] * d[j][k];      // h - x
         }
         if constexpr (NEXT) {
-          x[j][k] = (x[j][k] + e) * rh;                 // h^
-          const float u = gn[j][k] * wn[j][k];
+          x[j][k] = (x[j][k] + e) * rh;  // h^
+          const float u = gn[j][k] * w[k];
           an[j][k] += gn[j][k] * x[j][k];
           s[0] += u * x[j][k];
           if constexpr (DELTA) s[2] += e * x[j][k];
@@ -299,16 +332,15 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * V;
       if (!live || c >= a.C) continue;
-      float o[V];
+      float o[V], wp[V];
+      if constexpr (DELTA) factors<V>(kq, c, a.C, wp);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float D = NEXT ? gh[j][k] - x[j][k] * mu : gh[j][k];
         gh[j][k] = D;
         if constexpr (DELTA) {
-          const float f = sc * D * d[j][k];
-          ap[j][k] += f * q[j][k];
-          aq[j][k] += f * wp[j][k];
-          o[k] = rd * (sc * q[j][k] * wp[j][k] * D - d[j][k] * me);
+          at_[j][k] += sc * D * d[j][k];
+          o[k] = rd * (sc * wp[k] * D - d[j][k] * me);
         }
       }
       stv<V>(a.dx, a.x_dt, at + c, gh[j]);
@@ -317,6 +349,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
   }
 
   float* out = a.part + (int64_t)blockIdx.x * a.arrays * a.C;
+  float* dyn = reinterpret_cast<float*>(dyn4);
   auto leave = [&](float (&v)[NV][V], int which) {
     float* to = out + (int64_t)which * a.C;
     if constexpr (RB > 1) {  // add the block's row groups in order
@@ -336,20 +369,15 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const int c = (j * G + lane) * V + k;
-          if (c < a.C) to[c] = v[j][k];
-        }
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + lane) * V;
+        if (c < a.C) stv<V>(to, OW_DTYPE_F32, c, v[j]);
+      }
     }
   };
   int which = 0;
   if constexpr (NEXT) leave(an, which++);
-  if constexpr (DELTA) {
-    leave(ap, which++);
-    leave(aq, which++);
-  }
+  if constexpr (DELTA) leave(at_, which++);
 }
 
 // Rows longer than the kernels above hold: one block a row, read again for
@@ -454,9 +482,7 @@ __global__ void __launch_bounds__(256) norm_long_bwd_kernel(const Args a) {
       }
       stv<1>(a.dx, a.x_dt, at + c, D);
       if constexpr (DELTA) {
-        const float f = sc * D[0] * r.d;
-        out[(int64_t)which * a.C + c] += f * r.q;
-        out[(int64_t)(which + 1) * a.C + c] += f * r.wp;
+        out[(int64_t)which * a.C + c] += sc * D[0] * r.d;
         const float o[1] = {rd * (sc * r.q * r.wp * D[0] - r.d * me)};
         stv<1>(a.ddelta, a.d_dt, at + c, o);
       }
@@ -464,50 +490,59 @@ __global__ void __launch_bounds__(256) norm_long_bwd_kernel(const Args a) {
   }
 }
 
-// Column sums of the partial rows: 32 channels a block, 8 threads a channel,
-// added in the order of the parts.  ``apart``: array ``q_at`` is summed for
-// each group of its own.
+// Column sums of the partial rows, 32 channels a block, 32 threads a channel,
+// added in an order that the shape alone fixes.  blockIdx.y: 0 the next norm's
+// gradient, 1 the post-norm's (sum over the groups of q t), 2 + g group g's
+// gate (wp t).  One chain of loads is what this kernel takes, so each thread
+// has four of them in flight.
 struct SumArgs {
   const float* part;
-  int C, arrays, per_group;
+  int C, arrays, per_group, at_t;   // at_t: the array of t (-1: none)
   int64_t groups;
-  void* out[3];
-  int dt[3];
-  int q_at;        // the array that is summed group by group (-1: none)
+  const void* wp;
+  const void* q;
+  int q_rows, wp_dt, q_dt, wn_dt;
+  void* dnext;
+  void* dpost;
+  void* dgate;
 };
 
-__global__ void __launch_bounds__(256) norm_sum_kernel(const SumArgs a) {
-  __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) norm_sum_kernel(const SumArgs a) {
+  __shared__ float sh[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
-  // blockIdx.y: the arrays summed over all groups first, then (q_at, group)
-  int which = 0;
-  int64_t p0 = 0, p1 = a.groups * a.per_group, orow = 0;
-  const int whole = a.arrays - (a.q_at >= 0 ? 1 : 0);
-  for (int64_t y = blockIdx.y; y < whole + (a.q_at >= 0 ? a.groups : 0); y += gridDim.y) {
-    if (y < whole) {
-      which = (int)y;
-      p0 = 0;
-      p1 = a.groups * a.per_group;
-      orow = 0;
-    } else {
-      which = a.q_at;
-      orow = y - whole;
-      p0 = orow * a.per_group;
-      p1 = p0 + a.per_group;
+  const int64_t ys = a.at_t < 0 ? 1 : 2 + (a.q_rows ? a.groups : 0);
+  for (int64_t y = blockIdx.y; y < ys; y += gridDim.y) {
+    void* out = y == 0 ? a.dnext : y == 1 ? a.dpost : a.dgate;
+    if (!out) continue;
+    const int64_t stride = (int64_t)a.arrays * a.C;
+    const float* p = a.part + (y == 0 ? 0 : (int64_t)a.at_t * a.C) + c;
+    int64_t n = a.groups * a.per_group;
+    if (y >= 2) {
+      p += (y - 2) * a.per_group * stride;
+      n = a.per_group;
     }
-    float t = 0.f;
-    if (c < a.C && a.out[which])
-      for (int64_t p = p0 + ry; p < p1; p += 8) t += a.part[(p * a.arrays + which) * a.C + c];
-    sh[ry][cx] = t;
+    const bool weigh = y == 1 && a.q_rows > 1;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.C)
+      for (int64_t i = ry; i < n; i += 128) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int64_t r = i + 32 * k;
+          if (r < n) t[k] += p[r * stride] * (weigh ? ld1(a.q, a.q_dt, r / a.per_group * a.C + c) : 1.f);
+        }
+      }
     __syncthreads();
-    if (ry == 0 && c < a.C && a.out[which]) {
+    sh[ry][cx] = (t[0] + t[1]) + (t[2] + t[3]);
+    __syncthreads();
+    if (ry == 0 && c < a.C) {
       float v[1] = {0.f};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[0] += sh[i][cx];
-      stv<1>(a.out[which], a.dt[which], orow * a.C + c, v);
+      for (int i = 0; i < 32; ++i) v[0] += sh[i][cx];
+      if (y == 1 && a.q_rows == 1) v[0] *= ld1(a.q, a.q_dt, c);
+      if (y >= 2) v[0] *= ld1(a.wp, a.wp_dt, c);
+      stv<1>(out, y == 0 ? a.wn_dt : y == 1 ? a.wp_dt : a.q_dt, (y >= 2 ? (y - 2) * a.C : 0) + c, v);
     }
-    __syncthreads();
   }
 }
 
@@ -602,22 +637,34 @@ int split_bwd(int C, bool vec, F&& f) {
 
 bool too_long(int C, bool vec) { return C > (vec ? LONG_V : LONG_1); }
 
+int reserve(const void* kern, size_t smem) {
+  if (smem <= 48 * 1024) return OW_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) {
+    set_error("ow_norm: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    return OW_ERR_CUDA;
+  }
+  return OW_OK;
+}
+
 template <class F>
 int modes(bool delta, bool next, F&& f) {
   if (delta) return next ? f(std::true_type(), std::true_type()) : f(std::true_type(), std::false_type());
   return f(std::false_type(), std::true_type());
 }
 
-// Blocks of the backward: a few waves of the device, no more than there are
-// rows, shared out over the groups.
-void parts(const ow_norm_t* a, Args* k) {
+// The blocks: ``per_sm`` an SM, no more than there are rows, shared out over
+// the groups of rows with a gate of their own.
+void parts(const ow_norm_t* a, Args* k, int per_sm) {
   k->groups = a->gate_rows > 1 ? a->samples : 1;
   k->group_rows = k->rows / std::max<int64_t>(k->groups, 1);
-  const int64_t want = (int64_t)device_sm_count() * 4;
+  const int64_t want = (int64_t)device_sm_count() * per_sm;
   const int64_t per = std::max<int64_t>(1, want / std::max<int64_t>(k->groups, 1));
   k->per_group = (int)std::max<int64_t>(1, std::min<int64_t>(per, k->group_rows));
-  k->arrays = (a->next_w ? 1 : 0) + (a->delta ? 2 : 0);
+  k->arrays = (a->next_w ? 1 : 0) + (a->delta ? 1 : 0);
 }
+
+constexpr int FWD_PER_SM = 6, BWD_PER_SM = 3;  // what the registers (40 and 80 a thread) let run at once
 
 }  // namespace
 }  // namespace ow
@@ -630,7 +677,7 @@ size_t ow_norm_bwd_workspace_size(const ow_norm_t* a) {
   clear_error();
   if (check(a) != OW_OK) return 0;
   Args k = base(a);
-  parts(a, &k);
+  parts(a, &k, BWD_PER_SM);
   return (size_t)k.groups * k.per_group * k.arrays * k.C * sizeof(float) + 256;
 }
 
@@ -646,15 +693,20 @@ int ow_norm_fwd(const ow_norm_t* a, void* stream) {
   const void* outs[] = {k.h, k.n};
   const bool vec = vectors(k, outs, 2);
   const cudaStream_t st = (cudaStream_t)stream;
-  const int sms = device_sm_count();
+  parts(a, &k, FWD_PER_SM);
   return modes(delta, next, [&](auto D, auto N) -> int {
     if (too_long(k.C, vec)) {
-      launch(norm_long_fwd_kernel<D.value, N.value>, (int)std::min<int64_t>(k.rows, sms * 8), 256, 0, st, k);
+      const int64_t grid = std::min<int64_t>(k.rows, (int64_t)device_sm_count() * FWD_PER_SM);
+      launch(norm_long_fwd_kernel<D.value, N.value>, (int)grid, 256, 0, st, k);
     } else {
       OW_RETURN_IF(split_fwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
         constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
-        const int grid = (int)std::min<int64_t>((k.rows + RB - 1) / RB, sms * 8);
-        launch(norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value>, grid, T, 0, st, k);
+        k.per_group = (int)std::min<int64_t>(k.per_group, (k.group_rows + RB - 1) / RB);
+        OW_CHECK_ARG(k.groups * k.per_group < (1LL << 31), "ow_norm_fwd: too many samples");
+        const size_t smem = (size_t)k.C * sizeof(float) * (D.value + N.value);
+        auto kern = norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value>;
+        OW_RETURN_IF(reserve((const void*)kern, smem));
+        launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
         return OW_OK;
       }));
     }
@@ -672,7 +724,7 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
   OW_CHECK_ARG(k.rows == 0 || (g->dx && (!next || g->dn) && (!delta || g->ddelta) && (g->dh || next) &&
                                (!delta || k.rd) && (!next || k.rh)),
                "ow_norm_bwd: a pointer is NULL");
-  parts(a, &k);
+  parts(a, &k, BWD_PER_SM);
   const size_t need = ow_norm_bwd_workspace_size(a);
   if (!a->workspace || a->workspace_bytes < need) {
     set_error("ow_norm_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
@@ -691,8 +743,11 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
     } else {
       OW_RETURN_IF(split_bwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
         constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
-        const size_t smem = RB > 1 ? (size_t)RB * k.C * sizeof(float) : 0;
-        launch(norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value>, (int)grid, T, smem, st, k);
+        k.per_group = (int)std::min<int64_t>(k.per_group, std::max<int64_t>(1, (k.group_rows + RB - 1) / RB));
+        const size_t smem = (size_t)k.C * sizeof(float) * std::max<int>(D.value + N.value, RB > 1 ? RB : 0);
+        auto kern = norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value>;
+        OW_RETURN_IF(reserve((const void*)kern, smem));
+        launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
         return OW_OK;
       }));
     }
@@ -701,17 +756,14 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
   }));
   SumArgs s{};
   s.part = k.part; s.C = k.C; s.arrays = k.arrays; s.per_group = k.per_group; s.groups = k.groups;
-  int which = 0;
-  if (next) { s.out[which] = g->dnext; s.dt[which++] = a->next_dtype; }
-  s.q_at = -1;
-  if (delta) {
-    s.out[which] = g->dpost; s.dt[which++] = a->post_dtype;
-    s.out[which] = a->gate_rows ? g->dgate : nullptr; s.dt[which] = a->gate_dtype;
-    if (a->gate_rows > 1) s.q_at = which;
-    ++which;
-  }
-  const int64_t ys = s.arrays - (s.q_at >= 0 ? 1 : 0) + (s.q_at >= 0 ? s.groups : 0);
-  launch(norm_sum_kernel, dim3((k.C + 31) / 32, (unsigned)std::min<int64_t>(ys, 32768)), 256, 0, st, s);
+  s.at_t = delta ? (next ? 1 : 0) : -1;
+  s.wp = k.wp; s.q = k.q; s.q_rows = k.q_rows;
+  s.wp_dt = k.wp_dt; s.q_dt = k.q_dt; s.wn_dt = k.wn_dt;
+  s.dnext = next ? g->dnext : nullptr;
+  s.dpost = delta ? g->dpost : nullptr;
+  s.dgate = a->gate_rows ? g->dgate : nullptr;
+  const int64_t ys = s.at_t < 0 ? 1 : 2 + (s.q_rows ? s.groups : 0);
+  launch(norm_sum_kernel, dim3((k.C + 31) / 32, (unsigned)std::min<int64_t>(ys, 32768)), 1024, 0, st, s);
   OW_CHECK_LAUNCH("norm_sum_kernel");
   return OW_OK;
 }

@@ -9,9 +9,10 @@
 // Layout.  Every tensor's state starts on a multiple of 256 slots of one flat
 // array, so a block of 256 slots belongs to one tensor and one warp does one
 // block: 8 elements a lane in two groups of four, each array read and written
-// with whole 128-byte lines.  A table of one int per block names the tensor;
-// the parameters' and gradients' pointers travel in the launch itself, so
-// gradients that move from step to step cost no copy.
+// with whole 128-byte lines.  A table tells each block's tensor, its place in it
+// and how much of it is used; a warp reads the record of its next block while it
+// works on this one.  The parameters' and gradients' pointers travel in the
+// launch itself, so gradients that move from step to step cost no copy.
 //
 // 8-bit moments.  A block holds 256 e4m3 codes and one f32 scale = max / 448.
 // They are rounded stochastically, by a hash of (slot, step): with b2 = 0.999
@@ -46,9 +47,7 @@ struct Ptrs {
 };
 
 struct Tables {
-  const int64_t* slot;     // [tensors + 1] first slot of each tensor
-  const int64_t* numel;    // [tensors]
-  const int32_t* tensor;   // [blocks] tensor of each block
+  const int4* block;       // [blocks]: tensor, block of the tensor, elements in use
   int t0;                  // first tensor of this launch
   int64_t blk0, nblk;      // its blocks
 };
@@ -61,7 +60,7 @@ struct Ctl {
 };
 
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float (&o)[4]) {
+__device__ __forceinline__ void load4(const T* p, int i, int n, bool vec, float (&o)[4]) {
   if (vec && i + 4 <= n) {
     if constexpr (sizeof(T) == 4) {
       const float4 v = *reinterpret_cast<const float4*>(p + i);
@@ -79,7 +78,7 @@ __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float (&v)[4]) {
+__device__ __forceinline__ void store4(T* p, int i, int n, bool vec, const float (&v)[4]) {
   if (vec && i + 4 <= n) {
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
@@ -102,6 +101,12 @@ __device__ __forceinline__ bool aligned4(const void* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
 
+__device__ __forceinline__ float fast_sqrt(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -109,9 +114,13 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // Two 16-bit numbers from (slot, step), as the 20 bits below an e4m3 mantissa
-// see them: 16 random bits and half of the last one.
-__device__ __forceinline__ void random20(int64_t slot, uint32_t step, uint32_t& r1, uint32_t& r2) {
-  uint32_t h = (uint32_t)slot * 0x9E3779B1u + (uint32_t)((uint64_t)slot >> 32) * 0x85EBCA6Bu + step * 0xC2B2AE35u;
+// see them: 16 random bits and half of the last one.  ``seed``: of the block's
+// first slot; the slots of a block differ in the low 8 bits only.
+__device__ __forceinline__ uint32_t random_seed(int64_t slot, uint32_t step) {
+  return (uint32_t)slot * 0x9E3779B1u + (uint32_t)((uint64_t)slot >> 32) * 0x85EBCA6Bu + step * 0xC2B2AE35u;
+}
+__device__ __forceinline__ void random20(uint32_t seed, uint32_t e, uint32_t& r1, uint32_t& r2) {
+  uint32_t h = seed + e * 0x9E3779B1u;
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;
   h ^= h >> 16;
@@ -163,14 +172,20 @@ __global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant
   const float lr = a.lr_ptr ? *a.lr_ptr : a.lr;
   const float decay = 1.f - lr * a.wd;
   float t_have = -1.f, alpha = 0.f, rc2 = 0.f;
-  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.tab.nblk; b += (int64_t)gridDim.x * WARPS) {
+  const int64_t stride = (int64_t)gridDim.x * WARPS;
+  int64_t b = (int64_t)blockIdx.x * WARPS + warp;
+  int4 next = b < a.tab.nblk ? a.tab.block[a.tab.blk0 + b] : make_int4(0, 0, 0, 0);
+  for (; b < a.tab.nblk; b += stride) {
+    const int4 rec = next;
+    if (b + stride < a.tab.nblk) next = a.tab.block[a.tab.blk0 + b + stride];
     const int64_t blk = a.tab.blk0 + b;
-    const int ti = a.tab.tensor[blk];
+    const int ti = rec.x;
     const T* g = reinterpret_cast<const T*>(ptr.g[ti - a.tab.t0]);
     if (!g) continue;  // no gradient: this tensor takes no step
-    T* p = reinterpret_cast<T*>(ptr.p[ti - a.tab.t0]);
+    g += (int64_t)rec.y * BLK;
+    T* p = reinterpret_cast<T*>(ptr.p[ti - a.tab.t0]) + (int64_t)rec.y * BLK;
     const int64_t slot = blk * BLK;
-    const int64_t n = a.tab.numel[ti], base = slot - a.tab.slot[ti];
+    const int n = rec.z;
     const float t = a.steps[ti] + 1.f;
     const bool vec = aligned4<T>(p) && aligned4<T>(g);
     float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
@@ -179,14 +194,14 @@ __global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int e = j * 128 + lane * 4;
-      load4(p, base + e, n, vec, pv[j]);
-      load4(g, base + e, n, vec, gv[j]);
+      load4(p, e, n, vec, pv[j]);
+      load4(g, e, n, vec, gv[j]);
       if constexpr (EIGHT) {
         mc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.m + slot + e);
         vc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.v + slot + e);
       } else {
-        load4((const float*)a.m, slot + e, slot + BLK, true, mv[j]);
-        load4((const float*)a.v, slot + e, slot + BLK, true, vv[j]);
+        load4((const float*)a.m + slot, e, BLK, true, mv[j]);
+        load4((const float*)a.v + slot, e, BLK, true, vv[j]);
       }
     }
     if constexpr (EIGHT) {
@@ -213,7 +228,7 @@ __global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant
         const float gg = __fmul_rn(gv[j][k], coef);
         const float m = __fadd_rn(__fmul_rn(a.b1, mv[j][k]), __fmul_rn(a.b1c, gg));
         const float v = __fadd_rn(__fmul_rn(a.b2, vv[j][k]), __fmul_rn(__fmul_rn(a.b2c, gg), gg));
-        pv[j][k] = pv[j][k] * decay - alpha * (m / (sqrtf(v) * rc2 + a.eps));
+        pv[j][k] = pv[j][k] * decay - alpha * __fdividef(m, fast_sqrt(v) * rc2 + a.eps);
         mv[j][k] = m;
         vv[j][k] = v;
         if constexpr (EIGHT) {
@@ -221,26 +236,27 @@ __global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant
           vmax = fmaxf(vmax, v);
         }
       }
-      store4(p, base + j * 128 + lane * 4, n, vec, pv[j]);
+      store4(p, j * 128 + lane * 4, n, vec, pv[j]);
       if constexpr (!EIGHT) {
-        store4((float*)a.m, slot + j * 128 + lane * 4, slot + BLK, true, mv[j]);
-        store4((float*)a.v, slot + j * 128 + lane * 4, slot + BLK, true, vv[j]);
+        store4((float*)a.m + slot, j * 128 + lane * 4, BLK, true, mv[j]);
+        store4((float*)a.v + slot, j * 128 + lane * 4, BLK, true, vv[j]);
       }
     }
     if constexpr (EIGHT) {
       mmax = warp_max(mmax);
       vmax = warp_max(vmax);
+      const uint32_t seed = random_seed(slot, (uint32_t)t) + lane * 4 * 0x9E3779B1u;
       const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
+      const uint32_t least = vinv > 0.f ? 1u : 0u;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t om = 0, ov = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t r1, r2;
-          random20(slot + j * 128 + lane * 4 + k, (uint32_t)t, r1, r2);
-          const uint32_t qm = hold8(mv[j][k], minv, r1) | (mv[j][k] < 0.f ? 128u : 0u);
-          uint32_t qv = hold8(vv[j][k], vinv, r2);
-          if (qv == 0 && vv[j][k] > 0.f && vinv > 0.f) qv = 1;
+          random20(seed, j * 128 + k, r1, r2);
+          const uint32_t qm = hold8(mv[j][k], minv, r1) | (__float_as_uint(mv[j][k]) >> 24 & 128u);
+          const uint32_t qv = max(hold8(vv[j][k], vinv, r2), vv[j][k] > 0.f ? least : 0u);
           om |= qm << (8 * k);
           ov |= qv << (8 * k);
         }
@@ -288,16 +304,19 @@ template <typename T, int MAXT>
 __global__ void __launch_bounds__(WARPS * 32) grad_norm_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const NormArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double s = 0.0;
-  for (int64_t b = (int64_t)blockIdx.x * WARPS + warp; b < a.tab.nblk; b += (int64_t)gridDim.x * WARPS) {
-    const int64_t blk = a.tab.blk0 + b;
-    const int ti = a.tab.tensor[blk];
-    const T* g = reinterpret_cast<const T*>(ptr.g[ti - a.tab.t0]);
+  const int64_t stride = (int64_t)gridDim.x * WARPS;
+  int64_t b = (int64_t)blockIdx.x * WARPS + warp;
+  int4 next = b < a.tab.nblk ? a.tab.block[a.tab.blk0 + b] : make_int4(0, 0, 0, 0);
+  for (; b < a.tab.nblk; b += stride) {
+    const int4 rec = next;
+    if (b + stride < a.tab.nblk) next = a.tab.block[a.tab.blk0 + b + stride];
+    const T* g = reinterpret_cast<const T*>(ptr.g[rec.x - a.tab.t0]);
     if (!g) continue;
-    const int64_t n = a.tab.numel[ti], base = blk * BLK - a.tab.slot[ti];
+    g += (int64_t)rec.y * BLK;
     const bool vec = aligned4<T>(g);
     float v[2][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) load4(g, base + j * 128 + lane * 4, n, vec, v[j]);
+    for (int j = 0; j < 2; ++j) load4(g, j * 128 + lane * 4, rec.z, vec, v[j]);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -355,7 +374,7 @@ int check(const ow_adamw_t* a) {
   OW_CHECK_ARG(a != nullptr, "ow_adamw: args is NULL");
   OW_CHECK_ARG(a->tensors > 0, "ow_adamw: tensors must be positive (got %d)", a->tensors);
   OW_CHECK_ARG(a->params && a->grads && a->slots, "ow_adamw: params, grads or slots is NULL");
-  OW_CHECK_ARG(a->dev_slots && a->dev_numel && a->dev_block_tensor && a->control, "ow_adamw: a device table is NULL");
+  OW_CHECK_ARG(a->dev_blocks && a->control, "ow_adamw: a device table is NULL");
   if (a->dtype != OW_DTYPE_F32 && a->dtype != OW_DTYPE_BF16 && a->dtype != OW_DTYPE_F16) {
     set_error("ow_adamw: parameters must be float32, bfloat16 or float16 (dtype code %d)", a->dtype);
     return OW_ERR_UNSUPPORTED;
@@ -371,8 +390,7 @@ template <class F>
 int each_launch(const ow_adamw_t* a, F&& f) {
   for (int t0 = 0; t0 < a->tensors; t0 += MAX_MANY) {
     const int n = std::min(MAX_MANY, a->tensors - t0);
-    Tables tab{a->dev_slots, a->dev_numel, a->dev_block_tensor, t0, a->slots[t0] / BLK,
-               (a->slots[t0 + n] - a->slots[t0]) / BLK};
+    Tables tab{(const int4*)a->dev_blocks, t0, a->slots[t0] / BLK, (a->slots[t0 + n] - a->slots[t0]) / BLK};
     const bool end = t0 + n == a->tensors;
     auto fill = [&](auto& ptr) {
       for (int i = 0; i < n; ++i) {

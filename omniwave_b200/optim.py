@@ -77,11 +77,14 @@ class _Bucket:
         self.slots = slots
         blocks = total // BLOCK
         self._slots = (ctypes.c_int64 * len(slots))(*slots)
-        numel = torch.tensor([p.numel() for p in params], dtype=torch.int64)
-        counts = (torch.tensor(slots[1:]) - torch.tensor(slots[:-1])) // BLOCK
-        self.dev_slots = torch.tensor(slots, dtype=torch.int64, device=dev)
-        self.dev_numel = numel.to(dev)
-        self.dev_tensor = torch.repeat_interleave(torch.arange(len(params), dtype=torch.int32), counts).to(dev)
+        # one record for each block: its tensor, its place in the tensor, its elements in use
+        numel = torch.tensor([p.numel() for p in params])
+        first = torch.tensor(slots[:-1]) // BLOCK
+        counts = torch.tensor(slots[1:]) // BLOCK - first
+        tensor = torch.repeat_interleave(torch.arange(len(params)), counts)
+        place = torch.arange(blocks) - first[tensor]
+        used = (numel[tensor] - place * BLOCK).clamp(max=BLOCK)
+        self.blocks = torch.stack([tensor, place, used, torch.zeros_like(used)], 1).to(torch.int32).to(dev)
         self.control = torch.zeros(_lib.ADAMW_CONTROL_BYTES, dtype=torch.uint8, device=dev)
         state = torch.float32 if bits == 32 else torch.float8_e4m3fn
         self.held: dict[str, Tensor] = {
@@ -97,8 +100,7 @@ class _Bucket:
         self._p, self._g = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)()
         self.args = _lib.AdamW(
             n, _lib.DTYPE_CODE[self.dtype], ctypes.addressof(self._p), ctypes.addressof(self._g),
-            ctypes.addressof(self._slots), self.dev_slots.data_ptr(), self.dev_numel.data_ptr(),
-            self.dev_tensor.data_ptr(), self.control.data_ptr(), bits, h["exp_avg"].data_ptr(),
+            ctypes.addressof(self._slots), self.blocks.data_ptr(), self.control.data_ptr(), bits, h["exp_avg"].data_ptr(),
             h["exp_avg_sq"].data_ptr(), _lib.ptr(h.get("exp_avg_scale")), _lib.ptr(h.get("exp_avg_sq_scale")),
             h["step"].data_ptr())
         self.partials = _lib.load().ow_grad_norm_partials(self.args)

@@ -2,11 +2,12 @@
 
 Tolerances count roundings.  u = 2^-24 is half a step of f32.  m and v take
 three roundings and one of a rounded constant each, relative to the magnitudes
-they are summed from: 4 u.  The update lr/c1 m/(sqrt(v) rc2 + eps) adds the
-constants' (lr, betas and their logarithms: 4), two corrections of two
-roundings and an expm1f of one step each (6), sqrt, product, sum, two
-divisions and products (6), and halves v's: 20 u of alpha M / denom with
-M = b1 |m| + (1 - b1) |g|; the decay and the last subtraction take 4 u of |p|.
+they are summed from: 4 u.  Of the update alpha m / (sqrt(v) rc2 + eps), with
+M = b1 |m| + (1 - b1) |g|: alpha = lr / (1 - b1^t) takes 6 u (lr, log b1 and its
+product, expm1f's one step = 2 u, the division), rc2 half of 4 u and rsqrtf's two
+steps = 4 u, sqrt(v) half of v's 4 u and its own step = 2 u, product and sum 2 u,
+the division's two steps = 4 u, the last product 1 u, and m itself 4 u: 27 u of
+alpha M / denom.  The decay and the last subtraction take 4 u of |p|.
 Clipping multiplies g once more, by a coefficient rounded once: 2 u on g, 4 u
 on v.  A 16-bit parameter is rounded once more, by half a step of its type.
 """
@@ -53,7 +54,7 @@ def _step64(p, g, m, v, t, clip=1.0, lr=LR, wd=WD):
     denom = (v / (1 - B2 ** t)).sqrt() + EPS
     alpha = lr / (1 - B1 ** t)
     pn = p * (1 - lr * wd) - alpha * m / denom
-    return pn, m, v, 4 * U * p.abs() + 22 * U * alpha * ms / denom, 6 * U * ms, 8 * U * vs
+    return pn, m, v, 4 * U * p.abs() + 30 * U * alpha * ms / denom, 6 * U * ms, 8 * U * vs
 
 
 @pytest.mark.parametrize("dtype", [F32, BF, HF], ids=["f32", "bf16", "f16"])

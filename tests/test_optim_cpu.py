@@ -62,7 +62,7 @@ def test_train_step_refuses_unknown_optimizers():
 
 def _args(**over):
     keep = [(ctypes.c_void_p * 2)(16, 16), (ctypes.c_void_p * 2)(16, None), (ctypes.c_int64 * 3)(0, 256, 1024)]
-    a = _lib.AdamW(2, 0, *[ctypes.addressof(k) for k in keep], 16, 16, 16, 16, 32, 16, 16, None, None, 16,
+    a = _lib.AdamW(2, 0, *[ctypes.addressof(k) for k in keep], 16, 16, 32, 16, 16, None, None, 16,
                    1e-3, 0.9, 0.999, 1e-8, 0.0, None, None, 0)
     for k, v in over.items():
         setattr(a, k, v)
@@ -72,7 +72,7 @@ def _args(**over):
 @pytest.mark.parametrize("over,status,msg", [
     (dict(tensors=0), 1, "tensors must be positive"),
     (dict(params=None), 1, "NULL"),
-    (dict(dev_slots=None), 1, "device table"),
+    (dict(dev_blocks=None), 1, "device table"),
     (dict(control=None), 1, "device table"),
     (dict(dtype=1), 2, "float32, bfloat16 or float16"),
     (dict(state_bits=4), 1, "state_bits"),
