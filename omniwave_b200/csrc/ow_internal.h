@@ -114,6 +114,9 @@ int device_sm_count();
 // error message.
 int encode_tiled_map(void* map, bool bf16, int rank, const void* base, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box, const char* who);
+// The same for f32, bf16 or f16, with the 128-byte or the 64-byte swizzle.
+int encode_tiled_map64(void* map, int dtype, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                       const uint32_t* box, bool swizzle64, const char* who);
 
 // RMSNorm backward of block mode from the gradient w.r.t. the normalised
 // input (``dxn``, f32 or the 16-bit compute type; CUDA cores, row-wise).  norm_bwd_take() carves its partials from

@@ -9,9 +9,9 @@
 // the forward, dz in dx), MN-major when they run across (W in dx, dz and x in
 // dW), so nothing is transposed in memory.
 //
-// Persistent, one CTA per SM, 320 threads: 8 epilogue warps, one thread that
-// issues the copies and one that issues the tcgen05.mma (M = 128, N = 64, 128
-// or 256).  A ring of 64-wide k blocks feeds the MMA; the accumulator is
+// Persistent, one CTA per SM, 576 threads: 16 epilogue warps, one thread that
+// issues the copies and one that issues the tcgen05.mma (M = 128, N = 64 or 128,
+// or M = 256, N = 256).  A ring of 64-wide k blocks feeds the MMA; the accumulator is
 // double-buffered in TMEM, so a tile's epilogue runs under the next tile's
 // products.  Tiles are walked in patches of 12 row blocks, so that the SMs at
 // work share A and B blocks in L2.
@@ -44,27 +44,33 @@ namespace {
 using namespace sm100;
 
 constexpr int TM = 128, KE = 64;
-constexpr int EPI_WARPS = 8, PROD_W = 8, MMA_W = 9, THREADS = 320;
+constexpr int EPI_WARPS = 16, PROD_W = 16, MMA_W = 17, THREADS = 576;
 constexpr int A_ST = TM * 128;
-constexpr int STG_W = 4096;  // a warp's staging: 2 KB for the residual, 2 KB for what it stores
+constexpr int BLOCK_ST = 2048;  // a 32 x 32 block of 16-bit values, or half a block of f32, in staging
 constexpr int PATCH = 12;
 
 // BN columns of a tile; CG CTAs share it (2: 256 rows, BN / 2 rows of B each).
 template <int BN, int CG>
 struct GC {
   static constexpr int B_ROWS = BN / CG;
-  static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
+  static constexpr int CW = BN == 256 ? 64 : 32;   // columns of an epilogue warp
+  static constexpr int NBLK = CW / 32;
+  static constexpr int ACTIVE = 4 * (BN / CW);     // epilogue warps at work
+  static constexpr int STG_W = NBLK * BLOCK_ST;
+  static constexpr int STAGES = BN == 256 ? 5 : BN == 128 ? 6 : 8;
   static constexpr int B_ST = B_ROWS * 128;
   static constexpr int OFF_B = STAGES * A_ST;
   static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
-  static constexpr int OFF_BAR = OFF_STG + EPI_WARPS * STG_W;
-  static constexpr int NBAR = 2 * STAGES + 4 + 1;  // full, empty, tfull[2], tfree[2], probe
+  static constexpr int OFF_BAR = OFF_STG + ACTIVE * STG_W;
+  static constexpr int NBAR = 2 * STAGES + 4 + 1 + EPI_WARPS;  // full, empty, tfull[2], tfree[2], probe, residual
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
   static_assert(SMEM <= 232448, "shared memory budget");
 };
 
-// What happens to a block of D on its way out.
+// What happens to a block of D on its way out.  Arrays whose rows TMA can
+// address (vz, vr, vo) move as 32 x 32 boxes between staging and memory, the
+// others element by element.
 struct Epi {
   const void* bias;
   int bias_dt;
@@ -77,7 +83,7 @@ struct Epi {
   void* out;         // 16-bit, or f32 (partials, an f32 weight gradient)
   int64_t ldo;
   int out32;
-  int vz, vr, vo;    // rows take 16-byte accesses
+  int vz, vr, vo;
 };
 
 struct GemmArgs {
@@ -86,7 +92,6 @@ struct GemmArgs {
   int kblocks;       // 64-wide blocks of k
   int mtiles, ntiles;
   int splits;        // of the k blocks; with more than one, out is the partials
-  int64_t part_stride;
   Epi e;
   int* fault;
   uint32_t probe_ns;
@@ -117,7 +122,9 @@ __device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void arrive_in(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  // release at the scope of the CTA: what it orders is this thread's reads of
+  // TMEM (a release at cluster scope waits for every global store before it)
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A load into this CTA that completes on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
@@ -190,24 +197,32 @@ __device__ __forceinline__ float normal_cdf(float z, float& bell) {
   return z > 0.f ? 1.f - tail : tail;
 }
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-  if (act == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if (act == OW_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
-  if (act == OW_ACT_GELU) {
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+  if constexpr (ACT == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if constexpr (ACT == OW_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
+  if constexpr (ACT == OW_ACT_GELU) {
     float bell;
     return z * normal_cdf(z, bell);
   }
   return z;
 }
+__device__ __forceinline__ float act_fwd(float z, int act) {
+  return act == OW_ACT_RELU   ? act_fwd<OW_ACT_RELU>(z)
+         : act == OW_ACT_SILU ? act_fwd<OW_ACT_SILU>(z)
+         : act == OW_ACT_GELU ? act_fwd<OW_ACT_GELU>(z)
+                              : z;
+}
 
 // act'(z)
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == OW_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
-  if (act == OW_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == OW_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
+  if constexpr (ACT == OW_ACT_SILU) {
     const float s = __fdividef(1.f, 1.f + __expf(-z));
     return s * (1.f + z * (1.f - s));
   }
-  if (act == OW_ACT_GELU) {
+  if constexpr (ACT == OW_ACT_GELU) {
     float bell;
     const float cdf = normal_cdf(z, bell);
     return fmaf(z * 0.39894228040143268f, bell, cdf);
@@ -235,104 +250,93 @@ __device__ __forceinline__ uint32_t pk(float a, float b, int bf16) { return bf16
 __device__ __forceinline__ float2 upk(uint32_t v, int bf16) { return bf16 ? unpack2<true>(v) : unpack2<false>(v); }
 
 // ---------------------------------------------------------------- epilogue
-// A warp's 32 rows x 32 columns, a row a lane, through 2 KB of staging
-// (16-byte units rotated by the row pair: conflict free both ways) to or from
-// 64-byte row segments.
+// A warp's block of 32 rows, a row a lane: 64-byte rows in staging under the
+// 64-byte swizzle of the TMA boxes that carry it (conflict free for a warp that
+// writes its rows 16 bytes at a time).
 __device__ __forceinline__ uint32_t stg_at(int row, int u) { return row * 64 + ((u ^ ((row >> 1) & 3)) << 4); }
 
-__device__ __forceinline__ void store_block16(unsigned char* stg, const float (&v)[32], int bf16, void* out, int64_t ld,
-                                              int64_t m0, int64_t M, int n0, int N, bool vec) {
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int c0, int c1, int c2, const void* src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(src))
+               : "memory");
+}
+
+// The lanes' rows of 32 16-bit values, staged and sent to rows m0.. and
+// columns n0.. of an array.  The caller waits for the copy before it writes
+// the staging again.
+__device__ __forceinline__ void put16(unsigned char* stg, const float (&v)[32], int bf16, const CUtensorMap* map, bool boxes,
+                                      void* out, int64_t ld, int64_t m0, int64_t M, int n0, int N) {
   const int lane = threadIdx.x & 31;
-  __syncwarp();
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     *reinterpret_cast<uint4*>(stg + stg_at(lane, u)) =
         make_uint4(pk(v[8 * u], v[8 * u + 1], bf16), pk(v[8 * u + 2], v[8 * u + 3], bf16),
                    pk(v[8 * u + 4], v[8 * u + 5], bf16), pk(v[8 * u + 6], v[8 * u + 7], bf16));
-  __syncwarp();
-  uint16_t* o = reinterpret_cast<uint16_t*>(out);
-  if (vec && n0 + 32 <= N) {
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int row = it * 8 + (lane >> 2), u = lane & 3;
-      const uint4 w = *reinterpret_cast<const uint4*>(stg + stg_at(row, u));
-      if (m0 + row < M) *reinterpret_cast<uint4*>(o + (m0 + row) * ld + n0 + 8 * u) = w;
+  if (boxes) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(map, n0, (int)m0, 0, stg);
+      bulk_commit();
     }
   } else {
+    __syncwarp();
+    uint16_t* o = reinterpret_cast<uint16_t*>(out);
     for (int row = 0; row < 32 && m0 + row < M; ++row)
       if (n0 + lane < N)
         o[(m0 + row) * ld + n0 + lane] =
             *reinterpret_cast<const uint16_t*>(stg + stg_at(row, lane >> 3) + (lane & 7) * 2);
+    fence_proxy_async_smem();  // before a copy writes the staging again
+    __syncwarp();
   }
 }
 
-__device__ __forceinline__ void store_block32(unsigned char* stg, const float (&v)[32], float* out, int64_t ld, int64_t m0,
-                                              int64_t M, int n0, int N, bool vec) {
+// The same in f32, half a block of 16 columns at a time; waits for its copies.
+__device__ __forceinline__ void put32(unsigned char* stg, const float (&v)[32], const CUtensorMap* map, bool boxes, float* out,
+                                      int64_t ld, int64_t m0, int64_t M, int n0, int N, int split) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    __syncwarp();
+    const int nb = n0 + 16 * h;
+    if (nb >= N) break;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       *reinterpret_cast<float4*>(stg + stg_at(lane, u)) =
           make_float4(v[16 * h + 4 * u], v[16 * h + 4 * u + 1], v[16 * h + 4 * u + 2], v[16 * h + 4 * u + 3]);
-    __syncwarp();
-    const int nb = n0 + 16 * h;
-    if (vec && nb + 16 <= N) {
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int row = it * 8 + (lane >> 2), u = lane & 3;
-        const float4 w = *reinterpret_cast<const float4*>(stg + stg_at(row, u));
-        if (m0 + row < M) *reinterpret_cast<float4*>(out + (m0 + row) * ld + nb + 4 * u) = w;
+    if (boxes) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(map, nb, (int)m0, split, stg);
+        bulk_commit();
+        bulk_wait_read();
       }
     } else {
+      __syncwarp();
       for (int row = lane >> 4; row < 32 && m0 + row < M; row += 2) {
         const int c = lane & 15;
         if (nb + c < N) out[(m0 + row) * ld + nb + c] = *reinterpret_cast<const float*>(stg + stg_at(row, c >> 2) + (c & 3) * 4);
       }
+      fence_proxy_async_smem();
     }
+    __syncwarp();
   }
 }
 
-// The residual's 64-byte row segments of a block, as the coalesced loads of
-// the warp (kept in registers until the block is due).
-struct ResBlock {
-  uint4 w[4];
-};
-__device__ __forceinline__ void fetch_res(ResBlock& r, const Epi& e, int64_t m0, int64_t M, int n0, int N) {
+// This lane's row of the staged residual.
+__device__ __forceinline__ void take_res(const unsigned char* stg, uint4 (&r)[4]) {
   const int lane = threadIdx.x & 31;
-  if (!e.res || !e.vr || n0 + 32 > N) return;
-  const uint16_t* p = reinterpret_cast<const uint16_t*>(e.res);
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int row = it * 8 + (lane >> 2), u = lane & 3;
-    r.w[it] = m0 + row < M ? *reinterpret_cast<const uint4*>(p + (m0 + row) * e.ldr + n0 + 8 * u) : make_uint4(0, 0, 0, 0);
-  }
+  for (int u = 0; u < 4; ++u) r[u] = *reinterpret_cast<const uint4*>(stg + stg_at(lane, u));
 }
-__device__ __forceinline__ void add_res(float (&v)[32], const ResBlock& r, unsigned char* stg, const Epi& e, int64_t m0,
-                                        int64_t M, int n0, int N) {
+// A residual whose rows TMA cannot address, staged element by element.
+__device__ __forceinline__ void stage_res(unsigned char* stg, const Epi& e, int64_t m0, int64_t M, int n0, int N) {
   const int lane = threadIdx.x & 31;
+  for (int row = 0; row < 32; ++row)
+    *reinterpret_cast<uint16_t*>(stg + stg_at(row, lane >> 3) + (lane & 7) * 2) =
+        m0 + row < M && n0 + lane < N ? reinterpret_cast<const uint16_t*>(e.res)[(m0 + row) * e.ldr + n0 + lane] : 0;
   __syncwarp();
-  if (e.vr && n0 + 32 <= N) {
-#pragma unroll
-    for (int it = 0; it < 4; ++it) *reinterpret_cast<uint4*>(stg + stg_at(it * 8 + (lane >> 2), lane & 3)) = r.w[it];
-  } else {
-    for (int row = 0; row < 32; ++row)
-      *reinterpret_cast<uint16_t*>(stg + stg_at(row, lane >> 3) + (lane & 7) * 2) =
-          m0 + row < M && n0 + lane < N ? reinterpret_cast<const uint16_t*>(e.res)[(m0 + row) * e.ldr + n0 + lane] : 0;
-  }
-  __syncwarp();
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const uint4 w = *reinterpret_cast<const uint4*>(stg + stg_at(lane, u));
-    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = upk(q[k], e.bf16);
-      v[8 * u + 2 * k] += f.x;
-      v[8 * u + 2 * k + 1] += f.y;
-    }
-  }
 }
 
 __device__ __forceinline__ void add_bias(float (&v)[32], const Epi& e, int n0, int N) {
@@ -362,30 +366,6 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const Epi& e, int n0, i
   }
 }
 
-__device__ __forceinline__ void finish_block(float (&v)[32], const ResBlock& r, unsigned char* stg, const Epi& e, int64_t m0,
-                                             int64_t M, int n0, int N) {
-  if (e.bias) add_bias(v, e, n0, N);
-  if (e.z) {
-    float z[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] = keep_z(v[i], e.bf16);
-    store_block16(stg + 2048, z, e.bf16, e.z, e.ldz, m0, M, n0, N, e.vz);
-  }
-  if (e.act == OW_ACT_RELU) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_RELU);
-  } else if (e.act == OW_ACT_SILU) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_SILU);
-  } else if (e.act == OW_ACT_GELU) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = act_fwd(v[i], OW_ACT_GELU);
-  }
-  if (e.res) add_res(v, r, stg, e, m0, M, n0, N);
-  if (e.out32) store_block32(stg + 2048, v, (float*)e.out, e.ldo, m0, M, n0, N, e.vo);
-  else store_block16(stg + 2048, v, e.bf16, e.out, e.ldo, m0, M, n0, N, e.vo);
-}
-
 // ---------------------------------------------------------------- GEMM
 struct Unit {
   int mt, nt, split, kb0, kb1;
@@ -407,9 +387,12 @@ __device__ __forceinline__ Unit unit_of(const GemmArgs& a, int u) {
   return r;
 }
 
-template <int BN, int CG, bool AMN, bool BMN, bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap, const GemmArgs a) {
+struct Maps {
+  CUtensorMap a, b, out, z, res;
+};
+
+template <int BN, int CG, bool AMN, bool BMN, bool BF16, int ACT>
+__global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant__ Maps maps, const GemmArgs a) {
   using C = GC<BN, CG>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -418,6 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tfree = tfull + 2;
   uint64_t* probe = tfree + 2;
+  uint64_t* rbar = probe + 1;  // [EPI_WARPS] a warp's residual has landed
   uint32_t* tmem = reinterpret_cast<uint32_t*>(full + C::NBAR);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -432,8 +416,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull + i, 1);
-      mbar_init(tfree + i, EPI_WARPS * CG);
+      mbar_init(tfree + i, C::ACTIVE * CG);
     }
+    for (int i = 0; i < EPI_WARPS; ++i) mbar_init(rbar + i, 1);
     mbar_init(probe, 1);
     *abort = 0;
     fence_mbar_init();
@@ -466,15 +451,15 @@ __global__ void __launch_bounds__(THREADS, 1)
           };
           if constexpr (AMN) {
 #pragma unroll
-            for (int i = 0; i < TM / 64; ++i) load(sa + i * 8192, &amap, am0 + i * 64, kb * KE);
+            for (int i = 0; i < TM / 64; ++i) load(sa + i * 8192, &maps.a, am0 + i * 64, kb * KE);
           } else {
-            load(sa, &amap, kb * KE, am0);
+            load(sa, &maps.a, kb * KE, am0);
           }
           if constexpr (BMN) {
 #pragma unroll
-            for (int i = 0; i < C::B_ROWS / 64; ++i) load(sb + i * 8192, &bmap, bn0 + i * 64, kb * KE);
+            for (int i = 0; i < C::B_ROWS / 64; ++i) load(sb + i * 8192, &maps.b, bn0 + i * 64, kb * KE);
           } else {
-            load(sb, &bmap, kb * KE, bn0);
+            load(sb, &maps.b, kb * KE, bn0);
           }
         }
       }
@@ -506,45 +491,100 @@ __global__ void __launch_bounds__(THREADS, 1)
         commit<CG>(tfull + acc);
       }
     }
-  } else {
-    unsigned char* stg = sm + C::OFF_STG + warp * STG_W;
-    const int q = warp & 3, half = warp >> 2;
-    constexpr int NCH = BN / 64;  // 32-column blocks of a warp
-    int tl = 0;
+  } else if (warp < C::ACTIVE) {
+    unsigned char* stg = sm + C::OFF_STG + warp * C::STG_W;
+    const int q = warp & 3, group = warp >> 2;
+    const Epi& e = a.e;
+    int tl = 0, fetched = 0;
     for (int u = first; u < units && !*abort; u += step, ++tl) {
       const Unit t = unit_of(a, u);
       const int acc = tl & 1;
       const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
-      const int nb = t.nt * BN + half * (BN / 2);
-      Epi e = a.e;
-      if (a.splits > 1) e.out = (float*)a.e.out + (int64_t)t.split * a.part_stride;
-      ResBlock r;
-      fetch_res(r, e, m0, a.M, nb, a.N);
+      const int nb = t.nt * BN + group * C::CW;
+      const bool some = m0 < a.M && nb < a.N;
+      const int blocks = !some ? 0 : nb + 32 < a.N ? C::NBLK : 1;
+      // The staging is free once the last tile's copies have read it; the
+      // residual is on its way there while the products are still at work.
+      if (lane == 0) {
+        bulk_wait_read();
+        if (e.res && e.vr && some) {
+          mbar_arrive_expect_tx(rbar + warp, blocks * BLOCK_ST);
+          for (int j = 0; j < blocks; ++j) tma_load_2d(stg + j * BLOCK_ST, &maps.res, nb + 32 * j, (int)m0, rbar + warp);
+        }
+      }
+      __syncwarp();
       if (!mbar_wait(tfull + acc, (tl >> 1) & 1, abort)) break;
       __syncwarp();
       tc_fence_after();
-#pragma unroll 1
-      for (int cb = 0; cb < NCH; ++cb) {
-        const int n0 = nb + cb * 32;
-        if (n0 >= a.N) break;
+      if (e.res && e.vr && some) {
+        if (!mbar_wait(rbar + warp, fetched++ & 1, abort)) break;
+        __syncwarp();
+      }
+#pragma unroll
+      for (int j = 0; j < C::NBLK; ++j) {
+        if (j >= blocks) break;
+        const int n0 = nb + 32 * j;
+        unsigned char* sj = stg + j * BLOCK_ST;
         uint32_t w[32];
-        tmem_ld32(tbase + acc * BN + half * (BN / 2) + cb * 32 + ((uint32_t)(q * 32) << 16), w);
+        tmem_ld32(tbase + acc * BN + group * C::CW + j * 32 + ((uint32_t)(q * 32) << 16), w);
         tmem_ld_wait();
+        if (j + 1 == blocks) {  // the accumulator is read: the next but one tile may have it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(tfree + acc);
+            else arrive_in(in_cta(tfree + acc, 0));
+          }
+        }
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]);
-        if (m0 < a.M) {
-          finish_block(v, r, stg, e, m0, a.M, n0, a.N);
-          if (cb + 1 < NCH) fetch_res(r, e, m0, a.M, n0 + 32, a.N);
+        uint4 r[4];
+        if (e.res) {
+          if (!e.vr) stage_res(sj, e, m0, a.M, n0, a.N);
+          take_res(sj, r);
+          __syncwarp();
+        }
+        if (e.bias) add_bias(v, e, n0, a.N);
+        if (e.z) {
+          float z[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = keep_z(v[i], BF16);
+          put16(sj, z, BF16, &maps.z, true, nullptr, 0, m0, a.M, n0, a.N);
+        }
+        if constexpr (ACT != OW_ACT_NONE) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT>(v[i]);
+        }
+        if (e.res) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t p[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = upk(p[i], BF16);
+              v[8 * k + 2 * i] += f.x;
+              v[8 * k + 2 * i + 1] += f.y;
+            }
+          }
+        }
+        if (e.z) {  // z's copy has left the staging
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+        }
+        if (e.out32) put32(sj, v, &maps.out, e.vo, (float*)e.out, e.ldo, m0, a.M, n0, a.N, t.split);
+        else put16(sj, v, BF16, &maps.out, e.vo, e.out, e.ldo, m0, a.M, n0, a.N);
+      }
+      if (blocks == 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 1) mbar_arrive(tfree + acc);
+          else arrive_in(in_cta(tfree + acc, 0));
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 1) mbar_arrive(tfree + acc);
-        else arrive_in(in_cta(tfree + acc, 0));
-      }
     }
+    if (lane == 0) bulk_wait_all();
   }
 
   __syncwarp();
@@ -680,11 +720,12 @@ struct DzArgs {
   void* dz;          // [M, ldz] or NULL (only the sums are wanted)
   float* part;       // [chunks][N] column sums, or NULL
   int64_t M, ldz, chunk;
-  int N, act, bf16, vec;
+  int N, bf16, vec;
 };
 
 // dz = dy act'(z), rounded to the 16-bit type (the GEMMs take it so), and its
 // f32 column sums for the bias.  A block does 256 columns of a chunk of rows.
+template <int ACT>
 __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
   __shared__ float sh[8][264];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -716,7 +757,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      g[k] *= act_slope(z[k], a.act);
+      g[k] *= act_slope<ACT>(z[k]);
       s[k] += g[k];
     }
     if (a.dz)  // rows of dz start on 16 bytes and have room for whole vectors
@@ -781,8 +822,8 @@ struct Mat {
 // Shape of one GEMM: the tile's width, whether pairs of SMs share it, and the
 // k splits that a simple model finds fastest, in cycles.  A 64-wide k block
 // takes its products (BN * 2 cycles on an SM) or its copies at 64 bytes a
-// cycle, whichever is longer: 384 cycles for 128 x 64, 512 for 128 x 128, 768
-// for 128 x 256, and 512 for the pair's 256 x 256.  A tile adds its start and
+// cycle, whichever is longer: 384 cycles for 128 x 64, 512 for 128 x 128 and for
+// the pair's 256 x 256.  A tile adds its start and
 // the last one its epilogue (20 cycles a column and 2000); splits write and
 // read f32 partials at about 3 KB a cycle and start one more kernel (6000).
 struct Plan {
@@ -793,7 +834,7 @@ Plan plan_gemm(int64_t M, int N, int kblocks) {
   Plan best{128, 1, 1};
   double least = 1e300;
   struct Tile { int bn, cg, block; };
-  for (const Tile t : {Tile{64, 1, 384}, Tile{128, 1, 512}, Tile{256, 1, 768}, Tile{256, 2, 512}}) {
+  for (const Tile t : {Tile{64, 1, 384}, Tile{128, 1, 512}, Tile{256, 2, 512}}) {
     const int64_t tiles = (M + TM * t.cg - 1) / (TM * t.cg) * ((N + t.bn - 1) / t.bn);
     const int slots = sms / t.cg;
     // more splits than fill the SMs twice gain nothing
@@ -847,38 +888,42 @@ int map_of(CUtensorMap* map, const Mat& m, bool bf16, uint32_t box_rows) {
   return encode_tiled_map(map, bf16, 2, m.p, dims, strides, box, "ow_linear");
 }
 
-template <int BN, int CG, bool AMN, bool BMN, bool BF16>
-int run_gemm(const CUtensorMap& am, const CUtensorMap& bm, const GemmArgs& k, int grid, cudaStream_t st) {
+// An output or residual as boxes of 32 rows x 64 bytes: [splits][rows][cols].
+int block_map(CUtensorMap* map, int dtype, const void* p, int64_t rows, int cols, int64_t ld, int splits) {
+  const uint64_t es = dtype == OW_DTYPE_F32 ? 4 : 2;
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)splits};
+  const uint64_t strides[2] = {(uint64_t)ld * es, (uint64_t)ld * rows * es};
+  const uint32_t box[3] = {(uint32_t)(64 / es), 32, 1};
+  return encode_tiled_map64(map, dtype, splits > 0 ? 3 : 2, p, dims, strides, box, true, "ow_linear");
+}
+
+template <int BN, int CG, bool AMN, bool BMN, bool BF16, int ACT>
+int run_gemm(const Maps& maps, const GemmArgs& k, int grid, cudaStream_t st) {
   using C = GC<BN, CG>;
-  auto kern = gemm_kernel<BN, CG, AMN, BMN, BF16>;
+  auto kern = gemm_kernel<BN, CG, AMN, BMN, BF16, ACT>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) {
     set_error("ow_linear: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e));
     return OW_ERR_CUDA;
   }
-  if constexpr (CG == 1) {
-    launch(kern, grid, THREADS, C::SMEM, st, am, bm, k);
-  } else {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = CG;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    count_launches(1);
-    e = cudaLaunchKernelEx(&cfg, kern, am, bm, k);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      set_error("gemm_kernel: launch failed: %s", cudaGetErrorString(e));
-      return OW_ERR_CUDA;
-    }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = CG;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  count_launches(1);
+  e = cudaLaunchKernelEx(&cfg, kern, maps, k);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("gemm_kernel: launch failed: %s", cudaGetErrorString(e));
+    return OW_ERR_CUDA;
   }
-  OW_CHECK_LAUNCH("gemm_kernel");
   return OW_OK;
 }
 
@@ -888,9 +933,9 @@ template <bool AMN, bool BMN>
 int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs& w, const Epi& e, bool bf16, cudaStream_t st) {
   if (w.a) OW_RETURN_IF(pad_rows(A, w.a, st));
   if (w.b) OW_RETURN_IF(pad_rows(B, w.b, st));
-  CUtensorMap am, bm;
-  OW_RETURN_IF(map_of(&am, A, bf16, AMN ? KE : TM));
-  OW_RETURN_IF(map_of(&bm, B, bf16, BMN ? KE : p.bn / p.cg));
+  Maps maps{};
+  OW_RETURN_IF(map_of(&maps.a, A, bf16, AMN ? KE : TM));
+  OW_RETURN_IF(map_of(&maps.b, B, bf16, BMN ? KE : p.bn / p.cg));
   GemmArgs k{};
   k.M = M;
   k.N = N;
@@ -901,31 +946,44 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   k.e = e;
   if (p.splits > 1) {
     k.e = Epi{};
-    k.e.bf16 = e.bf16;
     k.e.out = w.part;
     k.e.ldo = w.part_ld;
     k.e.out32 = 1;
     k.e.vo = 1;
-    k.part_stride = M * w.part_ld;
   }
+  const int t16 = bf16 ? OW_DTYPE_BF16 : OW_DTYPE_F16;
+  if (k.e.vo) OW_RETURN_IF(block_map(&maps.out, k.e.out32 ? OW_DTYPE_F32 : t16, k.e.out, M, N, k.e.ldo, p.splits));
+  if (k.e.z) OW_RETURN_IF(block_map(&maps.z, t16, k.e.z, M, N, k.e.ldz, 1));
+  if (k.e.res && k.e.vr) OW_RETURN_IF(block_map(&maps.res, t16, k.e.res, M, N, k.e.ldr, 0));
   OW_RETURN_IF(fault_word(&k.fault));
   k.probe_ns = wait_probe_ns();
   const int64_t units = (int64_t)k.mtiles * k.ntiles * k.splits;
   OW_CHECK_ARG(units < (1LL << 31) - 1024, "ow_linear: too many tiles");
   const int grid = (int)std::min<int64_t>(units, device_sm_count() / p.cg) * p.cg;
-  auto go = [&](auto bn, auto cg) -> int {
-    constexpr int BN = decltype(bn)::value, CG = decltype(cg)::value;
-    return bf16 ? run_gemm<BN, CG, AMN, BMN, true>(am, bm, k, grid, st) : run_gemm<BN, CG, AMN, BMN, false>(am, bm, k, grid, st);
+  auto go = [&](auto act) -> int {
+    constexpr int ACT = decltype(act)::value;
+    auto tile = [&](auto bn, auto cg) -> int {
+      constexpr int BN = decltype(bn)::value, CG = decltype(cg)::value;
+      return bf16 ? run_gemm<BN, CG, AMN, BMN, true, ACT>(maps, k, grid, st) : run_gemm<BN, CG, AMN, BMN, false, ACT>(maps, k, grid, st);
+    };
+    if (p.cg == 2) return tile(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    if (p.bn == 64) return tile(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    return tile(std::integral_constant<int, 128>(), std::integral_constant<int, 1>());
   };
-  using I1 = std::integral_constant<int, 1>;
-  if (p.cg == 2) OW_RETURN_IF(go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>()));
-  else if (p.bn == 64) OW_RETURN_IF(go(std::integral_constant<int, 64>(), I1()));
-  else if (p.bn == 128) OW_RETURN_IF(go(std::integral_constant<int, 128>(), I1()));
-  else OW_RETURN_IF(go(std::integral_constant<int, 256>(), I1()));
+  if constexpr (!AMN && !BMN) {  // only the forward has an activation
+    switch (k.e.act) {
+      case OW_ACT_RELU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_RELU>())); break;
+      case OW_ACT_SILU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_SILU>())); break;
+      case OW_ACT_GELU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_GELU>())); break;
+      default: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_NONE>()));
+    }
+  } else {
+    OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_NONE>()));
+  }
   if (p.splits > 1) {
     const int64_t total = M * ((N + 3) / 4);
     const int g2 = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);
-    launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, k.part_stride, w.part_ld, M, N, e);
+    launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, M * w.part_ld, w.part_ld, M, N, e);
     OW_CHECK_LAUNCH("gemm_sum_kernel");
   }
   return OW_OK;
@@ -1083,9 +1141,14 @@ int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream
   Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
   const BwdWs b = bwd_take(a, g, ws);
   if (b.dz || g->dbias) {
-    DzArgs k{g->dout, a->activation == OW_ACT_NONE ? nullptr : a->z, b.dz, b.bias, M, up8(N), b.chunk, N, a->activation, bf,
-             tma_rows(g->dout, N)};
-    launch(dz_kernel, dim3((N + 255) / 256, b.chunks), 256, 0, st, k);
+    DzArgs k{g->dout, a->activation == OW_ACT_NONE ? nullptr : a->z, b.dz, b.bias, M, up8(N), b.chunk, N, bf, tma_rows(g->dout, N)};
+    const dim3 grid((N + 255) / 256, b.chunks);
+    switch (a->activation) {
+      case OW_ACT_NONE: launch(dz_kernel<OW_ACT_NONE>, grid, 256, 0, st, k); break;
+      case OW_ACT_RELU: launch(dz_kernel<OW_ACT_RELU>, grid, 256, 0, st, k); break;
+      case OW_ACT_SILU: launch(dz_kernel<OW_ACT_SILU>, grid, 256, 0, st, k); break;
+      default: launch(dz_kernel<OW_ACT_GELU>, grid, 256, 0, st, k);
+    }
     OW_CHECK_LAUNCH("dz_kernel");
     if (g->dbias) {
       launch(dbias_kernel, (N + 31) / 32, 256, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype);

@@ -802,6 +802,11 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 int encode_tiled_map(void* map, bool bf16, int rank, const void* base, const uint64_t* dims,
                      const uint64_t* strides, const uint32_t* box, const char* who) {
+  return encode_tiled_map64(map, bf16 ? OW_DTYPE_BF16 : OW_DTYPE_F16, rank, base, dims, strides, box, false, who);
+}
+
+int encode_tiled_map64(void* map, int dtype, int rank, const void* base, const uint64_t* dims, const uint64_t* strides,
+                       const uint32_t* box, bool swizzle64, const char* who) {
   auto encode = encode_fn();
   if (!encode) {
     set_error("%s: cuTensorMapEncodeTiled is not available from the CUDA driver", who);
@@ -820,9 +825,11 @@ int encode_tiled_map(void* map, bool bf16, int rank, const void* base, const uin
     if (i + 1 < rank) s[i] = strides[i];
   }
   const CUresult r = encode(static_cast<CUtensorMap*>(map),
-                            bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            dtype == OW_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                            : dtype == OW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                             (cuuint32_t)rank, const_cast<void*>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            swizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("%s: cuTensorMapEncodeTiled failed (CUresult %d)", who, (int)r);
