@@ -820,12 +820,15 @@ struct Mat {
 };
 
 // Shape of one GEMM: the tile's width, whether pairs of SMs share it, and the
-// k splits that a simple model finds fastest, in cycles.  A 64-wide k block
-// takes its products (BN * 2 cycles on an SM) or its copies at 64 bytes a
-// cycle, whichever is longer: 384 cycles for 128 x 64, 512 for 128 x 128 and for
-// the pair's 256 x 256.  A tile adds its start and
-// the last one its epilogue (20 cycles a column and 2000); splits write and
-// read f32 partials at about 3 KB a cycle and start one more kernel (6000).
+// k splits that a model finds fastest, in cycles of an SM.  Its figures are
+// measured (B200, 1.75 GHz): a 64-wide k block takes 600 cycles in a 128 x 64
+// tile, 670 in 128 x 128 and 680 in the pair's 256 x 256 (products alone: 128,
+// 256, 512; an SM's copies at 64 bytes a cycle: 384, 512, 512); an epilogue
+// 2000 + 12.5 a column, under the next tile's products; a launch with its first
+// copies 6000; splits write and read f32 partials at about 3 KB a cycle and
+// start one more kernel (4000).  With few tiles the narrow ones win by filling
+// the SMs (2000 x 512 x 512: 7.4, 7.9, 9.5 us), with many the pair's
+// (200704 x 128 x 256: 60.7, 39.7, 30.3 us).
 struct Plan {
   int bn, cg, splits;
 };
@@ -834,17 +837,17 @@ Plan plan_gemm(int64_t M, int N, int kblocks) {
   Plan best{128, 1, 1};
   double least = 1e300;
   struct Tile { int bn, cg, block; };
-  for (const Tile t : {Tile{64, 1, 384}, Tile{128, 1, 512}, Tile{256, 2, 512}}) {
+  for (const Tile t : {Tile{64, 1, 600}, Tile{128, 1, 670}, Tile{256, 2, 680}}) {
     const int64_t tiles = (M + TM * t.cg - 1) / (TM * t.cg) * ((N + t.bn - 1) / t.bn);
     const int slots = sms / t.cg;
+    const double epilogue = 2000.0 + 12.5 * t.bn;
     // more splits than fill the SMs twice gain nothing
     const int smax = (int)std::min<int64_t>(std::min(kblocks, 64), 1 + 2 * slots / tiles);
     for (int s = 1; s <= smax; ++s) {
       const int64_t waves = (tiles * s + slots - 1) / slots;
       const int kb = (kblocks + s - 1) / s;
-      const double main = std::max<double>((double)kb * t.block, t.bn * 20.0);  // an epilogue runs under the next tile
-      double c = waves * main + t.bn * 20.0 + 2000.0;
-      if (s > 1) c += 6000.0 + (double)s * M * N * 8.0 / 3000.0;
+      double c = waves * std::max<double>((double)kb * t.block, epilogue) + epilogue + 6000.0;
+      if (s > 1) c += 4000.0 + (double)s * M * N * 8.0 / 3000.0;
       if (c < least) {
         least = c;
         best = Plan{t.bn, t.cg, s};

@@ -294,6 +294,27 @@ def test_captured_and_on_another_stream(cuda_device):
     assert all(torch.equal(p, q) for p, q in zip(outs, want))
 
 
+def test_first_cuda_call_of_a_thread(cuda_device):
+    """A thread without a context of its own yet (as autograd's may be) can make the call."""
+    import threading
+
+    x, w, *_ = _inputs(cuda_device, 200, 64, 64, BF)
+    linear.linear(x, w)  # its workspace is in the allocator's cache now: the thread's first CUDA call is the kernel's
+    got: list = []
+
+    def call():
+        try:
+            got.append(linear.linear(x, w))
+        except Exception as exc:  # handed to the test
+            got.append(exc)
+
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    assert torch.is_tensor(got[0]), got[0]
+    assert torch.equal(got[0], linear.linear(x, w))
+
+
 def test_wait_that_runs_out_is_reported(cuda_device):
     """The GEMM's bounded waits report to the library's fault word, as every pipelined kernel's do."""
     x, w, *_ = _inputs(cuda_device, 200, 64, 64, BF)
