@@ -105,6 +105,17 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// mbar_wait, without a look at the abort flag where the phase is complete.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort);
+}
+// One lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---------------------------------------------------------------- CTA pairs
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -434,17 +445,22 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   if (*abort) {
     // the wait-timeout self-check ran out: nothing is issued
   } else if (warp == PROD_W) {
-    if (lane == 0) {
-      int g = 0;
-      for (int u = first; u < units && !*abort; u += step) {
-        const Unit t = unit_of(a, u);
-        const int am0 = (t.mt * CG + (int)rank) * TM, bn0 = t.nt * BN + (int)rank * C::B_ROWS;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
-          const int s = g % C::STAGES;
-          if (g >= C::STAGES && !mbar_wait(empty + s, ((g / C::STAGES) - 1) & 1, abort)) break;
+    // This warp and the next run their loops with all lanes and let one issue:
+    // what the instructions take (barriers, descriptors, coordinates) is then
+    // computed once for the warp.  With a single lane in the loop, moving it to
+    // the uniform registers cost 125 cycles an MMA, whatever its size.
+    const bool one = elect_lane();
+    int g = 0;
+    for (int u = first; u < units && !*abort; u += step) {
+      const Unit t = unit_of(a, u);
+      const int am0 = (t.mt * CG + (int)rank) * TM, bn0 = t.nt * BN + (int)rank * C::B_ROWS;
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
+        const int s = g % C::STAGES;
+        if (g >= C::STAGES && !wait_for(empty + s, ((g / C::STAGES) - 1) & 1, abort)) break;
+        unsigned char* sa = sm + s * A_ST;
+        unsigned char* sb = sm + C::OFF_B + s * C::B_ST;
+        if (one) {
           if (rank == 0) mbar_arrive_expect_tx(full + s, CG * (A_ST + C::B_ST));
-          unsigned char* sa = sm + s * A_ST;
-          unsigned char* sb = sm + C::OFF_B + s * C::B_ST;
           auto load = [&](void* dst, const CUtensorMap* map, int c0, int c1) {
             if constexpr (CG == 1) tma_load_2d(dst, map, c0, c1, full + s);
             else tma_load_2d_pair(dst, map, c0, c1, in_cta(full + s, 0));
@@ -462,33 +478,40 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             load(sb, &maps.b, kb * KE, bn0);
           }
         }
+        __syncwarp();
       }
     }
   } else if (warp == MMA_W) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t ID = idesc_f16(TM * CG, BN, BF16) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
       const uint32_t s0 = smem_u32(sm);
+      const uint32_t tmem0 = __shfl_sync(0xffffffffu, tbase, 0);
+      const bool one = elect_lane();
       int g = 0, tl = 0;
       for (int u = first; u < units && !*abort; u += step, ++tl) {
         const Unit t = unit_of(a, u);
         const int acc = tl & 1;
-        if (tl >= 2 && !mbar_wait(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
+        if (tl >= 2 && !wait_for(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
         tc_fence_after();
-        const uint32_t tacc = tbase + acc * BN;
+        const uint32_t tacc = tmem0 + acc * BN;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
           const int s = g % C::STAGES;
-          if (!mbar_wait(full + s, (g / C::STAGES) & 1, abort)) break;
+          if (!wait_for(full + s, (g / C::STAGES) & 1, abort)) break;
           tc_fence_after();
           const uint32_t aA = s0 + s * A_ST, aB = s0 + C::OFF_B + s * C::B_ST;
+          const uint64_t da = AMN ? sdesc_mn(aA, 8192) : sdesc_sw128(aA);
+          const uint64_t db = BMN ? sdesc_mn(aB, 8192) : sdesc_sw128(aB);
+          if (one) {
+            // a 16-wide k step further: 2048 bytes (MN-major) or 32, in units of 16
 #pragma unroll
-          for (int kk = 0; kk < KE / 16; ++kk) {
-            const uint64_t da = AMN ? sdesc_mn(aA + kk * 2048, 8192) : sdesc_sw128(aA + kk * 32);
-            const uint64_t db = BMN ? sdesc_mn(aB + kk * 2048, 8192) : sdesc_sw128(aB + kk * 32);
-            umma<CG>(tacc, da, db, ID, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < KE / 16; ++kk)
+              umma<CG>(tacc, da + kk * (AMN ? 128 : 2), db + kk * (BMN ? 128 : 2), ID, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+            commit<CG>(empty + s);
           }
-          commit<CG>(empty + s);
+          __syncwarp();
         }
-        commit<CG>(tfull + acc);
+        if (one) commit<CG>(tfull + acc);
+        __syncwarp();
       }
     }
   } else if (warp < C::ACTIVE) {
@@ -513,11 +536,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         }
       }
       __syncwarp();
-      if (!mbar_wait(tfull + acc, (tl >> 1) & 1, abort)) break;
+      if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
       __syncwarp();
       tc_fence_after();
       if (e.res && e.vr && some) {
-        if (!mbar_wait(rbar + warp, fetched++ & 1, abort)) break;
+        if (!wait_for(rbar + warp, fetched++ & 1, abort)) break;
         __syncwarp();
       }
 #pragma unroll
