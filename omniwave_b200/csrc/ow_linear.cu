@@ -105,6 +105,9 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 // mbar_wait, without a look at the abort flag where the phase is complete.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort);
@@ -194,28 +197,41 @@ __device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t lbo) {
 }
 
 // ---------------------------------------------------------------- activations
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and exp(-z^2 / 2): one exponential serves
-// the function and its slope.  erfc by Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2),
-// t = 1 / (1 + p x), off by 1.5e-7 at most; a value that is rounded to 16 bits
-// next.  About 16 instructions where erff and expf take 40, which bound the
-// epilogue (25088 x 512 x 1024 forward 88 us) and the backward's first pass.
-__device__ __forceinline__ float normal_cdf(float z, float& bell) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  bell = __expf(-0.5f * z * z);
-  const float tail = 0.5f * bell * t * fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f);
+// 2^x and 1 / x by the special-function units, subnormals taken as 0 (two
+// instructions less each than without): what follows is rounded to 16 bits.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float z) { return rcp(1.f + ex2(z * -1.44269504f)); }
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 by Abramowitz and Stegun, Handbook of
+// Mathematical Functions, 7.1.28: erfc(x) = (1 + a1 x + ... + a6 x^6)^-16, off by
+// 3e-7 at most, here in |z| = sqrt(2) x.  One special-function result an
+// element where an exponential and a quotient take two; erff and expf took 40
+// instructions and bound the epilogue.
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float a = fabsf(z);
+  float p = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(5.3829750e-6f, a, 4.8890636e-5f), a, 3.8003575e-5f), a, 3.2776263e-3f), a, 2.1141006e-2f), a,
+                      4.9867347e-2f), a, 1.f);
+  p *= p;
+  p *= p;
+  p *= p;
+  p *= p;
+  const float tail = 0.5f * rcp(p);
   return z > 0.f ? 1.f - tail : tail;
 }
-
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if constexpr (ACT == OW_ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
-  if constexpr (ACT == OW_ACT_GELU) {
-    float bell;
-    return z * normal_cdf(z, bell);
-  }
+  if constexpr (ACT == OW_ACT_SILU) return z * sigmoid(z);
+  if constexpr (ACT == OW_ACT_GELU) return z * normal_cdf(z);
   return z;
 }
 __device__ __forceinline__ float act_fwd(float z, int act) {
@@ -230,14 +246,11 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == OW_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
   if constexpr (ACT == OW_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-z));
-    return s * (1.f + z * (1.f - s));
+    const float s = sigmoid(z);
+    return s * fmaf(z, 1.f - s, 1.f);
   }
-  if constexpr (ACT == OW_ACT_GELU) {
-    float bell;
-    const float cdf = normal_cdf(z, bell);
-    return fmaf(z * 0.39894228040143268f, bell, cdf);
-  }
+  if constexpr (ACT == OW_ACT_GELU)
+    return fmaf(z * 0.39894228040143268f, ex2(z * z * -0.72134752f), normal_cdf(z));
   return 1.f;
 }
 
@@ -420,20 +433,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(full + s, 1);
-      mbar_init(empty + s, 1);
+  if (warp == 0) {  // a lane a barrier
+    for (int i = lane; i < C::NBAR; i += 32) {
+      uint64_t* b = full + i;
+      mbar_init(b, b == tfree || b == tfree + 1 ? C::ACTIVE * CG : 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(tfull + i, 1);
-      mbar_init(tfree + i, C::ACTIVE * CG);
-    }
-    for (int i = 0; i < EPI_WARPS; ++i) mbar_init(rbar + i, 1);
-    mbar_init(probe, 1);
-    *abort = 0;
     fence_mbar_init();
-    wait_probe(probe, abort, a.probe_ns);
+    __syncwarp();
+    if (lane == 0) {
+      *abort = 0;
+      wait_probe(probe, abort, a.probe_ns);
+    }
+  } else if (threadIdx.x == PROD_W * 32) {
+    prefetch_map(&maps.a);
+    prefetch_map(&maps.b);
   }
   if (warp == MMA_W) tmem_take<CG>(tmem, C::TMEM_COLS);
   tc_fence_before();
@@ -607,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         }
       }
     }
-    if (lane == 0) bulk_wait_all();
+    if (lane == 0) bulk_wait_read();  // the staging stays until it is read
   }
 
   __syncwarp();
@@ -800,18 +813,22 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
   }
 }
 
-__global__ void __launch_bounds__(256) dbias_kernel(const float* __restrict__ part, int chunks, int N, void* out, int dt) {
-  __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) dbias_kernel(const float* __restrict__ part, int chunks, int N, void* out, int dt) {
+  __shared__ float sh[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
-  float t = 0.f;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};  // four loads in flight: a chain of them is what this kernel takes
   if (c < N)
-    for (int p = ry; p < chunks; p += 8) t += part[(int64_t)p * N + c];
-  sh[ry][cx] = t;
+    for (int p = ry; p < chunks; p += 128) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (p + 32 * k < chunks) t[k] += part[(int64_t)(p + 32 * k) * N + c];
+    }
+  sh[ry][cx] = (t[0] + t[1]) + (t[2] + t[3]);
   __syncthreads();
   if (ry == 0 && c < N) {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += sh[i][cx];
+    for (int i = 0; i < 32; ++i) v += sh[i][cx];
     if (dt == OW_DTYPE_F32) ((float*)out)[c] = v;
     else st16(out, c, dt == OW_DTYPE_BF16, v);
   }
@@ -844,14 +861,14 @@ struct Mat {
 
 // Shape of one GEMM: the tile's width, whether pairs of SMs share it, and the
 // k splits that a model finds fastest, in cycles of an SM.  Its figures are
-// measured (B200, 1.75 GHz): a 64-wide k block takes 600 cycles in a 128 x 64
-// tile, 670 in 128 x 128 and 680 in the pair's 256 x 256 (products alone: 128,
+// measured (B200, 1.75 GHz): a 64-wide k block takes 400 cycles in a 128 x 64
+// tile, 460 in 128 x 128 and 600 in the pair's 256 x 256 (products alone: 128,
 // 256, 512; an SM's copies at 64 bytes a cycle: 384, 512, 512); an epilogue
-// 2000 + 12.5 a column, under the next tile's products; a launch with its first
+// 1300 + 9.5 a column, under the next tile's products; a launch with its first
 // copies 6000; splits write and read f32 partials at about 3 KB a cycle and
-// start one more kernel (4000).  With few tiles the narrow ones win by filling
-// the SMs (2000 x 512 x 512: 7.4, 7.9, 9.5 us), with many the pair's
-// (200704 x 128 x 256: 60.7, 39.7, 30.3 us).
+// start one more kernel (5000).  With few tiles the narrow ones win by filling
+// the SMs (2000 x 512 x 512: 6.3, 7.0, 8.9 us), with many the pair's
+// (12544 x 2048 x 1024: 81, 52, 39 us).
 struct Plan {
   int bn, cg, splits;
 };
@@ -860,17 +877,17 @@ Plan plan_gemm(int64_t M, int N, int kblocks) {
   Plan best{128, 1, 1};
   double least = 1e300;
   struct Tile { int bn, cg, block; };
-  for (const Tile t : {Tile{64, 1, 600}, Tile{128, 1, 670}, Tile{256, 2, 680}}) {
+  for (const Tile t : {Tile{64, 1, 400}, Tile{128, 1, 460}, Tile{256, 2, 600}}) {
     const int64_t tiles = (M + TM * t.cg - 1) / (TM * t.cg) * ((N + t.bn - 1) / t.bn);
     const int slots = sms / t.cg;
-    const double epilogue = 2000.0 + 12.5 * t.bn;
+    const double epilogue = 1300.0 + 9.5 * t.bn;
     // more splits than fill the SMs twice gain nothing
     const int smax = (int)std::min<int64_t>(std::min(kblocks, 64), 1 + 2 * slots / tiles);
     for (int s = 1; s <= smax; ++s) {
       const int64_t waves = (tiles * s + slots - 1) / slots;
       const int kb = (kblocks + s - 1) / s;
       double c = waves * std::max<double>((double)kb * t.block, epilogue) + epilogue + 6000.0;
-      if (s > 1) c += 4000.0 + (double)s * M * N * 8.0 / 3000.0;
+      if (s > 1) c += 5000.0 + (double)s * M * N * 8.0 / 3000.0;
       if (c < least) {
         least = c;
         best = Plan{t.bn, t.cg, s};
@@ -1177,7 +1194,7 @@ int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream
     }
     OW_CHECK_LAUNCH("dz_kernel");
     if (g->dbias) {
-      launch(dbias_kernel, (N + 31) / 32, 256, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype);
+      launch(dbias_kernel, (N + 31) / 32, 1024, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype);
       OW_CHECK_LAUNCH("dbias_kernel");
     }
   }
