@@ -88,6 +88,20 @@ __device__ __forceinline__ void ldv(const void* p, int dt, int64_t i, float (&o)
   }
 }
 
+// The same 8 channels of a 16-bit array, fetched and widened apart.
+__device__ __forceinline__ uint4 fetch8(const void* p, int64_t i) { return *reinterpret_cast<const uint4*>((const uint16_t*)p + i); }
+__device__ __forceinline__ void widen8(const uint4& r, int dt, float (&o)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 f;
+    if (dt == OW_DTYPE_BF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k]));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    o[2 * k] = f.x;
+    o[2 * k + 1] = f.y;
+  }
+}
+
 template <int V>
 __device__ __forceinline__ void stv(void* p, int dt, int64_t i, const float (&v)[V]) {
   if (dt == OW_DTYPE_F32) {
@@ -186,7 +200,10 @@ __device__ __forceinline__ int64_t sample_of(const Args& a, int64_t row) {
 }
 
 // Block (group, part) strides over its group's rows, ``blockDim / G`` at a time.
-template <int V, int G, int NV, bool DELTA, bool NEXT>
+// H16: x, delta and n are 16-bit; a row is then half the bytes of an f32 one,
+// too few in flight to fill the memory's pipe, so each row is asked for while
+// the one before it is worked on (128 x 196 x 512: forward 34 -> 25 us).
+template <int V, int G, int NV, bool DELTA, bool NEXT, bool H16>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args a) {
   constexpr int T = G > 256 ? G : 256, RB = T / G;
   extern __shared__ float4 dyn4[];
@@ -198,20 +215,44 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args 
   const int64_t group = blockIdx.x / a.per_group;
   const int part = blockIdx.x % a.per_group;
   const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
+  const int64_t stride = (int64_t)a.per_group * RB;
+  int64_t r0 = group * a.group_rows + (int64_t)part * RB;
+  uint4 fx[NV], fd[NV];  // H16: the next row
+  auto fetch_row = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+      fx[j] = fd[j] = make_uint4(0, 0, 0, 0);
+      if (row < row_end && c < a.C) {
+        fx[j] = fetch8(a.x, row * a.C + c);
+        if constexpr (DELTA) fd[j] = fetch8(a.delta, row * a.C + c);
+      }
+    }
+  };
+  if constexpr (H16) fetch_row(r0 + sub);
   load_factors<V, DELTA, NEXT>(a, group, kq, wn);
-  for (int64_t r0 = group * a.group_rows + (int64_t)part * RB; r0 < row_end; r0 += (int64_t)a.per_group * RB) {
+  for (; r0 < row_end; r0 += stride) {
     const int64_t row = r0 + sub;
     const bool live = row < row_end;
     const int64_t at = row * a.C;
     float x[NV][V], d[NV][V];
+    if constexpr (H16) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * G + lane) * V;
+      for (int j = 0; j < NV; ++j) {
+        widen8(fx[j], a.x_dt, x[j]);
+        if constexpr (DELTA) widen8(fd[j], a.d_dt, d[j]);
+      }
+      fetch_row(row + stride);
+    } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = 0.f;
-      if (live && c < a.C) {
-        ldv<V>(a.x, a.x_dt, at + c, x[j]);
-        if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[j][k] = d[j][k] = 0.f;
+        if (live && c < a.C) {
+          ldv<V>(a.x, a.x_dt, at + c, x[j]);
+          if constexpr (DELTA) ldv<V>(a.delta, a.d_dt, at + c, d[j]);
+        }
       }
     }
     if constexpr (DELTA) {
@@ -259,7 +300,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_fwd_kernel(const Args 
 }
 
 // Block (group, part) strides over its group's rows; ``part`` gets its sums.
-template <int V, int G, int NV, bool DELTA, bool NEXT>
+template <int V, int G, int NV, bool DELTA, bool NEXT, bool H16>
 __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args a) {
   constexpr int T = G > 256 ? G : 256, RB = T / G;
   extern __shared__ float4 dyn4[];  // the channel factors, later the sums of the block's row groups
@@ -271,6 +312,31 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
   const int64_t group = blockIdx.x / a.per_group;
   const int part = blockIdx.x % a.per_group;
   const int64_t row_end = min(a.rows, (group + 1) * a.group_rows);
+  const int64_t stride = (int64_t)a.per_group * RB;
+  int64_t r0 = group * a.group_rows + (int64_t)part * RB;
+  uint4 fx[NV], fd[NV], fh[NV], fn[NV];  // H16: the next row
+  float fr[2];
+  auto fetch_row = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * V;
+      fx[j] = fd[j] = fh[j] = fn[j] = make_uint4(0, 0, 0, 0);
+      if (row < row_end && c < a.C) {
+        const int64_t i = row * a.C + c;
+        if constexpr (NEXT) {
+          fx[j] = fetch8(a.x, i);
+          fn[j] = fetch8(a.dn, i);
+        }
+        if constexpr (DELTA) {
+          fd[j] = fetch8(a.delta, i);
+          if (a.dh) fh[j] = fetch8(a.dh, i);
+        }
+      }
+    }
+    fr[0] = DELTA && row < row_end ? a.rd[row] : 0.f;
+    fr[1] = NEXT && row < row_end ? a.rh[row] : 0.f;
+  };
+  if constexpr (H16) fetch_row(r0 + sub);
   load_factors<V, DELTA, NEXT>(a, group, kq, wn);
   float an[NV][V], at_[NV][V];
 #pragma unroll
@@ -278,11 +344,24 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
 #pragma unroll
     for (int k = 0; k < V; ++k) an[j][k] = at_[j][k] = 0.f;
 
-  for (int64_t r0 = group * a.group_rows + (int64_t)part * RB; r0 < row_end; r0 += (int64_t)a.per_group * RB) {
+  for (; r0 < row_end; r0 += stride) {
     const int64_t row = r0 + sub;
     const bool live = row < row_end;
     const int64_t at = row * a.C;
     float x[NV][V], d[NV][V], gh[NV][V], gn[NV][V];
+    float rd, rh;
+    if constexpr (H16) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        widen8(fx[j], a.x_dt, x[j]);
+        widen8(fd[j], a.d_dt, d[j]);
+        widen8(fh[j], a.x_dt, gh[j]);
+        widen8(fn[j], a.n_dt, gn[j]);
+      }
+      rd = fr[0];
+      rh = fr[1];
+      fetch_row(row + stride);
+    } else {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * V;
@@ -297,7 +376,9 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) norm_bwd_kernel(const Args 
         if (DELTA && a.dh) ldv<V>(a.dh, a.x_dt, at + c, gh[j]);
       }
     }
-    const float rd = DELTA && live ? a.rd[row] : 0.f, rh = NEXT && live ? a.rh[row] : 0.f;
+    rd = DELTA && live ? a.rd[row] : 0.f;
+    rh = NEXT && live ? a.rh[row] : 0.f;
+    }
     const float sc = DELTA && a.scale && live ? a.scale[sample_of(a, row)] : 1.f;
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -492,8 +573,8 @@ __global__ void __launch_bounds__(256) norm_long_bwd_kernel(const Args a) {
 
 // Column sums of the partial rows, 32 channels a block, 32 threads a channel,
 // added in an order that the shape alone fixes.  blockIdx.y: 0 the next norm's
-// gradient, 1 the post-norm's (sum over the groups of q t), 2 + g group g's
-// gate (wp t).  One chain of loads is what this kernel takes, so each thread
+// gradient, 1 the post-norm's (sum over the groups of q t), 2 and on the
+// groups' gates (wp t).  One chain of loads is what this kernel takes, so each thread
 // has four of them in flight.
 struct SumArgs {
   const float* part;
@@ -502,6 +583,8 @@ struct SumArgs {
   const void* wp;
   const void* q;
   int q_rows, wp_dt, q_dt, wn_dt;
+  int few;        // the groups have few parts: a thread adds up a group's
+  int64_t ys;
   void* dnext;
   void* dpost;
   void* dgate;
@@ -511,10 +594,22 @@ __global__ void __launch_bounds__(1024) norm_sum_kernel(const SumArgs a) {
   __shared__ float sh[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
-  const int64_t ys = a.at_t < 0 ? 1 : 2 + (a.q_rows ? a.groups : 0);
+  const int64_t ys = a.ys;
   for (int64_t y = blockIdx.y; y < ys; y += gridDim.y) {
     void* out = y == 0 ? a.dnext : y == 1 ? a.dpost : a.dgate;
     if (!out) continue;
+    if (y >= 2 && a.few) {  // 32 groups at once, a thread each
+      const int64_t g = (y - 2) * 32 + ry;
+      if (c < a.C && g < a.groups) {
+        float v[1] = {0.f};
+        const float* p = a.part + (g * a.per_group * a.arrays + a.at_t) * a.C + c;
+#pragma unroll 4
+        for (int i = 0; i < a.per_group; ++i) v[0] += p[(int64_t)i * a.arrays * a.C];
+        v[0] *= ld1(a.wp, a.wp_dt, c);
+        stv<1>(out, a.q_dt, g * a.C + c, v);
+      }
+      continue;
+    }
     const int64_t stride = (int64_t)a.arrays * a.C;
     const float* p = a.part + (y == 0 ? 0 : (int64_t)a.at_t * a.C) + c;
     int64_t n = a.groups * a.per_group;
@@ -637,6 +732,10 @@ int split_bwd(int C, bool vec, F&& f) {
 
 bool too_long(int C, bool vec) { return C > (vec ? LONG_V : LONG_1); }
 
+bool all16(const Args& k, bool delta, bool next) {
+  return k.x_dt != OW_DTYPE_F32 && (!delta || k.d_dt != OW_DTYPE_F32) && (!next || k.n_dt != OW_DTYPE_F32);
+}
+
 int reserve(const void* kern, size_t smem) {
   if (smem <= 48 * 1024) return OW_OK;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -653,8 +752,8 @@ int modes(bool delta, bool next, F&& f) {
   return f(std::false_type(), std::true_type());
 }
 
-// The blocks: ``per_sm`` an SM, no more than there are rows, shared out over
-// the groups of rows with a gate of their own.
+// The blocks: at most ``per_sm`` an SM, no more than there are rows, shared out
+// over the groups of rows with a gate of their own.
 void parts(const ow_norm_t* a, Args* k, int per_sm) {
   k->groups = a->gate_rows > 1 ? a->samples : 1;
   k->group_rows = k->rows / std::max<int64_t>(k->groups, 1);
@@ -664,7 +763,11 @@ void parts(const ow_norm_t* a, Args* k, int per_sm) {
   k->arrays = (a->next_w ? 1 : 0) + (a->delta ? 1 : 0);
 }
 
-constexpr int FWD_PER_SM = 6, BWD_PER_SM = 3;  // what the registers (40 and 80 a thread) let run at once
+// Blocks an SM runs at once, by the registers of the kernels' threads (40 to 61
+// forward, 80 to 112 backward): more would make a second, half empty wave.
+constexpr int FWD_PER_SM = 6, BWD_PER_SM = 3;
+constexpr int fwd_per_sm(int nv, bool h16) { return nv == 1 ? (h16 ? 5 : 6) : nv == 2 ? (h16 ? 3 : 4) : (h16 ? 2 : 3); }
+constexpr int bwd_per_sm(int T, bool h16) { return T > 256 ? 1 : h16 ? 2 : 3; }
 
 }  // namespace
 }  // namespace ow
@@ -701,13 +804,19 @@ int ow_norm_fwd(const ow_norm_t* a, void* stream) {
     } else {
       OW_RETURN_IF(split_fwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
         constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
+        const bool h16 = V.value == 8 && all16(k, D.value, N.value);
+        parts(a, &k, V.value == 8 ? fwd_per_sm(NV.value, h16) : FWD_PER_SM);
         k.per_group = (int)std::min<int64_t>(k.per_group, (k.group_rows + RB - 1) / RB);
         OW_CHECK_ARG(k.groups * k.per_group < (1LL << 31), "ow_norm_fwd: too many samples");
         const size_t smem = (size_t)k.C * sizeof(float) * (D.value + N.value);
-        auto kern = norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value>;
-        OW_RETURN_IF(reserve((const void*)kern, smem));
-        launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
-        return OW_OK;
+        auto go = [&](auto kern) -> int {
+          OW_RETURN_IF(reserve((const void*)kern, smem));
+          launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
+          return OW_OK;
+        };
+        if constexpr (V.value == 8)
+          if (h16) return go(norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value, true>);
+        return go(norm_fwd_kernel<V.value, G.value, NV.value, D.value, N.value, false>);
       }));
     }
     OW_CHECK_LAUNCH("norm_fwd_kernel");
@@ -743,12 +852,20 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
     } else {
       OW_RETURN_IF(split_bwd(k.C, vec, [&](auto V, auto G, auto NV) -> int {
         constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
+        // with 1024 threads a row to come does not fit in their 64 registers
+        constexpr bool ROOM = V.value == 8 && T <= 512;
+        const bool h16 = ROOM && all16(k, D.value, N.value);
+        parts(a, &k, bwd_per_sm(T, h16));
         k.per_group = (int)std::min<int64_t>(k.per_group, std::max<int64_t>(1, (k.group_rows + RB - 1) / RB));
         const size_t smem = (size_t)k.C * sizeof(float) * std::max<int>(D.value + N.value, RB > 1 ? RB : 0);
-        auto kern = norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value>;
-        OW_RETURN_IF(reserve((const void*)kern, smem));
-        launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
-        return OW_OK;
+        auto go = [&](auto kern) -> int {
+          OW_RETURN_IF(reserve((const void*)kern, smem));
+          launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
+          return OW_OK;
+        };
+        if constexpr (ROOM)
+          if (h16) return go(norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value, true>);
+        return go(norm_bwd_kernel<V.value, G.value, NV.value, D.value, N.value, false>);
       }));
     }
     OW_CHECK_LAUNCH("norm_bwd_kernel");
@@ -762,8 +879,9 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
   s.dnext = next ? g->dnext : nullptr;
   s.dpost = delta ? g->dpost : nullptr;
   s.dgate = a->gate_rows ? g->dgate : nullptr;
-  const int64_t ys = s.at_t < 0 ? 1 : 2 + (s.q_rows ? s.groups : 0);
-  launch(norm_sum_kernel, dim3((k.C + 31) / 32, (unsigned)std::min<int64_t>(ys, 32768)), 1024, 0, st, s);
+  s.few = s.per_group <= 16;
+  s.ys = s.at_t < 0 ? 1 : 2 + (!s.q_rows ? 0 : s.few ? (s.groups + 31) / 32 : s.groups);
+  launch(norm_sum_kernel, dim3((k.C + 31) / 32, (unsigned)std::min<int64_t>(s.ys, 32768)), 1024, 0, st, s);
   OW_CHECK_LAUNCH("norm_sum_kernel");
   return OW_OK;
 }

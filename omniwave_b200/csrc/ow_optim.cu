@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_fp8.h>
 
@@ -130,11 +131,11 @@ __device__ __forceinline__ void random20(uint32_t seed, uint32_t e, uint32_t& r1
 
 // |x| inv, at most 448, as an e4m3 magnitude.  Times 2^-120 the exponents of
 // e4m3 (subnormals included) are those of f32, so the code is the top bits and
-// adding a random number below them rounds.  A NaN keeps being one.
-__device__ __forceinline__ uint32_t hold8(float x, float inv, uint32_t r20) {
+// adding a random number below them rounds.  ``most``: 126, or 127 (a NaN) in a
+// block that holds values that are not finite.
+__device__ __forceinline__ uint32_t hold8(float x, float inv, uint32_t r20, uint32_t most) {
   const float y = __fmul_rn(fabsf(x), inv);
-  const uint32_t q = (__float_as_uint(y * 7.52316384526264e-37f) + r20) >> 20;  // 2^-120
-  return y != y ? 127u : min(q, 126u);
+  return min((__float_as_uint(y * 7.52316384526264e-37f) + r20) >> 20, most);  // 2^-120
 }
 
 __device__ __forceinline__ void unhold4(uint32_t codes, float scale, float (&o)[4]) {
@@ -159,8 +160,72 @@ struct StepArgs {
   int ntensors;
 };
 
+// A block's values as they come from memory.
+template <typename T, bool EIGHT>
+struct Fetched {
+  int used;     // elements of the block in use
+  const T* g;   // the block's first gradient; NULL: nothing to do
+  T* p;
+  bool vec;
+  float t;      // the tensor's steps, this one included
+  using W = std::conditional_t<sizeof(T) == 4, float4, uint2>;
+  W pw[2], gw[2];
+  uint32_t mc[2], vc[2];  // 8 bits
+  float ms, vs;
+  float4 mw[2], vw[2];    // 32 bits
+};
+
 template <typename T, bool EIGHT, int MAXT>
-__global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const StepArgs a) {
+__device__ __forceinline__ void fetch(Fetched<T, EIGHT>& f, const Ptrs<MAXT>& ptr, const StepArgs& a, int64_t blk, int4 rec) {
+  const int lane = threadIdx.x & 31;
+  f.used = rec.z;
+  const T* g = reinterpret_cast<const T*>(ptr.g[rec.x - a.tab.t0]);
+  f.g = g;
+  if (!g) return;
+  f.g = g + (int64_t)rec.y * BLK;
+  f.p = reinterpret_cast<T*>(ptr.p[rec.x - a.tab.t0]) + (int64_t)rec.y * BLK;
+  f.vec = aligned4<T>(f.p) && aligned4<T>(f.g) && rec.z == BLK;
+  f.t = a.steps[rec.x] + 1.f;
+  const int64_t slot = blk * BLK;
+  using W = typename Fetched<T, EIGHT>::W;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int e = j * 128 + lane * 4;
+    if (f.vec) {
+      f.pw[j] = *reinterpret_cast<const W*>(f.p + e);
+      f.gw[j] = *reinterpret_cast<const W*>(f.g + e);
+    }
+    if constexpr (EIGHT) {
+      f.mc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.m + slot + e);
+      f.vc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.v + slot + e);
+    } else {
+      f.mw[j] = *reinterpret_cast<const float4*>((const float*)a.m + slot + e);
+      f.vw[j] = *reinterpret_cast<const float4*>((const float*)a.v + slot + e);
+    }
+  }
+  if constexpr (EIGHT) {
+    f.ms = a.ms[blk];
+    f.vs = a.vs[blk];
+  }
+}
+
+template <typename T, typename W>
+__device__ __forceinline__ void widen(const W& w, float (&o)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
+  } else {
+    const T* h = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = Elem<T>::to_f(h[k]);
+  }
+}
+
+// 8-bit moments take some 55 instructions and 20 bytes an element, so a warp
+// asks for its next block before it works on this one; with 32 bits and 28
+// bytes the loads of the warps at hand fill the memory's pipe already (94% of
+// the copy bandwidth) and the registers are better spent on more warps.
+template <typename T, bool EIGHT, int MAXT>
+__global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const StepArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // A step that was called off leaves everything as it is.
   if (a.found_in && *a.found_in != 0.f) return;
@@ -172,102 +237,107 @@ __global__ void __launch_bounds__(WARPS * 32) adamw_kernel(const __grid_constant
   const float lr = a.lr_ptr ? *a.lr_ptr : a.lr;
   const float decay = 1.f - lr * a.wd;
   float t_have = -1.f, alpha = 0.f, rc2 = 0.f;
-  const int64_t stride = (int64_t)gridDim.x * WARPS;
+  const int64_t stride = (int64_t)gridDim.x * WARPS, nblk = a.tab.nblk;
+  const int4* records = a.tab.block + a.tab.blk0;
   int64_t b = (int64_t)blockIdx.x * WARPS + warp;
-  int4 next = b < a.tab.nblk ? a.tab.block[a.tab.blk0 + b] : make_int4(0, 0, 0, 0);
-  for (; b < a.tab.nblk; b += stride) {
-    const int4 rec = next;
-    if (b + stride < a.tab.nblk) next = a.tab.block[a.tab.blk0 + b + stride];
+  Fetched<T, EIGHT> now, next;
+  int4 ahead = b < nblk ? records[b] : make_int4(0, 0, 0, 0);
+  if (EIGHT && b < nblk) {
+    fetch(now, ptr, a, a.tab.blk0 + b, ahead);
+    if (b + stride < nblk) ahead = records[b + stride];
+  }
+  for (; b < nblk; b += stride) {
     const int64_t blk = a.tab.blk0 + b;
-    const int ti = rec.x;
-    const T* g = reinterpret_cast<const T*>(ptr.g[ti - a.tab.t0]);
-    if (!g) continue;  // no gradient: this tensor takes no step
-    g += (int64_t)rec.y * BLK;
-    T* p = reinterpret_cast<T*>(ptr.p[ti - a.tab.t0]) + (int64_t)rec.y * BLK;
-    const int64_t slot = blk * BLK;
-    const int n = rec.z;
-    const float t = a.steps[ti] + 1.f;
-    const bool vec = aligned4<T>(p) && aligned4<T>(g);
-    float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
-    uint32_t mc[2], vc[2];
-    float msc = 0.f, vsc = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int e = j * 128 + lane * 4;
-      load4(p, e, n, vec, pv[j]);
-      load4(g, e, n, vec, gv[j]);
-      if constexpr (EIGHT) {
-        mc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.m + slot + e);
-        vc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.v + slot + e);
-      } else {
-        load4((const float*)a.m + slot, e, BLK, true, mv[j]);
-        load4((const float*)a.v + slot, e, BLK, true, vv[j]);
-      }
-    }
-    if constexpr (EIGHT) {
-      msc = a.ms[blk];
-      vsc = a.vs[blk];
-    }
-    if (t != t_have) {  // most often all tensors are at the same step
-      t_have = t;
-      alpha = lr / -expm1f(t * a.ln_b1);
-      rc2 = rsqrtf(-expm1f(t * a.ln_b2));
-    }
-    float mmax = 0.f, vmax = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if constexpr (EIGHT) {
-        unhold4(mc[j], msc, mv[j]);
-        unhold4(vc[j], vsc, vv[j]);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // Every product and sum of the moments is rounded on its own (no fused
-        // multiply-add), so they, and with them the codes, are those of the
-        // formula taken operation by operation in f32, on any machine.
-        const float gg = __fmul_rn(gv[j][k], coef);
-        const float m = __fadd_rn(__fmul_rn(a.b1, mv[j][k]), __fmul_rn(a.b1c, gg));
-        const float v = __fadd_rn(__fmul_rn(a.b2, vv[j][k]), __fmul_rn(__fmul_rn(a.b2c, gg), gg));
-        pv[j][k] = pv[j][k] * decay - alpha * __fdividef(m, fast_sqrt(v) * rc2 + a.eps);
-        mv[j][k] = m;
-        vv[j][k] = v;
-        if constexpr (EIGHT) {
-          mmax = fmaxf(mmax, fabsf(m));
-          vmax = fmaxf(vmax, v);
-        }
-      }
-      store4(p, j * 128 + lane * 4, n, vec, pv[j]);
-      if constexpr (!EIGHT) {
-        store4((float*)a.m + slot, j * 128 + lane * 4, BLK, true, mv[j]);
-        store4((float*)a.v + slot, j * 128 + lane * 4, BLK, true, vv[j]);
-      }
-    }
-    if constexpr (EIGHT) {
-      mmax = warp_max(mmax);
-      vmax = warp_max(vmax);
-      const uint32_t seed = random_seed(slot, (uint32_t)t) + lane * 4 * 0x9E3779B1u;
-      const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
-      const uint32_t least = vinv > 0.f ? 1u : 0u;
+    constexpr int AHEAD = EIGHT ? 2 : 1;
+    const int4 rec = ahead;
+    if (b + AHEAD * stride < nblk) ahead = records[b + AHEAD * stride];
+    if (!EIGHT) fetch(now, ptr, a, blk, rec);
+    else if (b + stride < nblk) fetch(next, ptr, a, blk + stride, rec);
+    if (now.g) {  // without a gradient a tensor takes no step
+      const int64_t slot = blk * BLK;
+      const int n = now.used;
+      const bool vec = now.vec;
+      float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint32_t om = 0, ov = 0;
+        if (vec) {
+          widen<T>(now.pw[j], pv[j]);
+          widen<T>(now.gw[j], gv[j]);
+        } else {
+          load4(now.p, j * 128 + lane * 4, n, false, pv[j]);
+          load4(now.g, j * 128 + lane * 4, n, false, gv[j]);
+        }
+        if constexpr (EIGHT) {
+          unhold4(now.mc[j], now.ms, mv[j]);
+          unhold4(now.vc[j], now.vs, vv[j]);
+        } else {
+          widen<float>(now.mw[j], mv[j]);
+          widen<float>(now.vw[j], vv[j]);
+        }
+      }
+      if (now.t != t_have) {  // most often all tensors are at the same step
+        t_have = now.t;
+        alpha = lr / -expm1f(t_have * a.ln_b1);
+        rc2 = rsqrtf(-expm1f(t_have * a.ln_b2));
+      }
+      float mmax = 0.f;
+      uint32_t vtop = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint32_t r1, r2;
-          random20(seed, j * 128 + k, r1, r2);
-          const uint32_t qm = hold8(mv[j][k], minv, r1) | (__float_as_uint(mv[j][k]) >> 24 & 128u);
-          const uint32_t qv = max(hold8(vv[j][k], vinv, r2), vv[j][k] > 0.f ? least : 0u);
-          om |= qm << (8 * k);
-          ov |= qv << (8 * k);
+          // Every product and sum of the moments is rounded on its own (no fused
+          // multiply-add), so they, and with them the codes, are those of the
+          // formula taken operation by operation in f32, on any machine.
+          const float gg = __fmul_rn(gv[j][k], coef);
+          const float m = __fadd_rn(__fmul_rn(a.b1, mv[j][k]), __fmul_rn(a.b1c, gg));
+          const float v = __fadd_rn(__fmul_rn(a.b2, vv[j][k]), __fmul_rn(__fmul_rn(a.b2c, gg), gg));
+          pv[j][k] = pv[j][k] * decay - alpha * __fdividef(m, fast_sqrt(v) * rc2 + a.eps);
+          mv[j][k] = m;
+          vv[j][k] = v;
+          if constexpr (EIGHT) {
+            mmax = fmaxf(mmax, fabsf(m));
+            vtop = max(vtop, __float_as_uint(v));  // v is not negative; an inf or a NaN is the largest
+          }
         }
-        *reinterpret_cast<uint32_t*>((unsigned char*)a.m + slot + j * 128 + lane * 4) = om;
-        *reinterpret_cast<uint32_t*>((unsigned char*)a.v + slot + j * 128 + lane * 4) = ov;
+        store4(now.p, j * 128 + lane * 4, n, vec, pv[j]);
+        if constexpr (!EIGHT) {
+          store4((float*)a.m + slot, j * 128 + lane * 4, BLK, true, mv[j]);
+          store4((float*)a.v + slot, j * 128 + lane * 4, BLK, true, vv[j]);
+        }
       }
-      if (lane == 0) {
-        a.ms[blk] = mmax > TINY ? __fmul_rn(mmax, 1.f / 448.f) : 0.f;
-        a.vs[blk] = vmax > TINY ? __fmul_rn(vmax, 1.f / 448.f) : 0.f;
+      if constexpr (EIGHT) {
+        mmax = warp_max(mmax);
+        vtop = __reduce_max_sync(0xffffffffu, vtop);
+        const float vmax = __uint_as_float(vtop);
+        const uint32_t seed = random_seed(slot, (uint32_t)t_have) + lane * 4 * 0x9E3779B1u;
+        const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
+        const uint32_t least = vinv > 0.f ? 1u : 0u;
+        // A gradient that is not finite (and was not called off) makes v so; then
+        // the codes of the elements concerned are NaN.
+        const uint32_t odd = vtop >= 0x7F800000u ? 127u : 126u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t om = 0, ov = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t r1, r2;
+            random20(seed, j * 128 + k, r1, r2);
+            const uint32_t qm = hold8(mv[j][k], minv, r1, odd) | (__float_as_uint(mv[j][k]) >> 24 & 128u);
+            const uint32_t qv = max(hold8(vv[j][k], vinv, r2, odd), min(__float_as_uint(vv[j][k]), least));
+            om |= qm << (8 * k);
+            ov |= qv << (8 * k);
+          }
+          *reinterpret_cast<uint32_t*>((unsigned char*)a.m + slot + j * 128 + lane * 4) = om;
+          *reinterpret_cast<uint32_t*>((unsigned char*)a.v + slot + j * 128 + lane * 4) = ov;
+        }
+        if (lane == 0) {
+          a.ms[blk] = mmax > TINY ? __fmul_rn(mmax, 1.f / 448.f) : 0.f;
+          a.vs[blk] = vmax > TINY ? __fmul_rn(vmax, 1.f / 448.f) : 0.f;
+        }
       }
     }
+    if constexpr (EIGHT) now = next;
   }
   // The last block counts the step: every block has read the counts by then.
   __shared__ bool last;
@@ -418,7 +488,7 @@ int by_type(int dtype, F&& f) {
   return f((__half*)nullptr);
 }
 
-constexpr int NORM_PER_SM = 6, STEP_PER_SM = 8;
+constexpr int NORM_PER_SM = 8, STEP_PER_SM = 3, STEP8_PER_SM = 2;  // blocks the registers let run at once
 
 }  // namespace
 }  // namespace ow
@@ -490,7 +560,7 @@ int ow_adamw_step(const ow_adamw_t* a, void* stream) {
     return each_launch(a, [&](auto& ptr, const Tables& tab, int n, bool) -> int {
       k.tab = tab;
       k.ntensors = n;
-      const int grid = grid_for(tab.nblk, STEP_PER_SM);
+      const int grid = grid_for(tab.nblk, a->state_bits == 8 ? STEP8_PER_SM : STEP_PER_SM);
       using P = std::remove_reference_t<decltype(ptr)>;
       constexpr int MAXT = sizeof(ptr.p) / sizeof(void*);
       if (a->state_bits == 8)
