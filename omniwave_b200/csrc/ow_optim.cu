@@ -102,10 +102,17 @@ __device__ __forceinline__ bool aligned4(const void* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
 
+// sqrt(v) and m / d in three and two instructions, within two steps of f32.
+// Below 2^-126 the root is taken a little small instead of as 0.
 __device__ __forceinline__ float fast_sqrt(float v) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(v, 1.17549435e-38f)));
+  return v * r;
+}
+__device__ __forceinline__ float fast_div(float m, float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return m * r;
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -246,37 +253,31 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
     fetch(now, ptr, a, a.tab.blk0 + b, ahead);
     if (b + stride < nblk) ahead = records[b + stride];
   }
-  for (; b < nblk; b += stride) {
-    const int64_t blk = a.tab.blk0 + b;
-    constexpr int AHEAD = EIGHT ? 2 : 1;
-    const int4 rec = ahead;
-    if (b + AHEAD * stride < nblk) ahead = records[b + AHEAD * stride];
-    if (!EIGHT) fetch(now, ptr, a, blk, rec);
-    else if (b + stride < nblk) fetch(next, ptr, a, blk + stride, rec);
-    if (now.g) {  // without a gradient a tensor takes no step
+  auto work = [&](const Fetched<T, EIGHT>& f, int64_t blk) {
+    if (f.g) {  // without a gradient a tensor takes no step
       const int64_t slot = blk * BLK;
-      const int n = now.used;
-      const bool vec = now.vec;
+      const int n = f.used;
+      const bool vec = f.vec;
       float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (vec) {
-          widen<T>(now.pw[j], pv[j]);
-          widen<T>(now.gw[j], gv[j]);
+          widen<T>(f.pw[j], pv[j]);
+          widen<T>(f.gw[j], gv[j]);
         } else {
-          load4(now.p, j * 128 + lane * 4, n, false, pv[j]);
-          load4(now.g, j * 128 + lane * 4, n, false, gv[j]);
+          load4(f.p, j * 128 + lane * 4, n, false, pv[j]);
+          load4(f.g, j * 128 + lane * 4, n, false, gv[j]);
         }
         if constexpr (EIGHT) {
-          unhold4(now.mc[j], now.ms, mv[j]);
-          unhold4(now.vc[j], now.vs, vv[j]);
+          unhold4(f.mc[j], f.ms, mv[j]);
+          unhold4(f.vc[j], f.vs, vv[j]);
         } else {
-          widen<float>(now.mw[j], mv[j]);
-          widen<float>(now.vw[j], vv[j]);
+          widen<float>(f.mw[j], mv[j]);
+          widen<float>(f.vw[j], vv[j]);
         }
       }
-      if (now.t != t_have) {  // most often all tensors are at the same step
-        t_have = now.t;
+      if (f.t != t_have) {  // most often all tensors are at the same step
+        t_have = f.t;
         alpha = lr / -expm1f(t_have * a.ln_b1);
         rc2 = rsqrtf(-expm1f(t_have * a.ln_b2));
       }
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
           const float gg = __fmul_rn(gv[j][k], coef);
           const float m = __fadd_rn(__fmul_rn(a.b1, mv[j][k]), __fmul_rn(a.b1c, gg));
           const float v = __fadd_rn(__fmul_rn(a.b2, vv[j][k]), __fmul_rn(__fmul_rn(a.b2c, gg), gg));
-          pv[j][k] = pv[j][k] * decay - alpha * __fdividef(m, fast_sqrt(v) * rc2 + a.eps);
+          pv[j][k] = pv[j][k] * decay - alpha * fast_div(m, fast_sqrt(v) * rc2 + a.eps);
           mv[j][k] = m;
           vv[j][k] = v;
           if constexpr (EIGHT) {
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
             vtop = max(vtop, __float_as_uint(v));  // v is not negative; an inf or a NaN is the largest
           }
         }
-        store4(now.p, j * 128 + lane * 4, n, vec, pv[j]);
+        store4(f.p, j * 128 + lane * 4, n, vec, pv[j]);
         if constexpr (!EIGHT) {
           store4((float*)a.m + slot, j * 128 + lane * 4, BLK, true, mv[j]);
           store4((float*)a.v + slot, j * 128 + lane * 4, BLK, true, vv[j]);
@@ -337,7 +338,27 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
         }
       }
     }
-    if constexpr (EIGHT) now = next;
+  };
+  if constexpr (EIGHT) {
+    // two sets of registers in turn: nothing is moved from one to the other
+    auto turn = [&](Fetched<T, EIGHT>& f, Fetched<T, EIGHT>& g) {
+      const int4 rec = ahead;
+      if (b + 2 * stride < nblk) ahead = records[b + 2 * stride];
+      if (b + stride < nblk) fetch(g, ptr, a, a.tab.blk0 + b + stride, rec);
+      work(f, a.tab.blk0 + b);
+      b += stride;
+      return b < nblk;
+    };
+    if (b < nblk)
+      while (turn(now, next) && turn(next, now)) {
+      }
+  } else {
+    for (; b < nblk; b += stride) {
+      const int4 rec = ahead;
+      if (b + stride < nblk) ahead = records[b + stride];
+      fetch(now, ptr, a, a.tab.blk0 + b, rec);
+      work(now, a.tab.blk0 + b);
+    }
   }
   // The last block counts the step: every block has read the counts by then.
   __shared__ bool last;
@@ -488,7 +509,7 @@ int by_type(int dtype, F&& f) {
   return f((__half*)nullptr);
 }
 
-constexpr int NORM_PER_SM = 8, STEP_PER_SM = 3, STEP8_PER_SM = 2;  // blocks the registers let run at once
+constexpr int NORM_PER_SM = 6, STEP_PER_SM = 3, STEP8_PER_SM = 2;  // blocks the registers let run at once
 
 }  // namespace
 }  // namespace ow
