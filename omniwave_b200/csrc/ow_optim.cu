@@ -167,7 +167,9 @@ struct StepArgs {
   int ntensors;
 };
 
-// A block's values as they come from memory.
+// Where a block's values are and, with 32 bits, the values as they come from
+// memory.  With 8 bits they come by asynchronous copies to the thread's own
+// slots in shared memory: every thread reads back what it asked for itself.
 template <typename T, bool EIGHT>
 struct Fetched {
   int used;     // elements of the block in use
@@ -175,15 +177,28 @@ struct Fetched {
   T* p;
   bool vec;
   float t;      // the tensor's steps, this one included
+  float ms, vs; // 8 bits
   using W = std::conditional_t<sizeof(T) == 4, float4, uint2>;
-  W pw[2], gw[2];
-  uint32_t mc[2], vc[2];  // 8 bits
-  float ms, vs;
-  float4 mw[2], vw[2];    // 32 bits
+  W pw[EIGHT ? 1 : 2], gw[EIGHT ? 1 : 2];
+  float4 mw[EIGHT ? 1 : 2], vw[EIGHT ? 1 : 2];
 };
 
+template <typename T>
+struct Slots {
+  using W = typename Fetched<T, true>::W;
+  W p[2][WARPS * 32], g[2][WARPS * 32];
+  uint32_t m[2][WARPS * 32], v[2][WARPS * 32];
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES)
+               : "memory");
+}
+
 template <typename T, bool EIGHT, int MAXT>
-__device__ __forceinline__ void fetch(Fetched<T, EIGHT>& f, const Ptrs<MAXT>& ptr, const StepArgs& a, int64_t blk, int4 rec) {
+__device__ __forceinline__ void fetch(Fetched<T, EIGHT>& f, Slots<T>* to, const Ptrs<MAXT>& ptr, const StepArgs& a, int64_t blk,
+                                      int4 rec) {
   const int lane = threadIdx.x & 31;
   f.used = rec.z;
   const T* g = reinterpret_cast<const T*>(ptr.g[rec.x - a.tab.t0]);
@@ -198,14 +213,18 @@ __device__ __forceinline__ void fetch(Fetched<T, EIGHT>& f, const Ptrs<MAXT>& pt
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int e = j * 128 + lane * 4;
-    if (f.vec) {
-      f.pw[j] = *reinterpret_cast<const W*>(f.p + e);
-      f.gw[j] = *reinterpret_cast<const W*>(f.g + e);
-    }
     if constexpr (EIGHT) {
-      f.mc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.m + slot + e);
-      f.vc[j] = *reinterpret_cast<const uint32_t*>((const unsigned char*)a.v + slot + e);
+      if (f.vec) {
+        copy_async<sizeof(W)>(&to->p[j][threadIdx.x], f.p + e);
+        copy_async<sizeof(W)>(&to->g[j][threadIdx.x], f.g + e);
+      }
+      copy_async<4>(&to->m[j][threadIdx.x], (const unsigned char*)a.m + slot + e);
+      copy_async<4>(&to->v[j][threadIdx.x], (const unsigned char*)a.v + slot + e);
     } else {
+      if (f.vec) {
+        f.pw[j] = *reinterpret_cast<const W*>(f.p + e);
+        f.gw[j] = *reinterpret_cast<const W*>(f.g + e);
+      }
       f.mw[j] = *reinterpret_cast<const float4*>((const float*)a.m + slot + e);
       f.vw[j] = *reinterpret_cast<const float4*>((const float*)a.v + slot + e);
     }
@@ -227,12 +246,12 @@ __device__ __forceinline__ void widen(const W& w, float (&o)[4]) {
   }
 }
 
-// 8-bit moments take some 55 instructions and 20 bytes an element, so a warp
-// asks for its next block before it works on this one; with 32 bits and 28
-// bytes the loads of the warps at hand fill the memory's pipe already (94% of
-// the copy bandwidth) and the registers are better spent on more warps.
+// 8-bit moments take some 80 instructions and 10 to 16 bytes an element, so a
+// warp asks for its next block before it works on this one, by copies that hold
+// no registers; with 32 bits and 28 bytes the loads of the warps at hand fill
+// the memory's pipe already (88% of the copy bandwidth).
 template <typename T, bool EIGHT, int MAXT>
-__global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const StepArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, 3) adamw_kernel(const __grid_constant__ Ptrs<MAXT> ptr, const StepArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // A step that was called off leaves everything as it is.
   if (a.found_in && *a.found_in != 0.f) return;
@@ -248,12 +267,14 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
   const int4* records = a.tab.block + a.tab.blk0;
   int64_t b = (int64_t)blockIdx.x * WARPS + warp;
   Fetched<T, EIGHT> now, next;
+  __shared__ Slots<T> slots[EIGHT ? 2 : 1];
   int4 ahead = b < nblk ? records[b] : make_int4(0, 0, 0, 0);
   if (EIGHT && b < nblk) {
-    fetch(now, ptr, a, a.tab.blk0 + b, ahead);
+    fetch(now, slots, ptr, a, a.tab.blk0 + b, ahead);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (b + stride < nblk) ahead = records[b + stride];
   }
-  auto work = [&](const Fetched<T, EIGHT>& f, int64_t blk) {
+  auto work = [&](const Fetched<T, EIGHT>& f, const Slots<T>& in, int64_t blk) {
     if (f.g) {  // without a gradient a tensor takes no step
       const int64_t slot = blk * BLK;
       const int n = f.used;
@@ -261,16 +282,19 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
       float pv[2][4], gv[2][4], mv[2][4], vv[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (vec) {
-          widen<T>(f.pw[j], pv[j]);
-          widen<T>(f.gw[j], gv[j]);
+        if (vec && EIGHT) {
+          widen<T>(in.p[j][threadIdx.x], pv[j]);
+          widen<T>(in.g[j][threadIdx.x], gv[j]);
+        } else if (vec) {
+          widen<T>(f.pw[EIGHT ? 0 : j], pv[j]);
+          widen<T>(f.gw[EIGHT ? 0 : j], gv[j]);
         } else {
           load4(f.p, j * 128 + lane * 4, n, false, pv[j]);
           load4(f.g, j * 128 + lane * 4, n, false, gv[j]);
         }
         if constexpr (EIGHT) {
-          unhold4(f.mc[j], f.ms, mv[j]);
-          unhold4(f.vc[j], f.vs, vv[j]);
+          unhold4(in.m[j][threadIdx.x], f.ms, mv[j]);
+          unhold4(in.v[j][threadIdx.x], f.vs, vv[j]);
         } else {
           widen<float>(f.mw[j], mv[j]);
           widen<float>(f.vw[j], vv[j]);
@@ -340,24 +364,26 @@ __global__ void __launch_bounds__(WARPS * 32, EIGHT ? 2 : 3) adamw_kernel(const 
     }
   };
   if constexpr (EIGHT) {
-    // two sets of registers in turn: nothing is moved from one to the other
-    auto turn = [&](Fetched<T, EIGHT>& f, Fetched<T, EIGHT>& g) {
+    // two sets of slots in turn; the newest copies are left under way
+    auto turn = [&](Fetched<T, EIGHT>& f, int at, Fetched<T, EIGHT>& g) {
       const int4 rec = ahead;
       if (b + 2 * stride < nblk) ahead = records[b + 2 * stride];
-      if (b + stride < nblk) fetch(g, ptr, a, a.tab.blk0 + b + stride, rec);
-      work(f, a.tab.blk0 + b);
+      if (b + stride < nblk) fetch(g, slots + (at ^ 1), ptr, a, a.tab.blk0 + b + stride, rec);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      work(f, slots[at], a.tab.blk0 + b);
       b += stride;
       return b < nblk;
     };
     if (b < nblk)
-      while (turn(now, next) && turn(next, now)) {
+      while (turn(now, 0, next) && turn(next, 1, now)) {
       }
   } else {
     for (; b < nblk; b += stride) {
       const int4 rec = ahead;
       if (b + stride < nblk) ahead = records[b + stride];
-      fetch(now, ptr, a, a.tab.blk0 + b, rec);
-      work(now, a.tab.blk0 + b);
+      fetch(now, slots, ptr, a, a.tab.blk0 + b, rec);
+      work(now, slots[0], a.tab.blk0 + b);
     }
   }
   // The last block counts the step: every block has read the counts by then.
@@ -509,7 +535,7 @@ int by_type(int dtype, F&& f) {
   return f((__half*)nullptr);
 }
 
-constexpr int NORM_PER_SM = 6, STEP_PER_SM = 3, STEP8_PER_SM = 2;  // blocks the registers let run at once
+constexpr int NORM_PER_SM = 6, STEP_PER_SM = 3;  // blocks the registers let run at once
 
 }  // namespace
 }  // namespace ow
@@ -581,7 +607,7 @@ int ow_adamw_step(const ow_adamw_t* a, void* stream) {
     return each_launch(a, [&](auto& ptr, const Tables& tab, int n, bool) -> int {
       k.tab = tab;
       k.ntensors = n;
-      const int grid = grid_for(tab.nblk, a->state_bits == 8 ? STEP8_PER_SM : STEP_PER_SM);
+      const int grid = grid_for(tab.nblk, STEP_PER_SM);
       using P = std::remove_reference_t<decltype(ptr)>;
       constexpr int MAXT = sizeof(ptr.p) / sizeof(void*);
       if (a->state_bits == 8)
