@@ -1,6 +1,6 @@
 // Host side of the operators around the block, as a Python module
 // (omniwave_b200._host): argument checks, autograd and the calls of the C ABI
-// for the norms and the linear layer, and the pointer lists of AdamW.
+// for the norms and the linear layer, and AdamW's step over its buckets.
 //
 // It is native because these operators are short: a few rows take the GPU 2 to
 // 5 us, and the same checks, allocations and autograd nodes took 25 us in
@@ -16,7 +16,9 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
+#include <variant>
 #include <vector>
 
 #include "omniwave_b200.h"
@@ -428,27 +430,32 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, int64_t 
 }
 
 // ------------------------------------------------------------------ AdamW
-// The parameters of one bucket as they were added; gather() writes down where
-// they and their gradients are now.
-struct Gather {
+// The parameters of one bucket as they were added, and the arguments of its
+// calls (an ow_adamw_t and the arrays it points to, which the optimizer owns).
+struct Bucket {
   std::vector<Tensor> params;
   std::vector<std::vector<int64_t>> sizes, strides;
   at::ScalarType dtype;
   at::Device device;
+  ow_adamw_t* args;
+  void** p;
+  void** g;
+  int32_t partials;
+  std::vector<Tensor> copied;  // gradients of this step in other strides than their parameters'
 
-  explicit Gather(std::vector<Tensor> ps) : params(std::move(ps)), dtype(params.at(0).scalar_type()), device(params.at(0).device()) {
-    for (const Tensor& p : params) {
-      sizes.push_back(p.sizes().vec());
-      strides.push_back(p.strides().vec());
+  Bucket(std::vector<Tensor> ps, uintptr_t args_, uintptr_t p_, uintptr_t g_)
+      : params(std::move(ps)), dtype(params.at(0).scalar_type()), device(params.at(0).device()),
+        args(reinterpret_cast<ow_adamw_t*>(args_)), p(reinterpret_cast<void**>(p_)), g(reinterpret_cast<void**>(g_)),
+        partials(ow_grad_norm_partials(args)) {
+    for (const Tensor& t : params) {
+      sizes.push_back(t.sizes().vec());
+      strides.push_back(t.strides().vec());
     }
   }
 
-  // (whether any parameter has a gradient, the gradients that had to be copied)
-  std::pair<bool, std::vector<Tensor>> gather(uintptr_t p_at, uintptr_t g_at) const {
-    void** p = reinterpret_cast<void**>(p_at);
-    void** g = reinterpret_cast<void**>(g_at);
+  // Writes down where the parameters and gradients are now; false if no parameter has a gradient.
+  bool gather() {
     bool some = false;
-    std::vector<Tensor> copied;
     for (size_t i = 0; i < params.size(); ++i) {
       const Tensor& t = params[i];
       TORCH_CHECK(t.scalar_type() == dtype && t.device() == device && t.layout() == at::kStrided &&
@@ -470,9 +477,68 @@ struct Gather {
       g[i] = d.data_ptr();
       some = true;
     }
-    return {some, copied};
+    return some;
   }
 };
+
+// A bucket's group: lr (or a device lr), betas, eps, weight decay.
+using Hyper = std::tuple<std::variant<double, Tensor>, std::pair<double, double>, double, double>;
+
+// One step over the buckets, with the norm of all gradients first when it is
+// asked for (``partials`` given).
+void adamw_step(const std::vector<Bucket*>& buckets, const std::vector<Hyper>& hyper, const OptTensor& found_,
+                const OptTensor& partials_, const OptTensor& norm_, double max_norm, bool skip_nonfinite) {
+  const at::NoGradGuard no_grad;
+  const at::Device device = buckets.at(0)->device;
+  const c10::cuda::CUDAGuard guard(device);
+  const Tensor found = value(found_), partials = value(partials_);
+  if (found.defined())
+    OW_VALUE(found.scalar_type() == at::kFloat && found.numel() == 1 && found.device() == device,
+             "found_inf must be one float32 on the parameters' device");
+  void* stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  std::vector<size_t> todo;
+  for (size_t i = 0; i < buckets.size(); ++i) {
+    buckets[i]->copied.clear();
+    if (buckets[i]->gather()) todo.push_back(i);
+    if (const Tensor* lr = std::get_if<Tensor>(&std::get<0>(hyper.at(i))))
+      OW_VALUE(lr->scalar_type() == at::kFloat && lr->numel() == 1 && lr->device() == device,
+               "a tensor lr must be one float32 on the parameters' device");
+  }
+  if (partials.defined()) {
+    int32_t first = 0;
+    for (size_t i : todo) {
+      Bucket& b = *buckets[i];
+      b.args->control = buckets[0]->args->control;
+      ow_grad_norm_t o{};
+      o.partials = (double*)ptr(partials);
+      o.first = first;
+      o.capacity = (int32_t)partials.numel();
+      o.finish = i == todo.back();
+      o.max_norm = (float)max_norm;
+      o.skip_nonfinite = skip_nonfinite;
+      o.norm = (float*)ptr(value(norm_));
+      o.found = (float*)ptr(found);
+      check_status(ow_grad_norm(b.args, &o, stream), "ow_grad_norm");
+      first += b.partials;
+    }
+  }
+  for (size_t i : todo) {
+    Bucket& b = *buckets[i];
+    const auto& [lr, betas, eps, decay] = hyper.at(i);
+    ow_adamw_t& a = *b.args;
+    a.lr = std::holds_alternative<double>(lr) ? std::get<double>(lr) : 0.0;
+    a.lr_ptr = std::holds_alternative<Tensor>(lr) ? (const float*)ptr(std::get<Tensor>(lr)) : nullptr;
+    a.beta1 = betas.first;
+    a.beta2 = betas.second;
+    a.eps = eps;
+    a.weight_decay = decay;
+    a.found = (const float*)ptr(found);
+    a.use_norm = partials.defined();
+    a.control = buckets[0]->args->control;
+    check_status(ow_adamw_step(&a, stream), "ow_adamw_step");
+  }
+  for (Bucket* b : buckets) b->copied.clear();
+}
 
 std::pair<bool, std::optional<std::string>> told(const std::optional<std::string>& why) { return {!why.has_value(), why}; }
 
@@ -492,5 +558,8 @@ PYBIND11_MODULE(_host, m) {
   m.def("linear_supported", [](const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r) {
     return told(linear_unsupported(x, w, value(b), value(r)));
   });
-  py::class_<Gather>(m, "Gather").def(py::init<std::vector<Tensor>>()).def("gather", &Gather::gather, nogil);
+  py::class_<Bucket>(m, "Bucket")
+      .def(py::init<std::vector<Tensor>, uintptr_t, uintptr_t, uintptr_t>())
+      .def_readonly("partials", &Bucket::partials);
+  m.def("adamw_step", &adamw_step, nogil);
 }

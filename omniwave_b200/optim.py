@@ -69,7 +69,6 @@ class _Bucket:
         self.group, self.params, self.bits = group, params, bits
         dev = self.device = params[0].device
         self.dtype = params[0].dtype
-        self._gather = _lib.host().Gather(params)
         slots, total = [0], 0
         for p in params:
             total += -(-p.numel() // BLOCK) * BLOCK
@@ -103,7 +102,8 @@ class _Bucket:
             ctypes.addressof(self._slots), self.blocks.data_ptr(), self.control.data_ptr(), bits, h["exp_avg"].data_ptr(),
             h["exp_avg_sq"].data_ptr(), _lib.ptr(h.get("exp_avg_scale")), _lib.ptr(h.get("exp_avg_sq_scale")),
             h["step"].data_ptr())
-        self.partials = _lib.load().ow_grad_norm_partials(self.args)
+        self.native = _lib.host().Bucket(params, ctypes.addressof(self.args), ctypes.addressof(self._p),
+                                         ctypes.addressof(self._g))
 
     def views(self, i: int) -> dict[str, Tensor]:
         """Parameter i's share of the state, in its shape."""
@@ -115,11 +115,6 @@ class _Bucket:
             for k in ("exp_avg_scale", "exp_avg_sq_scale"):
                 out[k] = h[k][o // BLOCK:self.slots[i + 1] // BLOCK]
         return out
-
-    def gather(self) -> list[Tensor]:
-        """Write down this step's pointers; returns the gradients that had to be copied."""
-        self.some, copied = self._gather.gather(ctypes.addressof(self._p), ctypes.addressof(self._g))
-        return copied
 
 
 class AdamW(torch.optim.Optimizer):
@@ -205,7 +200,7 @@ class AdamW(torch.optim.Optimizer):
     def _norm_buffers(self) -> None:
         if self._buckets and (self.max_norm is not None or self.skip_nonfinite):
             dev = self._buckets[0].device
-            self._partials = torch.empty(sum(b.partials for b in self._buckets), dtype=torch.float64, device=dev)
+            self._partials = torch.empty(sum(b.native.partials for b in self._buckets), dtype=torch.float64, device=dev)
             if self.grad_norm is None:
                 self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
 
@@ -226,40 +221,9 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if not self._buckets:
             return loss
-        lib = _lib.load()
-        dev = self._buckets[0].device
-        if found_inf is not None and (found_inf.dtype != torch.float32 or found_inf.numel() != 1
-                                      or found_inf.device != dev):
-            raise ValueError("found_inf must be one float32 on the parameters' device")
-        found = _lib.ptr(found_inf)
-        keep = [b.gather() for b in self._buckets]
-        todo = [b for b in self._buckets if b.some]
-        if not todo:
-            return loss
-        normed = self.max_norm is not None or self.skip_nonfinite
-        control = self._buckets[0].control.data_ptr()
-        with torch.cuda.device(dev):  # the library launches on the current device
-            stream = _lib.stream_handle(dev)
-            if normed:
-                first, room = 0, self._partials.numel()
-                for b in todo:
-                    b.args.control = control
-                    opt = _lib.GradNorm(self._partials.data_ptr(), first, room, int(b is todo[-1]),
-                                        self.max_norm or 0.0, int(self.skip_nonfinite),
-                                        self.grad_norm.data_ptr(), found)
-                    _lib.check(lib.ow_grad_norm(b.args, opt, stream), "ow_grad_norm")
-                    first += b.partials
-            for b in todo:
-                a, g = b.args, b.group
-                lr = g["lr"]
-                if isinstance(lr, Tensor):
-                    a.lr, a.lr_ptr = 0.0, lr.data_ptr()
-                else:
-                    a.lr, a.lr_ptr = lr, None
-                (a.beta1, a.beta2), a.eps, a.weight_decay = g["betas"], g["eps"], g["weight_decay"]
-                a.found, a.use_norm, a.control = found, int(normed), control
-                _lib.check(lib.ow_adamw_step(a, stream), "ow_adamw_step")
-        del keep
+        hyper = [(g["lr"], g["betas"], g["eps"], g["weight_decay"]) for g in (b.group for b in self._buckets)]
+        _lib.host().adamw_step([b.native for b in self._buckets], hyper, found_inf, self._partials, self.grad_norm,
+                               self.max_norm or 0.0, self.skip_nonfinite)
         return loss
 
     # ------------------------------------------------------------ checkpoints

@@ -219,6 +219,22 @@ def test_nonfinite_gradient_leaves_everything(cuda_device, bits, bad):
     assert not torch.equal(before[1], ps[1].detach()) and float(opt.state[ps[1]]["step"]) == 2
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nonfinite_gradient_that_is_not_called_off(cuda_device, bits):
+    """It makes its own parameter NaN at once, and spoils no other block's."""
+    ps = _params(cuda_device, [1024])
+    opt = optim.AdamW(ps, lr=LR, state_bits=bits)
+    ps[0].grad[300] = float("nan")
+    opt.step()
+    bad = torch.isnan(ps[0].detach())
+    assert bad[300] and int(bad.sum()) == 1
+    ps[0].grad[300] = 0.0
+    opt.step()
+    bad = torch.isnan(ps[0].detach())
+    assert bad[300] and not bad[:256].any() and not bad[512:].any()
+    assert bits == 8 or int(bad.sum()) == 1
+
+
 def test_huge_finite_gradients_are_finite(cuda_device):
     """Squares that overflow f32 do not call a step off."""
     p = torch.nn.Parameter(torch.zeros(1000, device=cuda_device))
@@ -357,6 +373,10 @@ def test_refusals(cuda_device):
     p.grad = torch.zeros_like(p)
     with pytest.raises(ValueError, match="found_inf"):
         opt.step(found_inf=torch.zeros(2, device=cuda_device))
+    opt.param_groups[0]["lr"] = torch.zeros((), dtype=torch.float64, device=cuda_device)
+    with pytest.raises(ValueError, match="tensor lr"):
+        opt.step()
+    opt.param_groups[0]["lr"] = 1e-3
     p.data = p.data.to(BF)
     p.grad = torch.zeros_like(p)
     with pytest.raises(RuntimeError, match="moved"):
