@@ -108,9 +108,11 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
-// mbar_wait, without a look at the abort flag where the phase is complete.
+// mbar_wait for a whole warp, without a look at the abort flag where the phase
+// is complete.  The lanes agree on the answer: if the wait of one gave up, all
+// leave their loop together and none is left behind in a __syncwarp.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort);
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort));
 }
 // One lane of a converged warp, the same one each time.
 __device__ __forceinline__ bool elect_lane() {
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     // the uniform registers cost 125 cycles an MMA, whatever its size.
     const bool one = elect_lane();
     int g = 0;
-    for (int u = first; u < units && !*abort; u += step) {
+    for (int u = first; u < units; u += step) {
       const Unit t = unit_of(a, u);
       const int am0 = (t.mt * CG + (int)rank) * TM, bn0 = t.nt * BN + (int)rank * C::B_ROWS;
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       const uint32_t tmem0 = __shfl_sync(0xffffffffu, tbase, 0);
       const bool one = elect_lane();
       int g = 0, tl = 0;
-      for (int u = first; u < units && !*abort; u += step, ++tl) {
+      for (int u = first; u < units; u += step, ++tl) {
         const Unit t = unit_of(a, u);
         const int acc = tl & 1;
         if (tl >= 2 && !wait_for(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     const int q = warp & 3, group = warp >> 2;
     const Epi& e = a.e;
     int tl = 0, fetched = 0;
-    for (int u = first; u < units && !*abort; u += step, ++tl) {
+    for (int u = first; u < units; u += step, ++tl) {
       const Unit t = unit_of(a, u);
       const int acc = tl & 1;
       const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
   __shared__ float sh[8][264];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n = blockIdx.x * 256 + tx * 8;
-  const int64_t m1 = min(a.M, (blockIdx.y + 1) * a.chunk);
+  const int64_t m1 = min(a.M, (int64_t)(blockIdx.y + 1) * a.chunk);
   float s[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[k] = 0.f;

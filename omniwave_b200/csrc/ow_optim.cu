@@ -535,7 +535,10 @@ int by_type(int dtype, F&& f) {
   return f((__half*)nullptr);
 }
 
-constexpr int NORM_PER_SM = 6, STEP_PER_SM = 3;  // blocks the registers let run at once
+// Blocks an SM.  8-bit blocks are fetched ahead by warps that stay (three are
+// what the registers let run); with 32 bits more blocks than run at once even
+// out what the memory's channels take (10.2 M parameters: 46.5 against 49.5 us).
+constexpr int NORM_PER_SM = 6, STEP_PER_SM = 8, STEP8_PER_SM = 3;
 
 }  // namespace
 }  // namespace ow
@@ -607,7 +610,7 @@ int ow_adamw_step(const ow_adamw_t* a, void* stream) {
     return each_launch(a, [&](auto& ptr, const Tables& tab, int n, bool) -> int {
       k.tab = tab;
       k.ntensors = n;
-      const int grid = grid_for(tab.nblk, STEP_PER_SM);
+      const int grid = grid_for(tab.nblk, a->state_bits == 8 ? STEP8_PER_SM : STEP_PER_SM);
       using P = std::remove_reference_t<decltype(ptr)>;
       constexpr int MAXT = sizeof(ptr.p) / sizeof(void*);
       if (a->state_bits == 8)
