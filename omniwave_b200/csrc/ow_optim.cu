@@ -115,12 +115,6 @@ __device__ __forceinline__ float fast_div(float m, float d) {
   return m * r;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
 // Two 16-bit numbers from (slot, step), as the 20 bits below an e4m3 mantissa
 // see them: 16 random bits and half of the last one.  ``seed``: of the block's
 // first slot; the slots of a block differ in the low 8 bits only.
@@ -132,8 +126,8 @@ __device__ __forceinline__ void random20(uint32_t seed, uint32_t e, uint32_t& r1
   h = (h ^ (h >> 16)) * 0x7FEB352Du;
   h = (h ^ (h >> 15)) * 0x846CA68Bu;
   h ^= h >> 16;
-  r1 = ((h & 0xFFFFu) << 4) | 8u;
-  r2 = ((h >> 16) << 4) | 8u;
+  r1 = (h << 4 & 0xFFFF0u) | 8u;
+  r2 = (h >> 12 & 0xFFFF0u) | 8u;
 }
 
 // |x| inv, at most 448, as an e4m3 magnitude.  Times 2^-120 the exponents of
@@ -332,7 +326,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) adamw_kernel(const __grid_const
         }
       }
       if constexpr (EIGHT) {
-        mmax = warp_max(mmax);
+        mmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));  // not negative
         vtop = __reduce_max_sync(0xffffffffu, vtop);
         const float vmax = __uint_as_float(vtop);
         const uint32_t seed = random_seed(slot, (uint32_t)t_have) + lane * 4 * 0x9E3779B1u;
