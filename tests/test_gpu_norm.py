@@ -223,6 +223,49 @@ def test_layouts_devices_and_autocast(cuda_device):
         assert grads[2].dtype == wt
 
 
+@pytest.mark.parametrize("c", [64, 70, 300, 1025])
+@pytest.mark.parametrize("st,dt", [(F32, BF), (BF, BF)], ids=["f32bf16", "bf16"])
+def test_unaligned_arrays(cuda_device, c, st, dt):
+    """Inputs and incoming gradients that start beside a 16-byte boundary, forward and gradients."""
+    d = _inputs(cuda_device, (3, 11, c), st, dt, "bc", seed=8)
+    for k in ("x", "delta", "dh", "dn"):
+        buf = torch.empty(d[k].numel() + 1, dtype=d[k].dtype, device=cuda_device)
+        d[k] = buf[1:].view(d[k].shape).copy_(d[k])
+    want, mag = _define(d, True, "pair")
+    names = ["x", "delta", "post", "gate", "pre"]
+    leaves = {k: d[k].detach().requires_grad_() for k in names}
+    out = _call({**d, **leaves}, True, "pair")
+    _check({k: v.detach() for k, v in out.items()}, want, mag, c, 33)
+    grads = torch.autograd.grad(list(out.values()), list(leaves.values()), [d["dh"], d["dn"]])
+    _check({"d_" + k: g for k, g in zip(names, grads)}, want, mag, c, 33)
+
+
+@pytest.mark.parametrize("c", [7, 70, 129, 2049])
+@pytest.mark.parametrize("t", [F32, BF])
+def test_rows_do_not_see_their_neighbours(cuda_device, c, t):
+    """A row of NaN between others, whose 16-byte units it shares when C is ragged: they are as without it."""
+    d = _inputs(cuda_device, (2, 9, c), t, t, "c", seed=4)
+    names = ["x", "delta"]
+
+    def run(d):
+        leaves = {k: d[k].clone().requires_grad_() for k in names}
+        out = _call({**d, **leaves}, True, "pair")
+        grads = torch.autograd.grad(list(out.values()), list(leaves.values()), [d["dh"], d["dn"]])
+        return [v.detach().reshape(18, c) for v in out.values()] + [g.reshape(18, c) for g in grads]
+
+    want = run(d)
+    bad = {**d, "x": d["x"].clone(), "delta": d["delta"].clone(), "dh": d["dh"].clone()}
+    for r in (0, 5, 17):
+        for k in ("x", "delta", "dh"):
+            bad[k].view(18, c)[r] = float("nan")
+    got = run(bad)
+    fine = torch.ones(18, dtype=torch.bool, device=cuda_device)
+    fine[[0, 5, 17]] = False
+    for g, w in zip(got, want):
+        assert torch.equal(g[fine], w[fine])
+        assert torch.isnan(g[0]).all() and torch.isnan(g[17]).all()
+
+
 def test_empty(cuda_device):
     w = torch.ones(16, device=cuda_device, requires_grad=True)
     x = torch.zeros(0, 5, 16, device=cuda_device, requires_grad=True)
