@@ -389,8 +389,10 @@ OW_API int ow_pool_head_fwd(const ow_pool_head_t* args, void* stream);
  *
  * ``params``, ``grads`` and ``slots`` are host arrays, read during the call
  * (a captured graph keeps the pointers it was captured with).  A NULL
- * gradient leaves its tensor, its state and its step count as they are.
- * Neither function allocates or synchronises.
+ * gradient leaves its tensor, its state and its step count as they are.  A
+ * gradient that is inf or NaN and does not call the step off makes its
+ * parameter and its moments so, and with 8 bits spoils the moments of its whole
+ * block.  Neither function allocates or synchronises.
  */
 #define OW_ADAMW_BLOCK 256
 #define OW_ADAMW_CONTROL_BYTES 64
