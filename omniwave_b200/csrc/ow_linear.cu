@@ -29,6 +29,12 @@
 //
 // A few rows (serving) are a matter of reading W once: a CUDA-core kernel, a
 // warp (or several, for few features) a feature.
+//
+// Bound and measured (B200, device time in a CUDA graph; torch.matmul without an
+// epilogue beside it): the tensor pipe for 8192^3, 713 us = 1542 TFLOP/s (675);
+// 12544 x 2048 x 1024 39.7 us (38), its last wave two thirds full; HBM for
+// 401408 x 128 x 256, 58 us (57); 25088 x 512 x 1024 25.3 us (25.7), with gelu,
+// bias and kept z 40; one row 1024 -> 2048 3 us.
 #include <cuda.h>
 
 #include <algorithm>

@@ -315,9 +315,10 @@ def test_first_cuda_call_of_a_thread(cuda_device):
     assert torch.equal(got[0], linear.linear(x, w))
 
 
-def test_wait_that_runs_out_is_reported(cuda_device):
+@pytest.mark.parametrize("m,k,n", [(200, 64, 64), (8192, 128, 1024)], ids=["one-sm", "sm-pairs"])
+def test_wait_that_runs_out_is_reported(cuda_device, m, k, n):
     """The GEMM's bounded waits report to the library's fault word, as every pipelined kernel's do."""
-    x, w, *_ = _inputs(cuda_device, 200, 64, 64, BF)
+    x, w, *_ = _inputs(cuda_device, m, k, n, BF)
     want = linear.linear(x, w)
     lib = _lib.load()
     assert lib.ow_debug_wait_probe(1_000_000) == 0
@@ -327,6 +328,53 @@ def test_wait_that_runs_out_is_reported(cuda_device):
         lib.ow_debug_wait_probe(0)
     assert _lib.device_fault(cuda_device.index or 0, reset=True) == 1
     assert torch.equal(linear.linear(x, w), want)
+
+
+def test_two_threads_and_streams_at_once(cuda_device):
+    """Calls of two threads on streams of their own, small and pair-sized products mixed, give what each gives alone."""
+    import threading
+
+    shapes = [(8192, 256, 512), (300, 512, 256), (5, 1024, 777), (2000, 72, 1000)]
+    ins = [_inputs(cuda_device, *s, BF, seed=i) for i, s in enumerate(shapes)]
+    want = [linear.linear(x, w, b, activation="gelu", residual=r) for x, w, b, r, _ in ins]
+    torch.cuda.synchronize()
+    got: dict = {}
+
+    def work(name):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[name] = [[linear.linear(x, w, b, activation="gelu", residual=r) for x, w, b, r, _ in ins]
+                         for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    for rounds in got.values():
+        for outs in rounds:
+            assert all(torch.equal(a, e) for a, e in zip(outs, want))
+    assert len(got) == 2
+
+
+def test_outputs_of_more_than_2_31_elements(cuda_device):
+    m, k, n = 2_100_000, 16, 1032
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    x = torch.randn(m, k, generator=g, device=cuda_device, dtype=BF)
+    w = torch.randn(n, k, generator=g, device=cuda_device, dtype=BF)
+    y = linear.linear(x, w, activation="silu")
+    tail = slice(m - 300, m)
+    assert torch.equal(y[tail], linear.linear(x[tail], w, activation="silu"))
+    assert torch.equal(y[:300], linear.linear(x[:300], w, activation="silu"))
+    wl = w.requires_grad_()
+    y = linear.linear(x, wl, activation="silu")
+    dy = torch.zeros_like(y)
+    dy[tail] = 1.0  # only the last rows count
+    (dw,) = torch.autograd.grad(y, wl, dy)
+    (want,) = torch.autograd.grad(linear.linear(x[tail], wl, activation="silu"), wl, dy[tail])
+    # the same products, grouped otherwise: f32 sums of 300 terms, then one rounding each
+    mag = x[tail].float().abs().sum(0)[None, :] * 1.13
+    assert ((dw.float() - want.float()).abs() <= 2 * 308 * U * mag + 2 * _half(BF) * want.float().abs()).all()
 
 
 def test_run_of_the_operators_together(cuda_device):

@@ -266,6 +266,26 @@ def test_rows_do_not_see_their_neighbours(cuda_device, c, t):
         assert torch.isnan(g[0]).all() and torch.isnan(g[17]).all()
 
 
+def test_more_than_2_31_elements(cuda_device):
+    rows, c = 33_600_000, 64
+    x = torch.randn(1, rows, c, device=cuda_device, dtype=BF)
+    d = x.roll(1, 1)
+    w = torch.linspace(0.5, 1.5, c, device=cuda_device)
+    h, n = norm.norm_residual(x, d, w, w, next_weight=w)
+    for part in (slice(0, 40), slice(rows - 40, rows)):
+        hp, np_ = norm.norm_residual(x[:, part].contiguous(), d[:, part].contiguous(), w, w, next_weight=w)
+        assert torch.equal(h[:, part], hp) and torch.equal(n[:, part], np_)
+    del h, n
+    xl, dl = x.requires_grad_(), d.requires_grad_()
+    h, n = norm.norm_residual(xl, dl, w, w, next_weight=w)
+    gx, gd = torch.autograd.grad([h, n], [xl, dl], [d.detach(), x.detach()])
+    part = slice(rows - 40, rows)
+    xs, ds = (t.detach()[:, part].contiguous().requires_grad_() for t in (x, d))
+    hs, ns = norm.norm_residual(xs, ds, w, w, next_weight=w)
+    sx, sd = torch.autograd.grad([hs, ns], [xs, ds], [ds.detach(), xs.detach()])
+    assert torch.equal(gx[:, part], sx) and torch.equal(gd[:, part], sd)
+
+
 def test_empty(cuda_device):
     w = torch.ones(16, device=cuda_device, requires_grad=True)
     x = torch.zeros(0, 5, 16, device=cuda_device, requires_grad=True)

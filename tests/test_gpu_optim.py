@@ -247,6 +247,43 @@ def test_huge_finite_gradients_are_finite(cuda_device):
     assert torch.allclose(p.detach(), torch.full_like(p, -LR), rtol=1e-4)  # the first step's size is lr
 
 
+def test_norm_over_more_tensors_than_one_launch_takes(cuda_device):
+    sizes = [(11 * i) % 700 + 1 for i in range(1100)]
+    ps = _params(cuda_device, sizes, seed=6)
+    for p in ps[::7]:
+        p.grad = None
+    opt = optim.AdamW(ps, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, state_bits=8, max_norm=0.3)
+    old = [p.detach().double() for p in ps]
+    opt.step()
+    norm = torch.cat([p.grad.double() for p in ps if p.grad is not None]).norm()
+    assert abs(float(opt.grad_norm) - float(norm)) <= 2 * U * float(norm)
+    clip = min(1.0, 0.3 / (float(norm) + 1e-6))
+    for i, (p, o) in enumerate(zip(ps, old)):
+        if i % 7 == 0:
+            assert torch.equal(p.detach().double(), o) and float(opt.state[p]["step"]) == 0
+            continue
+        z = torch.zeros_like(o)
+        want, _, _, ep, _, _ = _step64(o, p.grad.double(), z, z, 1, clip)
+        assert ((p.detach().double() - want).abs() <= ep).all()
+        assert float(opt.state[p]["step"]) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_of_more_than_2_31_elements(cuda_device, bits):
+    n = 2 ** 31 + 777
+    p = torch.nn.Parameter(torch.zeros(n, device=cuda_device, dtype=BF))
+    p.grad = torch.zeros_like(p)
+    tail = torch.randn(5000, device=cuda_device).to(BF)
+    p.grad[-5000:] = tail
+    opt = optim.AdamW([p], lr=LR, weight_decay=0.0, state_bits=bits, max_norm=1e9)
+    opt.step()
+    q = torch.nn.Parameter(torch.zeros(5000, device=cuda_device, dtype=BF))
+    q.grad = tail.clone()
+    optim.AdamW([q], lr=LR, weight_decay=0.0, state_bits=bits, max_norm=1e9).step()
+    assert torch.equal(p.detach()[-5000:], q.detach()) and not p.detach()[:-5000].any()
+    assert abs(float(opt.grad_norm) - float(tail.double().norm())) <= 2 * U * float(tail.double().norm())
+
+
 def test_without_gradient_no_step_and_groups(cuda_device):
     a, b, c = _params(cuda_device, [500, 300, 200])
     b.grad = None
