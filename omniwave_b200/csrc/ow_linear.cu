@@ -27,14 +27,15 @@
 // are split over CTAs; each leaves an f32 partial, and a second kernel adds
 // them in a fixed order and does the epilogue.
 //
-// A few rows (serving) are a matter of reading W once: a CUDA-core kernel, a
-// warp (or several, for few features) a feature.
+// A few rows (serving) are a matter of reading W once, with no tile to stage:
+// the warp-wide MMA straight from global memory where rows are 16-byte units,
+// CUDA cores where they are not.
 //
 // Bound and measured (B200, device time in a CUDA graph; torch.matmul without an
 // epilogue beside it): the tensor pipe for 8192^3, 713 us = 1542 TFLOP/s (675);
 // 12544 x 2048 x 1024 39.7 us (38), its last wave two thirds full; HBM for
 // 401408 x 128 x 256, 58 us (57); 25088 x 512 x 1024 25.3 us (25.7), with gelu,
-// bias and kept z 40; one row 1024 -> 2048 3 us.
+// bias and kept z 40; one row 1024 -> 2048 2.7 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -142,6 +143,11 @@ __device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
+}
+__device__ __forceinline__ float ld_in(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ void arrive_in(uint32_t bar) {
   // release at the scope of the CTA: what it orders is this thread's reads of
@@ -681,80 +687,166 @@ struct RowsArgs {
   const void* w;
   int64_t ldw;
   int M, N, K;
-  int vec;
   Epi e;
 };
 
-// P warps share a feature (its k range dealt out in 256-element turns); a
-// block of 8 warps does 8 / P features.  MR rows are taken at a time.
-template <int MR, int P>
+// One output from its sum: bias, the kept z, the activation, the residual.
+__device__ __forceinline__ void finish_one(const Epi& e, float z, int64_t m, int n, int bf) {
+  if (e.bias) z += ld_any(e.bias, e.bias_dt, n);
+  if (e.z) st16(e.z, m * e.ldz + n, bf, keep_z(z, bf));
+  z = act_fwd(z, e.act);
+  if (e.res) z += ld16(e.res, m * e.ldr + n, bf);
+  st16(e.out, m * e.ldo + n, bf, z);
+}
+
+// Rows that are not 16-byte units.  Four warps share a feature (its k dealt out
+// in turns of 32), a block of 8 warps does two; MR rows at once.
+template <int MR>
 __global__ void __launch_bounds__(256) linear_rows_kernel(const RowsArgs a) {
   __shared__ float sh[8][MR];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % P;
-  const int n = blockIdx.x * (8 / P) + warp / P;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp & 3;
+  const int n = blockIdx.x * 2 + (warp >> 2);
   const int bf = a.e.bf16;
-  for (int m0 = 0; m0 < a.M; m0 += MR) {
-    float s[MR];
+  float s[MR];
 #pragma unroll
-    for (int r = 0; r < MR; ++r) s[r] = 0.f;
-    if (n < a.N) {
-      const uint16_t* w = reinterpret_cast<const uint16_t*>(a.w) + n * a.ldw;
-      const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
-      if (a.vec) {
+  for (int r = 0; r < MR; ++r) s[r] = 0.f;
+  if (n < a.N) {
+    const uint16_t* w = reinterpret_cast<const uint16_t*>(a.w) + n * a.ldw;
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x);
 #pragma unroll 4
-        for (int k = part * 256 + lane * 8; k < a.K; k += P * 256) {
-          const uint4 wv = __ldg(reinterpret_cast<const uint4*>(w + k));
-          const uint32_t wq[4] = {wv.x, wv.y, wv.z, wv.w};
-#pragma unroll
-          for (int r = 0; r < MR; ++r) {
-            if (m0 + r >= a.M) break;
-            const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + (m0 + r) * a.ldx + k));
-            const uint32_t xq[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 p = upk(wq[i], bf), q = upk(xq[i], bf);
-              s[r] = fmaf(p.x, q.x, s[r]);
-              s[r] = fmaf(p.y, q.y, s[r]);
-            }
-          }
-        }
-      } else {
-        for (int k = part * 32 + lane; k < a.K; k += P * 32) {
-          const float wk = ld16(w, k, bf);
-#pragma unroll
-          for (int r = 0; r < MR; ++r)
-            if (m0 + r < a.M) s[r] = fmaf(wk, ld16(x, (m0 + r) * a.ldx + k, bf), s[r]);
-        }
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < MR; ++r)
-#pragma unroll
-      for (int o = 16; o; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
-    float mine = 0.f;  // row ``lane``'s sum
-    if constexpr (P == 1) {
+    for (int64_t k = part * 32 + lane; k < a.K; k += 128) {
+      const float wk = ld16(w, k, bf);
 #pragma unroll
       for (int r = 0; r < MR; ++r)
-        if (lane == r) mine = s[r];
-    } else {
-      if (lane == 0)
-#pragma unroll
-        for (int r = 0; r < MR; ++r) sh[warp][r] = s[r];
-      __syncthreads();
-      if (lane < MR)
-#pragma unroll
-        for (int i = 0; i < P; ++i) mine += sh[warp - part + i][lane];
-      __syncthreads();
-    }
-    if (part == 0 && lane < MR && m0 + lane < a.M && n < a.N) {
-      const int64_t m = m0 + lane;
-      if (a.e.bias) mine += ld_any(a.e.bias, a.e.bias_dt, n);
-      if (a.e.z) st16(a.e.z, m * a.e.ldz + n, bf, keep_z(mine, bf));
-      mine = act_fwd(mine, a.e.act);
-      if (a.e.res) mine += ld16(a.e.res, m * a.e.ldr + n, bf);
-      st16(a.e.out, m * a.e.ldo + n, bf, mine);
+        if (r < a.M) s[r] = fmaf(wk, ld16(x, r * a.ldx + k, bf), s[r]);
     }
   }
+#pragma unroll
+  for (int r = 0; r < MR; ++r)
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+  if (lane == 0)
+#pragma unroll
+    for (int r = 0; r < MR; ++r) sh[warp][r] = s[r];
+  __syncthreads();
+  if (part == 0 && lane < MR && lane < a.M && n < a.N)
+    finish_one(a.e, ((sh[warp][lane] + sh[warp + 1][lane]) + sh[warp + 2][lane]) + sh[warp + 3][lane], lane, n, bf);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes that are read once: not kept in L1, which holds x.  These loads and
+// the MMAs are volatile so that all loads of a pass stay ahead of its products.
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint4 ld_again(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// Rows of 16-byte units, up to 8 NB of them, on the warp-wide MMA: a warp takes
+// 16 features and, 64 of k a turn, a share of k.  A lane's 16 bytes are 8
+// neighbouring k, where the MMA wants k 2t, 2t + 1, 2t + 8, 2t + 9 in lane t; a
+// sum does not mind in which order its terms come, so the units go in as they
+// lie, W's and x's alike: no shuffle, no shared memory.  Reading W bounds it;
+// the loads of some turns are under way before the first product, as many as
+// the registers hold beside x's: 4, 3 and 1 turns for NB = 1, 2 and 4 (16 rows,
+// 4096 x 4096: 13.1 us with 2 turns, 10.6 with 3; 32 rows: 19 with 2, 13.5 with
+// 1, whose blocks are more).  A block's warps meet in shared memory.  Where the
+// features give too few blocks to fill the SMs, a cluster of blocks (along y)
+// splits k and its first adds them.  All sums in a fixed order.
+//
+// On CUDA cores (a warp a feature) 8 rows of 4096 x 4096 took 38.7 us, here 8.7;
+// one row 11.7 and 8.3; one row of 8192 x 8192 38.3 and 23.9 (5.6 TB/s).
+constexpr int UNIT_WARPS = 8;
+constexpr int unit_turns(int nb) { return nb == 1 ? 4 : nb == 2 ? 3 : 1; }
+
+template <int NB, bool BF16>
+__global__ void __launch_bounds__(UNIT_WARPS * 32) linear_units_kernel(const RowsArgs a) {
+  constexpr int U = unit_turns(NB), warps = UNIT_WARPS, ROW = 8 * NB + 1;
+  extern __shared__ float sh[];  // [warps][16][ROW], [8 NB][16]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16, units = a.K >> 3, splits = gridDim.y, all = warps * splits * 8;
+  const uint16_t* w = reinterpret_cast<const uint16_t*>(a.w) + t * 8;
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x) + t * 8;
+  // features and rows past the end repeat the last; what they give is not stored
+  const uint16_t* w0 = w + min(n0 + g, a.N - 1) * a.ldw;
+  const uint16_t* w1 = w + min(n0 + g + 8, a.N - 1) * a.ldw;
+  const uint16_t* xr[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) xr[j] = x + min(8 * j + g, a.M - 1) * a.ldx;
+  float c[NB][4];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int q = (blockIdx.y * warps + warp) * 8; q < units; q += all * U) {
+    uint4 p[U][2][2], v[U][2][NB];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = q + u * all + h * 4;  // in units; K < 2^30
+        const bool in = k + t < units;
+        p[u][h][0] = in ? ld_once(w0 + k * 8) : zero;
+        p[u][h][1] = in ? ld_once(w1 + k * 8) : zero;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) v[u][h][j] = in ? ld_again(xr[j] + k * 8) : zero;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          mma16<BF16>(c[j], p[u][h][0].x, p[u][h][1].x, p[u][h][0].y, p[u][h][1].y, v[u][h][j].x, v[u][h][j].y);
+          mma16<BF16>(c[j], p[u][h][0].z, p[u][h][1].z, p[u][h][0].w, p[u][h][1].w, v[u][h][j].z, v[u][h][j].w);
+        }
+  }
+  float* mine = sh + warp * 16 * ROW;
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine[(g + 8 * (i >> 1)) * ROW + 8 * j + 2 * t + (i & 1)] = c[j][i];
+  __syncthreads();
+  float* sum = sh + warps * 16 * ROW;  // this block's sums, for the cluster's first block
+  for (int i = threadIdx.x; i < 16 * a.M; i += warps * 32) {
+    const int n = n0 + (i & 15), m = i >> 4;
+    float z = 0.f;
+#pragma unroll
+    for (int p = 0; p < warps; ++p) z += sh[(p * 16 + (i & 15)) * ROW + m];
+    if (splits > 1) sum[i] = z;
+    else if (n < a.N) finish_one(a.e, z, m, n, BF16);
+  }
+  if (splits == 1) return;
+  cluster_sync();
+  if (blockIdx.y == 0) {
+    for (int i = threadIdx.x; i < 16 * a.M; i += warps * 32) {
+      const int n = n0 + (i & 15), m = i >> 4;
+      float z = sum[i];
+#pragma unroll 4
+      for (int p = 1; p < splits; ++p) z += ld_in(in_cta(sum + i, p));
+      if (n < a.N) finish_one(a.e, z, m, n, BF16);
+    }
+  }
+  cluster_sync();  // a block's sums stay until the first has read them
 }
 
 // ---------------------------------------------------------------- backward of the epilogue
@@ -867,6 +959,31 @@ struct Mat {
   int64_t ld;
 };
 
+template <typename... KArgs, typename... Args>
+int launch_cluster(const char* name, void (*kern)(KArgs...), dim3 grid, dim3 cluster, int threads, size_t smem, cudaStream_t st,
+                   const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cluster.x;
+  at.val.clusterDim.y = cluster.y;
+  at.val.clusterDim.z = cluster.z;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  count_launches(1);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s: launch failed: %s", name, cudaGetErrorString(e));
+    return OW_ERR_CUDA;
+  }
+  return OW_OK;
+}
+
 // Shape of one GEMM: the tile's width, whether pairs of SMs share it, and the
 // k splits that a model finds fastest, in cycles of an SM.  Its figures are
 // measured (B200, 1.75 GHz): a 64-wide k block takes 400 cycles in a 128 x 64
@@ -957,25 +1074,7 @@ int run_gemm(const Maps& maps, const GemmArgs& k, int grid, cudaStream_t st) {
     set_error("ow_linear: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e));
     return OW_ERR_CUDA;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = CG;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  count_launches(1);
-  e = cudaLaunchKernelEx(&cfg, kern, maps, k);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    set_error("gemm_kernel: launch failed: %s", cudaGetErrorString(e));
-    return OW_ERR_CUDA;
-  }
-  return OW_OK;
+  return launch_cluster("gemm_kernel", kern, dim3(grid), dim3(CG), THREADS, C::SMEM, st, maps, k);
 }
 
 // D[M, N] = sum_k A B with the epilogue ``e``.  AMN/BMN: the operand's rows
@@ -1058,8 +1157,18 @@ int check(const ow_linear_t* a) {
   return OW_OK;
 }
 
-// Up to this many rows the kernel that reads W once from CUDA cores is used.
-constexpr int FEW_ROWS = 8;
+bool in_units(const ow_linear_t* a) {
+  return a->in_features % 8 == 0 && tma_rows(a->x, a->ldx) && tma_rows(a->weight, a->ldw);
+}
+// Whether the kernels for a few rows serve.  In units, against the GEMM: 16 rows
+// 1024 -> 2048 3.3 and 7.5 us, 4096 -> 4096 10.6 and 14.1, 8192 -> 8192 32 and 30;
+// 32 rows 4.1 and 7.6, 13.5 and 14.1, 42 and 31.  Other rows, where the GEMM
+// copies x and W first: 4 rows 1001 -> 1000 3.8 and 14, 4090 -> 4096 22 and 57; 8 rows
+// 9.5 and 14, 65 and 57.
+bool few_rows(const ow_linear_t* a) {
+  if (!in_units(a)) return a->rows <= 4;
+  return a->rows <= 16 || (a->rows <= 32 && (int64_t)a->in_features * a->out_features <= (1 << 24));
+}
 
 Mat mat_x(const ow_linear_t* a) { return Mat{a->x, a->rows, a->in_features, a->ldx}; }
 Mat mat_w(const ow_linear_t* a) { return Mat{a->weight, a->out_features, a->in_features, a->ldw}; }
@@ -1113,7 +1222,7 @@ size_t ow_linear_workspace_size(const ow_linear_t* a, const ow_linear_grads_t* g
   if (a->rows > 0) {
     if (g) {
       bwd_take(a, g, c);
-    } else if (a->rows > FEW_ROWS) {
+    } else if (!few_rows(a)) {
       gemm_take(mat_x(a), mat_w(a), a->rows, a->out_features, plan_gemm(a->rows, a->out_features, blocks_of(a->in_features)), c);
     }
   }
@@ -1141,26 +1250,37 @@ int ow_linear_fwd(const ow_linear_t* a, void* stream) {
   e.z = a->z; e.ldz = up8(N); e.vz = 1;
   e.res = a->residual; e.ldr = a->ldr; e.vr = tma_rows(a->residual, a->ldr);
   e.out = a->out; e.ldo = N; e.vo = tma_rows(a->out, N);
-  if (a->rows <= FEW_ROWS) {
-    RowsArgs k{a->x, a->ldx, a->weight, a->ldw, (int)a->rows, N, K,
-               K % 8 == 0 && tma_rows(a->x, a->ldx) && tma_rows(a->weight, a->ldw), e};
-    // warps for a feature: enough that few features still fill the SMs
-    const int want = device_sm_count() * 16;
-    auto go = [&](auto p) -> int {
-      constexpr int P = decltype(p)::value, F = 8 / P;
-      const int grid = (N + F - 1) / F;
-      if (a->rows == 1) launch(linear_rows_kernel<1, P>, grid, 256, 0, st, k);
-      else if (a->rows == 2) launch(linear_rows_kernel<2, P>, grid, 256, 0, st, k);
-      else if (a->rows <= 4) launch(linear_rows_kernel<4, P>, grid, 256, 0, st, k);
-      else launch(linear_rows_kernel<8, P>, grid, 256, 0, st, k);
+  if (few_rows(a)) {
+    const RowsArgs k{a->x, a->ldx, a->weight, a->ldw, (int)a->rows, N, K, e};
+    if (in_units(a)) {
+      const int blocks = (N + 15) / 16;
+      auto go = [&](auto nb, auto b16) -> int {
+        constexpr int NB = decltype(nb)::value, W = UNIT_WARPS, turns = std::max(unit_turns(NB), 2);
+        // A split costs 0.7 us (2048 -> 1024: 3.5 us whole, 3.9 in two), and pays where each
+        // warp keeps the turns that it has under way at once (4096 -> 64: 4.5 whole, 4.0 in two).
+        int splits = 1;
+        while (splits < 8 && blocks * splits * 2 <= device_sm_count() && K >= 64 * W * turns * splits * 2) splits *= 2;
+        const size_t smem = ((size_t)W * 16 * (8 * NB + 1) + 128 * NB) * 4;
+        if (splits > 1)
+          return launch_cluster("linear_units_kernel", linear_units_kernel<NB, decltype(b16)::value>, dim3(blocks, splits),
+                                dim3(1, splits), W * 32, smem, st, k);
+        launch(linear_units_kernel<NB, decltype(b16)::value>, blocks, W * 32, smem, st, k);
+        OW_CHECK_LAUNCH("linear_units_kernel");
+        return OW_OK;
+      };
+      auto of = [&](auto nb) { return bf ? go(nb, std::true_type()) : go(nb, std::false_type()); };
+      if (a->rows <= 8) return of(std::integral_constant<int, 1>());
+      if (a->rows <= 16) return of(std::integral_constant<int, 2>());
+      return of(std::integral_constant<int, 4>());
+    }
+    auto go = [&](auto mr) -> int {
+      launch(linear_rows_kernel<decltype(mr)::value>, (N + 1) / 2, 256, 0, st, k);
       OW_CHECK_LAUNCH("linear_rows_kernel");
       return OW_OK;
     };
-    const int turns = (K + 255) / 256;
-    if (turns >= 8 && N * 8 <= want) return go(std::integral_constant<int, 8>());
-    if (turns >= 4 && N * 4 <= want) return go(std::integral_constant<int, 4>());
-    if (turns >= 2 && N * 2 <= want) return go(std::integral_constant<int, 2>());
-    return go(std::integral_constant<int, 1>());
+    if (a->rows == 1) return go(std::integral_constant<int, 1>());
+    if (a->rows == 2) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, 4>());
   }
   Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
   const Plan p = plan_gemm(a->rows, N, blocks_of(K));

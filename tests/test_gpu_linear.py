@@ -213,6 +213,46 @@ def test_gradients_against_differences(cuda_device):
         assert abs(got - want) <= 4 * _half(HF) * size  # z, dz and each gradient rounded to f16
 
 
+@pytest.mark.parametrize("k", [8, 56, 72, 1000, 2048, 4104, 8192])
+@pytest.mark.parametrize("t", [BF, HF], ids=["bf16", "f16"])
+def test_a_few_rows(cuda_device, k, t):
+    # around the row counts where the kernel changes; features that do not fill a warp's 16; long k, that is split
+    for m in (1, 7, 8, 9, 16, 17, 31, 32, 33):
+        for n in (1, 15, 16, 17, 64, 1000):
+            x, w, b, r, dy = _inputs(cuda_device, m, k, n, t, seed=m)
+            want, tol = _define(x, w, b, r, dy, "silu", t)
+            y = linear.linear(x, w, b, activation="silu", residual=r)
+            _ok(y, want["y"], tol["y"], f"{m}x{k}x{n}")
+            assert torch.equal(y, linear.linear(x, w, b, activation="silu", residual=r))
+            # rows that lie apart, in 16-byte units and out of them: the same function, perhaps another kernel
+            for pad in (8, 3):
+                xs, ws, rs = (torch.full((a.shape[0], a.shape[1] + pad), float("nan"), dtype=t, device=cuda_device)
+                              for a in (x, w, r))
+                for a, c in ((xs, x), (ws, w), (rs, r)):
+                    a[:, : c.shape[1]] = c
+                y = linear.linear(xs[:, :k], ws[:, :k], b, activation="silu", residual=rs[:, :n])
+                _ok(y, want["y"], tol["y"], f"{m}x{k}x{n} pad {pad}")
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 8192, 4096), (17, 4096, 4096), (32, 4096, 4097), (2, 4090, 4096)])
+def test_a_few_rows_of_large_weights(cuda_device, m, k, n):
+    _both(*_inputs(cuda_device, m, k, n, BF), "gelu", f"{m}x{k}x{n}")
+
+
+def test_rows_and_features_do_not_mix(cuda_device):
+    # what is not a number in one row of x or of the weight stays in its row or column of the result
+    for m in (4, 16, 30, 40):
+        for k in (64, 70, 4096):
+            x, w, *_ = _inputs(cuda_device, m, k, 50, BF)
+            want = linear.linear(x, w)
+            x[m // 2, k // 3], w[7, k - 1], w[49, 0] = float("nan"), float("inf"), float("-inf")
+            y = linear.linear(x, w)
+            rows, cols = torch.arange(m, device=cuda_device) != m // 2, torch.ones(50, dtype=torch.bool, device=cuda_device)
+            cols[7] = cols[49] = False
+            assert torch.isnan(y[m // 2]).all() and not torch.isfinite(y[:, ~cols]).any()
+            assert torch.equal(y[rows][:, cols], want[rows][:, cols])
+
+
 def test_special_values(cuda_device):
     x = torch.zeros(4, 16, dtype=BF, device=cuda_device)
     x[1, 0], x[2, 0], x[3, 0] = float("inf"), float("nan"), -3e4
