@@ -1235,7 +1235,7 @@ int ow_linear_fwd(const ow_linear_t* a, void* stream) {
   if (a->rows == 0) return OW_OK;
   OW_CHECK_ARG(a->x && a->weight && a->out, "ow_linear_fwd: a pointer is NULL");
   OW_CHECK_ARG(((uintptr_t)a->x | (uintptr_t)a->weight | (uintptr_t)a->out | (uintptr_t)a->residual) % 2 == 0 &&
-                   (uintptr_t)a->z % 16 == 0,
+                   (uintptr_t)a->z % 16 == 0 && (!a->bias || (uintptr_t)a->bias % dtype_size(a->bias_dtype) == 0),
                "ow_linear_fwd: a tensor is not aligned");
   const size_t need = ow_linear_workspace_size(a, nullptr);
   if (!a->workspace || a->workspace_bytes < need) {
@@ -1300,6 +1300,10 @@ int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream
   OW_CHECK_ARG(a->rows > 0, "ow_linear_bwd: no rows");
   OW_CHECK_ARG(g->dout && (!g->dx || a->weight) && (!g->dweight || a->x) && (a->activation == OW_ACT_NONE || a->z),
                "ow_linear_bwd: a pointer is NULL");
+  OW_CHECK_ARG(((uintptr_t)a->x | (uintptr_t)a->weight | (uintptr_t)g->dout | (uintptr_t)g->dx) % 2 == 0 &&
+                   (uintptr_t)a->z % 16 == 0 && (uintptr_t)g->dweight % dtype_size(g->dweight ? g->dweight_dtype : a->dtype) == 0 &&
+                   (!g->dbias || (uintptr_t)g->dbias % dtype_size(a->bias_dtype) == 0),
+               "ow_linear_bwd: a tensor is not aligned");
   const size_t need = ow_linear_workspace_size(a, g);
   if (!a->workspace || a->workspace_bytes < need) {
     set_error("ow_linear_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);

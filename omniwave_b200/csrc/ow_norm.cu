@@ -748,6 +748,12 @@ int check(const ow_norm_t* a) {
     return OW_ERR_UNSUPPORTED;
   }
   OW_CHECK_ARG(a->eps >= 0.0, "ow_norm: eps must not be negative");
+  auto at = [](const void* p, int dt) { return (uintptr_t)p % dtype_size(dt) == 0; };
+  OW_CHECK_ARG(at(a->x, a->x_dtype) && (!d || (at(a->delta, a->delta_dtype) && at(a->post_w, a->post_dtype) && at(a->h, a->x_dtype))) &&
+                   (!a->gate_rows || at(a->gate, a->gate_dtype)) &&
+                   (!a->next_w || (at(a->next_w, a->next_dtype) && at(a->n, a->n_dtype))) &&
+                   ((uintptr_t)a->sample_scale | (uintptr_t)a->rstd_delta | (uintptr_t)a->rstd_h) % 4 == 0,
+               "ow_norm: a tensor is not aligned");
   return OW_OK;
 }
 
@@ -943,6 +949,11 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
   OW_CHECK_ARG(k.rows == 0 || (g->dx && (!next || g->dn) && (!delta || g->ddelta) && (g->dh || next) &&
                                (!delta || k.rd) && (!next || k.rh)),
                "ow_norm_bwd: a pointer is NULL");
+  auto at = [](const void* p, int dt) { return !p || (uintptr_t)p % dtype_size(dt) == 0; };
+  OW_CHECK_ARG(at(g->dh, a->x_dtype) && at(g->dx, a->x_dtype) && (!next || (at(g->dn, a->n_dtype) && at(g->dnext, a->next_dtype))) &&
+                   (!delta || (at(g->ddelta, a->delta_dtype) && at(g->dpost, a->post_dtype))) &&
+                   (!a->gate_rows || at(g->dgate, a->gate_dtype)),
+               "ow_norm_bwd: a gradient is not aligned");
   parts(a, &k, BWD_PER_SM);
   const size_t need = ow_norm_bwd_workspace_size(a);
   if (!a->workspace || a->workspace_bytes < need) {

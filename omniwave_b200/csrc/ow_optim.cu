@@ -493,6 +493,10 @@ int check(const ow_adamw_t* a) {
     set_error("ow_adamw: parameters must be float32, bfloat16 or float16 (dtype code %d)", a->dtype);
     return OW_ERR_UNSUPPORTED;
   }
+  const size_t es = dtype_size(a->dtype);
+  OW_CHECK_ARG((uintptr_t)a->dev_blocks % 16 == 0 && (uintptr_t)a->control % 4 == 0, "ow_adamw: a device table is not aligned");
+  for (int i = 0; i < a->tensors; ++i)
+    OW_CHECK_ARG(((uintptr_t)a->params[i] | (uintptr_t)a->grads[i]) % es == 0, "ow_adamw: tensor %d is not aligned", i);
   for (int i = 0; i < a->tensors; ++i)
     OW_CHECK_ARG(a->slots[i] >= 0 && a->slots[i] % BLK == 0 && a->slots[i + 1] % BLK == 0 && a->slots[i] < a->slots[i + 1],
                  "ow_adamw: slots of tensor %d must be a rising multiple of %d", i, BLK);
@@ -562,6 +566,8 @@ int ow_grad_norm(const ow_adamw_t* a, const ow_grad_norm_t* o, void* stream) {
   clear_error();
   OW_RETURN_IF(check(a));
   OW_CHECK_ARG(o && o->partials, "ow_grad_norm: options or partials is NULL");
+  OW_CHECK_ARG((uintptr_t)o->partials % 8 == 0 && ((uintptr_t)o->norm | (uintptr_t)o->found) % 4 == 0,
+               "ow_grad_norm: an output is not aligned");
   OW_CHECK_ARG(o->first >= 0 && o->capacity >= o->first + ow_grad_norm_partials(a),
                "ow_grad_norm: room for %d partial sums from %d on is needed, got %d", ow_grad_norm_partials(a), o->first,
                o->capacity);
@@ -586,6 +592,10 @@ int ow_adamw_step(const ow_adamw_t* a, void* stream) {
   OW_CHECK_ARG(a->state_bits == 32 || a->state_bits == 8, "ow_adamw_step: state_bits must be 32 or 8 (got %d)", a->state_bits);
   OW_CHECK_ARG(a->exp_avg && a->exp_avg_sq && a->dev_steps, "ow_adamw_step: a state pointer is NULL");
   OW_CHECK_ARG(a->state_bits == 32 || (a->exp_avg_scale && a->exp_avg_sq_scale), "ow_adamw_step: 8-bit states need their scales");
+  OW_CHECK_ARG(((uintptr_t)a->exp_avg | (uintptr_t)a->exp_avg_sq) % (a->state_bits == 32 ? 16 : 4) == 0 &&
+                   ((uintptr_t)a->exp_avg_scale | (uintptr_t)a->exp_avg_sq_scale | (uintptr_t)a->dev_steps |
+                    (uintptr_t)a->lr_ptr | (uintptr_t)a->found) % 4 == 0,
+               "ow_adamw_step: the state is not aligned");
   OW_CHECK_ARG(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "ow_adamw_step: betas must be in [0, 1)");
   for (int i = 0; i < a->tensors; ++i)
     OW_CHECK_ARG(a->params[i] || !a->grads[i], "ow_adamw_step: parameter %d is NULL", i);

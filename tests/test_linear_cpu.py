@@ -87,3 +87,19 @@ def test_workspace_covers_padded_operands():
     assert lib.ow_linear_workspace_size(_args(dtype=0), None) == 0
     g = _lib.LinearGrads(16, 16, 16, 2, 16)
     assert lib.ow_linear_workspace_size(_args(), g) >= 100 * 40 * 2  # dz
+
+
+@pytest.mark.parametrize("over,grads", [
+    (dict(bias=17), None), (dict(z=8), {}), (dict(x=17), {}), ({}, dict(dout=17)), ({}, dict(dx=17)), ({}, dict(dweight=17)),
+    ({}, dict(dweight=18, dweight_dtype=0)), ({}, dict(dbias=17)),
+])
+def test_c_entries_refuse_pointers_off_their_alignment(over, grads):
+    lib = _lib.load()
+    if grads is None:
+        status = lib.ow_linear_fwd(ctypes.byref(_args(**over)), None)
+    else:
+        g = _lib.LinearGrads(16, 16, 16, 2, 16)
+        for k, v in grads.items():
+            setattr(g, k, v)
+        status = lib.ow_linear_bwd(ctypes.byref(_args(**over)), ctypes.byref(g), None)
+    assert status == 1 and "not aligned" in lib.ow_last_error().decode()

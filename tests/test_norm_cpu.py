@@ -91,3 +91,21 @@ def test_post_norm_block_parameters():
         assert torch.equal(v, post.state_dict()[k])
     with pytest.raises(RuntimeError, match="CUDA is unavailable"):
         post(torch.zeros(1, 4, 4, 64))
+
+
+@pytest.mark.parametrize("over,grads", [
+    (dict(x=18), None), (dict(delta=17), None), (dict(post_w=18), None), (dict(gate=18), None), (dict(next_w=18), None),
+    (dict(h=18), None), (dict(n=17), None), (dict(sample_scale=18), None), (dict(rstd_h=18), {}), ({}, dict(dh=18)),
+    ({}, dict(dn=17)), ({}, dict(dx=18)), ({}, dict(ddelta=17)), ({}, dict(dpost=18)), ({}, dict(dgate=18)), ({}, dict(dnext=18)),
+])
+def test_c_entries_refuse_pointers_off_their_alignment(over, grads):
+    lib = _lib.load()
+    a = _args(n_dtype=2, **over)
+    if grads is None:
+        status = lib.ow_norm_fwd(ctypes.byref(a), None)
+    else:
+        g = _lib.NormGrads(16, 16, 16, 16, 16, 16, 16)
+        for k, v in grads.items():
+            setattr(g, k, v)
+        status = lib.ow_norm_bwd(ctypes.byref(a), ctypes.byref(g), None)
+    assert status == 1 and "not aligned" in lib.ow_last_error().decode()

@@ -103,3 +103,25 @@ def test_c_entry_checks_slots_and_partials():
     opt = _lib.GradNorm(None, 0, need, 1, 1.0, 0, None, None)
     assert lib.ow_grad_norm(a, opt, None) == 1
     assert lib.ow_grad_norm_partials(None) == 0
+
+
+@pytest.mark.parametrize("over", [
+    dict(dev_blocks=24), dict(control=18), dict(exp_avg=24), dict(exp_avg_sq=20), dict(dev_steps=18), dict(lr_ptr=18),
+    dict(found=18), dict(state_bits=8, exp_avg=18, exp_avg_scale=16, exp_avg_sq_scale=16),
+    dict(state_bits=8, exp_avg_scale=18, exp_avg_sq_scale=16),
+])
+def test_c_entry_refuses_pointers_off_their_alignment(over):
+    lib = _lib.load()
+    a, keep = _args(**over)
+    assert lib.ow_adamw_step(a, None) == 1
+    assert "not aligned" in lib.ow_last_error().decode()
+    a, keep = _args()
+    for which in (0, 1):
+        keep[which][0] = 18  # f32
+        assert lib.ow_adamw_step(a, None) == 1 and "tensor 0 is not aligned" in lib.ow_last_error().decode()
+        keep[which][0] = 16
+    for bad in (dict(partials=20), dict(norm=18), dict(found=18)):
+        opt = _lib.GradNorm(16, 0, 1000, 1, 1.0, 0, None, None)
+        for k, v in bad.items():
+            setattr(opt, k, v)
+        assert lib.ow_grad_norm(a, opt, None) == 1 and "not aligned" in lib.ow_last_error().decode()
