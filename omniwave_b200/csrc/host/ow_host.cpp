@@ -228,6 +228,9 @@ at::ScalarType norm_out(const Tensor& x, const std::optional<at::ScalarType>& as
   return t;
 }
 
+// The C structs hold a row's length in 32 bits.
+constexpr int64_t MOST = (int64_t)1 << 30;
+
 void check_vector(const char* name, const Tensor& w, int64_t c) {
   OW_VALUE(w.dim() == 1 && w.size(0) == c, name, " must be [", c, "], got ", shape_text(w.sizes()));
 }
@@ -246,6 +249,7 @@ variable_list norm_call(const Tensor& x, const Tensor& delta, const Tensor& post
 
 Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps, std::optional<at::ScalarType> out_dtype) {
   OW_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must be [..., C], got ", shape_text(x.sizes()));
+  OW_VALUE(x.size(-1) < MOST, "x has too many channels: ", x.size(-1));
   OW_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
   check_vector("weight", weight, x.size(-1));
   if (auto why = unsupported(x, {weight})) TORCH_CHECK(false, "norm not supported: ", *why);
@@ -256,6 +260,7 @@ variable_list norm_residual(const Tensor& x, const Tensor& delta, const Tensor& 
                             const OptTensor& scale_, const OptTensor& next_, double eps,
                             std::optional<at::ScalarType> out_dtype) {
   OW_VALUE(x.dim() >= 2 && x.size(-1) > 0, "x must be [B, ..., C], got ", shape_text(x.sizes()));
+  OW_VALUE(x.size(-1) < MOST, "x has too many channels: ", x.size(-1));
   OW_VALUE(delta.sizes() == x.sizes(), "delta must be ", shape_text(x.sizes()), ", got ", shape_text(delta.sizes()));
   OW_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
   const Tensor gate = value(gate_), next = value(next_);
@@ -416,6 +421,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, int64_t 
   Tensor bias = value(bias_);
   OW_VALUE(w.dim() == 2 && w.numel() > 0, "weight must be [N, K], got ", shape_text(w.sizes()));
   const int64_t n = w.size(0), kk = w.size(1);
+  OW_VALUE(n < MOST && kk < MOST, "weight is too large: ", shape_text(w.sizes()));
   OW_VALUE(x.dim() >= 1 && x.size(-1) == kk, "x must be [..., ", kk, "], got ", shape_text(x.sizes()));
   if (bias.defined())
     OW_VALUE(bias.dim() == 1 && bias.size(0) == n, "bias must be [", n, "], got ", shape_text(bias.sizes()));

@@ -737,6 +737,7 @@ int check(const ow_norm_t* a) {
   OW_CHECK_ARG(a->samples >= 0 && a->tokens >= 0 && a->channels > 0, "ow_norm: bad shape [%lld, %lld, %d]",
                (long long)a->samples, (long long)a->tokens, a->channels);
   OW_CHECK_ARG(a->samples < (1LL << 31) && a->tokens < (1LL << 31) && a->samples * a->tokens < (1LL << 40), "ow_norm: too many rows");
+  OW_CHECK_ARG(a->channels < (1 << 30), "ow_norm: too many channels (%d)", a->channels);
   const bool d = a->delta != nullptr;
   OW_CHECK_ARG(a->x && (!d || a->post_w) && (d || a->next_w), "ow_norm: an input pointer is NULL");
   OW_CHECK_ARG(a->gate_rows == 0 || (d && a->gate && (a->gate_rows == 1 || a->gate_rows == a->samples)),

@@ -103,3 +103,11 @@ def test_c_entries_refuse_pointers_off_their_alignment(over, grads):
             setattr(g, k, v)
         status = lib.ow_linear_bwd(ctypes.byref(_args(**over)), ctypes.byref(g), None)
     assert status == 1 and "not aligned" in lib.ow_last_error().decode()
+
+
+def test_refuses_features_that_their_field_does_not_hold():
+    k = 2 ** 32 + 8  # 8 in 32 bits
+    with pytest.raises(ValueError, match="too large"):
+        linear.linear(torch.zeros(1, 1).expand(1, k), torch.zeros(1, 1).expand(2, k))
+    with pytest.raises(ValueError, match="too large"):
+        linear.linear(torch.zeros(1, 8), torch.zeros(1, 8).expand(k, 8))

@@ -109,3 +109,15 @@ def test_c_entries_refuse_pointers_off_their_alignment(over, grads):
             setattr(g, k, v)
         status = lib.ow_norm_bwd(ctypes.byref(a), ctypes.byref(g), None)
     assert status == 1 and "not aligned" in lib.ow_last_error().decode()
+
+
+def test_refuses_rows_that_their_length_field_does_not_hold():
+    c = 2 ** 32 + 8  # 8 in 32 bits
+    x, w = torch.zeros(1, 1).expand(1, c), torch.zeros(1).expand(c)
+    with pytest.raises(ValueError, match="too many channels"):
+        norm.rms_norm(x, w)
+    with pytest.raises(ValueError, match="too many channels"):
+        norm.norm_residual(x, x, w)
+    lib = _lib.load()
+    assert lib.ow_norm_fwd(ctypes.byref(_args(channels=2 ** 31 - 1)), None) == 1
+    assert "too many channels" in lib.ow_last_error().decode()
