@@ -221,9 +221,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if not self._buckets:
             return loss
+        norm = self.max_norm is not None or self.skip_nonfinite
+        if norm and self._partials is None:  # asked for since the parameters were added
+            self._norm_buffers()
         hyper = [(g["lr"], g["betas"], g["eps"], g["weight_decay"]) for g in (b.group for b in self._buckets)]
-        _lib.host().adamw_step([b.native for b in self._buckets], hyper, found_inf, self._partials, self.grad_norm,
-                               self.max_norm or 0.0, self.skip_nonfinite)
+        _lib.host().adamw_step([b.native for b in self._buckets], hyper, found_inf, self._partials if norm else None,
+                               self.grad_norm, self.max_norm or 0.0, self.skip_nonfinite)
         return loss
 
     # ------------------------------------------------------------ checkpoints

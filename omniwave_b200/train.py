@@ -219,6 +219,7 @@ class TrainStep:
         loss = loss.detach()
         self._found.copy_((~torch.isfinite(loss)).to(torch.float32))
         if self._fused:
+            self.optimizer.max_norm = self.clip_norm
             self.optimizer.step(found_inf=self._found)  # also sets it for a non-finite gradient
         else:
             self._torch_update()

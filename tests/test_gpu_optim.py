@@ -197,6 +197,25 @@ def test_clip_norm_and_reproducibility(cuda_device):
         assert ((p.detach().double() - want).abs() <= ep).all()
 
 
+def test_clipping_asked_for_later_and_no_more(cuda_device):
+    sizes = [300, 5000]
+    late, first, never = (_params(cuda_device, sizes, seed=4) for _ in range(3))
+    kw = dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD)
+    a, b, c = optim.AdamW(late, **kw), optim.AdamW(first, max_norm=0.25, **kw), optim.AdamW(never, **kw)
+    a.max_norm = 0.25
+    a.step(), b.step(), c.step()
+    assert torch.equal(a.grad_norm, b.grad_norm)
+    for key in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(a.buffers[0][key], b.buffers[0][key]) and not torch.equal(a.buffers[0][key], c.buffers[0][key])
+    a.load_state_dict(c.state_dict())
+    with torch.no_grad():
+        for p, q in zip(late, never):
+            p.copy_(q)
+    a.max_norm = None
+    a.step(), c.step()
+    assert all(torch.equal(p, q) for p, q in zip(late, never))
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_nonfinite_gradient_leaves_everything(cuda_device, bits, bad):
