@@ -263,8 +263,16 @@ __device__ __forceinline__ float act_slope(float z) {
     const float s = sigmoid(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
-  if constexpr (ACT == OW_ACT_GELU)
-    return fmaf(z * 0.39894228040143268f, ex2(z * z * -0.72134752f), normal_cdf(z));
+  if constexpr (ACT == OW_ACT_GELU) {
+    // Phi by the same handbook's 7.1.26, off by 1e-7, whose exponential the density needs as well
+    const float e = ex2(z * z * -0.72134752f);  // exp(-z^2 / 2)
+    const float t = rcp(fmaf(fabsf(z), 0.23164189f, 1.f));
+    float tail = fmaf(t, 0.5307027145f, -0.7265760135f);
+    tail = fmaf(tail, t, 0.7107068705f);
+    tail = fmaf(tail, t, -0.142248368f);
+    tail = fmaf(tail, t, 0.127414796f) * t * e;
+    return fmaf(z * 0.39894228040143268f, e, z > 0.f ? 1.f - tail : tail);
+  }
   return 1.f;
 }
 
@@ -856,12 +864,15 @@ struct DzArgs {
   void* dz;          // [M, ldz] or NULL (only the sums are wanted)
   float* part;       // [chunks][N] column sums, or NULL
   int64_t M, ldz, chunk;
-  int N, bf16, vec;
+  int N, vec;
 };
 
 // dz = dy act'(z), rounded to the 16-bit type (the GEMMs take it so), and its
 // f32 column sums for the bias.  A block does 256 columns of a chunk of rows.
-template <int ACT>
+// HBM and arithmetic bound it together: 25088 x 1024 bf16 gelu 29.3 us, silu 28.1
+// (5.5 TB/s), none (sums alone) 17; without the row ahead, and with the type
+// a value instead of a parameter, 34.8, 30.6 and 17.
+template <int ACT, bool BF16>
 __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
   __shared__ float sh[8][264];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -870,25 +881,33 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
   float s[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[k] = 0.f;
-  for (int64_t m = blockIdx.y * a.chunk + ty; m < m1; m += 8) {
+  const bool whole = a.vec && n + 8 <= a.N;
+  // the row to come is asked for while the one before it is worked on
+  uint4 gv = make_uint4(0, 0, 0, 0), zv = gv;
+  auto fetch = [&](int64_t m) {
+    if (!whole || m >= m1) return;
+    gv = *reinterpret_cast<const uint4*>((const uint16_t*)a.dy + m * a.N + n);
+    if constexpr (ACT != OW_ACT_NONE) zv = *reinterpret_cast<const uint4*>((const uint16_t*)a.z + m * a.ldz + n);
+  };
+  int64_t m = blockIdx.y * a.chunk + ty;
+  fetch(m);
+  for (; m < m1; m += 8) {
     if (n >= a.N) continue;
     float g[8], z[8];
-    if (a.vec && n + 8 <= a.N) {
-      const uint4 gv = *reinterpret_cast<const uint4*>((const uint16_t*)a.dy + m * a.N + n);
-      uint4 zv = make_uint4(0, 0, 0, 0);
-      if (a.z) zv = *reinterpret_cast<const uint4*>((const uint16_t*)a.z + m * a.ldz + n);
+    if (whole) {
       const uint32_t gq[4] = {gv.x, gv.y, gv.z, gv.w}, zq[4] = {zv.x, zv.y, zv.z, zv.w};
+      fetch(m + 8);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 f = upk(gq[k], a.bf16), h = upk(zq[k], a.bf16);
+        const float2 f = unpack2<BF16>(gq[k]), h = unpack2<BF16>(zq[k]);
         g[2 * k] = f.x; g[2 * k + 1] = f.y;
         z[2 * k] = h.x; z[2 * k + 1] = h.y;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        g[k] = n + k < a.N ? ld16(a.dy, m * a.N + n + k, a.bf16) : 0.f;
-        z[k] = a.z && n + k < a.N ? ld16(a.z, m * a.ldz + n + k, a.bf16) : 0.f;
+        g[k] = n + k < a.N ? ld16(a.dy, m * a.N + n + k, BF16) : 0.f;
+        z[k] = ACT != OW_ACT_NONE && n + k < a.N ? ld16(a.z, m * a.ldz + n + k, BF16) : 0.f;
       }
     }
 #pragma unroll
@@ -898,7 +917,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzArgs a) {
     }
     if (a.dz)  // rows of dz start on 16 bytes and have room for whole vectors
       *reinterpret_cast<uint4*>((uint16_t*)a.dz + m * a.ldz + n) =
-          make_uint4(pk(g[0], g[1], a.bf16), pk(g[2], g[3], a.bf16), pk(g[4], g[5], a.bf16), pk(g[6], g[7], a.bf16));
+          make_uint4(pack2<BF16>(g[0], g[1]), pack2<BF16>(g[2], g[3]), pack2<BF16>(g[4], g[5]), pack2<BF16>(g[6], g[7]));
   }
   if (!a.part) return;
 #pragma unroll
@@ -1316,13 +1335,17 @@ int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream
   Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
   const BwdWs b = bwd_take(a, g, ws);
   if (b.dz || g->dbias) {
-    DzArgs k{g->dout, a->activation == OW_ACT_NONE ? nullptr : a->z, b.dz, b.bias, M, up8(N), b.chunk, N, bf, tma_rows(g->dout, N)};
+    DzArgs k{g->dout, a->activation == OW_ACT_NONE ? nullptr : a->z, b.dz, b.bias, M, up8(N), b.chunk, N, tma_rows(g->dout, N)};
     const dim3 grid((N + 255) / 256, b.chunks);
+    auto go = [&](auto act) {
+      if (bf) launch(dz_kernel<decltype(act)::value, true>, grid, 256, 0, st, k);
+      else launch(dz_kernel<decltype(act)::value, false>, grid, 256, 0, st, k);
+    };
     switch (a->activation) {
-      case OW_ACT_NONE: launch(dz_kernel<OW_ACT_NONE>, grid, 256, 0, st, k); break;
-      case OW_ACT_RELU: launch(dz_kernel<OW_ACT_RELU>, grid, 256, 0, st, k); break;
-      case OW_ACT_SILU: launch(dz_kernel<OW_ACT_SILU>, grid, 256, 0, st, k); break;
-      default: launch(dz_kernel<OW_ACT_GELU>, grid, 256, 0, st, k);
+      case OW_ACT_NONE: go(std::integral_constant<int, OW_ACT_NONE>()); break;
+      case OW_ACT_RELU: go(std::integral_constant<int, OW_ACT_RELU>()); break;
+      case OW_ACT_SILU: go(std::integral_constant<int, OW_ACT_SILU>()); break;
+      default: go(std::integral_constant<int, OW_ACT_GELU>());
     }
     OW_CHECK_LAUNCH("dz_kernel");
     if (g->dbias) {
