@@ -99,6 +99,7 @@ struct GemmArgs {
   int kblocks;       // 64-wide blocks of k
   int mtiles, ntiles;
   int splits;        // of the k blocks; with more than one, out is the partials
+  int kq, kr;        // kblocks / splits and the rest: the first kr splits have a block more
   Epi e;
   int* fault;
   uint32_t probe_ns;
@@ -120,6 +121,15 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 // leave their loop together and none is left behind in a __syncwarp.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort));
+}
+// Whether a phase is complete, without waiting; the same for all lanes.
+__device__ __forceinline__ bool is_done(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return __all_sync(0xffffffffu, ok);
 }
 // One lane of a converged warp, the same one each time.
 __device__ __forceinline__ bool elect_lane() {
@@ -420,16 +430,17 @@ struct Unit {
 // Unit u: the splits outermost (CTAs at work then read the same k range),
 // tiles in patches of PATCH row blocks.
 __device__ __forceinline__ Unit unit_of(const GemmArgs& a, int u) {
-  const int tiles = a.mtiles * a.ntiles;
+  // a division here is a hundred cycles before the first copy; most launches need one
+  const uint32_t tiles = (uint32_t)(a.mtiles * a.ntiles);
   Unit r;
-  r.split = u / tiles;
-  const int t = u - r.split * tiles;
-  const int per = PATCH * a.ntiles, p = t / per, q = t - p * per;
-  const int rows = min(PATCH, a.mtiles - p * PATCH);
-  r.nt = q / rows;
-  r.mt = p * PATCH + (q - r.nt * rows);
-  r.kb0 = (int)((int64_t)a.kblocks * r.split / a.splits);
-  r.kb1 = (int)((int64_t)a.kblocks * (r.split + 1) / a.splits);
+  r.split = a.splits == 1 ? 0 : (int)((uint32_t)u / tiles);
+  const uint32_t t = (uint32_t)u - (uint32_t)r.split * tiles;
+  const uint32_t per = (uint32_t)(PATCH * a.ntiles), p = a.mtiles <= PATCH ? 0 : t / per, q = t - p * per;
+  const uint32_t rows = (uint32_t)min(PATCH, a.mtiles - (int)p * PATCH);
+  r.nt = (int)(q / rows);
+  r.mt = (int)(p * PATCH + (q - (uint32_t)r.nt * rows));
+  r.kb0 = r.split * a.kq + min(r.split, a.kr);
+  r.kb1 = r.kb0 + a.kq + (r.split < a.kr ? 1 : 0);
   return r;
 }
 
@@ -454,6 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   const int units = a.mtiles * a.ntiles * a.splits;
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  Unit t = unit_of(a, first);  // while the barriers are set up
 
   if (warp == 0) {  // a lane a barrier
     for (int i = lane; i < C::NBAR; i += 32) {
@@ -485,13 +497,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     // computed once for the warp.  With a single lane in the loop, moving it to
     // the uniform registers cost 125 cycles an MMA, whatever its size.
     const bool one = elect_lane();
-    int g = 0;
-    for (int u = first; u < units; u += step) {
-      const Unit t = unit_of(a, u);
+    int s = 0, turn = 0;
+    for (int u = first; u < units;) {
       const int am0 = (t.mt * CG + (int)rank) * TM, bn0 = t.nt * BN + (int)rank * C::B_ROWS;
-      for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
-        const int s = g % C::STAGES;
-        if (g >= C::STAGES && !wait_for(empty + s, ((g / C::STAGES) - 1) & 1, abort)) break;
+      for (int kb = t.kb0; kb < t.kb1; ++kb) {
+        if (turn > 0 && !wait_for(empty + s, (turn - 1) & 1, abort)) break;
         unsigned char* sa = sm + s * A_ST;
         unsigned char* sb = sm + C::OFF_B + s * C::B_ST;
         if (one) {
@@ -514,7 +524,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
           }
         }
         __syncwarp();
+        if (++s == C::STAGES) {
+          s = 0;
+          ++turn;
+        }
       }
+      if ((u += step) < units) t = unit_of(a, u);
     }
   } else if (warp == MMA_W) {
     if (rank == 0) {
@@ -522,16 +537,22 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       const uint32_t s0 = smem_u32(sm);
       const uint32_t tmem0 = __shfl_sync(0xffffffffu, tbase, 0);
       const bool one = elect_lane();
-      int g = 0, tl = 0;
-      for (int u = first; u < units; u += step, ++tl) {
-        const Unit t = unit_of(a, u);
+      int s = 0, tl = 0;
+      uint32_t phase = 0;
+      // Whether block s has landed, asked while the one before it is issued.  A block's
+      // turn of this loop (432 cycles with the wait in front of its products, and as
+      // many for 64 columns as for 256) bounds narrow tiles: 2048 x 1024 x 2048 12.0 -> 11.5 us.
+      bool ready = false;
+      for (int u = first; u < units; ++tl) {
         const int acc = tl & 1;
         if (tl >= 2 && !wait_for(tfree + acc, ((tl >> 1) - 1) & 1, abort)) break;
         tc_fence_after();
         const uint32_t tacc = tmem0 + acc * BN;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
-          const int s = g % C::STAGES;
-          if (!wait_for(full + s, (g / C::STAGES) & 1, abort)) break;
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!ready && !wait_for(full + s, phase, abort)) break;
+          const int s1 = s + 1 == C::STAGES ? 0 : s + 1;
+          const uint32_t phase1 = s1 == 0 ? phase ^ 1 : phase;
+          ready = is_done(full + s1, phase1);
           tc_fence_after();
           const uint32_t aA = s0 + s * A_ST, aB = s0 + C::OFF_B + s * C::B_ST;
           const uint64_t da = AMN ? sdesc_mn(aA, 8192) : sdesc_sw128(aA);
@@ -544,9 +565,12 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             commit<CG>(empty + s);
           }
           __syncwarp();
+          s = s1;
+          phase = phase1;
         }
         if (one) commit<CG>(tfull + acc);
         __syncwarp();
+        if ((u += step) < units) t = unit_of(a, u);
       }
     }
   } else if (warp < C::ACTIVE) {
@@ -554,8 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     const int q = warp & 3, group = warp >> 2;
     const Epi& e = a.e;
     int tl = 0, fetched = 0;
-    for (int u = first; u < units; u += step, ++tl) {
-      const Unit t = unit_of(a, u);
+    for (int u = first; u < units; ++tl) {
       const int acc = tl & 1;
       const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
       const int nb = t.nt * BN + group * C::CW;
@@ -641,6 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
           else arrive_in(in_cta(tfree + acc, 0));
         }
       }
+      if ((u += step) < units) t = unit_of(a, u);
     }
     if (lane == 0) bulk_wait_read();  // the staging stays until it is read
   }
@@ -1112,6 +1136,8 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   k.mtiles = (int)((M + TM * p.cg - 1) / (TM * p.cg));
   k.ntiles = (N + p.bn - 1) / p.bn;
   k.splits = p.splits;
+  k.kq = k.kblocks / p.splits;
+  k.kr = k.kblocks % p.splits;
   k.e = e;
   if (p.splits > 1) {
     k.e = Epi{};
