@@ -105,12 +105,13 @@ __device__ __forceinline__ bool aligned4(const void* p) {
   return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
 }
 
-// sqrt(v) and m / d in three and two instructions, within two steps of f32.
-// Below 2^-126 the root is taken a little small instead of as 0.
+// sqrt(v) and m / d, each within two steps of f32.  The root is right for every
+// v: below 2^-126 too (gradients of 1e-19 and less), which counts with a small eps,
+// and inf for a v that overflowed, so that m / inf takes 0 off the parameter.
 __device__ __forceinline__ float fast_sqrt(float v) {
   float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(v, 1.17549435e-38f)));
-  return v * r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float fast_div(float m, float d) {
   float r;

@@ -464,3 +464,45 @@ def test_train_step_fused_follows_torch(cuda_device, graph):
     with pytest.raises(FloatingPointError):
         b.check_finite()
     assert all(torch.equal(p, q) for p, q in zip(before, mb.parameters()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+def test_unclipped_gradients_whose_squares_overflow(cuda_device, dtype):
+    """v = inf takes m / inf = 0 off its parameter, as the formula in f32 does, at once and for good; others go on."""
+    (p,) = _params(cuda_device, [1000], dtype, seed=8)
+    huge = torch.tensor([1e21, -1e21, 1e25, -1e30, 3e38], device=cuda_device)  # (1 - b2) g^2 is past f32
+    large = torch.tensor([1e10, -1e18, 1e19, 3e20], device=cuda_device)        # and here it is not
+    p.grad[:5], p.grad[500:504] = huge.to(dtype), large.to(dtype)
+    opt = optim.AdamW([p], lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, skip_nonfinite=True)
+    found = torch.zeros((), device=cuda_device)
+    m, v = torch.zeros(1000, dtype=torch.float64, device=cuda_device), torch.zeros(1000, dtype=torch.float64, device=cuda_device)
+    half = 0.0 if dtype == F32 else torch.finfo(dtype).eps / 2
+    for t in (1, 2, 3):
+        old, g = p.detach().double(), p.grad.double()
+        opt.step(found_inf=found)
+        want, _, _, ep, _, _ = _step64(old, g, m, v, t)
+        want[:5], ep[:5] = old[:5] * (1 - LR * WD), 4 * U * old[:5].abs()
+        err = (p.detach().double() - want).abs()
+        assert (err <= ep + half * want.abs() * (1 + 1e-3)).all(), (t, err.max())
+        m, v = opt.state[p]["exp_avg"].double(), opt.state[p]["exp_avg_sq"].double()
+        assert torch.isinf(v[:5]).all() and torch.isfinite(v[5:]).all() and torch.isfinite(m).all()
+        p.grad[:5] = 1e-2
+        p.grad[500:504] *= 0.5
+    assert float(found) == 0.0
+
+
+def test_small_second_moments_without_eps(cuda_device):
+    """Steps of gradients so small that v is below the smallest normal f32, taken from the v that is held."""
+    n = 1000
+    p = torch.nn.Parameter(torch.zeros(n, device=cuda_device))
+    p.grad = torch.logspace(-20.6, -17, n, device=cuda_device)
+    p.grad[::2] *= -1
+    opt = optim.AdamW([p], lr=LR, betas=(B1, B2), eps=0.0, weight_decay=0.0)
+    for t in (1, 2, 3):
+        old = p.detach().double()
+        opt.step()
+        m, v = opt.state[p]["exp_avg"].double(), opt.state[p]["exp_avg_sq"].double()
+        assert (v > 0).all() and float(v[0]) < 2.0 ** -140
+        step = LR / (1 - B1 ** t) * m / (v / (1 - B2 ** t)).sqrt()
+        # m and v are the held ones here, so less than the 30 u of a step from the gradient
+        assert ((p.detach().double() - (old - step)).abs() <= 30 * U * step.abs() + 4 * U * old.abs()).all(), t
