@@ -390,9 +390,12 @@ OW_API int ow_pool_head_fwd(const ow_pool_head_t* args, void* stream);
  * ``params``, ``grads`` and ``slots`` are host arrays, read during the call
  * (a captured graph keeps the pointers it was captured with).  A NULL
  * gradient leaves its tensor, its state and its step count as they are.  A
- * gradient that is inf or NaN and does not call the step off makes its
- * parameter and its moments so, and with 8 bits spoils the moments of its whole
- * block.  Neither function allocates or synchronises.
+ * gradient that is inf or NaN and does not call the step off makes its own
+ * parameter and moments NaN, and no others.  A finite one whose square is past
+ * f32 (above 6e20 with b2 = 0.999) is no reason to call a step off: its v is inf
+ * and its update 0, for good with 32 bits; with 8 its m is then held as 0 and
+ * its v as its block's largest finite one, and it goes on from there.  Neither
+ * function allocates or synchronises.
  */
 #define OW_ADAMW_BLOCK 256
 #define OW_ADAMW_CONTROL_BYTES 64

@@ -136,11 +136,42 @@ __device__ __forceinline__ void random20(uint32_t seed, uint32_t e, uint32_t& r1
 
 // |x| inv, at most 448, as an e4m3 magnitude.  Times 2^-120 the exponents of
 // e4m3 (subnormals included) are those of f32, so the code is the top bits and
-// adding a random number below them rounds.  ``most``: 126, or 127 (a NaN) in a
-// block that holds values that are not finite.
-__device__ __forceinline__ uint32_t hold8(float x, float inv, uint32_t r20, uint32_t most) {
+// adding a random number below them rounds.
+__device__ __forceinline__ uint32_t hold8(float x, float inv, uint32_t r20) {
   const float y = __fmul_rn(fabsf(x), inv);
-  return min((__float_as_uint(y * 7.52316384526264e-37f) + r20) >> 20, most);  // 2^-120
+  return min((__float_as_uint(y * 7.52316384526264e-37f) + r20) >> 20, 126u);  // 2^-120
+}
+
+constexpr uint32_t INF = 0x7F800000u;
+
+// A block whose v are not all finite, before it is held; a format with one scale
+// has no room for them, and they are kept from the block's other elements.  An
+// element that a gradient (or its own state) has made NaN or inf is marked by
+// v = NaN and held so.  One with a finite m whose v overflowed took a step of 0;
+// it goes on from m = 0 and the largest finite v of its block.  ``mmax`` and
+// ``vtop`` (as bits): the largest of the finite ones, of the whole block.
+__device__ __forceinline__ void mend_odd(float (&m)[2][4], float (&v)[2][4], float& mmax, uint32_t& vtop) {
+  float mm = 0.f;
+  uint32_t vt = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool lost = (__float_as_uint(m[j][k]) & INF) == INF || v[j][k] != v[j][k];
+      if (lost) v[j][k] = __uint_as_float(0x7FFFFFFFu);
+      else if (__float_as_uint(v[j][k]) == INF) m[j][k] = 0.f;
+      else {
+        mm = fmaxf(mm, fabsf(m[j][k]));
+        vt = max(vt, __float_as_uint(v[j][k]));
+      }
+    }
+  mmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mm)));
+  vtop = __reduce_max_sync(0xffffffffu, vt);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (__float_as_uint(v[j][k]) == INF) v[j][k] = __uint_as_float(vtop);
 }
 
 __device__ __forceinline__ void unhold4(uint32_t codes, float scale, float (&o)[4]) {
@@ -332,13 +363,12 @@ __global__ void __launch_bounds__(WARPS * 32, 3) adamw_kernel(const __grid_const
       if constexpr (EIGHT) {
         mmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));  // not negative
         vtop = __reduce_max_sync(0xffffffffu, vtop);
+        const bool odd = vtop >= INF;
+        if (odd) mend_odd(mv, vv, mmax, vtop);
         const float vmax = __uint_as_float(vtop);
         const uint32_t seed = random_seed(slot, (uint32_t)t_have) + lane * 4 * 0x9E3779B1u;
         const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
         const uint32_t least = vinv > 0.f ? 1u : 0u;
-        // A gradient that is not finite (and was not called off) makes v so; then
-        // the codes of the elements concerned are NaN.
-        const uint32_t odd = vtop >= 0x7F800000u ? 127u : 126u;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t om = 0, ov = 0;
@@ -346,10 +376,18 @@ __global__ void __launch_bounds__(WARPS * 32, 3) adamw_kernel(const __grid_const
           for (int k = 0; k < 4; ++k) {
             uint32_t r1, r2;
             random20(seed, j * 128 + k, r1, r2);
-            const uint32_t qm = hold8(mv[j][k], minv, r1, odd) | (__float_as_uint(mv[j][k]) >> 24 & 128u);
-            const uint32_t qv = max(hold8(vv[j][k], vinv, r2, odd), min(__float_as_uint(vv[j][k]), least));
+            const uint32_t qm = hold8(mv[j][k], minv, r1) | (__float_as_uint(mv[j][k]) >> 24 & 128u);
+            const uint32_t qv = max(hold8(vv[j][k], vinv, r2), min(__float_as_uint(vv[j][k]), least));
             om |= qm << (8 * k);
             ov |= qv << (8 * k);
+          }
+          if (odd) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (vv[j][k] != vv[j][k]) {
+                om |= 127u << (8 * k);
+                ov |= 127u << (8 * k);
+              }
           }
           *reinterpret_cast<uint32_t*>((unsigned char*)a.m + slot + j * 128 + lane * 4) = om;
           *reinterpret_cast<uint32_t*>((unsigned char*)a.v + slot + j * 128 + lane * 4) = ov;

@@ -506,3 +506,79 @@ def test_small_second_moments_without_eps(cuda_device):
         step = LR / (1 - B1 ** t) * m / (v / (1 - B2 ** t)).sqrt()
         # m and v are the held ones here, so less than the 30 u of a step from the gradient
         assert ((p.detach().double() - (old - step)).abs() <= 30 * U * step.abs() + 4 * U * old.abs()).all(), t
+
+
+def _twins(dev, n, at, grad, **kw):
+    """Two 8-bit optimizers over the same parameter, the first with ``grad`` at ``at`` and the second with 0 there."""
+    (p,), (q,) = _params(dev, [n], seed=9), _params(dev, [n], seed=9)
+    p.grad[at], q.grad[at] = grad, 0.0
+    kw = dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, state_bits=8) | kw
+    return p, q, optim.AdamW([p], **kw), optim.AdamW([q], **kw)
+
+
+def _others_equal(p, q, a, b, at):
+    rest = torch.ones(p.numel(), dtype=torch.bool, device=p.device)
+    rest[at] = False
+    assert torch.equal(p.detach()[rest], q.detach()[rest])
+    for k, t in a.buffers[0].items():
+        t, w = t.view(torch.uint8), b.buffers[0][k].view(torch.uint8)
+        if k in ("exp_avg", "exp_avg_sq"):
+            t, w = t[:p.numel()][rest], w[:p.numel()][rest]
+        assert torch.equal(t, w), k
+
+
+def test_8bit_overflow_of_one_element_stays_with_it(cuda_device):
+    """Its v is past f32, so it takes no step; it goes on from m = 0 and its block's largest v, the others as ever."""
+    at = torch.tensor([300, 301, 1023], device=cuda_device)
+    p, q, a, b = _twins(cuda_device, 1024, at, torch.tensor([1e30, -1e25, 3e38], device=cuda_device), skip_nonfinite=True)
+    found = torch.zeros((), device=cuda_device)
+    old = p.detach().double()
+    a.step(found_inf=found), b.step()
+    assert float(found) == 0.0
+    assert ((p.detach().double() - old * (1 - LR * WD)).abs() <= 4 * U * old.abs())[at].all()
+    _others_equal(p, q, a, b, at)
+    h = a.buffers[0]
+    assert not h["exp_avg"].float()[at].any()
+    v = h["exp_avg_sq"].float()
+    assert (v[at] == 448).all() and (v.view(-1, 256)[torch.tensor([1, 3])].amax(1) == 448).all()
+    p.grad[at] = q.grad[at]  # 0: the block's largest v falls like any, so the scales stay alike
+    a.step(), b.step()
+    _others_equal(p, q, a, b, at)
+    before = p.detach().clone()
+    p.grad[at] = 1e-2
+    a.step()
+    moved = (p.detach() - before * (1 - LR * WD))[at]
+    # m = 0.1 g, c1 = 0.271; v >= 0.001 g^2, c2 = 0.003: at most 0.37 / 0.577 lr
+    assert (moved < 0).all() and (moved.abs() <= LR).all()
+
+
+def test_8bit_overflow_of_a_whole_block(cuda_device):
+    """No v of the block can be held: it is zeros, and its moments start over."""
+    at = torch.arange(256, 512, device=cuda_device)
+    p, q, a, b = _twins(cuda_device, 1024, at, torch.full((256,), 1e30, device=cuda_device), skip_nonfinite=True)
+    old = p.detach().double()
+    a.step(), b.step()
+    assert ((p.detach().double() - old * (1 - LR * WD)).abs() <= 4 * U * old.abs())[at].all()
+    _others_equal(p, q, a, b, at)
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert float(a.buffers[0][k + "_scale"][1]) == 0.0 and not a.buffers[0][k].float()[at].any()
+    p.grad[at] = 1e-2
+    before = p.detach().clone()
+    a.step()
+    moved = (p.detach() - before * (1 - LR * WD))[at]
+    # m = 0.1 g, c1 = 0.19; v = 0.001 g^2, c2 = 0.001999: 0.526 / 0.707 lr
+    assert ((moved / -LR - 0.744).abs() < 0.01).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_8bit_gradient_that_is_not_finite_stays_with_its_element(cuda_device, bad):
+    """When it does not call the step off: its parameter and moments are NaN from then on, and no other's."""
+    at = torch.tensor([300, 777], device=cuda_device)
+    p, q, a, b = _twins(cuda_device, 1024, at, bad)
+    for _ in range(3):
+        a.step(), b.step()
+        assert torch.isnan(p.detach()[at]).all()
+        _others_equal(p, q, a, b, at)
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.isnan(a.buffers[0][k].float()[at]).all()
+        p.grad[at] = 0.0
