@@ -385,7 +385,9 @@ OW_API int ow_pool_head_fwd(const ow_pool_head_t* args, void* stream);
  * state_bits == 32 the moments are f32.  With 8 they are e4m3 codes, with one
  * f32 scale (largest magnitude / 448) for each block of OW_ADAMW_BLOCK slots;
  * they are rounded stochastically by a hash of (slot, step), so a run is
- * reproducible bit for bit, and a positive second moment is never held as 0.
+ * reproducible bit for bit.  A positive second moment is held as the smallest
+ * code at least; a block of which none is above 2^-100 is held as zeros, its
+ * first moments too.  eps must be positive with 8 bits.
  *
  * ``params``, ``grads`` and ``slots`` are host arrays, read during the call
  * (a captured graph keeps the pointers it was captured with).  A NULL

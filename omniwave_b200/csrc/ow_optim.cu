@@ -19,8 +19,11 @@
 // a step moves v by 0.1% or less, far under half a step of a 3-bit mantissa
 // (3 to 6%), so rounding to nearest would hold v where it is for good, while
 // this keeps its expectation.  The update itself uses the unrounded moments.
-// A positive v is never held as 0: an element with v = 0 and m != 0 would
-// next move by m / eps.
+// A positive v is never held as 0 beside an m that is not: the element would
+// next move by m / eps.  In a block with a v above 2^-100 it is held as the
+// smallest code at least; in one without, v and m are zeros, and a step is then
+// at most that from moments of zero, 3.2 lr (gradients below 3e-14 of which eps,
+// 1e-8 as a rule, leaves nothing to see).
 //
 // Bound: with 32-bit moments HBM: an f32 parameter costs 28 bytes (p, m, v read
 // and written, g read); 10.2 M take 46.5 us (6.2 TB/s), 40 M 177 us (6.3).  With 8
@@ -42,7 +45,7 @@ namespace {
 
 constexpr int BLK = OW_ADAMW_BLOCK;  // slots a warp works on, and that share a scale
 constexpr int WARPS = 8;
-constexpr float TINY = 7.888609052210118e-31f;  // 2^-100: a block below it is held as zeros
+constexpr float TINY = 7.888609052210118e-31f;  // 2^-100: a block whose values are all below it is held as zeros
 
 template <int MAXT>
 struct Ptrs {
@@ -367,6 +370,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) adamw_kernel(const __grid_const
         if (odd) mend_odd(mv, vv, mmax, vtop);
         const float vmax = __uint_as_float(vtop);
         const uint32_t seed = random_seed(slot, (uint32_t)t_have) + lane * 4 * 0x9E3779B1u;
+        if (!(vmax > TINY)) mmax = 0.f;  // v held as zeros: an m held beside them would next move by m / eps
         const float minv = mmax > TINY ? __fdiv_rn(448.f, mmax) : 0.f, vinv = vmax > TINY ? __fdiv_rn(448.f, vmax) : 0.f;
         const uint32_t least = vinv > 0.f ? 1u : 0u;
 #pragma unroll
@@ -635,6 +639,8 @@ int ow_adamw_step(const ow_adamw_t* a, void* stream) {
                    ((uintptr_t)a->exp_avg_scale | (uintptr_t)a->exp_avg_sq_scale | (uintptr_t)a->dev_steps |
                     (uintptr_t)a->lr_ptr | (uintptr_t)a->found) % 4 == 0,
                "ow_adamw_step: the state is not aligned");
+  OW_CHECK_ARG(a->state_bits == 32 || (float)a->eps > 0.f,
+               "ow_adamw_step: 8-bit states need a positive eps (both moments may be held as 0)");
   OW_CHECK_ARG(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "ow_adamw_step: betas must be in [0, 1)");
   for (int i = 0; i < a->tensors; ++i)
     OW_CHECK_ARG(a->params[i] || !a->grads[i], "ow_adamw_step: parameter %d is NULL", i);

@@ -123,7 +123,7 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` is a number, or a float32 tensor of one element on the parameters'
     device, which the kernel reads when it runs (so a captured step follows a
     schedule).  ``state_bits`` is 32 or 8 (also as a parameter group's own
-    option).  ``max_norm`` clips the gradients by their global norm, as
+    option); 8 needs a positive ``eps``.  ``max_norm`` clips the gradients by their global norm, as
     ``clip_grad_norm_`` does but without writing them; ``skip_nonfinite`` leaves
     parameters and state untouched in a step whose gradients hold an inf or a
     NaN.  With either, ``grad_norm`` is the norm of the last step, on the
@@ -163,6 +163,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"invalid weight_decay: {group['weight_decay']}")
         if group["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+        if group["state_bits"] == 8 and not ctypes.c_float(group["eps"]).value > 0.0:
+            raise ValueError(f"8-bit moments need a positive eps (both may be held as 0), got {group['eps']}")
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)

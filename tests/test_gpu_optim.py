@@ -582,3 +582,21 @@ def test_8bit_gradient_that_is_not_finite_stays_with_its_element(cuda_device, ba
         for k in ("exp_avg", "exp_avg_sq"):
             assert torch.isnan(a.buffers[0][k].float()[at]).all()
         p.grad[at] = 0.0
+
+
+def test_8bit_second_moments_too_small_to_hold(cuda_device):
+    """Where a block's v are held as zeros its m are too, so no step is longer than one from moments of zero."""
+    p = torch.nn.Parameter(torch.zeros(512, device=cuda_device))
+    p.grad = torch.full_like(p, 1e-17)  # (1 - b2) g^2 = 1e-37, below 2^-100
+    opt = optim.AdamW([p], lr=LR, betas=(B1, B2), eps=1e-30, weight_decay=0.0, state_bits=8)
+    opt.buffers[0]["step"].fill_(20_000)  # both corrections are 1
+    for k in range(8):
+        before = p.detach().clone()
+        opt.step()
+        # 0.1 / sqrt(0.001), where moments held apart would reach 1 / sqrt(0.001)
+        assert ((before - p.detach()).abs() <= LR * 0.1 / 0.001 ** 0.5 * (1 + 1e-5)).all(), k
+        assert not any(t.view(torch.uint8).any() for name, t in opt.buffers[0].items() if name != "step")
+    p.grad.zero_()
+    before = p.detach().clone()
+    opt.step()
+    assert torch.equal(p.detach(), before)

@@ -125,3 +125,16 @@ def test_c_entry_refuses_pointers_off_their_alignment(over):
         for k, v in bad.items():
             setattr(opt, k, v)
         assert lib.ow_grad_norm(a, opt, None) == 1 and "not aligned" in lib.ow_last_error().decode()
+
+
+def test_8bit_moments_need_a_positive_eps():
+    """Both moments may be held as 0, where a step is 0 / eps."""
+    group = dict(lr=1e-3, betas=(0.9, 0.999), eps=0.0, weight_decay=0.0, state_bits=32)
+    optim.AdamW._check_hyper(group, torch.device("cpu"))
+    lib = _lib.load()
+    for eps in (0.0, 1e-60):  # 0 in f32
+        with pytest.raises(ValueError, match="positive eps"):
+            optim.AdamW._check_hyper(group | dict(state_bits=8, eps=eps), torch.device("cpu"))
+        a, keep = _args(state_bits=8, exp_avg_scale=16, exp_avg_sq_scale=16, eps=eps)
+        assert lib.ow_adamw_step(a, None) == 1 and "positive eps" in lib.ow_last_error().decode()
+        del keep
