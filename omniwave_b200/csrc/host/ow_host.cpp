@@ -542,6 +542,9 @@ void adamw_step(const std::vector<Bucket*>& buckets, const std::vector<Hyper>& h
     a.use_norm = partials.defined();
     a.control = buckets[0]->args->control;
     check_status(ow_adamw_step(&a, stream), "ow_adamw_step");
+    // The kernel wrote the parameters: autograd nodes that saved one as it was before must not take it as it is now.
+    for (size_t k = 0; k < b.params.size(); ++k)
+      if (b.g[k] && !b.params[k].is_inference()) b.params[k].unsafeGetTensorImpl()->bump_version();
   }
   for (Bucket* b : buckets) b->copied.clear();
 }

@@ -600,3 +600,22 @@ def test_8bit_second_moments_too_small_to_hold(cuda_device):
     before = p.detach().clone()
     opt.step()
     assert torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_counts_as_a_write_to_its_parameters(cuda_device, bits):
+    """A backward pass that needs the weights from before a step is refused, as after torch's AdamW."""
+    from omniwave_b200 import linear, norm
+
+    x = torch.randn(64, 64, device=cuda_device, dtype=BF).requires_grad_()
+    w, idle = (torch.nn.Parameter(torch.randn(64, 64, device=cuda_device, dtype=BF) / 8) for _ in range(2))
+    scale = torch.nn.Parameter(torch.ones(64, device=cuda_device))
+    opt = optim.AdamW([w, idle, scale], lr=LR, state_bits=bits)
+    for out in (linear.linear(x, w), norm.rms_norm(x, scale)):
+        before = [t._version for t in (w, scale)]
+        out.float().sum().backward(retain_graph=True)
+        opt.step()
+        moved = [t._version > v for t, v in zip((w, scale), before)]
+        assert any(moved) and idle._version == 0
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.float().sum().backward()
