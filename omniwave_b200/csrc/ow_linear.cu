@@ -35,7 +35,7 @@
 // epilogue beside it): the tensor pipe for 8192^3, 713 us = 1542 TFLOP/s (675);
 // 12544 x 2048 x 1024 39.7 us (38), its last wave two thirds full; HBM for
 // 401408 x 128 x 256, 58 us (57); 25088 x 512 x 1024 25.3 us (25.7), with gelu,
-// bias and kept z 40; one row 1024 -> 2048 2.7 us.
+// bias and kept z 41; one row 1024 -> 2048 2.7 us.
 #include <cuda.h>
 
 #include <algorithm>
@@ -222,7 +222,8 @@ __device__ __forceinline__ uint64_t sdesc_mn(uint32_t addr, uint32_t lbo) {
 
 // ---------------------------------------------------------------- activations
 // 2^x and 1 / x by the special-function units, subnormals taken as 0 (two
-// instructions less each than without): what follows is rounded to 16 bits.
+// instructions less each than without).  A quotient below 2^-126 is 0, which of
+// silu drops values under 1.1e-36 (z < -87.3); all others keep their 22 bits.
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -235,33 +236,57 @@ __device__ __forceinline__ float rcp(float x) {
 }
 __device__ __forceinline__ float sigmoid(float z) { return rcp(1.f + ex2(z * -1.44269504f)); }
 
-// Phi(z) = (1 + erf(z / sqrt 2)) / 2 by Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.28: erfc(x) = (1 + a1 x + ... + a6 x^6)^-16, off by
-// 3e-7 at most, here in |z| = sqrt(2) x.  One special-function result an
-// element where an exponential and a quotient take two; erff and expf took 40
-// instructions and bound the epilogue.
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float a = fabsf(z);
-  float p = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(5.3829750e-6f, a, 4.8890636e-5f), a, 3.8003575e-5f), a, 3.2776263e-3f), a, 2.1141006e-2f), a,
-                      4.9867347e-2f), a, 1.f);
-  p *= p;
-  p *= p;
-  p *= p;
-  p *= p;
-  const float tail = 0.5f * rcp(p);
-  return z > 0.f ? 1.f - tail : tail;
+// gelu(z) = z Phi(z) for a result of the 16-bit type.  Phi's tail, Phi(-|z|), is
+// 2^q(|z|): its logarithm is so near a parabola that a polynomial of degree 8
+// serves, and its error is one of the tail relative to itself, so gelu keeps its
+// bits where it is small (a form whose error is bounded absolutely was off by 8
+// steps of f16 at z = -4).  q is this file's own fit, by a linear program over the
+// coefficients, one for each type:
+//   f16   off by 7e-6 of the tail up to |z| = 6, from where z Phi rounds to 0 (q
+//         falls on without end), and by 4e-7 of 1;
+//   bf16  by 3.1e-4 of the tail up to 6 and 6.3e-4 up to 13.5, by 6e-7 of 1; from
+//         z = -12.9 on the exponential, and gelu below 1.6e-37 with it, is 0.
+// One special-function result an element: with erff, or with an exponential and a
+// quotient, the epilogue is slower (25088 x 512 x 1024 with bias and kept z 56 and
+// 47 us, here 41).
+template <bool BF16>
+__device__ __forceinline__ float gelu(float z) {
+  float q;
+  if constexpr (BF16) {
+    const float a = fminf(fabsf(z), 13.5f);
+    q = fmaf(a, 3.98267339e-8f, -2.39384553e-6f);
+    q = fmaf(q, a, 6.14833989e-5f);
+    q = fmaf(q, a, -8.9382549e-4f);
+    q = fmaf(q, a, 8.29635281e-3f);
+    q = fmaf(q, a, -5.3509552e-2f);
+    q = fmaf(q, a, -0.458847046f);
+    q = fmaf(q, a, -1.15114152f);
+    q = fmaf(q, a, -1.00000072f);
+  } else {
+    const float a = fabsf(z);
+    q = fmaf(a, -1.39922733e-7f, 1.43002126e-6f);
+    q = fmaf(q, a, 3.0813193e-5f);
+    q = fmaf(q, a, -7.80530798e-4f);
+    q = fmaf(q, a, 8.10782891e-3f);
+    q = fmaf(q, a, -5.33918403e-2f);
+    q = fmaf(q, a, -0.458847821f);
+    q = fmaf(q, a, -1.15115714f);
+    q = fmaf(q, a, -0.999998868f);
+  }
+  const float tail = ex2(q);
+  return z * (z > 0.f ? 1.f - tail : tail);
 }
-template <int ACT>
+template <int ACT, bool BF16>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == OW_ACT_RELU) return z > 0.f || z != z ? z : 0.f;
   if constexpr (ACT == OW_ACT_SILU) return z * sigmoid(z);
-  if constexpr (ACT == OW_ACT_GELU) return z * normal_cdf(z);
+  if constexpr (ACT == OW_ACT_GELU) return gelu<BF16>(z);
   return z;
 }
-__device__ __forceinline__ float act_fwd(float z, int act) {
-  return act == OW_ACT_RELU   ? act_fwd<OW_ACT_RELU>(z)
-         : act == OW_ACT_SILU ? act_fwd<OW_ACT_SILU>(z)
-         : act == OW_ACT_GELU ? act_fwd<OW_ACT_GELU>(z)
+__device__ __forceinline__ float act_fwd(float z, int act, int bf16) {
+  return act == OW_ACT_RELU   ? act_fwd<OW_ACT_RELU, false>(z)
+         : act == OW_ACT_SILU ? act_fwd<OW_ACT_SILU, false>(z)
+         : act == OW_ACT_GELU ? (bf16 ? gelu<true>(z) : gelu<false>(z))
                               : z;
 }
 
@@ -274,13 +299,17 @@ __device__ __forceinline__ float act_slope(float z) {
     return s * fmaf(z, 1.f - s, 1.f);
   }
   if constexpr (ACT == OW_ACT_GELU) {
-    // Phi by the same handbook's 7.1.26, off by 1e-7, whose exponential the density needs as well
-    const float e = ex2(z * z * -0.72134752f);  // exp(-z^2 / 2)
-    const float t = rcp(fmaf(fabsf(z), 0.23164189f, 1.f));
-    float tail = fmaf(t, 0.5307027145f, -0.7265760135f);
-    tail = fmaf(tail, t, 0.7107068705f);
-    tail = fmaf(tail, t, -0.142248368f);
-    tail = fmaf(tail, t, 0.127414796f) * t * e;
+    // Phi(z) + z phi(z).  The density needs exp(-z^2 / 2) anyway, and the tail is
+    // t P(t) times it with t = 1 / (1 + 0.35 |z|): this file's own fit again, off by
+    // 1e-7 of 1, 3e-7 of the tail up to |z| = 6 and 3e-5 up to 14
+    const float e = ex2(z * z * -0.72134752f);
+    const float t = rcp(fmaf(fabsf(z), 0.35f, 1.f));
+    float tail = fmaf(t, 0.0471570618f, -0.194429092f);
+    tail = fmaf(tail, t, 0.226878741f);
+    tail = fmaf(tail, t, -0.00380232154f);
+    tail = fmaf(tail, t, 0.148624128f);
+    tail = fmaf(tail, t, 0.135697883f);
+    tail = fmaf(tail, t, 0.139873699f) * t * e;
     return fmaf(z * 0.39894228040143268f, e, z > 0.f ? 1.f - tail : tail);
   }
   return 1.f;
@@ -635,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         }
         if constexpr (ACT != OW_ACT_NONE) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT>(v[i]);
+          for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT, BF16>(v[i]);
         }
         if (e.res) {
 #pragma unroll
@@ -704,7 +733,7 @@ __global__ void __launch_bounds__(256) gemm_sum_kernel(const float* __restrict__
       float z = v[k];
       if (e.bias) z += ld_any(e.bias, e.bias_dt, n + k);
       if (e.z) st16(e.z, m * e.ldz + n + k, e.bf16, keep_z(z, e.bf16));
-      z = act_fwd(z, e.act);
+      z = act_fwd(z, e.act, e.bf16);
       if (e.res) z += ld16(e.res, m * e.ldr + n + k, e.bf16);
       if (e.out32) ((float*)e.out)[m * e.ldo + n + k] = z;
       else st16(e.out, m * e.ldo + n + k, e.bf16, z);
@@ -726,7 +755,7 @@ struct RowsArgs {
 __device__ __forceinline__ void finish_one(const Epi& e, float z, int64_t m, int n, int bf) {
   if (e.bias) z += ld_any(e.bias, e.bias_dt, n);
   if (e.z) st16(e.z, m * e.ldz + n, bf, keep_z(z, bf));
-  z = act_fwd(z, e.act);
+  z = act_fwd(z, e.act, bf);
   if (e.res) z += ld16(e.res, m * e.ldr + n, bf);
   st16(e.out, m * e.ldo + n, bf, z);
 }
@@ -893,7 +922,7 @@ struct DzArgs {
 
 // dz = dy act'(z), rounded to the 16-bit type (the GEMMs take it so), and its
 // f32 column sums for the bias.  A block does 256 columns of a chunk of rows.
-// HBM and arithmetic bound it together: 25088 x 1024 bf16 gelu 29.3 us, silu 28.1
+// HBM and arithmetic bound it together: 25088 x 1024 bf16 gelu 30.7 us, silu 28.0
 // (5.5 TB/s), none (sums alone) 17; without the row ahead, and with the type
 // a value instead of a parameter, 34.8, 30.6 and 17.
 template <int ACT, bool BF16>

@@ -459,3 +459,65 @@ def test_run_of_the_operators_together(cuda_device):
         step = ps[k].detach().double() - before[k].double()
         sure = g.abs() > tol * g.abs().max()  # a first step is lr against the gradient's sign
         assert ((step + 1e-2 * torch.sign(g)).abs()[sure] <= 1e-4 + _half(BF) * 1.01 * ps[k].double().abs()[sure]).all(), k
+
+
+def _gelu_cases(dev, t):
+    """Every finite z of the type with -20 < z < 20, as inputs that an identity weight passes on exactly."""
+    v = torch.arange(65536, dtype=torch.int32, device=dev).to(torch.int16).view(t)
+    v = v[torch.isfinite(v) & (v.abs() < 20)]
+    return torch.cat([v, v.new_zeros(-v.numel() % 1920)])
+
+
+def _gelu_bound(z, t):
+    """gelu, its slope, and how far a result may be off.
+
+    Forward: the tail Phi(-|z|) is 2^q(|z|), whose fit is off by 7e-6 of it (f16, up to |z| = 6), 3.1e-4 (bf16, up to 6)
+    or 6.3e-4 (further out), under a third of bf16's half step.  Of q's 8 fused steps each is rounded by u of its partial
+    sum; the sums' magnitudes add up to less than 8.5 (1 + z^2) after all later factors, and log 2 of that is the tail's:
+    12 (1 + z^2) u, with 4 u of the exponential and 2 u of the products.
+    Slope: the tail is t P(t) exp(-z^2 / 2), fitted to 3e-7 up to 6 and 3e-5 further out.  The exponent's three roundings
+    make 3 u z^2 / 2, the exponential 4 u, t 3 u, the seven terms, whose magnitudes add up to twice their sum, 12 u, the
+    products 3 u; the density takes no more.
+    Below 2^-126 an exponential is 0: of gelu that drops |z| Phi(-|z|) where the tail is less than that (z < -12.8), of
+    the slope z phi = z exp(-z^2 / 2) / sqrt(2 pi), less than 0.4 |z| 2^-126 (z < -13.2), and less than 2^-126 of Phi.
+    Past 6, f16's gelu is under half its smallest step."""
+    a = z.abs()
+    phi, cdf, tail = (torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5,
+                      *(0.5 * torch.special.erfc(v / 2 ** 0.5) for v in (-z, a)))
+    fit = torch.full_like(z, 7e-6) if t == HF else torch.where(a <= 6, 3.1e-4, 6.3e-4)
+    rel = fit + (18 + 12 * z * z) * U
+    tiny, h = 2.0 ** -25 if t == HF else 2.0 ** -126, _half(t)
+    y, s = z * cdf, cdf + z * phi
+    drop = torch.where(tail < 1.001 * 2.0 ** -126, a * tail, 0.0)
+    ty = (rel * a * tail + 2 * U * y.abs()) * (1 + h) + h * y.abs() + tiny + drop
+    ts = (torch.where(a <= 6, 3e-7, 3e-5) + (24 + 2 * z * z) * U) * (cdf + a * phi) * (1 + h) + h * s.abs()
+    return (y, ty), (s, ts + tiny * (1 + 0.4 * a))
+
+
+@pytest.mark.parametrize("t", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("k,rows", [(16, None), (16, 8), (15, 4)], ids=["gemm", "units", "rows"])
+def test_gelu_keeps_its_bits_in_the_tail(cuda_device, t, k, rows):
+    """Forward (all three kernels) and slope, to little more than the rounding of the result, for every 16-bit z."""
+    v = _gelu_cases(cuda_device, t)
+    eye = torch.eye(k, device=cuda_device, dtype=t)
+    for x in [v.view(-1, k)] if rows is None else v.view(-1, rows, k)[::7]:
+        (y, ty), (s, ts) = _gelu_bound(x.double(), t)
+        x = x.detach().requires_grad_(rows is None)
+        got = linear.linear(x, eye, activation="gelu")
+        err = (got.detach().double() - y).abs()
+        assert (err <= ty).all(), (float((err / ty).max()), float(x.detach().reshape(-1)[(err / ty).argmax()]))
+        if rows is None:
+            (dx,) = torch.autograd.grad(got, x, torch.ones_like(got))  # dz, rounded to 16 bits
+            err = (dx.double() - s).abs()
+            assert (err <= ts).all(), (float((err / ts).max()), float(x.detach().reshape(-1)[(err / ts).argmax()]))
+
+
+def test_gelu_keeps_its_bits_where_k_is_split(cuda_device):
+    """The same through the kernel that adds split products: one row block, 8192 of k, of which one term is not 0."""
+    t, k = HF, 8192
+    v = _gelu_cases(cuda_device, t)[-64 * 64:].view(64, 64)
+    x, w = torch.zeros(64, k, device=cuda_device, dtype=t), torch.zeros(64, k, device=cuda_device, dtype=t)
+    x[:, 5000:5064] = v
+    w[:, 5000:5064] = torch.eye(64, device=cuda_device, dtype=t)
+    (y, ty), _ = _gelu_bound(v.double(), t)
+    assert ((linear.linear(x, w, activation="gelu").double() - y).abs() <= ty).all()
