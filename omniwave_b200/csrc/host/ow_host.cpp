@@ -102,6 +102,12 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// A forward-mode tangent would be dropped without a word: the nodes below have no formula for it.
+void no_tangents(const char* what, std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " not supported: forward-mode differentiation");
+}
+
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward is not differentiable (create_graph is not supported)");
 }
@@ -252,6 +258,7 @@ Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps, std::optional
   OW_VALUE(x.size(-1) < MOST, "x has too many channels: ", x.size(-1));
   OW_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
   check_vector("weight", weight, x.size(-1));
+  no_tangents("norm", {x, weight});
   if (auto why = unsupported(x, {weight})) TORCH_CHECK(false, "norm not supported: ", *why);
   return norm_call(x, Tensor(), Tensor(), Tensor(), Tensor(), weight, eps, norm_out(x, out_dtype))[0];
 }
@@ -275,6 +282,7 @@ variable_list norm_residual(const Tensor& x, const Tensor& delta, const Tensor& 
     OW_VALUE(scale.dim() == 1 && scale.size(0) == b, "sample_scale must be [", b, "], got ", shape_text(scale.sizes()));
     OW_VALUE(!scale.requires_grad(), "sample_scale takes no gradient");
   }
+  no_tangents("norm", {x, delta, weight, gate, scale, next});
   if (auto why = unsupported(x, {delta, weight, gate, next})) TORCH_CHECK(false, "norm not supported: ", *why);
   if (scale.defined()) {
     TORCH_CHECK(scale.device() == x.device(), "norm not supported: tensors on ", x.device(), " and ", scale.device());
@@ -428,6 +436,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, int64_t 
   const auto shape = out_shape(x, n);
   if (res.defined())
     OW_VALUE(res.sizes() == at::IntArrayRef(shape), "residual must be ", shape_text(shape), ", got ", shape_text(res.sizes()));
+  no_tangents("linear", {x, w, bias, res});
   if (auto why = linear_unsupported(x, w, bias, res)) TORCH_CHECK(false, "linear not supported: ", *why);
   const at::ScalarType t = linear_compute(x);
   bias = dense(bias);

@@ -38,7 +38,8 @@ def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activation:
     (an f32 weight gets an f32 gradient); else x's, which must be 16-bit, and
     weight and residual must have it too.  Bad shapes raise ``ValueError``, what
     the kernels do not take ``RuntimeError``.  The backward holds the
-    pre-activation in the compute type; it cannot be differentiated again.
+    pre-activation in the compute type; it cannot be differentiated again, and
+    forward-mode differentiation is refused.
     """
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:

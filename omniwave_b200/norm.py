@@ -33,7 +33,8 @@ def rms_norm(x: Tensor, weight: Tensor, *, eps: float = RMS_EPS, out_dtype: torc
     ``x`` is ``[..., C]`` in float32, bfloat16 or float16, ``weight`` ``[C]``.  The
     result is in ``out_dtype``: by default the autocast type where autocast is
     on, else x's.  Bad shapes raise ``ValueError``, what the kernels do not take
-    ``RuntimeError``.  The backward cannot be differentiated again.
+    ``RuntimeError``.  The backward cannot be differentiated again, and forward-mode
+    differentiation is refused.
     """
     return _lib.host().rms_norm(x, weight, eps, out_dtype)
 

@@ -521,3 +521,17 @@ def test_gelu_keeps_its_bits_where_k_is_split(cuda_device):
     w[:, 5000:5064] = torch.eye(64, device=cuda_device, dtype=t)
     (y, ty), _ = _gelu_bound(v.double(), t)
     assert ((linear.linear(x, w, activation="gelu").double() - y).abs() <= ty).all()
+
+
+def test_forward_mode_is_refused(cuda_device):
+    import torch.autograd.forward_ad as fw
+
+    from omniwave_b200 import norm
+
+    x, w, g = torch.randn(4, 64, device=cuda_device, dtype=BF), torch.eye(64, device=cuda_device, dtype=BF), torch.ones(64, device=cuda_device)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: linear.linear(d, w), lambda: linear.linear(x, w, residual=d), lambda: norm.rms_norm(d, g),
+                     lambda: norm.norm_residual(x, d, g), lambda: linear.linear(d, torch.nn.Parameter(w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

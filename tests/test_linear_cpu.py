@@ -111,3 +111,17 @@ def test_refuses_features_that_their_field_does_not_hold():
         linear.linear(torch.zeros(1, 1).expand(1, k), torch.zeros(1, 1).expand(2, k))
     with pytest.raises(ValueError, match="too large"):
         linear.linear(torch.zeros(1, 8), torch.zeros(1, 8).expand(k, 8))
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+def test_refuses_forward_mode(which):
+    """A tangent would be dropped: there is no formula for it here."""
+    import torch.autograd.forward_ad as fw
+
+    t = {"x": torch.zeros(2, 8), "weight": torch.zeros(4, 8), "bias": torch.zeros(4), "residual": torch.zeros(2, 4)}
+    with fw.dual_level():
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear.linear(t["x"], t["weight"], t["bias"], residual=t["residual"])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            linear.linear(t["x"], t["weight"], t["bias"], residual=t["residual"])

@@ -121,3 +121,19 @@ def test_refuses_rows_that_their_length_field_does_not_hold():
     lib = _lib.load()
     assert lib.ow_norm_fwd(ctypes.byref(_args(channels=2 ** 31 - 1)), None) == 1
     assert "too many channels" in lib.ow_last_error().decode()
+
+
+@pytest.mark.parametrize("which", ["x", "delta", "weight", "gate", "scale", "next"])
+def test_refuses_forward_mode(which):
+    """A tangent would be dropped: there is no formula for it here."""
+    import torch.autograd.forward_ad as fw
+
+    t = {"x": torch.zeros(2, 3, 8), "delta": torch.zeros(2, 3, 8), "weight": torch.ones(8), "gate": torch.ones(8),
+         "scale": torch.ones(2), "next": torch.ones(8)}
+    with fw.dual_level():
+        t[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            norm.norm_residual(t["x"], t["delta"], t["weight"], t["gate"], sample_scale=t["scale"], next_weight=t["next"])
+        if which in ("x", "weight"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                norm.rms_norm(t["x"], t["weight"])
