@@ -840,9 +840,11 @@ int room(int C, bool vec) { return ragged(C, vec) ? C + 7 : C; }
 bool too_long(int C, bool vec) { return room(C, vec) > (vec ? LONG_V : LONG_1); }
 
 // Blocks of a group for ragged rows: a block's rows ``parts`` x RB apart start
-// alike when that is a multiple of 8.
-int alike(int parts, int RB) {
+// alike when that is a multiple of 8.  Fewer blocks than that makes do when each
+// takes its rows at once and has none further on.
+int alike(int parts, int RB, int64_t rows) {
   const int m = RB >= 8 ? 1 : 8 / RB;
+  if (parts < m && (int64_t)parts * RB >= rows) return parts;
   return std::max(m, parts / m * m);
 }
 
@@ -880,6 +882,21 @@ constexpr int fwd_per_sm(int nv, bool h16, bool rag) {
   return rag ? (nv == 1 ? 4 : 2) : nv == 1 ? (h16 ? 5 : 6) : nv == 2 ? (h16 ? 3 : 4) : (h16 ? 2 : 3);
 }
 constexpr int bwd_per_sm(int T, bool h16) { return T > 512 ? 1 : T > 256 ? (h16 ? 1 : 2) : h16 ? 2 : 3; }
+// With 1024 threads a row to come does not fit in their 64 registers.
+constexpr bool bwd_ahead(int V, int T) { return V == 8 && T <= 512; }
+
+// The blocks of the backward, rows moved in units or not, and with them the rows of its partial sums.
+void bwd_parts(const ow_norm_t* a, Args* k, bool vec) {
+  parts(a, k, BWD_PER_SM);
+  if (too_long(k->C, vec)) return;
+  split_bwd(room(k->C, vec), vec, [&](auto V, auto G, auto) -> int {
+    constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
+    parts(a, k, bwd_per_sm(T, bwd_ahead(V.value, T) && all16(*k, a->delta, a->next_w)));
+    k->per_group = (int)std::min<int64_t>(k->per_group, std::max<int64_t>(1, (k->group_rows + RB - 1) / RB));
+    if (ragged(k->C, vec)) k->per_group = alike(k->per_group, RB, k->group_rows);
+    return OW_OK;
+  });
+}
 
 }  // namespace
 }  // namespace ow
@@ -892,8 +909,11 @@ size_t ow_norm_bwd_workspace_size(const ow_norm_t* a) {
   clear_error();
   if (check(a) != OW_OK) return 0;
   Args k = base(a);
-  parts(a, &k, BWD_PER_SM);
-  return (size_t)k.groups * std::max(k.per_group, 8) * k.arrays * k.C * sizeof(float) + 256;
+  // whether the rows are moved in units depends on the gradients' addresses too
+  bwd_parts(a, &k, false);
+  const int others = k.per_group;
+  bwd_parts(a, &k, true);
+  return (size_t)k.groups * std::max(k.per_group, others) * k.arrays * k.C * sizeof(float) + 256;
 }
 
 int ow_norm_fwd(const ow_norm_t* a, void* stream) {
@@ -919,7 +939,7 @@ int ow_norm_fwd(const ow_norm_t* a, void* stream) {
         const bool h16 = V.value == 8 && all16(k, D.value, N.value);
         parts(a, &k, V.value == 8 ? fwd_per_sm(NV.value, h16, rag) : FWD_PER_SM);
         k.per_group = (int)std::min<int64_t>(k.per_group, (k.group_rows + RB - 1) / RB);
-        if (rag) k.per_group = alike(k.per_group, RB);
+        if (rag) k.per_group = alike(k.per_group, RB, k.group_rows);
         OW_CHECK_ARG(k.groups * k.per_group < (1LL << 31), "ow_norm_fwd: too many samples");
         const size_t smem = (size_t)(rag ? factor_floats<8, true>(k.C) : k.C) * sizeof(float) * (D.value + N.value);
         auto go = [&](auto kern) -> int {
@@ -955,7 +975,6 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
                    (!delta || (at(g->ddelta, a->delta_dtype) && at(g->dpost, a->post_dtype))) &&
                    (!a->gate_rows || at(g->dgate, a->gate_dtype)),
                "ow_norm_bwd: a gradient is not aligned");
-  parts(a, &k, BWD_PER_SM);
   const size_t need = ow_norm_bwd_workspace_size(a);
   if (!a->workspace || a->workspace_bytes < need) {
     set_error("ow_norm_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
@@ -966,6 +985,7 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
   const void* more[] = {k.dh, k.dn, k.dx, k.ddelta};
   const bool vec = units(k, delta, next, more, 4), rag = ragged(k.C, vec);
   const cudaStream_t st = (cudaStream_t)stream;
+  bwd_parts(a, &k, vec);
   const int64_t grid = k.groups * k.per_group;
   OW_CHECK_ARG(grid < (1LL << 31), "ow_norm_bwd: too many samples");
   if (grid > 0) OW_RETURN_IF(modes(delta, next, [&](auto D, auto N) -> int {
@@ -974,21 +994,16 @@ int ow_norm_bwd(const ow_norm_t* a, const ow_norm_grads_t* g, void* stream) {
     } else {
       OW_RETURN_IF(split_bwd(room(k.C, vec), vec, [&](auto V, auto G, auto NV) -> int {
         constexpr int T = G.value > 256 ? G.value : 256, RB = T / G.value;
-        // with 1024 threads a row to come does not fit in their 64 registers
-        constexpr bool ROOM = V.value == 8 && T <= 512;
-        const bool h16 = ROOM && all16(k, D.value, N.value);
-        parts(a, &k, bwd_per_sm(T, h16));
-        k.per_group = (int)std::min<int64_t>(k.per_group, std::max<int64_t>(1, (k.group_rows + RB - 1) / RB));
-        if (rag) k.per_group = alike(k.per_group, RB);
-        OW_CHECK_ARG(k.groups * k.per_group < (1LL << 31), "ow_norm_bwd: too many samples");
+        constexpr bool AHEAD = bwd_ahead(V.value, T);
+        const bool h16 = AHEAD && all16(k, D.value, N.value);
         const size_t smem = sizeof(float) * std::max<size_t>((size_t)(rag ? factor_floats<8, true>(k.C) : k.C) * (D.value + N.value),
                                                              RB > 1 ? (size_t)RB * k.C : 0);
         auto go = [&](auto kern) -> int {
           OW_RETURN_IF(reserve((const void*)kern, smem));
-          launch(kern, (int)(k.groups * k.per_group), T, smem, st, k);
+          launch(kern, (int)grid, T, smem, st, k);
           return OW_OK;
         };
-        if constexpr (ROOM) {
+        if constexpr (AHEAD) {
           if (h16)
             return rag ? go(norm_bwd_kernel<8, G.value, NV.value, D.value, N.value, true, true>)
                        : go(norm_bwd_kernel<8, G.value, NV.value, D.value, N.value, true, false>);

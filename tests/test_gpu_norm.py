@@ -399,3 +399,51 @@ def test_post_norm_blocks(cuda_device):
     y1 = d(x)
     torch.manual_seed(1)
     assert torch.equal(y1, d(x))
+
+
+@pytest.mark.parametrize("c", [64, 70, 777])
+def test_a_gate_for_each_of_many_samples_of_one_token(cuda_device, c):
+    shape, st = (100_000, 1, c), BF
+    d = _inputs(cuda_device, shape, st, st, "bc")
+    want, mag = _define(d, True, "pair")
+    names = ["x", "delta", "post", "gate", "pre"]
+    leaves = {k: d[k].requires_grad_() for k in names}
+    out = _call(d | leaves, True, "pair")
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(list(out.values()), [leaves[k] for k in names], [d["dh"], d["dn"]])
+    # dx, ddelta, the gate's f32 gradient and the partial sums: two rows of f32 a sample
+    assert torch.cuda.max_memory_allocated() - held <= 1.05 * 100_000 * c * (2 * 2 + 4 + 2 * 4) + (1 << 22)
+    got = {k: v.detach() for k, v in out.items()} | {"d_" + k: g for k, g in zip(names, grads)}
+    _check(got, want, mag, c, 100_000, f"c={c}")
+
+
+@pytest.mark.parametrize("c", [40, 64, 70, 129, 512, 777, 1000, 1032, 2049, 4096, 8200])
+@pytest.mark.parametrize("samples,tokens", [(300, 1), (300, 7), (3, 500), (700, 40)])
+@pytest.mark.parametrize("t,off", [(BF, 0), (BF, 1), (F32, 0)], ids=["bf16", "bf16-off", "f32"])
+def test_backward_stays_in_its_workspace(cuda_device, c, samples, tokens, t, off):
+    """The C entry, given the bytes that it asked for in front of a guard; gradients off 16 bytes as well."""
+    if samples * tokens * c > 30_000_000:
+        tokens = max(1, 30_000_000 // (samples * c))
+    shape = (samples, tokens, c)
+    d = _inputs(cuda_device, shape, t, t, "bc")
+    rows, n = samples * tokens, samples * tokens * c
+    code = _lib.DTYPE_CODE[t]
+    stats = torch.ones(2, rows, device=cuda_device)
+    outs = {k: torch.zeros(n + 1, dtype=t, device=cuda_device)[off:off + n] for k in ("dx", "dd")}
+    dp, dg, dq = torch.empty(c, device=cuda_device), torch.empty(samples, c, device=cuda_device), torch.empty(c, device=cuda_device)
+    a = _lib.Norm(samples, tokens, c, d["x"].data_ptr(), code, d["delta"].data_ptr(), code, d["post"].data_ptr(), 0,
+                  d["gate"].data_ptr(), 0, samples, None, d["pre"].data_ptr(), 0, EPS, None, None, code,
+                  stats[0].data_ptr(), stats[1].data_ptr(), None, 0)
+    g = _lib.NormGrads(d["dh"].data_ptr(), d["dn"].data_ptr(), outs["dx"].data_ptr(), outs["dd"].data_ptr(), dp.data_ptr(),
+                       dg.data_ptr(), dq.data_ptr())
+    lib = _lib.load()
+    need = lib.ow_norm_bwd_workspace_size(a)
+    ws = torch.full((need + (1 << 20),), 0x5A, dtype=torch.uint8, device=cuda_device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _lib.check(lib.ow_norm_bwd(a, g, torch.cuda.current_stream().cuda_stream), "ow_norm_bwd")
+    assert (ws[need:] == 0x5A).all()
+    # the sums against the definition, with the 1 / rms that was given (1): dnext = sum dn h, h = x + q wp delta
+    h = d["x"].double() + d["gate"].double()[:, None] * d["post"].double() * d["delta"].double()
+    want, mag = (d["dn"].double() * h).sum((0, 1)), (d["dn"].double().abs() * h.abs()).sum((0, 1))
+    assert ((dq.double() - want).abs() <= (64 + rows / 4 + 64) * U * mag + U * want.abs()).all()

@@ -137,3 +137,18 @@ def test_refuses_forward_mode(which):
         if which in ("x", "weight"):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 norm.rms_norm(t["x"], t["weight"])
+
+
+@pytest.mark.parametrize("samples,tokens,c,bf16,parts", [
+    (50176, 1, 1024, True, 1),   # a row a sample: one part each
+    (262144, 1, 1024, True, 1),
+    (128, 196, 512, True, 3),    # as many as make three blocks an SM
+    (100_000, 1, 70, False, 1),  # ragged rows as well, while a block takes a sample's rows at once
+    (100_000, 1, 777, True, 1),
+    (128, 49, 777, True, 4),     # and here every fourth row of a block starts alike
+])
+def test_backward_workspace_is_what_the_parts_take(samples, tokens, c, bf16, parts):
+    lib = _lib.load()
+    t = 2 if bf16 else 0
+    a = _args(samples=samples, tokens=tokens, channels=c, x_dtype=t, delta_dtype=t, n_dtype=t, gate_rows=samples)
+    assert lib.ow_norm_bwd_workspace_size(ctypes.byref(a)) <= samples * parts * 2 * c * 4 + 256
