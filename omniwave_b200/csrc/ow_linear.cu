@@ -1250,7 +1250,8 @@ int blocks_of(int64_t k) { return (int)((k + KE - 1) / KE); }
 
 // Everything a backward call needs, carved from its workspace.
 struct BwdWs {
-  void* dz;        // [rows, up8(N)], or NULL: dout serves as it is
+  bool own_dz;     // dz is made; else dout serves as it is
+  void* dz;        // [rows, up8(N)] (NULL too where only the size is asked for)
   float* bias;     // [chunks][N]
   int chunks;
   int64_t chunk;
@@ -1262,15 +1263,15 @@ BwdWs bwd_take(const ow_linear_t* a, const ow_linear_grads_t* g, Carver& ws) {
   BwdWs b{};
   const int N = a->out_features, K = a->in_features;
   const int64_t M = a->rows;
-  if ((g->dx || g->dweight) && (a->activation != OW_ACT_NONE || !tma_rows(g->dout, N)))
-    b.dz = ws.take((size_t)M * up8(N) * 2);
+  b.own_dz = (g->dx || g->dweight) && (a->activation != OW_ACT_NONE || !tma_rows(g->dout, N));
+  if (b.own_dz) b.dz = ws.take((size_t)M * up8(N) * 2);
   // chunks of rows: a few blocks an SM, at least 8 rows each
   const int64_t col_blocks = (N + 255) / 256;
   b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
   b.chunk = (M + b.chunks - 1) / b.chunks;
   b.chunks = (int)((M + b.chunk - 1) / b.chunk);
   if (g->dbias) b.bias = (float*)ws.take((size_t)b.chunks * N * 4);
-  const Mat dz = b.dz ? Mat{nullptr, M, N, up8(N)} : Mat{g->dout, M, N, N};
+  const Mat dz = b.own_dz ? Mat{nullptr, M, N, up8(N)} : Mat{g->dout, M, N, N};
   if (g->dx) {
     b.px = plan_gemm(M, K, blocks_of(N));
     b.x = gemm_take(dz, mat_w(a), M, K, b.px, ws);

@@ -125,3 +125,17 @@ def test_refuses_forward_mode(which):
             linear.linear(t["x"], t["weight"], t["bias"], residual=t["residual"])
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             linear.linear(t["x"], t["weight"], t["bias"], residual=t["residual"])
+
+
+@pytest.mark.parametrize("n", [4095, 4089])
+def test_backward_workspace_has_no_copies_that_are_not_made(n):
+    """dz is made in rows that TMA reads, so an odd width asks for no more than the next multiple of 8 does."""
+    lib = _lib.load()
+    g = _lib.LinearGrads(16, 16, 16, 2, 16)
+    kw = dict(rows=32768, in_features=4096, activation=3, ldx=4096, ldw=4096, residual=None)
+    even = lib.ow_linear_workspace_size(_args(out_features=4096, **kw), g)
+    odd = lib.ow_linear_workspace_size(_args(out_features=n, **kw), g)
+    assert 32768 * 4096 * 2 <= odd <= even + 4096
+    # without an activation dy itself is read: where its rows are no 16-byte units it is copied once, as dz
+    plain = lib.ow_linear_workspace_size(_args(out_features=n, **(kw | dict(activation=0))), g)
+    assert plain == odd
