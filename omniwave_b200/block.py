@@ -19,6 +19,7 @@ from collections.abc import Iterable
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.nn.modules import module as _module
 
 from omniwave_b200.norm import norm_residual, rms_norm
 from omniwave_b200.ops import (bigemm_delta_cuda, block_forward, cuda_is_supported, drop_path_scale,
@@ -92,7 +93,7 @@ class OmniWeaveBlock(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         """``x``: ``[B, H, W, C]`` -> ``[B, H, W, C]``."""
         if self.post_norm:
-            return forward_blocks([self], x)
+            return _forward_post_norm([self], x)
         self._check_backend(x)
         return block_forward(
             x, self.plan, self.norm_weight, self.a_u, self.a_v, self.a_o,
@@ -101,25 +102,43 @@ class OmniWeaveBlock(nn.Module):
         )
 
 
-def forward_blocks(blocks: Iterable[OmniWeaveBlock], x: Tensor) -> Tensor:
+def _plain_call(blk: nn.Module) -> bool:
+    """Whether calling ``blk`` is ``OmniWeaveBlock.forward`` and nothing else: no hook, wrapper or override sees the call."""
+    hooks = (blk._forward_hooks, blk._forward_pre_hooks, blk._backward_hooks, blk._backward_pre_hooks,
+             _module._global_forward_hooks, _module._global_forward_pre_hooks, _module._global_backward_hooks,
+             _module._global_backward_pre_hooks)
+    return (type(blk).forward is OmniWeaveBlock.forward and type(blk).__call__ is nn.Module.__call__
+            and "forward" not in vars(blk) and blk._compiled_call_impl is None and not any(hooks))
+
+
+def forward_blocks(blocks: Iterable[nn.Module], x: Tensor) -> Tensor:
     """Run blocks one after another, ``x`` ``[B, H, W, C]`` -> ``[B, H, W, C]``.
 
     Between two post-norm blocks the first one's norm, gate and residual add
     and the second one's pre-norm are one kernel.  The residual stream keeps
     x's type there; the operator runs in the compute type (autocast's, or x's).
+    Plain blocks, other modules (a wrapper around a block among them) and
+    blocks with hooks or a ``forward`` of their own are called as they are.
     """
-    todo = list(blocks)
-    n = None  # the pre-norm of x, where the block before has taken it
-    for i, blk in enumerate(todo):
-        if not blk.post_norm:
-            x, n = blk(x), None
+    run: list[OmniWeaveBlock] = []  # post-norm blocks to run together
+    for blk in blocks:
+        if isinstance(blk, OmniWeaveBlock) and blk.post_norm and _plain_call(blk):
+            run.append(blk)
             continue
+        x = blk(_forward_post_norm(run, x))
+        run = []
+    return _forward_post_norm(run, x)
+
+
+def _forward_post_norm(blocks: list[OmniWeaveBlock], x: Tensor) -> Tensor:
+    n = None  # the pre-norm of x, where the block before has taken it
+    for i, blk in enumerate(blocks):
         blk._check_backend(x)
         if n is None:
             n = rms_norm(x, blk.norm_weight)
         delta = bigemm_delta_cuda(x=n, plan=blk.plan, a_u=blk.a_u, a_v=blk.a_v, a_o=blk.a_o,
                                   b_u=blk.b_u, b_v=blk.b_v, b_o=blk.b_o, gamma=blk._unit)
-        nxt = todo[i + 1] if i + 1 < len(todo) and todo[i + 1].post_norm else None
+        nxt = blocks[i + 1] if i + 1 < len(blocks) else None
         out = norm_residual(x, delta, blk.post_norm_weight, blk.gamma,
                             sample_scale=drop_path_scale(x, blk.gamma, blk.drop_path_rate, blk.training),
                             next_weight=None if nxt is None else nxt.norm_weight)

@@ -447,3 +447,26 @@ def test_backward_stays_in_its_workspace(cuda_device, c, samples, tokens, t, off
     h = d["x"].double() + d["gate"].double()[:, None] * d["post"].double() * d["delta"].double()
     want, mag = (d["dn"].double() * h).sum((0, 1)), (d["dn"].double().abs() * h.abs()).sum((0, 1))
     assert ((dq.double() - want).abs() <= (64 + rows / 4 + 64) * U * mag + U * want.abs()).all()
+
+
+def test_forward_blocks_with_hooks(cuda_device):
+    """Hooked blocks see their own inputs and outputs, and the chain's result is that of the blocks called in turn."""
+    blocks = [_block(cuda_device, True, s) for s in range(3)]
+    x = torch.randn(2, 14, 14, 128, device=cuda_device, dtype=BF)
+    with torch.autocast("cuda", dtype=BF):
+        want = x
+        for b in blocks:
+            want = b(want)
+        seen = []
+        handles = [b.register_forward_hook(lambda m, a, o: seen.append((a[0], o))) for b in blocks]
+        got = forward_blocks(blocks, x)
+        assert torch.equal(got, want) and len(seen) == 3
+        assert seen[0][0] is x and seen[2][1] is got and all(torch.equal(seen[i][1], seen[i + 1][0]) for i in (0, 1))
+        handles.pop(1).remove()
+        handles.pop(0).remove()
+        seen.clear()
+        last = forward_blocks(blocks, x)  # the first two are fused, the third is called
+        assert len(seen) == 1 and torch.equal(blocks[2](forward_blocks(blocks[:2], x)), last)
+        handles.pop().remove()
+        blocks[1].register_forward_hook(lambda m, a, o: o * 0)
+        assert torch.equal(forward_blocks(blocks, x), blocks[2](torch.zeros_like(x)))

@@ -152,3 +152,44 @@ def test_backward_workspace_is_what_the_parts_take(samples, tokens, c, bf16, par
     t = 2 if bf16 else 0
     a = _args(samples=samples, tokens=tokens, channels=c, x_dtype=t, delta_dtype=t, n_dtype=t, gate_rows=samples)
     assert lib.ow_norm_bwd_workspace_size(ctypes.byref(a)) <= samples * parts * 2 * c * 4 + 256
+
+
+def test_forward_blocks_runs_hooks_and_other_modules():
+    """A block that is watched or wrapped is called, not taken apart; a hook in front of it runs before any CUDA call."""
+    from omniwave_b200.block import forward_blocks
+
+    class Wrapper(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            seen.append("wrapper")
+            return x + 1
+
+    seen = []
+    x = torch.zeros(1, 4, 4, 64)
+    for post in (False, True):
+        blk = OmniWeaveBlock(4, 4, 64, 64, "local", 0, post_norm=post)
+        blk.register_forward_pre_hook(lambda m, a: seen.append("pre"))
+        with pytest.raises(RuntimeError, match="CUDA is unavailable"):
+            forward_blocks([blk], x)
+    assert seen == ["pre", "pre"]
+    assert torch.equal(forward_blocks([Wrapper(blk), Wrapper(blk)], x), x + 2)
+    assert seen[2:] == ["wrapper", "wrapper"]
+
+    class Shifted(OmniWeaveBlock):
+        def forward(self, x):
+            return x + 3
+
+    assert torch.equal(forward_blocks([Shifted(4, 4, 64, 64, "local", 0, post_norm=True)], x), x + 3)
+    patched = OmniWeaveBlock(4, 4, 64, 64, "local", 0, post_norm=True)
+    patched.forward = lambda x: x + 5
+    assert torch.equal(forward_blocks([patched], x), x + 5)
+    handle = torch.nn.modules.module.register_module_forward_pre_hook(lambda m, a: seen.append("global"))
+    try:
+        with pytest.raises(RuntimeError, match="CUDA is unavailable"):
+            forward_blocks([OmniWeaveBlock(4, 4, 64, 64, "local", 0, post_norm=True)], x)
+    finally:
+        handle.remove()
+    assert seen[-1] == "global"
