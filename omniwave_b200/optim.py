@@ -16,7 +16,8 @@ element's place and the step, so a run repeats bit for bit.
 
 The state lives in flat buffers (``AdamW.buffers``); ``state[p]`` holds views of
 them in ``p``'s shape under the names ``torch.optim.AdamW`` uses, so its
-checkpoints load here (and, with 32 bits, this one's load there).
+checkpoints load here (and, with 32 bits, this one's load there), those of 16-bit
+parameters too, whose moments torch holds in the parameter's type.
 """
 
 from __future__ import annotations
@@ -234,7 +235,10 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------ checkpoints
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
-        """Copy a checkpoint's values into the state (its dtypes must be this optimizer's)."""
+        """Copy a checkpoint's values into the state, which must be held in as many bits.
+
+        A parameter that the checkpoint has no state for starts anew, as with torch's.
+        """
         groups, saved = self.param_groups, state_dict["param_groups"]
         if len(groups) != len(saved):
             raise ValueError("loaded state dict has a different number of parameter groups")
@@ -255,7 +259,10 @@ class AdamW(torch.optim.Optimizer):
                         moves.append((t, None))
                         continue
                     v = torch.as_tensor(v)
-                    if v.shape != t.shape or (k != "step" and v.dtype != t.dtype):
+                    # 32-bit moments take any of torch's (it holds a 16-bit parameter's in 16 bits); codes are codes
+                    wide = k in ("exp_avg", "exp_avg_sq") and t.dtype == torch.float32
+                    fits = k == "step" or v.dtype == t.dtype or (wide and v.dtype in (*_DTYPES, torch.float64))
+                    if v.shape != t.shape or not fits:
                         raise ValueError(f"loaded {k} is {v.dtype} {tuple(v.shape)}, expected {t.dtype} {tuple(t.shape)}")
                     moves.append((t, v))
         for t, v in moves:

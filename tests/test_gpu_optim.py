@@ -619,3 +619,29 @@ def test_a_step_counts_as_a_write_to_its_parameters(cuda_device, bits):
         assert any(moved) and idle._version == 0
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             out.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+def test_checkpoints_of_16_bit_parameters(cuda_device, dtype):
+    """torch holds their moments in their own type: they load here exactly, and this one's load there."""
+    ps, qs = _params(cuda_device, [1000, 33], dtype), _params(cuda_device, [1000, 33], dtype)
+    tor = torch.optim.AdamW(qs, lr=LR, weight_decay=WD)
+    tor.step()
+    opt = optim.AdamW(ps, lr=LR)
+    opt.load_state_dict(tor.state_dict())
+    for p, q in zip(ps, qs):
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert tor.state[q][k].dtype == dtype and opt.state[p][k].dtype == F32
+            assert torch.equal(opt.state[p][k], tor.state[q][k].float())
+        assert float(opt.state[p]["step"]) == 1
+    opt.step()
+    tor.load_state_dict(opt.state_dict())
+    for p, q in zip(ps, qs):
+        assert torch.equal(tor.state[q]["exp_avg"], opt.state[p]["exp_avg"].to(dtype)) and float(tor.state[q]["step"]) == 2
+    eight = optim.AdamW(ps, lr=LR, state_bits=8)
+    eight.step()
+    wrong = eight.state_dict()  # its inner dicts are the optimizer's own
+    wrong["state"] = {k: dict(v) for k, v in wrong["state"].items()}
+    wrong["state"][0]["exp_avg"] = wrong["state"][0]["exp_avg"].float()  # values, where codes belong
+    with pytest.raises(ValueError, match="exp_avg"):
+        eight.load_state_dict(wrong)
