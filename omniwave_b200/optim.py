@@ -238,12 +238,20 @@ class AdamW(torch.optim.Optimizer):
         """Copy a checkpoint's values into the state, which must be held in as many bits.
 
         A parameter that the checkpoint has no state for starts anew, as with torch's.
+        A checkpoint of another rule (``maximize``, ``amsgrad``, decay that is not
+        decoupled) raises ``ValueError``, and nothing is changed.
         """
         groups, saved = self.param_groups, state_dict["param_groups"]
         if len(groups) != len(saved):
             raise ValueError("loaded state dict has a different number of parameter groups")
         if any(len(g["params"]) != len(s["params"]) for g, s in zip(groups, saved)):
             raise ValueError("loaded state dict contains a parameter group that doesn't match the size of optimizer's group")
+        for s in saved:
+            for rule in ("maximize", "amsgrad"):
+                if s.get(rule):
+                    raise ValueError(f"loaded state is of an optimizer with {rule}, which this one does not do")
+            if not s.get("decoupled_weight_decay", True) and s.get("weight_decay"):
+                raise ValueError("loaded state is of an optimizer whose weight decay is not decoupled from the gradient")
         moves = []
         for g, s in zip(groups, saved):
             for p, key in zip(g["params"], s["params"]):

@@ -645,3 +645,27 @@ def test_checkpoints_of_16_bit_parameters(cuda_device, dtype):
     wrong["state"][0]["exp_avg"] = wrong["state"][0]["exp_avg"].float()  # values, where codes belong
     with pytest.raises(ValueError, match="exp_avg"):
         eight.load_state_dict(wrong)
+
+
+def test_checkpoints_of_other_rules_are_refused(cuda_device):
+    """What this optimizer does not do (maximize, amsgrad, coupled decay) is refused, before anything changes."""
+    def made(kind, **kw):
+        (q,) = _params(cuda_device, [500])
+        o = kind([q], lr=LR, weight_decay=WD, **kw)
+        o.step()
+        return o.state_dict()
+
+    (p,) = _params(cuda_device, [500])
+    opt = optim.AdamW([p], lr=0.5)
+    opt.step()
+    before = {k: t.clone() for k, t in opt.buffers[0].items()}
+    for sd, match in ((made(torch.optim.AdamW, maximize=True), "maximize"), (made(torch.optim.AdamW, amsgrad=True), "amsgrad"),
+                      (made(torch.optim.Adam), "decoupled")):
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(sd)
+        assert all(torch.equal(t, before[k]) for k, t in opt.buffers[0].items()) and opt.param_groups[0]["lr"] == 0.5
+    (q,) = _params(cuda_device, [500])
+    plain = torch.optim.Adam([q], lr=LR)  # without decay the rules are one
+    plain.step()
+    opt.load_state_dict(plain.state_dict())
+    assert opt.param_groups[0]["lr"] == LR and opt.param_groups[0]["weight_decay"] == 0
