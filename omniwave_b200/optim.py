@@ -22,6 +22,7 @@ parameters too, whose moments torch holds in the parameter's type.
 
 from __future__ import annotations
 
+import copy
 import ctypes
 from typing import Any
 
@@ -34,6 +35,9 @@ __all__ = ["AdamW", "adamw_supported"]
 
 BLOCK = _lib.ADAMW_BLOCK
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+# of a checkpoint's groups: what says which parameters they are and how they are held, and choices of torch's own code
+_NOT_LOADED = ("params", "param_names", "state_bits", "amsgrad", "maximize", "foreach", "capturable", "differentiable",
+               "fused", "decoupled_weight_decay")
 
 
 def _dense(p: Tensor) -> bool:
@@ -241,6 +245,10 @@ class AdamW(torch.optim.Optimizer):
         A checkpoint of another rule (``maximize``, ``amsgrad``, decay that is not
         decoupled) raises ``ValueError``, and nothing is changed.
         """
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups, saved = self.param_groups, state_dict["param_groups"]
         if len(groups) != len(saved):
             raise ValueError("loaded state dict has a different number of parameter groups")
@@ -278,14 +286,15 @@ class AdamW(torch.optim.Optimizer):
                 t, v = t.view(torch.uint8), None if v is None else v.view(torch.uint8)
             t.zero_() if v is None else t.copy_(v)
         for g, s in zip(groups, saved):
-            new = {k: s.get(k, g[k]) for k in ("lr", "betas", "eps", "weight_decay") if k in g}
+            new = {k: copy.deepcopy(v) for k, v in s.items() if k not in _NOT_LOADED}  # a scheduler's entries too
+            lr = new.pop("lr", g["lr"])
             if isinstance(g["lr"], Tensor) and g["params"]:
-                g["lr"].copy_(torch.as_tensor(new.pop("lr")))  # a captured step reads this tensor
-            elif isinstance(new["lr"], Tensor):
-                new["lr"] = float(new["lr"])
+                g["lr"].copy_(torch.as_tensor(lr))  # a captured step reads this tensor
+            else:
+                g["lr"] = float(lr) if isinstance(lr, Tensor) else lr
             g.update({k: tuple(v) if k == "betas" else v for k, v in new.items()})
-            if "initial_lr" in s:
-                g["initial_lr"] = s["initial_lr"]
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def __getstate__(self) -> dict[str, Any]:
         return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite}

@@ -669,3 +669,40 @@ def test_checkpoints_of_other_rules_are_refused(cuda_device):
     plain.step()
     opt.load_state_dict(plain.state_dict())
     assert opt.param_groups[0]["lr"] == LR and opt.param_groups[0]["weight_decay"] == 0
+
+
+def test_loading_keeps_a_schedule_and_runs_hooks(cuda_device):
+    """A scheduler's own entries of a group come with a checkpoint; registered load hooks run, as torch runs them."""
+    (p,), (q,) = _params(cuda_device, [300]), _params(cuda_device, [300])
+    tor = torch.optim.AdamW([q], lr=LR)
+    sched = torch.optim.lr_scheduler.OneCycleLR(tor, max_lr=0.3, total_steps=10)
+    for _ in range(3):
+        tor.step()
+        sched.step()
+    opt = optim.AdamW([p], lr=1.0)
+    calls = []
+
+    def pre(o, sd):
+        calls.append(("pre", o, float(o.state[p]["step"])))
+        sd["param_groups"][0]["eps"] = 0.25
+        return sd
+
+    handles = [opt.register_load_state_dict_pre_hook(pre),
+               opt.register_load_state_dict_post_hook(lambda o: calls.append(("post", o, float(o.state[p]["step"]))))]
+    sd = tor.state_dict()
+    opt.load_state_dict(sd)
+    assert calls == [("pre", opt, 0.0), ("post", opt, 3.0)]
+    g, t = opt.param_groups[0], tor.param_groups[0]
+    assert g["eps"] == 0.25 and g["state_bits"] == 32 and g["params"] == [p]
+    for k in ("lr", "betas", "initial_lr", "max_lr", "min_lr"):
+        assert g[k] == t[k], k
+    for h in handles:
+        h.remove()
+    here = torch.optim.lr_scheduler.OneCycleLR(opt, max_lr=0.3, total_steps=10)
+    here.load_state_dict(sched.state_dict())
+    opt.load_state_dict(tor.state_dict())
+    for _ in range(4):
+        for o, s in ((opt, here), (tor, sched)):
+            o.step()
+            s.step()
+        assert g["lr"] == t["lr"] and g["betas"] == t["betas"]
