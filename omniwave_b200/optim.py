@@ -197,10 +197,10 @@ class AdamW(torch.optim.Optimizer):
         for p in params:
             if p.numel():
                 by_dtype.setdefault(p.dtype, []).append(p)
-        for ps in by_dtype.values():
-            b = _Bucket(group, ps, group["state_bits"])
-            self._buckets.append(b)
-            for i, p in enumerate(ps):
+        made = [_Bucket(group, ps, group["state_bits"]) for ps in by_dtype.values()]  # all of them, or none
+        self._buckets += made
+        for b in made:
+            for i, p in enumerate(b.params):
                 self.state[p] = b.views(i)
         self._norm_buffers()
 

@@ -706,3 +706,29 @@ def test_loading_keeps_a_schedule_and_runs_hooks(cuda_device):
             o.step()
             s.step()
         assert g["lr"] == t["lr"] and g["betas"] == t["betas"]
+
+
+def test_a_group_that_cannot_be_added_leaves_nothing(cuda_device, monkeypatch):
+    """A failure half way (the memory of its second bucket, say) leaves no bucket that later steps would move."""
+    (kept,) = _params(cuda_device, [300])
+    opt = optim.AdamW([kept], lr=LR, max_norm=1.0)
+    more = _params(cuda_device, [500]) + _params(cuda_device, [500], BF)
+    before = [p.detach().clone() for p in more]
+    made, real = [], optim._Bucket
+
+    def failing(*args):
+        if made:
+            raise RuntimeError("no memory")
+        made.append(real(*args))
+        return made[0]
+
+    monkeypatch.setattr(optim, "_Bucket", failing)
+    with pytest.raises(RuntimeError, match="no memory"):
+        opt.add_param_group({"params": more})
+    monkeypatch.setattr(optim, "_Bucket", real)
+    assert len(opt.param_groups) == 1 and len(opt.buffers) == 1 and list(opt.state) == [kept]
+    opt.step()
+    assert all(torch.equal(p, b) for p, b in zip(more, before))
+    opt.add_param_group({"params": more})
+    opt.step()
+    assert len(opt.buffers) == 3 and not any(torch.equal(p, b) for p, b in zip(more, before))
