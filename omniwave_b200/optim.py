@@ -148,6 +148,7 @@ class AdamW(torch.optim.Optimizer):
         self.skip_nonfinite = bool(skip_nonfinite)
         self._buckets: list[_Bucket] = []
         self._partials: Tensor | None = None
+        self._replaced: list[Tensor | None] = []
         self.grad_norm: Tensor | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
@@ -207,7 +208,11 @@ class AdamW(torch.optim.Optimizer):
     def _norm_buffers(self) -> None:
         if self._buckets and (self.max_norm is not None or self.skip_nonfinite):
             dev = self._buckets[0].device
-            self._partials = torch.empty(sum(b.native.partials for b in self._buckets), dtype=torch.float64, device=dev)
+            need = sum(b.native.partials for b in self._buckets)
+            if self._partials is None or self._partials.numel() < need:
+                # a step that was captured before writes to the sums of its day for as long as it is replayed
+                self._replaced.append(self._partials)
+                self._partials = torch.empty(need, dtype=torch.float64, device=dev)
             if self.grad_norm is None:
                 self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
 
@@ -304,7 +309,7 @@ class AdamW(torch.optim.Optimizer):
         """Rebuild the flat buffers around the values of a copied or unpickled optimizer."""
         super().__setstate__(state)
         old, self.state = self.state, type(self.state)(dict)
-        self._buckets, self._partials, self.grad_norm = [], None, None
+        self._buckets, self._partials, self._replaced, self.grad_norm = [], None, [], None
         for g in self.param_groups:
             self._add_buckets(g)
         for p, mine in self.state.items():

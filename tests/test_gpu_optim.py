@@ -732,3 +732,24 @@ def test_a_group_that_cannot_be_added_leaves_nothing(cuda_device, monkeypatch):
     opt.add_param_group({"params": more})
     opt.step()
     assert len(opt.buffers) == 3 and not any(torch.equal(p, b) for p, b in zip(more, before))
+
+
+def test_a_captured_step_outlives_a_group_added_later(cuda_device):
+    """Its sums of squares stay its own: a replay writes to no memory that others have been given since."""
+    ps = _params(cuda_device, [5000, 300])
+    opt = optim.AdamW(ps, lr=LR, max_norm=0.5)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    at, size = opt._partials.data_ptr(), opt._partials.nbytes
+    opt.add_param_group({"params": _params(cuda_device, [700_000])})
+    assert opt._partials.data_ptr() != at and any(t is not None and t.data_ptr() == at for t in opt._replaced)
+    others = [torch.full((size,), 7, dtype=torch.uint8, device=cuda_device) for _ in range(200)]
+    want = _params(cuda_device, [5000, 300])
+    ref = optim.AdamW(want, lr=LR, max_norm=0.5)
+    ref.step(), ref.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all((t == 7).all() for t in others)
+    assert all(torch.equal(p, q) for p, q in zip(ps, want))
