@@ -784,9 +784,14 @@ constexpr int LONG_V = 8192, LONG_1 = 1024;  // channels a row may have in the r
 // Whether the rows are moved in aligned units of 8 channels: every array of
 // rows starts on 16 bytes (the channels' vectors are read one by one), and, for
 // ragged rows, it pays: it does for 16-bit arrays (100 channels: forward 75 us
-// against 100 element by element, with the backward 218 against 439), with f32
-// ones beside them from some 112 channels on (204: 117 against 129, 265 against
-// 409; 70: 183 against 98), and not for f32 alone (777: 90 against 74).
+// against 100 element by element, with the backward 218 against 439), and not for
+// f32 alone (777: 90 against 74).  With f32 arrays beside 16-bit ones the backward
+// gains and the forward loses; 112 channels is where training gains (20 M elements,
+// f32 stream, forward and with the backward, in units and by elements: 92 channels
+// 143, 314 and 75, 300; 108 123, 273 and 79, 310; 116 118, 258 and 76, 313; 150 162,
+// 355 and 152, 563; 204 116, 259 and 127, 482).  Between 122 and 128, whose units
+// take a split for 256 channels, elements would be better in both (124: 178, 398
+// and 73, 298).
 bool units(const Args& k, bool delta, bool next, const void* const* more, int n) {
   if ((uintptr_t)k.x % 16 || (uintptr_t)k.delta % 16) return false;
   for (int i = 0; i < n; ++i)

@@ -26,10 +26,12 @@
 // 1e-8 as a rule, leaves nothing to see).
 //
 // Bound: with 32-bit moments HBM: an f32 parameter costs 28 bytes (p, m, v read
-// and written, g read); 10.2 M take 46.5 us (6.2 TB/s), 40 M 177 us (6.3).  With 8
-// bits it costs 16 (a bf16 one 10), but 80 instructions, of which the hash and
-// the rounding are half, and these bound it: 10.2 M f32 parameters 38 us, 160 M
-// bf16 ones 502 us (3.2 TB/s).  The norm adds 13 us at 10.2 M.
+// and written, g read); 10.2 M take 51 us (5.6 TB/s; two sets of parameters in
+// turn, so nothing of one is left in L2), 40 M 182 us (6.1).  With 8 bits it costs
+// 16 (a bf16 one 10), but some 83 instructions, of which the hash and the rounding
+// are half, and these bound it: 10.2 M f32 parameters 39 us, 160 M bf16 ones 518 us
+// (3.1 TB/s); 3% of it is the root that is right for every v.  The norm adds 11 us
+// at 10.2 M.
 #include <math.h>
 
 #include <algorithm>
@@ -124,7 +126,10 @@ __device__ __forceinline__ float fast_div(float m, float d) {
 
 // Two 16-bit numbers from (slot, step), as the 20 bits below an e4m3 mantissa
 // see them: 16 random bits and half of the last one.  ``seed``: of the block's
-// first slot; the slots of a block differ in the low 8 bits only.
+// first slot; the slots of a block differ in the low 8 bits only.  The mixing steps
+// are a published 32-bit integer mixer's, found by search (C. Wellons, "Prospecting
+// for hash functions", 2018); the seed's multipliers are 2^32 over the golden ratio
+// (Knuth, TAOCP 6.4) and the two of A. Appleby's 32-bit finalizer (2011).
 __device__ __forceinline__ uint32_t random_seed(int64_t slot, uint32_t step) {
   return (uint32_t)slot * 0x9E3779B1u + (uint32_t)((uint64_t)slot >> 32) * 0x85EBCA6Bu + step * 0xC2B2AE35u;
 }
@@ -278,7 +283,7 @@ __device__ __forceinline__ void widen(const W& w, float (&o)[4]) {
   }
 }
 
-// 8-bit moments take some 80 instructions and 10 to 16 bytes an element, so a
+// 8-bit moments take some 83 instructions and 10 to 16 bytes an element, so a
 // warp asks for its next block before it works on this one, by copies that hold
 // no registers; with 32 bits and 28 bytes the loads of the warps at hand fill
 // the memory's pipe already.

@@ -9,7 +9,8 @@ autograd node in ``csrc/host/ow_host.cpp``).
 
 The products are taken in 16 bits with f32 accumulation (autocast bf16/f16, or
 a 16-bit model), as the rest of the cuda backend does; bias, activation and
-residual are applied in f32 and ``y`` is rounded once.
+residual are applied in f32 and ``y`` is rounded once.  gelu's own error is under a
+third of that rounding, for small results too.
 """
 
 from __future__ import annotations
