@@ -920,8 +920,12 @@ struct DzArgs {
   int N, vec;
 };
 
-// dz = dy act'(z), rounded to the 16-bit type (the GEMMs take it so), and its
-// f32 column sums for the bias.  A block does 256 columns of a chunk of rows.
+// dz = dy act'(z), rounded to the 16-bit type (the tensor core takes no other), and
+// its f32 column sums for the bias.  What that costs: a bf16 dW of 4096 x 512 x 256,
+// gelu, is off by 0.0024 of its norm, where its own rounding makes 0.0017 and
+// dz's as much again; z in 16 bits (half the traffic of f32 in both passes) is
+// not seen in it: 0.00234 with an exact z, 0.00240 so.
+// A block does 256 columns of a chunk of rows.
 // HBM and arithmetic bound it together: 25088 x 1024 bf16 gelu 30.7 us, silu 28.0
 // (5.5 TB/s), none (sums alone) 17; without the row ahead, and with the type
 // a value instead of a parameter, 34.8, 30.6 and 17.
