@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define OW_ABI_VERSION 6
+#define OW_ABI_VERSION 7
 
 #if defined(__GNUC__)
 #define OW_API __attribute__((visibility("default")))
@@ -508,6 +508,47 @@ OW_API int ow_norm_fwd(const ow_norm_t* args, void* stream);
 OW_API int ow_norm_bwd(const ow_norm_t* args, const ow_norm_grads_t* grads, void* stream);
 
 /*
+ * Layer norm over the channels of x [rows, channels]:
+ *
+ *   n = (x - mean(x)) rsqrt(mean((x - mean(x))^2) + eps) * weight + bias
+ *
+ * in f32, n rounded once.  bias may be NULL.  dtypes are f32, bf16 or f16,
+ * each array its own.  mean and rstd [rows] are written by the forward when
+ * not NULL (both or neither) and read by the backward, which takes dn (n's
+ * dtype) and writes, where not NULL, dx (x's dtype) and the gradients of
+ * weight and bias in their dtypes; these are added in f32 in a fixed order.
+ */
+typedef struct ow_layernorm_t {
+  int64_t rows;
+  int32_t channels;
+  const void* x;
+  int32_t x_dtype;
+  const void* weight;
+  int32_t weight_dtype;
+  const void* bias;            /* or NULL */
+  int32_t bias_dtype;
+  double eps;
+  void* n;                     /* forward only */
+  int32_t n_dtype;
+  float* mean;
+  float* rstd;
+  void* workspace;             /* backward only: ow_layernorm_bwd_workspace_size() bytes */
+  size_t workspace_bytes;
+} ow_layernorm_t;
+
+typedef struct ow_layernorm_grads_t {
+  const void* dn;
+  void* dx;
+  void* dweight;
+  void* dbias;                 /* of bias_dtype */
+} ow_layernorm_grads_t;
+
+/* Workspace bytes of ow_layernorm_bwd (0 if the arguments are invalid). */
+OW_API size_t ow_layernorm_bwd_workspace_size(const ow_layernorm_t* args);
+OW_API int ow_layernorm_fwd(const ow_layernorm_t* args, void* stream);
+OW_API int ow_layernorm_bwd(const ow_layernorm_t* args, const ow_layernorm_grads_t* grads, void* stream);
+
+/*
  * Linear layer with its epilogue, for the 16-bit compute types:
  *
  *   z = x W^T + bias;   out = act(z) + residual
@@ -560,6 +601,129 @@ typedef struct ow_linear_grads_t {
 OW_API size_t ow_linear_workspace_size(const ow_linear_t* args, const ow_linear_grads_t* grads);
 OW_API int ow_linear_fwd(const ow_linear_t* args, void* stream);
 OW_API int ow_linear_bwd(const ow_linear_t* args, const ow_linear_grads_t* grads, void* stream);
+
+/*
+ * Gated feed-forward block, for the 16-bit compute types:
+ *
+ *   g = x Wg^T + gate_bias;  u = x Wu^T + up_bias;  h = act(g) u
+ *   out = h Wd^T + down_bias + residual
+ *
+ * x [rows, in_features] with row stride ldx, gate_weight and up_weight [hidden,
+ * in_features] with row strides ldg and ldu, down_weight [out_features, hidden]
+ * with row stride ldd, residual [rows, out_features] with row stride ldr, all of
+ * ``dtype`` (bf16 or f16) with unit column stride; biases f32, bf16 or f16, or
+ * NULL; out [rows, out_features] contiguous.  Sums and activation are f32.  h
+ * [rows, ldh], ldh = hidden rounded up to 8, gets h rounded to ``dtype``; g and u
+ * (both NULL, or [rows, ldh]) g and u, for the backward.
+ *
+ * Backward, from dout: NULL outputs are not computed; dgate_weight and dup_weight
+ * come together, with one dtype.  h is needed for ddown_weight only, g, u and
+ * down_weight for all gradients but the projection back's.  dh, dg and du are
+ * rounded to ``dtype``, the biases' gradients are summed before that.  All sums
+ * are taken in a fixed order.
+ */
+typedef struct ow_ffn_t {
+  int64_t rows;
+  int32_t in_features, hidden, out_features;
+  int32_t dtype, activation;
+  const void* x;
+  int64_t ldx;
+  const void* gate_weight;
+  int64_t ldg;
+  const void* up_weight;
+  int64_t ldu;
+  const void* down_weight;
+  int64_t ldd;
+  const void* gate_bias;
+  int32_t gate_bias_dtype;
+  const void* up_bias;
+  int32_t up_bias_dtype;
+  const void* down_bias;
+  int32_t down_bias_dtype;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  void* h;
+  void* g;
+  void* u;
+  void* workspace;             /* ow_ffn_workspace_size() bytes */
+  size_t workspace_bytes;
+} ow_ffn_t;
+
+typedef struct ow_ffn_grads_t {
+  const void* dout;            /* [rows, out_features] contiguous */
+  void* dx;                    /* [rows, in_features] contiguous, or NULL, as the weights' and biases' */
+  void* dgate_weight;
+  int32_t dgate_dtype;         /* dtype, or f32 */
+  void* dup_weight;
+  int32_t dup_dtype;
+  void* ddown_weight;
+  int32_t ddown_dtype;
+  void* dgate_bias;            /* of their biases' dtypes */
+  void* dup_bias;
+  void* ddown_bias;
+} ow_ffn_grads_t;
+
+/* Workspace bytes of the forward (grads NULL) or of the backward; reads the
+ * shapes, dtypes, strides and pointers (their alignment).  0: invalid. */
+OW_API size_t ow_ffn_workspace_size(const ow_ffn_t* args, const ow_ffn_grads_t* grads);
+OW_API int ow_ffn_fwd(const ow_ffn_t* args, void* stream);
+OW_API int ow_ffn_bwd(const ow_ffn_t* args, const ow_ffn_grads_t* grads, void* stream);
+
+/*
+ * Loss of a classifier that learns from a teacher's top logits and from labels.
+ * logits [rows, classes] with row stride ld; a row has ``top`` entries of the
+ * teacher, top_logits t_j for top_classes c_j (both [rows, top]), and a label.
+ * With q_T = softmax(logits / T) and p = softmax(t / T) over the row's entries:
+ *
+ *   soft = T^2 sum_j p_j (log p_j - log q_T[c_j]);   hard = -log q_1[label]
+ *
+ * An entry whose class is negative is padding; a row without entries, or with
+ * none above -inf, has no soft, one with a negative label no hard.  A class or
+ * label that is not below ``classes`` makes its row NaN.  Entries may name a
+ * class more than once.  reduction NONE: loss [rows] = weight soft + (1 - weight)
+ * hard, a term that a row lacks being 0.  SUM: loss [1], the sum of these.  MEAN:
+ * weight times the mean of soft over the rows that have one, plus (1 - weight)
+ * times that of hard.  weight 0 leaves soft out, 1 hard.
+ *
+ * All in f32, sums over rows in f64, in a fixed order.  The forward leaves in
+ * stats [3 rows] and factors [2] (not with NONE) what the backward takes, which
+ * writes dlogits [rows, classes] of logits' dtype from dloss ([rows] with NONE,
+ * else [1]).
+ */
+#define OW_REDUCE_NONE 0
+#define OW_REDUCE_MEAN 1
+#define OW_REDUCE_SUM 2
+typedef struct ow_distill_t {
+  int64_t rows;
+  int32_t classes, top;        /* top at most 1024 */
+  const void* logits;
+  int32_t dtype;               /* f32, bf16 or f16 */
+  int64_t ld;
+  const void* top_logits;
+  int32_t top_dtype;           /* f32, bf16 or f16 */
+  const void* top_classes;
+  int32_t class_bytes;         /* 4 or 8: of a signed integer */
+  const void* labels;          /* [rows], or NULL */
+  int32_t label_bytes;
+  double temperature, weight;
+  int32_t reduction;
+  float* loss;                 /* forward only */
+  float* stats;
+  float* factors;
+  void* workspace;             /* forward only: ow_distill_workspace_size() bytes */
+  size_t workspace_bytes;
+} ow_distill_t;
+
+typedef struct ow_distill_grads_t {
+  const float* dloss;
+  void* dlogits;
+} ow_distill_grads_t;
+
+/* Workspace bytes of ow_distill_fwd (0 if the arguments are invalid). */
+OW_API size_t ow_distill_workspace_size(const ow_distill_t* args);
+OW_API int ow_distill_fwd(const ow_distill_t* args, void* stream);
+OW_API int ow_distill_bwd(const ow_distill_t* args, const ow_distill_grads_t* grads, void* stream);
 
 #ifdef __cplusplus
 }

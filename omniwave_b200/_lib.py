@@ -16,7 +16,7 @@ import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libomniwave_b200.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 DTYPE_CODE = {
     torch.float32: 0,
@@ -134,6 +134,19 @@ class NormGrads(ctypes.Structure):
     _fields_ = [(k, _vp) for k in ("dh", "dn", "dx", "ddelta", "dpost", "dgate", "dnext")]
 
 
+class LayerNorm(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("channels", _c_i32),
+        ("x", _vp), ("x_dtype", _c_i32), ("weight", _vp), ("weight_dtype", _c_i32), ("bias", _vp), ("bias_dtype", _c_i32),
+        ("eps", _c_f64), ("n", _vp), ("n_dtype", _c_i32), ("mean", _vp), ("rstd", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class LayerNormGrads(ctypes.Structure):
+    _fields_ = [("dn", _vp), ("dx", _vp), ("dweight", _vp), ("dbias", _vp)]
+
+
 class Linear(ctypes.Structure):
     _fields_ = [
         ("rows", ctypes.c_int64), ("in_features", _c_i32), ("out_features", _c_i32),
@@ -151,7 +164,44 @@ class LinearGrads(ctypes.Structure):
     ]
 
 
+class Ffn(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("in_features", _c_i32), ("hidden", _c_i32), ("out_features", _c_i32),
+        ("dtype", _c_i32), ("activation", _c_i32),
+        ("x", _vp), ("ldx", ctypes.c_int64), ("gate_weight", _vp), ("ldg", ctypes.c_int64),
+        ("up_weight", _vp), ("ldu", ctypes.c_int64), ("down_weight", _vp), ("ldd", ctypes.c_int64),
+        ("gate_bias", _vp), ("gate_bias_dtype", _c_i32), ("up_bias", _vp), ("up_bias_dtype", _c_i32),
+        ("down_bias", _vp), ("down_bias_dtype", _c_i32), ("residual", _vp), ("ldr", ctypes.c_int64),
+        ("out", _vp), ("h", _vp), ("g", _vp), ("u", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class FfnGrads(ctypes.Structure):
+    _fields_ = [
+        ("dout", _vp), ("dx", _vp), ("dgate_weight", _vp), ("dgate_dtype", _c_i32), ("dup_weight", _vp), ("dup_dtype", _c_i32),
+        ("ddown_weight", _vp), ("ddown_dtype", _c_i32), ("dgate_bias", _vp), ("dup_bias", _vp), ("ddown_bias", _vp),
+    ]
+
+
+class Distill(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("classes", _c_i32), ("top", _c_i32),
+        ("logits", _vp), ("dtype", _c_i32), ("ld", ctypes.c_int64),
+        ("top_logits", _vp), ("top_dtype", _c_i32), ("top_classes", _vp), ("class_bytes", _c_i32),
+        ("labels", _vp), ("label_bytes", _c_i32),
+        ("temperature", _c_f64), ("weight", _c_f64), ("reduction", _c_i32),
+        ("loss", _vp), ("stats", _vp), ("factors", _vp),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class DistillGrads(ctypes.Structure):
+    _fields_ = [("dloss", _vp), ("dlogits", _vp)]
+
+
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 ADAMW_BLOCK = 256
 ADAMW_CONTROL_BYTES = 64
 
@@ -168,7 +218,10 @@ EXPORTS = (
     "ow_d2s_linear_workspace_size", "ow_d2s_linear_fwd",
     "ow_grad_norm_partials", "ow_grad_norm", "ow_adamw_step",
     "ow_norm_bwd_workspace_size", "ow_norm_fwd", "ow_norm_bwd",
+    "ow_layernorm_bwd_workspace_size", "ow_layernorm_fwd", "ow_layernorm_bwd",
     "ow_linear_workspace_size", "ow_linear_fwd", "ow_linear_bwd",
+    "ow_ffn_workspace_size", "ow_ffn_fwd", "ow_ffn_bwd",
+    "ow_distill_workspace_size", "ow_distill_fwd", "ow_distill_bwd",
 )
 
 _lock = threading.Lock()
@@ -240,12 +293,30 @@ def load() -> ctypes.CDLL:
         lib.ow_norm_fwd.restype = ctypes.c_int
         lib.ow_norm_bwd.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(NormGrads), _vp]
         lib.ow_norm_bwd.restype = ctypes.c_int
+        lib.ow_layernorm_bwd_workspace_size.argtypes = [ctypes.POINTER(LayerNorm)]
+        lib.ow_layernorm_bwd_workspace_size.restype = ctypes.c_size_t
+        lib.ow_layernorm_fwd.argtypes = [ctypes.POINTER(LayerNorm), _vp]
+        lib.ow_layernorm_fwd.restype = ctypes.c_int
+        lib.ow_layernorm_bwd.argtypes = [ctypes.POINTER(LayerNorm), ctypes.POINTER(LayerNormGrads), _vp]
+        lib.ow_layernorm_bwd.restype = ctypes.c_int
         lib.ow_linear_workspace_size.argtypes = [ctypes.POINTER(Linear), ctypes.POINTER(LinearGrads)]
         lib.ow_linear_workspace_size.restype = ctypes.c_size_t
         lib.ow_linear_fwd.argtypes = [ctypes.POINTER(Linear), _vp]
         lib.ow_linear_fwd.restype = ctypes.c_int
         lib.ow_linear_bwd.argtypes = [ctypes.POINTER(Linear), ctypes.POINTER(LinearGrads), _vp]
         lib.ow_linear_bwd.restype = ctypes.c_int
+        lib.ow_ffn_workspace_size.argtypes = [ctypes.POINTER(Ffn), ctypes.POINTER(FfnGrads)]
+        lib.ow_ffn_workspace_size.restype = ctypes.c_size_t
+        lib.ow_ffn_fwd.argtypes = [ctypes.POINTER(Ffn), _vp]
+        lib.ow_ffn_fwd.restype = ctypes.c_int
+        lib.ow_ffn_bwd.argtypes = [ctypes.POINTER(Ffn), ctypes.POINTER(FfnGrads), _vp]
+        lib.ow_ffn_bwd.restype = ctypes.c_int
+        lib.ow_distill_workspace_size.argtypes = [ctypes.POINTER(Distill)]
+        lib.ow_distill_workspace_size.restype = ctypes.c_size_t
+        lib.ow_distill_fwd.argtypes = [ctypes.POINTER(Distill), _vp]
+        lib.ow_distill_fwd.restype = ctypes.c_int
+        lib.ow_distill_bwd.argtypes = [ctypes.POINTER(Distill), ctypes.POINTER(DistillGrads), _vp]
+        lib.ow_distill_bwd.restype = ctypes.c_int
         v = lib.ow_abi_version()
         if v != ABI_VERSION:
             raise NativeLibraryError(f"ABI version mismatch: library {v}, binding {ABI_VERSION}")

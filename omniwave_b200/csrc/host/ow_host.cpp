@@ -1,6 +1,7 @@
 // Host side of the operators around the block, as a Python module
 // (omniwave_b200._host): argument checks, autograd and the calls of the C ABI
-// for the norms and the linear layer, and AdamW's step over its buckets.
+// for the norms, the linear layer, the feed-forward block and the distillation
+// loss, and AdamW's step over its buckets.
 //
 // It is native because these operators are short: a few rows take the GPU 2 to
 // 5 us, and the same checks, allocations and autograd nodes took 25 us in
@@ -291,6 +292,98 @@ variable_list norm_residual(const Tensor& x, const Tensor& delta, const Tensor& 
   return norm_call(x, delta, weight, gate, scale, next, eps, norm_out(x, out_dtype));
 }
 
+// ------------------------------------------------------------------ layer norm
+ow_layernorm_t layernorm_args(const Tensor& x, const Tensor& w, const Tensor& b, double eps, at::ScalarType n_dtype,
+                              const Tensor& stats) {
+  ow_layernorm_t a{};
+  a.channels = (int32_t)x.size(-1);
+  a.rows = x.numel() / a.channels;
+  a.x = ptr(x);
+  a.x_dtype = code(x.scalar_type());
+  a.weight = ptr(w);
+  a.weight_dtype = code(w.scalar_type());
+  if (b.defined()) {
+    a.bias = ptr(b);
+    a.bias_dtype = code(b.scalar_type());
+  }
+  a.eps = eps;
+  a.n_dtype = code(n_dtype);
+  if (stats.defined()) {
+    a.mean = (float*)ptr(stats);
+    a.rstd = a.mean + a.rows;
+  }
+  return a;
+}
+
+// n, and the rows' means and inverse deviations [2, rows] when ``keep``.
+std::pair<Tensor, Tensor> layernorm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, at::ScalarType n_dtype,
+                                            bool keep) {
+  const Tensor n = at::empty(x.sizes(), x.options().dtype(n_dtype));
+  Tensor stats;
+  if (x.numel() == 0) return {n, stats};
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (keep) stats = at::empty({2, x.numel() / x.size(-1)}, x.options().dtype(at::kFloat));
+  ow_layernorm_t a = layernorm_args(x, w, b, eps, n_dtype, stats);
+  a.n = ptr(n);
+  check_status(ow_layernorm_fwd(&a, stream_of(x)), "ow_layernorm_fwd");
+  return {n, stats};
+}
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, double eps, int64_t n_dtype) {
+    auto [n, stats] = layernorm_forward(x, w, value(b), eps, (at::ScalarType)n_dtype, true);
+    ctx->save_for_backward({x, w, value(b), stats});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["n_dtype"] = n_dtype;
+    return n;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    once("layer_norm");
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], &b = s[2], &stats = s[3];
+    variable_list out(5);
+    if (!grads[0].defined()) return out;
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) dx = like(x);
+    if (ctx->needs_input_grad(1)) dw = like(w);
+    if (b.defined() && ctx->needs_input_grad(2)) db = like(b);
+    if (x.numel() == 0) {
+      for (Tensor* t : {&dw, &db})
+        if (t->defined()) t->zero_();
+    } else {
+      const Tensor dn = dense(grads[0]);
+      ow_layernorm_t a = layernorm_args(x, w, b, ctx->saved_data["eps"].toDouble(), (at::ScalarType)ctx->saved_data["n_dtype"].toInt(), stats);
+      const size_t size = ow_layernorm_bwd_workspace_size(&a);
+      const Tensor ws = at::empty({(int64_t)size}, x.options().dtype(at::kByte));
+      a.workspace = ptr(ws);
+      a.workspace_bytes = size;
+      const ow_layernorm_grads_t g{ptr(dn), ptr(dx), ptr(dw), ptr(db)};
+      check_status(ow_layernorm_bwd(&a, &g, stream_of(x)), "ow_layernorm_bwd");
+    }
+    out[0] = dx;
+    out[1] = dw;
+    out[2] = db;
+    return out;
+  }
+};
+
+Tensor layer_norm(const Tensor& x0, const Tensor& w0, const OptTensor& b_, double eps, std::optional<at::ScalarType> out_dtype) {
+  const Tensor b0 = value(b_);
+  OW_VALUE(x0.dim() >= 1 && x0.size(-1) > 0, "x must be [..., C], got ", shape_text(x0.sizes()));
+  OW_VALUE(x0.size(-1) < MOST, "x has too many channels: ", x0.size(-1));
+  OW_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
+  check_vector("weight", w0, x0.size(-1));
+  if (b0.defined()) check_vector("bias", b0, x0.size(-1));
+  no_tangents("layer_norm", {x0, w0, b0});
+  if (auto why = unsupported(x0, {w0, b0})) TORCH_CHECK(false, "layer_norm not supported: ", *why);
+  const at::ScalarType t = norm_out(x0, out_dtype);
+  const Tensor x = dense(x0), w = dense(w0), b = dense(b0);
+  if (wants_grad({x, w, b})) return LayerNormFn::apply(x, w, maybe(b), eps, (int64_t)t);
+  return layernorm_forward(x, w, b, eps, t, false).first;
+}
+
 // ------------------------------------------------------------------ linear
 // ``t`` as a matrix whose rows lie densely, copied only if they do not.
 Tensor as_rows(const Tensor& t0) {
@@ -444,6 +537,302 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, int64_t 
   return linear_forward(as_rows(cast(x, t)), as_rows(cast(w, t)), bias, as_rows(cast(res, t)), (int)act, false, shape).first;
 }
 
+// ------------------------------------------------------------------ gated feed-forward
+struct FfnCall {
+  Tensor x, wg, wu, wd, bg, bu, bd;  // matrices of the compute type, their rows dense
+  int act;
+
+  ow_ffn_t args() const {
+    ow_ffn_t a{};
+    a.rows = x.size(0);
+    a.in_features = (int32_t)x.size(1);
+    a.hidden = (int32_t)wg.size(0);
+    a.out_features = (int32_t)wd.size(0);
+    a.dtype = code(wg.scalar_type());
+    a.activation = act;
+    a.x = ptr(x);
+    a.ldx = ld(x);
+    a.gate_weight = ptr(wg);
+    a.ldg = ld(wg);
+    a.up_weight = ptr(wu);
+    a.ldu = ld(wu);
+    a.down_weight = ptr(wd);
+    a.ldd = ld(wd);
+    auto bias = [](const Tensor& b, const void** p, int32_t* dt) {
+      if (!b.defined()) return;
+      *p = ptr(b);
+      *dt = code(b.scalar_type());
+    };
+    bias(bg, &a.gate_bias, &a.gate_bias_dtype);
+    bias(bu, &a.up_bias, &a.up_bias_dtype);
+    bias(bd, &a.down_bias, &a.down_bias_dtype);
+    return a;
+  }
+
+  Tensor workspace(ow_ffn_t* a, const ow_ffn_grads_t* g) const {
+    const size_t size = ow_ffn_workspace_size(a, g);
+    TORCH_CHECK(size > 0, "ow_ffn_workspace_size failed: ", ow_last_error());
+    const Tensor ws = at::empty({(int64_t)size}, x.options().dtype(at::kByte));
+    a->workspace = ptr(ws);
+    a->workspace_bytes = size;
+    return ws;
+  }
+};
+
+struct FfnOut {
+  Tensor y, h, g, u;  // g and u for the backward
+};
+
+FfnOut ffn_forward(const FfnCall& k, const Tensor& res, bool keep, at::IntArrayRef shape) {
+  const c10::cuda::CUDAGuard guard(k.x.device());
+  const int64_t m = k.x.size(0), f = (k.wg.size(0) + 7) / 8 * 8;
+  FfnOut o;
+  o.y = at::empty(shape, k.x.options());
+  if (m == 0) return o;
+  o.h = at::empty({m, f}, k.x.options());
+  if (keep) {
+    o.g = at::empty({m, f}, k.x.options());
+    o.u = at::empty({m, f}, k.x.options());
+  }
+  ow_ffn_t a = k.args();
+  if (res.defined()) {
+    a.residual = ptr(res);
+    a.ldr = ld(res);
+  }
+  a.out = ptr(o.y);
+  a.h = ptr(o.h);
+  a.g = ptr(o.g);
+  a.u = ptr(o.u);
+  const Tensor ws = k.workspace(&a, nullptr);
+  check_status(ow_ffn_fwd(&a, stream_of(k.x)), "ow_ffn_fwd");
+  return o;
+}
+
+struct FfnFn : torch::autograd::Function<FfnFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                        const OptTensor& bg, const OptTensor& bu, const OptTensor& bd, const OptTensor& res_, int64_t act,
+                        int64_t compute) {
+    const auto t = (at::ScalarType)compute;
+    const Tensor res = value(res_);
+    const FfnCall k{as_rows(cast(x, t)), as_rows(cast(wg, t)), as_rows(cast(wu, t)), as_rows(cast(wd, t)), value(bg), value(bu), value(bd),
+                    (int)act};
+    auto needs = [](const Tensor& v) { return v.defined() && v.requires_grad(); };
+    // the projection back's own gradients take h alone
+    const bool keep = needs(x) || needs(wg) || needs(wu) || needs(k.bg) || needs(k.bu);
+    FfnOut o = ffn_forward(k, as_rows(cast(res, t)), keep, out_shape(x, wd.size(0)));
+    ctx->save_for_backward({k.x, k.wg, k.wu, k.wd, k.bg, k.bu, k.bd, o.h, o.g, o.u});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["x_shape"] = x.sizes().vec();
+    std::vector<int64_t> types;
+    for (const Tensor& v : {x, wg, wu, wd}) types.push_back((int64_t)v.scalar_type());
+    types.push_back(res.defined() ? (int64_t)res.scalar_type() : (int64_t)-1);
+    ctx->saved_data["types"] = types;
+    return o.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    once("gated_feed_forward");
+    const auto s = ctx->get_saved_variables();
+    const FfnCall k{s[0], s[1], s[2], s[3], s[4], s[5], s[6], (int)ctx->saved_data["act"].toInt()};
+    const std::vector<int64_t> types = ctx->saved_data["types"].toIntVector();
+    variable_list out(10);
+    const Tensor& dy = grads[0];
+    if (!dy.defined()) return out;
+    const c10::cuda::CUDAGuard guard(k.x.device());
+    // edges of the tensors that were given: those that were not have none
+    bool need[8];
+    for (int i = 0, edge = 0; i < 8; ++i) {
+      const bool given = i < 4 || (i < 7 ? s[i].defined() : types[4] >= 0);
+      need[i] = given && ctx->needs_input_grad(edge);
+      edge += given;
+    }
+    if (need[7]) out[7] = cast(dy, (at::ScalarType)types[4]);
+    if (!std::any_of(need, need + 7, [](bool b) { return b; })) return out;
+    const Tensor g = cast(dy, k.x.scalar_type()).reshape({-1, k.wd.size(0)}).contiguous();
+    auto type_of = [&](int i) { return types[i] == (int64_t)at::kFloat ? at::kFloat : k.x.scalar_type(); };
+    Tensor d[7];
+    if (need[0]) d[0] = at::empty({k.x.size(0), k.x.size(1)}, k.x.options());
+    if (need[1] || need[2]) {  // they come together, in f32 if either wants it
+      const auto t = type_of(1) == at::kFloat ? at::kFloat : type_of(2);
+      for (int i : {1, 2}) d[i] = at::empty(k.wg.sizes(), k.x.options().dtype(t));
+    }
+    if (need[3]) d[3] = at::empty(k.wd.sizes(), k.x.options().dtype(type_of(3)));
+    for (int i = 4; i < 7; ++i)
+      if (need[i]) d[i] = at::empty(s[i].sizes(), s[i].options());
+    if (k.x.size(0) == 0) {
+      for (Tensor& t : d)
+        if (t.defined()) t.zero_();
+    } else {
+      ow_ffn_t a = k.args();
+      a.h = ptr(s[7]);
+      a.g = ptr(s[8]);
+      a.u = ptr(s[9]);
+      auto dt = [](const Tensor& t) { return t.defined() ? code(t.scalar_type()) : 0; };
+      const ow_ffn_grads_t gr{ptr(g), ptr(d[0]), ptr(d[1]), dt(d[1]), ptr(d[2]), dt(d[2]), ptr(d[3]), dt(d[3]), ptr(d[4]), ptr(d[5]), ptr(d[6])};
+      const Tensor ws = k.workspace(&a, &gr);
+      check_status(ow_ffn_bwd(&a, &gr, stream_of(k.x)), "ow_ffn_bwd");
+    }
+    if (need[0]) out[0] = cast(d[0], (at::ScalarType)types[0]).view(ctx->saved_data["x_shape"].toIntVector());
+    for (int i = 1; i < 4; ++i)
+      if (need[i]) out[i] = cast(d[i], (at::ScalarType)types[i]);
+    for (int i = 4; i < 7; ++i) out[i] = d[i];
+    return out;
+  }
+};
+
+std::optional<std::string> ffn_unsupported(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const Tensor& bg,
+                                           const Tensor& bu, const Tensor& bd, const Tensor& res) {
+  if (!x.is_cuda()) return "CUDA is unavailable";
+  const at::ScalarType t = linear_compute(x);
+  if (!is16(t)) return "compute dtype " + dtype_text(t) + " is not 16-bit";
+  if (auto why = unsupported(x, {wg, wu, wd, bg, bu, bd, res})) return why;
+  if (!at::autocast::is_autocast_enabled(at::kCUDA))
+    for (const Tensor& v : {wg, wu, wd, res})
+      if (v.defined() && v.scalar_type() != t) return "weights and residual must be " + dtype_text(t) + " without autocast";
+  return std::nullopt;
+}
+
+Tensor gated_feed_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const OptTensor& bg_,
+                          const OptTensor& bu_, const OptTensor& bd_, int64_t act, const OptTensor& res_) {
+  const Tensor bg = dense(value(bg_)), bu = dense(value(bu_)), bd = dense(value(bd_)), res = value(res_);
+  OW_VALUE(wg.dim() == 2 && wg.numel() > 0, "gate_weight must be [F, K], got ", shape_text(wg.sizes()));
+  const int64_t f = wg.size(0), kk = wg.size(1);
+  OW_VALUE(wu.sizes() == wg.sizes(), "up_weight must be ", shape_text(wg.sizes()), ", got ", shape_text(wu.sizes()));
+  OW_VALUE(wd.dim() == 2 && wd.size(0) > 0 && wd.size(1) == f, "down_weight must be [N, ", f, "], got ", shape_text(wd.sizes()));
+  const int64_t n = wd.size(0);
+  OW_VALUE(n < MOST && kk < MOST && f < MOST / 2, "weights are too large: ", shape_text(wg.sizes()), ", ", shape_text(wd.sizes()));
+  OW_VALUE(x.dim() >= 1 && x.size(-1) == kk, "x must be [..., ", kk, "], got ", shape_text(x.sizes()));
+  if (bg.defined()) check_vector("gate_bias", bg, f);
+  if (bu.defined()) check_vector("up_bias", bu, f);
+  if (bd.defined()) check_vector("down_bias", bd, n);
+  const auto shape = out_shape(x, n);
+  if (res.defined())
+    OW_VALUE(res.sizes() == at::IntArrayRef(shape), "residual must be ", shape_text(shape), ", got ", shape_text(res.sizes()));
+  no_tangents("gated_feed_forward", {x, wg, wu, wd, bg, bu, bd, res});
+  if (auto why = ffn_unsupported(x, wg, wu, wd, bg, bu, bd, res)) TORCH_CHECK(false, "gated_feed_forward not supported: ", *why);
+  const at::ScalarType t = linear_compute(x);
+  if (wants_grad({x, wg, wu, wd, bg, bu, bd, res}))
+    return FfnFn::apply(x, wg, wu, wd, maybe(bg), maybe(bu), maybe(bd), maybe(res), act, (int64_t)t);
+  const FfnCall k{as_rows(cast(x, t)), as_rows(cast(wg, t)), as_rows(cast(wu, t)), as_rows(cast(wd, t)), bg, bu, bd, (int)act};
+  return ffn_forward(k, as_rows(cast(res, t)), false, shape).y;
+}
+
+// ------------------------------------------------------------------ distillation
+struct DistillCall {
+  Tensor logits, top, classes, labels;  // [N, V] (rows may lie apart), [N, K], [N, K], [N]
+  double temperature, weight;
+  int reduction;
+
+  ow_distill_t args(const Tensor& stats, const Tensor& factors) const {
+    ow_distill_t a{};
+    a.rows = logits.size(0);
+    a.classes = (int32_t)logits.size(1);
+    a.top = (int32_t)top.size(1);
+    a.logits = ptr(logits);
+    a.dtype = code(logits.scalar_type());
+    a.ld = ld(logits);
+    a.top_logits = ptr(top);
+    a.top_dtype = code(top.scalar_type());
+    a.top_classes = ptr(classes);
+    a.class_bytes = (int32_t)classes.element_size();
+    if (labels.defined()) {
+      a.labels = ptr(labels);
+      a.label_bytes = (int32_t)labels.element_size();
+    }
+    a.temperature = temperature;
+    a.weight = weight;
+    a.reduction = reduction;
+    a.stats = (float*)ptr(stats);
+    a.factors = (float*)ptr(factors);
+    return a;
+  }
+};
+
+// The loss, and what the backward takes: the rows' sums and the terms' factors.
+std::tuple<Tensor, Tensor, Tensor> distill_forward(const DistillCall& k, at::IntArrayRef shape) {
+  const auto f32 = k.logits.options().dtype(at::kFloat);
+  const int64_t rows = k.logits.size(0);
+  if (rows == 0) return {at::zeros(shape, f32), Tensor(), Tensor()};
+  const c10::cuda::CUDAGuard guard(k.logits.device());
+  const Tensor loss = at::empty(shape, f32), stats = at::empty({3, rows}, f32);
+  Tensor factors;
+  if (k.reduction != OW_REDUCE_NONE) factors = at::empty({2}, f32);
+  ow_distill_t a = k.args(stats, factors);
+  a.loss = (float*)ptr(loss);
+  const size_t size = ow_distill_workspace_size(&a);
+  const Tensor ws = at::empty({(int64_t)size}, f32.dtype(at::kByte));
+  a.workspace = ptr(ws);
+  a.workspace_bytes = size;
+  check_status(ow_distill_fwd(&a, stream_of(k.logits)), "ow_distill_fwd");
+  return {loss, stats, factors};
+}
+
+struct DistillFn : torch::autograd::Function<DistillFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& top, const Tensor& classes, const OptTensor& labels,
+                        double temperature, double weight, int64_t reduction, std::vector<int64_t> shape) {
+    const DistillCall k{as_rows(logits), top, classes, value(labels), temperature, weight, (int)reduction};
+    auto [loss, stats, factors] = distill_forward(k, shape);
+    ctx->save_for_backward({k.logits, top, classes, k.labels, stats, factors});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["weight"] = weight;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["shape"] = logits.sizes().vec();
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    once("distill_loss");
+    const auto s = ctx->get_saved_variables();
+    variable_list out(8);
+    if (!grads[0].defined() || !ctx->needs_input_grad(0)) return out;
+    const DistillCall k{s[0], s[1], s[2], s[3], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["weight"].toDouble(),
+                        (int)ctx->saved_data["reduction"].toInt()};
+    const c10::cuda::CUDAGuard guard(k.logits.device());
+    const Tensor dz = at::empty(ctx->saved_data["shape"].toIntVector(), k.logits.options());
+    if (dz.numel() > 0) {
+      const Tensor g = grads[0].to(at::kFloat).contiguous();
+      const ow_distill_t a = k.args(s[4], s[5]);
+      const ow_distill_grads_t d{(const float*)ptr(g), ptr(dz)};
+      check_status(ow_distill_bwd(&a, &d, stream_of(k.logits)), "ow_distill_bwd");
+    }
+    out[0] = dz;
+    return out;
+  }
+};
+
+Tensor distill_loss(const Tensor& logits, const Tensor& top0, const Tensor& classes0, const OptTensor& labels_, double temperature,
+                    double weight, int64_t reduction) {
+  const Tensor labels0 = value(labels_);
+  auto whole = [](const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; };
+  OW_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must be [..., V], got ", shape_text(logits.sizes()));
+  OW_VALUE(logits.size(-1) < MOST, "logits has too many classes: ", logits.size(-1));
+  OW_VALUE(top0.dim() == logits.dim() && top0.size(-1) > 0 && top0.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+           "top_logits must be ", shape_text(logits.sizes().slice(0, logits.dim() - 1)), " + (K,), got ", shape_text(top0.sizes()));
+  OW_VALUE(classes0.sizes() == top0.sizes(), "top_classes must be ", shape_text(top0.sizes()), ", got ", shape_text(classes0.sizes()));
+  OW_VALUE(whole(classes0), "top_classes must be int32 or int64, got ", dtype_text(classes0.scalar_type()));
+  if (labels0.defined()) {
+    OW_VALUE(labels0.sizes() == logits.sizes().slice(0, logits.dim() - 1), "labels must be ",
+             shape_text(logits.sizes().slice(0, logits.dim() - 1)), ", got ", shape_text(labels0.sizes()));
+    OW_VALUE(whole(labels0), "labels must be int32 or int64, got ", dtype_text(labels0.scalar_type()));
+  }
+  OW_VALUE(temperature >= 1e-4 && temperature <= 1e4, "temperature must be 1e-4 to 1e4, got ", temperature);
+  OW_VALUE(weight >= 0.0 && weight <= 1.0, "weight must be 0 to 1, got ", weight);
+  OW_VALUE(!top0.requires_grad() || !at::GradMode::is_enabled(), "top_logits takes no gradient");
+  no_tangents("distill_loss", {logits, top0});
+  if (auto why = unsupported(logits, {top0})) TORCH_CHECK(false, "distill_loss not supported: ", *why);
+  for (const Tensor& t : {classes0, labels0})
+    TORCH_CHECK(!t.defined() || t.device() == logits.device(), "distill_loss not supported: tensors on ", logits.device(), " and ", t.device());
+  const int64_t kk = top0.size(-1);
+  TORCH_CHECK(kk <= 1024, "distill_loss not supported: at most 1024 entries a row, got ", kk);
+  const Tensor top = dense(top0).view({-1, kk}), classes = dense(classes0).view({-1, kk});
+  const Tensor labels = labels0.defined() ? dense(labels0).view({-1}) : labels0;
+  std::vector<int64_t> shape;
+  if (reduction == OW_REDUCE_NONE) shape = logits.sizes().slice(0, logits.dim() - 1).vec();
+  if (wants_grad({logits}))
+    return DistillFn::apply(logits, top, classes, maybe(labels), temperature, weight, reduction, shape);
+  return std::get<0>(distill_forward(DistillCall{as_rows(logits), top, classes, labels, temperature, weight, (int)reduction}, shape));
+}
+
 // ------------------------------------------------------------------ AdamW
 // The parameters of one bucket as they were added, and the arguments of its
 // calls (an ow_adamw_t and the arrays it points to, which the optimizer owns).
@@ -567,7 +956,10 @@ PYBIND11_MODULE(_host, m) {
   auto nogil = py::call_guard<py::gil_scoped_release>();
   m.def("rms_norm", &rms_norm, nogil);
   m.def("norm_residual", &norm_residual, nogil);
+  m.def("layer_norm", &layer_norm, nogil);
   m.def("linear", &linear, nogil);
+  m.def("gated_feed_forward", &gated_feed_forward, nogil);
+  m.def("distill_loss", &distill_loss, nogil);
   m.def("norm_supported", [](const Tensor& x, const std::vector<OptTensor>& more) {
     for (const OptTensor& t : more)
       if (auto why = unsupported(x, {value(t)})) return told(why);
@@ -576,6 +968,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("linear_supported", [](const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r) {
     return told(linear_unsupported(x, w, value(b), value(r)));
   });
+  m.def("gated_feed_forward_supported",
+        [](const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const OptTensor& bg, const OptTensor& bu,
+           const OptTensor& bd, const OptTensor& r) { return told(ffn_unsupported(x, wg, wu, wd, value(bg), value(bu), value(bd), value(r))); });
   py::class_<Bucket>(m, "Bucket")
       .def(py::init<std::vector<Tensor>, uintptr_t, uintptr_t, uintptr_t>())
       .def_readonly("partials", &Bucket::partials);

@@ -1,0 +1,344 @@
+// The gated feed-forward block, forward and backward, on the tensor cores (sm_100a):
+//
+//   g = x Wg^T + bg;  u = x Wu^T + bu;  h = act(g) u;  y = h Wd^T + bd + r
+//   dh = dy Wd;  dg = dh u act'(g);  du = dh act(g)
+//   dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x;  dWd = dy^T h
+//
+// The products are the GEMM of the linear layer (ow_gemm.cuh) in three more forms:
+// g, u and h by one launch, whose tiles hold as many columns of g as of u, so that
+// the epilogue has both of an element at hand and x is read once; dx by one whose k
+// blocks are those of dg Wg and then those of du Wu, so that the sum never leaves
+// TMEM; dWg and dWu by one whose tiles are those of both.
+//
+// g, u, h, dg and du are held in 16 bits, as autocast would hold them: h, dg and du
+// because the tensor core takes no other, g and u for their traffic.
+#include "ow_gemm.cuh"
+
+namespace ow {
+namespace {
+
+struct GradArgs {
+  const void* dh;    // [M, N] contiguous
+  const void* g;     // [M, ld]
+  const void* u;     // [M, ld]
+  void* dg;          // [M, ld]
+  void* du;          // [M, ld]
+  float* part;       // [chunks][2][N] column sums of dg and of du, or NULL
+  int64_t M, ld, chunk;
+  int N, vec;
+};
+
+// dg and du, rounded to the 16-bit type, and their f32 column sums for the biases.
+// A block does 256 columns of a chunk of rows.
+template <int ACT, bool BF16>
+__global__ void __launch_bounds__(256) gate_grad_kernel(const GradArgs a) {
+  __shared__ float sh[8][264];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = blockIdx.x * 256 + tx * 8;
+  const int64_t m1 = min(a.M, (int64_t)(blockIdx.y + 1) * a.chunk);
+  float s[2][8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s[0][k] = s[1][k] = 0.f;
+  const bool whole = a.vec && n + 8 <= a.N;
+  for (int64_t m = blockIdx.y * a.chunk + ty; m < m1; m += 8) {
+    if (n >= a.N) continue;
+    float d[8], g[8], u[8];
+    if (whole) {
+      const uint4 dv = *reinterpret_cast<const uint4*>((const uint16_t*)a.dh + m * a.N + n);
+      const uint4 gv = *reinterpret_cast<const uint4*>((const uint16_t*)a.g + m * a.ld + n);
+      const uint4 uv = *reinterpret_cast<const uint4*>((const uint16_t*)a.u + m * a.ld + n);
+      const uint32_t dq[4] = {dv.x, dv.y, dv.z, dv.w}, gq[4] = {gv.x, gv.y, gv.z, gv.w}, uq[4] = {uv.x, uv.y, uv.z, uv.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2<BF16>(dq[k]), i = unpack2<BF16>(gq[k]), j = unpack2<BF16>(uq[k]);
+        d[2 * k] = f.x; d[2 * k + 1] = f.y;
+        g[2 * k] = i.x; g[2 * k + 1] = i.y;
+        u[2 * k] = j.x; u[2 * k + 1] = j.y;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool in = n + k < a.N;
+        d[k] = in ? ld16(a.dh, m * a.N + n + k, BF16) : 0.f;
+        g[k] = in ? ld16(a.g, m * a.ld + n + k, BF16) : 0.f;
+        u[k] = in ? ld16(a.u, m * a.ld + n + k, BF16) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      u[k] *= d[k] * act_slope<ACT>(g[k]);   // dg
+      d[k] *= act_fwd<ACT, BF16>(g[k]);      // du
+      s[0][k] += u[k];
+      s[1][k] += d[k];
+    }
+    // rows start on 16 bytes and have room for whole vectors
+    *reinterpret_cast<uint4*>((uint16_t*)a.dg + m * a.ld + n) =
+        make_uint4(pack2<BF16>(u[0], u[1]), pack2<BF16>(u[2], u[3]), pack2<BF16>(u[4], u[5]), pack2<BF16>(u[6], u[7]));
+    *reinterpret_cast<uint4*>((uint16_t*)a.du + m * a.ld + n) =
+        make_uint4(pack2<BF16>(d[0], d[1]), pack2<BF16>(d[2], d[3]), pack2<BF16>(d[4], d[5]), pack2<BF16>(d[6], d[7]));
+  }
+  if (!a.part) return;
+  for (int i = 0; i < 2; ++i) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sh[ty][tx * 8 + k] = i ? s[1][k] : s[0][k];
+    __syncthreads();
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < a.N) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t += sh[j][threadIdx.x];
+      a.part[((int64_t)i * gridDim.y + blockIdx.y) * a.N + c] = t;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+int check(const ow_ffn_t* a) {
+  OW_CHECK_ARG(a != nullptr, "ow_ffn: args is NULL");
+  OW_CHECK_ARG(a->rows >= 0 && a->in_features > 0 && a->hidden > 0 && a->out_features > 0, "ow_ffn: bad shape [%lld, %d] x [%d] x [%d]",
+               (long long)a->rows, a->in_features, a->hidden, a->out_features);
+  OW_CHECK_ARG(a->rows < (1LL << 31) - 256 && a->in_features < (1 << 30) && a->hidden < (1 << 29) && a->out_features < (1 << 30),
+               "ow_ffn: too large");
+  if (!is16(a->dtype)) {
+    set_error("ow_ffn: dtype must be bfloat16 or float16 (code %d)", a->dtype);
+    return OW_ERR_UNSUPPORTED;
+  }
+  OW_CHECK_ARG(a->activation >= OW_ACT_NONE && a->activation <= OW_ACT_GELU, "ow_ffn: unknown activation %d", a->activation);
+  OW_CHECK_ARG(a->ldx >= a->in_features && a->ldg >= a->in_features && a->ldu >= a->in_features && a->ldd >= a->hidden &&
+                   (!a->residual || a->ldr >= a->out_features),
+               "ow_ffn: a row stride is shorter than its row");
+  auto bias = [](const void* p, int dt) { return !p || is16(dt) || dt == OW_DTYPE_F32; };
+  OW_CHECK_ARG(bias(a->gate_bias, a->gate_bias_dtype) && bias(a->up_bias, a->up_bias_dtype) && bias(a->down_bias, a->down_bias_dtype),
+               "ow_ffn: a bias must be float32, bfloat16 or float16");
+  OW_CHECK_ARG(!a->g == !a->u, "ow_ffn: g and u are kept both or neither");
+  auto at = [](const void* p, int dt) { return !p || (uintptr_t)p % dtype_size(dt) == 0; };
+  OW_CHECK_ARG(((uintptr_t)a->x | (uintptr_t)a->gate_weight | (uintptr_t)a->up_weight | (uintptr_t)a->down_weight |
+                (uintptr_t)a->out | (uintptr_t)a->residual) % 2 == 0 &&
+                   ((uintptr_t)a->h | (uintptr_t)a->g | (uintptr_t)a->u) % 16 == 0 && at(a->gate_bias, a->gate_bias_dtype) &&
+                   at(a->up_bias, a->up_bias_dtype) && at(a->down_bias, a->down_bias_dtype),
+               "ow_ffn: a tensor is not aligned");
+  return OW_OK;
+}
+
+Mat mat_x(const ow_ffn_t* a) { return Mat{a->x, a->rows, a->in_features, a->ldx}; }
+Mat mat_g(const ow_ffn_t* a) { return Mat{a->gate_weight, a->hidden, a->in_features, a->ldg}; }
+Mat mat_u(const ow_ffn_t* a) { return Mat{a->up_weight, a->hidden, a->in_features, a->ldu}; }
+
+bool in_units(const ow_ffn_t* a) {
+  return a->in_features % 8 == 0 && tma_rows(a->x, a->ldx) && tma_rows(a->gate_weight, a->ldg) && tma_rows(a->up_weight, a->ldu);
+}
+// Whether the kernels for a few rows serve: as for the linear layer, of both weights.
+bool few_rows(const ow_ffn_t* a) {
+  if (!in_units(a)) return a->rows <= 4;
+  return a->rows <= 16 || (a->rows <= 32 && (int64_t)a->in_features * a->hidden <= (1 << 23));
+}
+
+// The projection back, as the linear layer has it.
+ow_linear_t down(const ow_ffn_t* a) {
+  ow_linear_t d{};
+  d.rows = a->rows;
+  d.in_features = a->hidden;
+  d.out_features = a->out_features;
+  d.dtype = a->dtype;
+  d.activation = OW_ACT_NONE;
+  d.x = a->h;
+  d.ldx = up8(a->hidden);
+  d.weight = a->down_weight;
+  d.ldw = a->ldd;
+  d.bias = a->down_bias;
+  d.bias_dtype = a->down_bias_dtype;
+  d.residual = a->residual;
+  d.ldr = a->ldr;
+  d.out = a->out;
+  return d;
+}
+
+Plan plan_gate(const ow_ffn_t* a) { return plan_gemm(a->rows, 2 * a->hidden, blocks_of(a->in_features)); }
+
+// Everything a backward call needs, carved from its workspace.
+struct BwdWs {
+  void *dh, *dg, *du;
+  float* bias;       // [2][chunks][hidden]
+  int chunks;
+  int64_t chunk;
+  Plan px, pw;
+  DualWs x, w;
+  void* down;        // the projection back's own workspace
+  size_t down_bytes;
+};
+
+bool wants_gate(const ow_ffn_grads_t* g) { return g->dx || g->dgate_weight || g->dup_weight || g->dgate_bias || g->dup_bias; }
+
+BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
+  BwdWs b{};
+  const int64_t M = a->rows, ld = up8(a->hidden);
+  const int F = a->hidden, K = a->in_features;
+  if (wants_gate(g)) {
+    b.dh = ws.take((size_t)M * F * 2);
+    b.dg = ws.take((size_t)M * ld * 2);
+    b.du = ws.take((size_t)M * ld * 2);
+    // chunks of rows: a few blocks an SM, at least 8 rows each
+    const int64_t col_blocks = (F + 255) / 256;
+    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
+    b.chunk = (M + b.chunks - 1) / b.chunks;
+    b.chunks = (int)((M + b.chunk - 1) / b.chunk);
+    if (g->dgate_bias || g->dup_bias) b.bias = (float*)ws.take((size_t)b.chunks * 2 * F * 4);
+    const Mat dg{nullptr, M, F, ld};
+    if (g->dx) {
+      b.px = plan_gemm(M, K, 2 * blocks_of(F));
+      b.x = dual_take<CAT_K>(dg, mat_g(a), Second{dg, mat_u(a)}, M, K, b.px, ws);
+    }
+    if (g->dgate_weight || g->dup_weight) {
+      b.pw = plan_gemm(2 * F, K, blocks_of(M));
+      b.w = dual_take<CAT_M>(dg, mat_x(a), Second{dg}, F, K, b.pw, ws);
+    }
+  }
+  const ow_linear_t d = down(a);
+  const ow_linear_grads_t dgr{g->dout, b.dh, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
+  // sized as if dh were wanted where it is: its address is not known when only the size is asked for
+  ow_linear_grads_t sized = dgr;
+  if (wants_gate(g)) sized.dx = (void*)16;
+  b.down_bytes = ow_linear_workspace_size(&d, &sized);
+  b.down = ws.take(b.down_bytes);
+  return b;
+}
+
+}  // namespace
+}  // namespace ow
+
+using namespace ow;
+
+extern "C" {
+
+size_t ow_ffn_workspace_size(const ow_ffn_t* a, const ow_ffn_grads_t* g) {
+  clear_error();
+  if (check(a) != OW_OK) return 0;
+  Carver c(nullptr);
+  if (a->rows > 0) {
+    if (g) {
+      bwd_take(a, g, c);
+    } else {
+      if (!few_rows(a)) dual_take<GATE>(mat_x(a), mat_g(a), Second{Mat{}, mat_u(a)}, a->rows, a->hidden, plan_gate(a), c);
+      const ow_linear_t d = down(a);
+      c.take(ow_linear_workspace_size(&d, nullptr));
+    }
+  }
+  return c.used + 256;
+}
+
+int ow_ffn_fwd(const ow_ffn_t* a, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  if (a->rows == 0) return OW_OK;
+  OW_CHECK_ARG(a->x && a->gate_weight && a->up_weight && a->down_weight && a->h && a->out, "ow_ffn_fwd: a pointer is NULL");
+  const size_t need = ow_ffn_workspace_size(a, nullptr);
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("ow_ffn_fwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
+    return OW_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool bf = a->dtype == OW_DTYPE_BF16;
+  const int F = a->hidden, K = a->in_features;
+  Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
+  Epi e{};
+  e.bias = a->gate_bias; e.bias_dt = a->gate_bias_dtype; e.act = a->activation; e.bf16 = bf;
+  e.z = a->g; e.ldz = up8(F); e.vz = 1;
+  e.out = a->h; e.ldo = up8(F); e.vo = 1;
+  const Second s{Mat{}, mat_u(a), a->up_bias, a->up_bias_dtype, a->u};
+  if (few_rows(a)) {
+    const GateRowsArgs k{{a->x, a->ldx, a->gate_weight, a->ldg, (int)a->rows, F, K, e}, a->up_weight, a->ldu,
+                         Gate{a->up_bias, a->up_bias_dtype, a->u}};
+    OW_RETURN_IF(in_units(a) ? run_units<true>(k, st) : run_rows<true>(k, st));
+  } else {
+    const Plan p = plan_gate(a);
+    const DualWs w = dual_take<GATE>(mat_x(a), mat_g(a), s, a->rows, F, p, ws);
+    OW_RETURN_IF((gemm_dual<GATE, false, false>(mat_x(a), mat_g(a), s, a->rows, F, K, p, w, e, bf, st)));
+  }
+  ow_linear_t d = down(a);
+  d.workspace_bytes = ow_linear_workspace_size(&d, nullptr);
+  d.workspace = ws.take(d.workspace_bytes);
+  return ow_linear_fwd(&d, stream);
+}
+
+int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
+  clear_error();
+  OW_RETURN_IF(check(a));
+  OW_CHECK_ARG(g != nullptr, "ow_ffn_bwd: grads is NULL");
+  OW_CHECK_ARG(a->rows > 0, "ow_ffn_bwd: no rows");
+  auto out = [&](const void* p, int dt) { return !p || dt == a->dtype || dt == OW_DTYPE_F32; };
+  if (!out(g->dgate_weight, g->dgate_dtype) || !out(g->dup_weight, g->dup_dtype) || !out(g->ddown_weight, g->ddown_dtype)) {
+    set_error("ow_ffn_bwd: a weight's gradient must be of dtype or float32");
+    return OW_ERR_UNSUPPORTED;
+  }
+  auto bias = [](const void* p, int dt) { return !p || is16(dt) || dt == OW_DTYPE_F32; };
+  OW_CHECK_ARG(bias(g->dgate_bias, a->gate_bias_dtype) && bias(g->dup_bias, a->up_bias_dtype) && bias(g->ddown_bias, a->down_bias_dtype),
+               "ow_ffn_bwd: a bias dtype is not set");
+  const bool gate = wants_gate(g), weights = g->dgate_weight || g->dup_weight;
+  OW_CHECK_ARG(g->dout && (!gate || (a->down_weight && a->g && a->u)) && (!g->dx || (a->gate_weight && a->up_weight)) &&
+                   (!weights || a->x) && (!g->ddown_weight || a->h) && !g->dgate_weight == !g->dup_weight &&
+                   (!weights || g->dgate_dtype == g->dup_dtype),
+               "ow_ffn_bwd: a pointer is NULL, or the gradients of gate and up are not asked for alike");
+  auto at = [](const void* p, int dt) { return !p || (uintptr_t)p % dtype_size(dt) == 0; };
+  OW_CHECK_ARG(((uintptr_t)g->dout | (uintptr_t)g->dx) % 2 == 0 && at(g->dgate_weight, g->dgate_dtype) && at(g->dup_weight, g->dup_dtype) &&
+                   at(g->ddown_weight, g->ddown_dtype) && at(g->dgate_bias, a->gate_bias_dtype) && at(g->dup_bias, a->up_bias_dtype) &&
+                   at(g->ddown_bias, a->down_bias_dtype),
+               "ow_ffn_bwd: a gradient is not aligned");
+  const size_t need = ow_ffn_workspace_size(a, g);
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("ow_ffn_bwd needs %zu workspace bytes, got %zu", need, a->workspace_bytes);
+    return OW_ERR_WORKSPACE;
+  }
+  const cudaStream_t st = (cudaStream_t)stream;
+  const bool bf = a->dtype == OW_DTYPE_BF16;
+  const int F = a->hidden, K = a->in_features;
+  const int64_t M = a->rows, ld = up8(F);
+  Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
+  const BwdWs b = bwd_take(a, g, ws);
+  if (gate || g->ddown_weight || g->ddown_bias) {
+    ow_linear_t d = down(a);
+    d.workspace = b.down;
+    d.workspace_bytes = b.down_bytes;
+    const ow_linear_grads_t dgr{g->dout, b.dh, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
+    OW_RETURN_IF(ow_linear_bwd(&d, &dgr, stream));
+  }
+  if (!gate) return OW_OK;
+  const GradArgs k{b.dh, a->g, a->u, b.dg, b.du, b.bias, M, ld, b.chunk, F, F % 8 == 0};
+  const dim3 grid((F + 255) / 256, b.chunks);
+  auto go = [&](auto act) {
+    if (bf) launch(gate_grad_kernel<decltype(act)::value, true>, grid, 256, 0, st, k);
+    else launch(gate_grad_kernel<decltype(act)::value, false>, grid, 256, 0, st, k);
+  };
+  switch (a->activation) {
+    case OW_ACT_NONE: go(std::integral_constant<int, OW_ACT_NONE>()); break;
+    case OW_ACT_RELU: go(std::integral_constant<int, OW_ACT_RELU>()); break;
+    case OW_ACT_SILU: go(std::integral_constant<int, OW_ACT_SILU>()); break;
+    default: go(std::integral_constant<int, OW_ACT_GELU>());
+  }
+  OW_CHECK_LAUNCH("gate_grad_kernel");
+  for (int i = 0; i < 2; ++i) {
+    void* db = i ? g->dup_bias : g->dgate_bias;
+    if (!db) continue;
+    launch(dbias_kernel, (F + 31) / 32, 1024, 0, st, (const float*)b.bias + (size_t)i * b.chunks * F, b.chunks, F, db,
+           i ? a->up_bias_dtype : a->gate_bias_dtype);
+    OW_CHECK_LAUNCH("dbias_kernel");
+  }
+  const Mat dg{b.dg, M, F, ld}, du{b.du, M, F, ld};
+  if (g->dx) {
+    Epi e{};
+    e.bf16 = bf;
+    e.out = g->dx; e.ldo = K; e.vo = tma_rows(g->dx, K);
+    OW_RETURN_IF((gemm_dual<CAT_K, false, true>(dg, mat_g(a), Second{du, mat_u(a)}, M, K, F, b.px, b.x, e, bf, st)));
+  }
+  if (weights) {
+    Epi e{};
+    e.bf16 = bf;
+    e.out = g->dgate_weight; e.ldo = K;
+    e.out32 = g->dgate_dtype == OW_DTYPE_F32;
+    e.vo = ((uintptr_t)g->dgate_weight | (uintptr_t)g->dup_weight) % 16 == 0 && K % (e.out32 ? 4 : 8) == 0;
+    OW_RETURN_IF((gemm_dual<CAT_M, true, true>(dg, mat_x(a), Second{du, Mat{}, nullptr, 0, g->dup_weight}, F, K, M, b.pw, b.w, e, bf, st)));
+  }
+  return OW_OK;
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""RMSNorm before and after a block, with the block's gate, residual scale and residual add.
+"""Norms: RMSNorm before and after a block, with the block's gate, residual scale and residual add; layer norm.
 
 The reference's block normalises its input only: ``x + s * gamma * f(rms(x) w)``
 (omniweave/models/block.py:80-108, fused by ``ops.block_forward``).  A block that
@@ -7,6 +7,9 @@ the next block starts with ``rms(h) * w_next``; ``norm_residual`` does both in o
 pass over ``x`` and ``delta``, and ``rms_norm`` is the norm in front of the first
 block.  Forward and backward are CUDA kernels (``ow_norm_fwd``, ``ow_norm_bwd``);
 argument checks and the autograd node are native too (``csrc/host/ow_host.cpp``).
+
+``layer_norm`` is the norm of blocks that subtract the mean and add a bias
+(``nn.LayerNorm``), with ``ow_layernorm_fwd`` and ``ow_layernorm_bwd``.
 
 All arithmetic is f32, whatever the tensors' types; each output is rounded once.
 """
@@ -19,11 +22,13 @@ from torch import Tensor
 from omniwave_b200 import _lib
 from omniwave_b200.ops import RMS_EPS
 
-__all__ = ["norm_residual", "norm_supported", "rms_norm"]
+__all__ = ["layer_norm", "norm_residual", "norm_supported", "rms_norm"]
+
+LN_EPS = 1e-5  # nn.LayerNorm's
 
 
 def norm_supported(x: Tensor, *others: Tensor | None) -> tuple[bool, str | None]:
-    """``(is_supported, reason_if_not)`` for tensors of ``rms_norm`` and ``norm_residual``."""
+    """``(is_supported, reason_if_not)`` for tensors of the norms."""
     return _lib.host().norm_supported(x, list(others))
 
 
@@ -53,3 +58,14 @@ def norm_residual(x: Tensor, delta: Tensor, weight: Tensor, gate: Tensor | None 
     """
     out = _lib.host().norm_residual(x, delta, weight, gate, sample_scale, next_weight, eps, out_dtype)
     return out[0] if next_weight is None else tuple(out)
+
+
+def layer_norm(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, eps: float = LN_EPS,
+               out_dtype: torch.dtype | None = None) -> Tensor:
+    """``(x - mean(x)) * rsqrt(var(x) + eps) * weight + bias`` over the last dimension.
+
+    ``x`` is ``[..., C]`` in float32, bfloat16 or float16, ``weight`` and ``bias``
+    ``[C]``, each of any of these types; ``var`` is the mean squared distance from
+    the mean.  Result type, errors and derivatives as for ``rms_norm``.
+    """
+    return _lib.host().layer_norm(x, weight, bias, eps, out_dtype)

@@ -32,6 +32,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from omniwave_b200.loss import distill_loss
 from omniwave_b200.optim import AdamW
 
 __all__ = ["DistInfo", "EMA", "init_distributed", "broadcast_parameters", "shard_range", "TrainStep"]
@@ -140,6 +141,10 @@ class TrainStep:
     and clipping in one pass over the gradients, the update in another, the
     moments in ``state_bits`` bits (32, or 8).
 
+    A step that is given a teacher's top logits takes ``loss.distill_loss`` (CUDA
+    only) in the place of the cross-entropy, with ``distill_weight`` and
+    ``distill_temperature``.
+
     ``cuda_graph=True`` (single process only) captures the whole step --
     forward, backward, finite check, optimizer and EMA -- into one CUDA
     graph after ``graph_warmup`` eager steps; later steps copy the batch
@@ -161,11 +166,18 @@ class TrainStep:
         graph_warmup: int = 3,
         optimizer: str = "torch",
         state_bits: int = 32,
+        distill_weight: float = 0.5,
+        distill_temperature: float = 1.0,
     ) -> None:
         if optimizer not in ("torch", "fused"):
             raise ValueError(f"optimizer must be 'torch' or 'fused', got {optimizer!r}")
         if state_bits != 32 and optimizer != "fused":
             raise ValueError("state_bits other than 32 needs optimizer='fused'")
+        if not 0.0 <= distill_weight <= 1.0:
+            raise ValueError(f"distill_weight must be 0 to 1, got {distill_weight!r}")
+        if not 1e-4 <= distill_temperature <= 1e4:
+            raise ValueError(f"distill_temperature must be 1e-4 to 1e4, got {distill_temperature!r}")
+        self.distill_weight, self.distill_temperature = distill_weight, distill_temperature
         self.device = next(model.parameters()).device
         distributed = dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
         if distributed and broadcast:
@@ -205,15 +217,21 @@ class TrainStep:
         self._graph = None
         self._graph_warmup = graph_warmup if cuda_graph else -1
         self._nsteps = 0
-        self._static: tuple[Tensor, Tensor, Tensor] | None = None
+        self._static: tuple[tuple[Tensor, ...], Tensor] | None = None
 
-    def _body(self, images: Tensor, labels: Tensor) -> Tensor:
+    def _loss(self, images: Tensor, labels: Tensor, *teacher: Tensor) -> Tensor:
+        logits = self.model(images)
+        if not teacher:
+            return F.cross_entropy(logits, labels)
+        return distill_loss(logits, *teacher, labels, temperature=self.distill_temperature, weight=self.distill_weight)
+
+    def _body(self, *batch: Tensor) -> Tensor:
         self.model.train()
         if self.amp_dtype is not None:
             with torch.autocast(self.device.type, dtype=self.amp_dtype, cache_enabled=False):
-                loss = F.cross_entropy(self.model(images), labels)
+                loss = self._loss(*batch)
         else:
-            loss = F.cross_entropy(self.model(images), labels)
+            loss = self._loss(*batch)
         self.optimizer.zero_grad(set_to_none=True)
         loss.backward()
         loss = loss.detach()
@@ -250,32 +268,36 @@ class TrainStep:
                 for p, old in zip(self._params, snapshot):
                     p.copy_(torch.where(keep, old, p))
 
-    def step(self, images: Tensor, labels: Tensor) -> Tensor:
+    def step(self, images: Tensor, labels: Tensor, teacher: tuple[Tensor, Tensor] | None = None) -> Tensor:
         """Forward, backward (gradients all-reduced by DDP), optimizer step.
 
-        Returns the loss as a device tensor; nothing here waits for the GPU.
+        ``teacher`` is ``(top_logits, top_classes)`` of ``loss.distill_loss``.  Returns
+        the loss as a device tensor; nothing here waits for the GPU.
         """
+        batch = (images, labels, *(teacher or ()))
+        if self._static is not None and len(self._static[0]) != len(batch):
+            raise ValueError("the step was captured " + ("without" if teacher else "with") + " a teacher")
         self._nsteps += 1
         if self._graph_warmup < 0:
-            return self._body(images, labels)
+            return self._body(*batch)
         if self._graph is None and self._nsteps <= self._graph_warmup:
             # Warm-up runs eagerly on a side stream, as graph capture requires.
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(side):
-                loss = self._body(images, labels)
+                loss = self._body(*batch)
             torch.cuda.current_stream(self.device).wait_stream(side)
             return loss
         if self._graph is None:
-            si, sl = images.clone(), labels.clone()
+            held = tuple(t.clone() for t in batch)
             torch.cuda.synchronize(self.device)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                sloss = self._body(si, sl)
-            self._graph, self._static = g, (si, sl, sloss)
-        si, sl, sloss = self._static
-        si.copy_(images, non_blocking=True)
-        sl.copy_(labels, non_blocking=True)
+                sloss = self._body(*held)
+            self._graph, self._static = g, (held, sloss)
+        held, sloss = self._static
+        for to, t in zip(held, batch):
+            to.copy_(t, non_blocking=True)
         self._graph.replay()
         return sloss
 
