@@ -12,23 +12,31 @@
 //   s = sum 2^(z k - mk),   log q = (z k - mk - log2 s) / k
 // where z k - mk is one rounding and the rounding of mk drops out.
 //
-// G threads share a row: a block, or a warp where rows are short.  The forward
-// reads z once, with a running maximum; the backward reads it again and writes
-// dz, first as if there were neither teacher nor label, then the entries of
-// those classes anew: each of them takes everything that falls on its class, is
-// computed in f32 and rounded once, in an order that the row alone fixes.
+// The forward reads z once, with a running maximum that is looked at once for
+// four vectors; the backward reads it again and writes dz, first as if there were
+// neither teacher nor label, then the entries of those classes anew: each of them
+// takes everything that falls on its class, is computed in f32 and rounded once,
+// in an order that the row alone fixes.
+//
+// What bounds it is HBM, if the exponentials do not: the special-function units do
+// 16 a cycle and SM, two for each logit of 16 bits are half as much again as the
+// memory takes.  So with T = 2 or 4 the second is the first one's power (POW; k / T
+// is exact then), and one serves where T = 1 or a term is left out.
+//
+// A row is a warp's, or a block's, of which the last warp has the teacher's entries
+// while the others have the logits: its loads depend on one another.
 #include <algorithm>
 #include <type_traits>
 
 #include "ow_common.cuh"
 #include "ow_internal.h"
+#include "ow_sm100.cuh"
 
 namespace ow {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int THREADS = 256;
-constexpr int MOST_TOP = 1024;
+constexpr int MOST_TOP = 1024;  // a lane's entries are 32 at most
 
 struct Args {
   int64_t rows, ld;
@@ -54,6 +62,7 @@ struct Args {
   int dloss_rows;        // a gradient for each row
   const float* coef;     // factors of soft and hard, or NULL: weight and 1 - weight
   void* dz;
+  int slots;             // of a row's table of classes: a power of two, at least 2 K
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -80,45 +89,88 @@ __device__ __forceinline__ int64_t ld_index(const void* p, int wide, int64_t i) 
   return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
 }
 
-// Calls f(first element, its index, whether V elements follow) for a row's elements in 16-byte units where it can.
-template <int G, typename T, class F>
-__device__ __forceinline__ void over_row(const T* z, int V, int lane, F&& f) {
-  constexpr int U = 16 / sizeof(T);
-  const int lead = min(V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
-  const int units = (V - lead) / U;
-  for (int i = lane; i < lead; i += G) f(i, std::integral_constant<int, 1>());
-  for (int i = lane; i < units; i += G) f(lead + i * U, std::integral_constant<int, U>());
-  for (int i = lead + units * U + lane; i < V; i += G) f(i, std::integral_constant<int, 1>());
-}
-template <int N, typename T>
-__device__ __forceinline__ void ldn(const T* p, float (&o)[N]) {
-  if constexpr (N == 1) {
-    o[0] = widen(p[0]);
+// ---------------------------------------------------------------- a row's logits
+using f2 = uint64_t;  // two floats
+__device__ __forceinline__ f2 both(float v) { return sm100::f2pack(v, v); }
+
+template <typename T>
+constexpr int PER = 16 / sizeof(T);  // elements of a 16-byte vector
+
+// A vector's elements as pairs of floats.
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& r, f2 (&o)[PER<T> / 2]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if constexpr (sizeof(T) == 4) {
+    o[0] = (f2)w[0] | (f2)w[1] << 32;
+    o[1] = (f2)w[2] | (f2)w[3] << 32;
   } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-    T v[N];
-    *reinterpret_cast<uint4*>(v) = r;
 #pragma unroll
-    for (int k = 0; k < N; ++k) o[k] = widen(v[k]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = sm100::unpack2<std::is_same_v<T, __nv_bfloat16>>(w[i]);
+      o[i] = sm100::f2pack(f.x, f.y);
+    }
   }
 }
-template <int N, typename T>
-__device__ __forceinline__ void stn(T* p, const float (&o)[N]) {
-  if constexpr (N == 1) {
-    p[0] = narrow<T>(o[0]);
+template <typename T>
+__device__ __forceinline__ uint4 narrow(const f2 (&v)[PER<T> / 2]) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+    w[0] = (uint32_t)v[0]; w[1] = (uint32_t)(v[0] >> 32);
+    w[2] = (uint32_t)v[1]; w[3] = (uint32_t)(v[1] >> 32);
   } else {
-    alignas(16) T v[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = narrow<T>(o[k]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = sm100::f2unpack(v[i]);
+      w[i] = sm100::pack2<std::is_same_v<T, __nv_bfloat16>>(f.x, f.y);
+    }
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The larger of two vectors, element by element.
+template <typename T>
+__device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      o[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&x[i]), *reinterpret_cast<const __half2*>(&y[i]));
+      o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]), *reinterpret_cast<const __nv_bfloat162*>(&y[i]));
+      o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 least() {  // a vector of -inf
+  constexpr uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same_v<T, __half> ? 0xFC00FC00u : 0xFF80FF80u;
+  return make_uint4(w, w, w, w);
+}
+__device__ __forceinline__ f2 ex2(f2 v) {
+  const float2 f = sm100::f2unpack(v);
+  return sm100::f2pack(ex2(f.x), ex2(f.y));
+}
+// e^(POW - 1) and e^POW of what POW says (0: not used, 1: one exponential serves for both).
+template <int POW>
+__device__ __forceinline__ f2 power1(f2 e) {
+  if constexpr (POW == 4) return sm100::mul2(sm100::mul2(e, e), e);
+  return e;
 }
 
-template <int G>
-__device__ __forceinline__ void row_sync() {
-  if constexpr (G == 32) __syncwarp();
-  else __syncthreads();
-}
+// How a row's elements lie in 16-byte units: up to ``lead`` singly, then whole units, then the rest singly.
+template <typename T>
+struct Lay {
+  int lead, units;
+  __device__ __forceinline__ Lay(const T* z, int V) {
+    lead = min(V, (int)((16 - ((uintptr_t)z & 15)) & 15) / (int)sizeof(T));
+    units = (V - lead) / PER<T>;
+  }
+  __device__ __forceinline__ int rest() const { return lead + units * PER<T>; }
+};
 
 // A maximum with the sums of 2^(x k - m k) around it: the running state of a softmax.
 struct Run {
@@ -137,105 +189,199 @@ __device__ __forceinline__ Run join(const Run& a, const Run& b, float kt) {
   return r;
 }
 
-template <int G, typename T>
-__global__ void __launch_bounds__(THREADS) distill_fwd_kernel(const Args a) {
-  constexpr int RB = THREADS / G;
-  __shared__ Run sh[THREADS / 32];
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.rows; r0 += (int64_t)gridDim.x * RB) {
-    const int64_t row = r0 + sub;
-    const bool live = row < a.rows;
-    const T* z = (const T*)a.z + row * a.ld;
-    const int64_t label = live && a.label ? ld_index(a.label, a.label8, row) : -1;
-    Run run{-INFINITY, 0.f, 0.f};
-    if (live)
-      over_row<G>(z, a.V, lane, [&](int i, auto n) {
-        constexpr int N = decltype(n)::value;
-        float v[N];
-        ldn<N>(z + i, v);
-        float m = run.m;
+// The softmax state of a thread's share of a row, every G-th unit from ``lane`` on.
+template <typename T, int G, int POW>
+__device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float kt) {
+  constexpr int N = 4, P = PER<T> / 2;  // vectors under way at once
+  const Lay<T> lay(z, V);
+  Run run{-INFINITY, 0.f, 0.f};
+  auto single = [&](int i) {
+    const float v = widen(z[i]), m = fmaxf(run.m, v), p = pivot(m);
+    run.st = run.st * moved(run.m, p, kt) + ex2(fmaf(v, kt, -p * kt));
+    run.s1 = run.s1 * moved(run.m, p, LOG2E) + ex2(fmaf(v, LOG2E, -p * LOG2E));
+    run.m = m;
+  };
+  for (int i = lane; i < lay.lead; i += G) single(i);
+  for (int i = lay.rest() + lane; i < V; i += G) single(i);
+  f2 st = sm100::f2pack(run.st, 0.f), s1 = sm100::f2pack(run.s1, 0.f);
+  const uint4* u = reinterpret_cast<const uint4*>(z + lay.lead);
+  const f2 k2 = both(kt), k1 = both(LOG2E);
+  for (int i = lane; i < lay.units; i += N * G) {
+    uint4 v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) m = fmaxf(m, v[k]);
-        const float p = pivot(m);
-        if (m > run.m) {
-          run.st *= moved(run.m, p, a.kt);
-          run.s1 *= moved(run.m, p, LOG2E);
-          run.m = m;
-        }
+    for (int n = 0; n < N; ++n) v[n] = i + n * G < lay.units ? __ldg(u + i + n * G) : least<T>();
+    f2 x[P];
+    widen<T>(larger<T>(larger<T>(v[0], v[1]), larger<T>(v[2], v[3])), x);
+    float m = run.m;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          run.st += ex2(fmaf(v[k], a.kt, -p * a.kt));
-          run.s1 += ex2(fmaf(v[k], LOG2E, -p * LOG2E));
-        }
-      });
+    for (int j = 0; j < P; ++j) {
+      const float2 f = sm100::f2unpack(x[j]);
+      m = fmaxf(m, fmaxf(f.x, f.y));
+    }
+    const float p = pivot(m);
+    if (m > run.m) {
+      st = sm100::mul2(st, both(moved(run.m, p, kt)));
+      if constexpr (POW != 1) s1 = sm100::mul2(s1, both(moved(run.m, p, LOG2E)));
+      run.m = m;
+    }
+    const f2 pt = both(-p * kt), p1 = both(-p * LOG2E);
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
-                          __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
-    if constexpr (G > 32) {
-      if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = run;
+    for (int n = 0; n < N; ++n) {
+      widen<T>(v[n], x);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const f2 e = ex2(sm100::fma2(x[j], k2, pt));
+        st = sm100::add2(st, e);
+        if constexpr (POW >= 2) s1 = sm100::fma2(power1<POW>(e), e, s1);
+        if constexpr (POW == 0) s1 = sm100::add2(s1, ex2(sm100::fma2(x[j], k1, p1)));
+      }
+    }
+  }
+  const float2 a = sm100::f2unpack(st), b = sm100::f2unpack(s1);
+  run.st = a.x + a.y;
+  run.s1 = POW == 1 ? run.st : b.x + b.y;
+  return run;
+}
+
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Threads of a block: eight warps with a row each, or a row's G and the warp of its entries.
+constexpr int block_of(int G) { return G == 32 ? 256 : G + 32; }
+constexpr int rows_of(int G) { return G == 32 ? 8 : 1; }
+
+// ---------------------------------------------------------------- forward
+// What a row's entries and label have to say without its logits' sums, by one warp:
+//   soft / (T^2 ln 2) = own + log2 of the sum of 2^(z kt)
+// in 64 bits, because large logits of the entries and the sum's take each other away.
+struct Said {
+  double own;
+  float top;             // +inf no entries, NaN not to be used
+  float label;           // the label's logit
+  int has_label;         // 1, 0, or -1: not a class
+};
+template <typename T>
+__device__ __forceinline__ Said listen(const Args& a, const T* z, int64_t row, int lane, float* sx, float* sz) {
+  Said s{0., INFINITY, 0.f, 0};
+  const int64_t at = row * a.K;
+  int64_t label = -1;
+  if (a.label && a.weight < 1.f) label = ld_index(a.label, a.label8, row);
+  float tm = -INFINITY;
+  bool bad = false;
+  if (a.weight > 0.f) {
+#pragma unroll 4
+    for (int j = lane; j < a.K; j += 32) {
+      const int64_t c = ld_index(a.cls, a.cls8, at + j);
+      const float t = ld_teacher(a, at + j);
+      const bool on = c >= 0, in = on && c < a.V;
+      bad |= on && (!in || t != t || t == INFINITY);
+      sx[j] = on ? t : -INFINITY;
+      sz[j] = in ? widen(z[c]) : 0.f;
+      if (on) tm = fmaxf(tm, t);
+    }
+  }
+  if (label >= 0) {
+    s.has_label = label < a.V ? 1 : -1;
+    if (label < a.V) s.label = widen(z[label]);
+  }
+  if (a.weight <= 0.f) return s;
+  __syncwarp();
+#pragma unroll
+  for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+  if (__any_sync(0xffffffffu, bad)) {
+    s.own = s.top = NAN;
+    return s;
+  }
+  if (tm == -INFINITY) return s;
+  const float tk = tm * a.kt;
+  float sd = 0.f;           // sum of e (x - tk)
+  double ts = 0., sq = 0.;  // of e, e z
+  for (int j = lane; j < a.K; j += 32) {
+    const float d = fmaf(sx[j], a.kt, -tk), e = ex2(d);
+    if (e > 0.f) {  // a probability of 0 has no part, whatever the student says
+      ts += e;
+      sd = fmaf(e, d, sd);
+      sq = fma((double)e, (double)sz[j], sq);
+    }
+  }
+  ts = warp_sum(ts);
+  sd = warp_sum(sd);
+  sq = warp_sum(sq);
+  const float log_s = log2f((float)ts);
+  s.own = (sd - sq * a.kt) / ts - log_s;
+  s.top = tk + log_s;
+  return s;
+}
+
+// Writes down a row's results.
+__device__ __forceinline__ void conclude(const Args& a, int64_t row, const Run& run, const Said& s) {
+  const float p = pivot(run.m), mt = p * a.kt, m1 = p * LOG2E;
+  const float log_t = log2f(run.st), log_1 = log2f(run.s1);
+  float soft = 0.f, hard = 0.f, lse_1 = INFINITY;
+  if (s.top != INFINITY) soft = LN2 * a.temp * a.temp * (float)(s.own + ((double)mt + log_t));
+  if (s.has_label > 0) {
+    hard = LN2 * (log_1 - fmaf(s.label, LOG2E, -m1));
+    lse_1 = m1 + log_1;
+  } else if (s.has_label < 0) {
+    hard = lse_1 = NAN;
+  }
+  a.lse_t[row] = mt + log_t;
+  a.lse_1[row] = lse_1;
+  a.top[row] = s.top;
+  if (a.soft) {
+    a.soft[row] = soft;
+    a.hard[row] = hard;
+  }
+  if (a.loss) a.loss[row] = a.weight * soft + (1.f - a.weight) * hard;
+}
+
+template <int G, typename T, int POW>
+__global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G)) distill_fwd_kernel(const Args a) {
+  extern __shared__ float dyn[];  // [rows][2][K]: the entries' logits, the student's there
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (G == 32) {
+    float* sx = dyn + warp * 2 * a.K;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.rows; row += (int64_t)gridDim.x * 8) {
+      const T* z = (const T*)a.z + row * a.ld;
+      Run run = softmax_share<T, 32, POW>(z, a.V, lane, a.kt);
+      const Said said = listen(a, z, row, lane, sx, sx + a.K);
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
+                            __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+      if (lane == 0) conclude(a, row, run, said);
+      __syncwarp();  // before the next row's entries overwrite these
+    }
+  } else {
+    constexpr int W = G / 32;
+    __shared__ Run sh[2][W];  // used in turn, so one barrier a row is enough
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+      const T* z = (const T*)a.z + row * a.ld;
+      Said said;
+      if (warp < W) {
+        Run run = softmax_share<T, G, POW>(z, a.V, threadIdx.x, a.kt);
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+          run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
+                              __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+        if (lane == 0) sh[turn][warp] = run;
+      } else {
+        said = listen(a, z, row, lane, dyn, dyn + a.K);
+      }
       __syncthreads();
-      run = sh[0];
+      if (warp == W) {
+        Run run = lane < W ? sh[turn][lane] : Run{-INFINITY, 0.f, 0.f};
 #pragma unroll
-      for (int i = 1; i < G / 32; ++i) run = join(run, sh[i], a.kt);
-      __syncthreads();
-    }
-    if (!live || lane >= 32) continue;
-    const float p = pivot(run.m), mt = p * a.kt, m1 = p * LOG2E;
-    const float log_t = log2f(run.st), log_1 = log2f(run.s1);
-    // The teacher's entries, by one warp.
-    float soft = 0.f, top = INFINITY;
-    if (a.weight > 0.f) {
-      const int64_t at = row * a.K;
-      float tm = -INFINITY, ts = 0.f;
-      bool bad = false;
-      for (int j = lane; j < a.K; j += 32) {
-        const int64_t c = ld_index(a.cls, a.cls8, at + j);
-        if (c < 0) continue;
-        bad |= c >= a.V;
-        const float t = ld_teacher(a, at + j);
-        bad |= t != t;
-        tm = fmaxf(tm, t);
+        for (int o = 16; o; o >>= 1)
+          run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
+                              __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+        if (lane == 0) conclude(a, row, run, said);
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-      bad = __any_sync(0xffffffffu, bad);
-      if (bad) {
-        soft = top = NAN;
-      } else if (tm > -INFINITY) {
-        const float tk = tm * a.kt;
-        for (int j = lane; j < a.K; j += 32)
-          if (ld_index(a.cls, a.cls8, at + j) >= 0) ts += ex2(fmaf(ld_teacher(a, at + j), a.kt, -tk));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) ts += __shfl_xor_sync(0xffffffffu, ts, o);
-        const float log_s = log2f(ts), inv = 1.f / ts;
-        for (int j = lane; j < a.K; j += 32) {
-          const int64_t c = ld_index(a.cls, a.cls8, at + j);
-          if (c < 0) continue;
-          const float d = fmaf(ld_teacher(a, at + j), a.kt, -tk), pj = ex2(d) * inv;
-          if (pj > 0.f) soft += pj * ((d - log_s) - (fmaf(widen(z[c]), a.kt, -mt) - log_t));
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) soft += __shfl_xor_sync(0xffffffffu, soft, o);
-        soft *= LN2 * a.temp * a.temp;
-        top = tk + log_s;
-        if (tm == INFINITY) soft = top = NAN;
-      }
-    }
-    float hard = 0.f, lse_1 = INFINITY;
-    if (label >= 0 && a.weight < 1.f) {
-      hard = label < a.V ? LN2 * (log_1 - fmaf(widen(z[label]), LOG2E, -m1)) : NAN;
-      lse_1 = label < a.V ? m1 + log_1 : NAN;
-    }
-    if (lane == 0) {
-      a.lse_t[row] = mt + log_t;
-      a.lse_1[row] = lse_1;
-      a.top[row] = top;
-      if (a.soft) {
-        a.soft[row] = soft;
-        a.hard[row] = hard;
-      }
-      if (a.loss) a.loss[row] = a.weight * soft + (1.f - a.weight) * hard;
     }
   }
 }
@@ -270,85 +416,169 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const Args a, int mea
   coef[1] = (float)ch;
 }
 
-template <int G, typename T>
-__global__ void __launch_bounds__(THREADS) distill_bwd_kernel(const Args a) {
-  constexpr int RB = THREADS / G;
-  extern __shared__ float dyn[];  // [RB][2][K]: the entries' classes and probabilities
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  int* sc = reinterpret_cast<int*>(dyn) + sub * 2 * a.K;
-  float* sp = dyn + sub * 2 * a.K + a.K;
-  for (int64_t r0 = (int64_t)blockIdx.x * RB; r0 < a.rows; r0 += (int64_t)gridDim.x * RB) {
-    const int64_t row = r0 + sub;
-    const bool live = row < a.rows;
-    const T* z = (const T*)a.z + row * a.ld;
-    T* dz = (T*)a.dz + row * a.V;
-    float lse_t = 0.f, lse_1 = 0.f, top = INFINITY, ks = 0.f, kh = 0.f;
-    int64_t label = -1;
-    if (live) {
-      lse_t = a.lse_t[row];
-      lse_1 = a.lse_1[row];
-      top = a.top[row];
-      const float g = a.dloss[a.dloss_rows ? row : 0];
-      if (top != INFINITY) ks = g * (a.coef ? a.coef[0] : a.weight) * a.temp;
-      if (lse_1 != INFINITY) {
-        kh = g * (a.coef ? a.coef[1] : 1.f - a.weight);
-        label = ld_index(a.label, a.label8, row);
-      }
-      if (top != top) ks = NAN;
-      const bool any = top != INFINITY || lse_1 != INFINITY;
-      const bool has_t = top != INFINITY, has_1 = lse_1 != INFINITY;
-      auto value = [&](float v) {
-        float d = 0.f;
-        if (has_t) d = ks * ex2(fmaf(v, a.kt, -lse_t));
-        if (has_1) d = fmaf(kh, ex2(fmaf(v, LOG2E, -lse_1)), d);
-        return d;
-      };
-      auto dense = [&](int i, auto n) {
-        constexpr int N = decltype(n)::value;
-        float v[N];
-        if (any) ldn<N>(z + i, v);
+// ---------------------------------------------------------------- backward
+// A row's gradient but for its entries and its label:
+//   ks 2^(z kt - lse_t) + kh 2^(z k - lse_1),   e (ks + c e^(POW - 1)) where POW says so
+template <int POW>
+struct Slope {
+  float kt, ks, kh, lse_t, lse_1, c;
+  bool none;  // a row that learns from nothing
+  __device__ __forceinline__ Slope(const Args& a, int64_t row, float top) : kt(a.kt), ks(0.f), kh(0.f), c(0.f) {
+    lse_t = a.lse_t[row];
+    lse_1 = a.lse_1[row];
+    const float g = a.dloss[a.dloss_rows ? row : 0];
+    if (top != INFINITY) ks = top == top ? g * (a.coef ? a.coef[0] : a.weight) * a.temp : NAN;
+    if (lse_1 != INFINITY) kh = lse_1 == lse_1 ? g * (a.coef ? a.coef[1] : 1.f - a.weight) : NAN;
+    none = top == INFINITY && lse_1 == INFINITY;
+    if constexpr (POW == 1) c = ks + kh;
+    if constexpr (POW >= 2) c = lse_1 == INFINITY ? 0.f : kh * ex2(fmaf((float)POW, lse_t, -lse_1));
+    if (lse_1 == INFINITY) lse_1 = 0.f;
+  }
+  __device__ __forceinline__ f2 operator()(f2 v) const {
+    const f2 e = ex2(sm100::fma2(v, both(kt), both(-lse_t)));
+    if constexpr (POW == 1) return sm100::mul2(e, both(c));
+    if constexpr (POW >= 2) return sm100::mul2(e, sm100::fma2(both(c), power1<POW>(e), both(ks)));
+    const f2 f = ex2(sm100::fma2(v, both(LOG2E), both(-lse_1)));
+    return sm100::fma2(e, both(ks), kh != 0.f ? sm100::mul2(f, both(kh)) : 0);
+  }
+  __device__ __forceinline__ float operator()(float v) const { return sm100::f2unpack((*this)(both(v))).x; }
+};
+
+// A thread's share of a row's gradient, every G-th unit from ``lane`` on.
+template <typename T, int G, int POW>
+__device__ __forceinline__ void slope_share(const T* z, T* dz, int V, int lane, const Slope<POW>& slope) {
+  constexpr int N = 4, P = PER<T> / 2;
+  const Lay<T> lay(dz, V);
+  auto single = [&](int i) { dz[i] = narrow<T>(slope.none ? 0.f : slope(widen(z[i]))); };
+  if (((uintptr_t)z ^ (uintptr_t)dz) & 15) {  // rows of z that start elsewhere in a unit
+    for (int i = lane; i < V; i += G) single(i);
+    return;
+  }
+  for (int i = lane; i < lay.lead; i += G) single(i);
+  for (int i = lay.rest() + lane; i < V; i += G) single(i);
+  const uint4* u = reinterpret_cast<const uint4*>(z + lay.lead);
+  uint4* o = reinterpret_cast<uint4*>(dz + lay.lead);
+  for (int i = lane; i < lay.units; i += N * G) {
+    uint4 v[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = any ? value(v[k]) : 0.f;
-        stn<N>(dz + i, v);
-      };
-      if (((uintptr_t)z & 15) == ((uintptr_t)dz & 15)) over_row<G>(z, a.V, lane, dense);
-      else
-        for (int i = lane; i < a.V; i += G) dense(i, std::integral_constant<int, 1>());
-      if (has_t)
-        for (int j = lane; j < a.K; j += G) {
-          const int64_t c = ld_index(a.cls, a.cls8, row * a.K + j);
-          sc[j] = c < 0 || c >= a.V ? -1 : (int)c;
-          sp[j] = sc[j] < 0 ? 0.f : ex2(fmaf(ld_teacher(a, row * a.K + j), a.kt, -top));
-        }
+    for (int n = 0; n < N; ++n) v[n] = !slope.none && i + n * G < lay.units ? __ldg(u + i + n * G) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      f2 x[P];
+      widen<T>(v[n], x);
+#pragma unroll
+      for (int j = 0; j < P; ++j) x[j] = slope.none ? 0 : slope(x[j]);
+      if (i + n * G < lay.units) o[i + n * G] = narrow<T>(x);
     }
-    row_sync<G>();
-    if (live) {
-      auto anew = [&](int c, float d) {  // class c with d to take off
-        const float v = widen(z[c]);
-        float u = lse_1 != INFINITY ? kh * ex2(fmaf(v, LOG2E, -lse_1)) : 0.f;
-        if (top != INFINITY) u = fmaf(ks, ex2(fmaf(v, a.kt, -lse_t)), u);
-        dz[c] = narrow<T>(u - d);
-      };
-      const int y = label >= 0 && label < a.V ? (int)label : -1;
-      bool met = false;  // the label is among the entries
-      if (top != INFINITY)
-        for (int j = lane; j < a.K; j += G) {
-          const int c = sc[j];
-          if (c < 0) continue;
-          bool first = true;
-          for (int i = 0; i < j; ++i) first &= sc[i] != c;
-          if (!first) continue;
-          float d = 0.f;
-          for (int i = j; i < a.K; ++i) d += sc[i] == c ? sp[i] : 0.f;
-          anew(c, ks * d + (c == y ? kh : 0.f));
-        }
-      if (y >= 0 && lane == 0) {
-        if (top != INFINITY)
-          for (int i = 0; i < a.K; ++i) met |= sc[i] == y;
-        if (!met) anew(y, kh);
+  }
+}
+
+// What is to be written at a row's entries and its label, by one warp.
+struct Amends {
+  uint32_t first;  // of this lane's entries (every 32nd): those whose value is to be written
+  int label;       // the label's class where no entry has it, or -1, and its value
+  float value;
+};
+// ``mem``: [K] classes, [K] probabilities, [K] values, [slots] of a table of classes.
+template <typename T, int POW>
+__device__ __forceinline__ Amends amends(const Args& a, const T* z, int64_t row, float top, int lane, const Slope<POW>& slope, float* mem) {
+  int* sc = reinterpret_cast<int*>(mem);
+  float *sp = mem + a.K, *sv = sp + a.K;
+  int* table = reinterpret_cast<int*>(sv + a.K);
+  Amends m{0u, -1, 0.f};
+  if (a.label && slope.kh != 0.f) {
+    const int64_t y = ld_index(a.label, a.label8, row);
+    if (y >= 0 && y < a.V) {
+      m.label = (int)y;
+      m.value = slope(widen(z[y])) - slope.kh;
+    }
+  }
+  if (top == INFINITY) return m;
+  for (int i = lane; i < a.slots; i += 32) table[i] = -1;
+#pragma unroll 4
+  for (int j = lane; j < a.K; j += 32) {
+    const int64_t c = ld_index(a.cls, a.cls8, row * a.K + j);
+    const float t = ld_teacher(a, row * a.K + j);
+    const bool in = c >= 0 && c < a.V;
+    const float p = in ? ex2(fmaf(t, a.kt, -top)) : 0.f;
+    sc[j] = p > 0.f ? (int)c : -1;  // what has no probability takes nothing off
+    sp[j] = p;
+    sv[j] = in ? slope(widen(z[c])) : 0.f;
+  }
+  __syncwarp();
+  // Whether a class is named twice: whichever entry comes to the table first, the answer is the same.
+  bool twice = false;
+  for (int j = lane; j < a.K; j += 32) {
+    const int c = sc[j];
+    if (c < 0) continue;
+    for (uint32_t h = (uint32_t)c * 2654435761u >> 16;; ++h) {
+      const int old = atomicCAS(table + (h & (a.slots - 1)), -1, c);
+      twice |= old == c;
+      if (old == -1 || old == c) break;
+    }
+  }
+  twice = __any_sync(0xffffffffu, twice);
+  bool met = false;  // the label is among the entries
+  for (int j = lane, k = 0; j < a.K; j += 32, ++k) {
+    const int c = sc[j];
+    if (c < 0) continue;
+    bool first = true;
+    float d = sp[j];
+    if (twice) {
+      for (int i = 0; i < j; ++i) first &= sc[i] != c;
+      for (int i = j + 1; i < a.K; ++i) d += sc[i] == c ? sp[i] : 0.f;
+    }
+    if (!first) continue;
+    met |= c == m.label;
+    sv[j] -= fmaf(slope.ks, d, c == m.label ? slope.kh : 0.f);
+    m.first |= 1u << k;
+  }
+  if (__any_sync(0xffffffffu, met)) m.label = -1;
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ void amend(const Args& a, T* dz, const Amends& m, int lane, const float* mem) {
+  const int* sc = reinterpret_cast<const int*>(mem);
+  const float* sv = mem + 2 * a.K;
+  if (m.first)
+    for (int j = lane, k = 0; j < a.K; j += 32, ++k)
+      if (m.first >> k & 1) dz[sc[j]] = narrow<T>(sv[j]);
+  if (lane == 0 && m.label >= 0) dz[m.label] = narrow<T>(m.value);
+}
+
+template <int G, typename T, int POW>
+__global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G)) distill_bwd_kernel(const Args a) {
+  extern __shared__ float dyn[];  // [rows][3 K + slots]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (G == 32) {
+    float* mem = dyn + warp * (3 * a.K + a.slots);
+    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.rows; row += (int64_t)gridDim.x * 8) {
+      const T* z = (const T*)a.z + row * a.ld;
+      T* dz = (T*)a.dz + row * a.V;
+      const float top = a.top[row];
+      const Slope<POW> slope(a, row, top);
+      const Amends m = amends<T>(a, z, row, top, lane, slope, mem);
+      slope_share<T, 32>(z, dz, a.V, lane, slope);
+      __syncwarp();
+      amend(a, dz, m, lane, mem);
+      __syncwarp();  // before the next row's entries overwrite these
+    }
+  } else {
+    constexpr int W = G / 32;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+      const T* z = (const T*)a.z + row * a.ld;
+      T* dz = (T*)a.dz + row * a.V;
+      const float top = a.top[row];
+      const Slope<POW> slope(a, row, top);
+      Amends m{};
+      if (warp < W) slope_share<T, G>(z, dz, a.V, threadIdx.x, slope);
+      else m = amends<T>(a, z, row, top, lane, slope, dyn);
+      __syncthreads();
+      if (warp == W) {
+        amend(a, dz, m, lane, dyn);
+        __syncwarp();
       }
     }
-    row_sync<G>();
   }
 }
 
@@ -391,28 +621,54 @@ Args base(const ow_distill_t* a) {
   k.kt = (float)(1.4426950408889634 / a->temperature);
   k.temp = (float)a->temperature;
   k.weight = (float)a->weight;
+  if (a->weight == 0.0) {  // T has no say
+    k.kt = LOG2E;
+    k.temp = 1.f;
+  }
   k.lse_t = a->stats;
   k.lse_1 = a->stats + a->rows;
   k.top = a->stats + 2 * a->rows;
   return k;
 }
 
-constexpr int WARP_ROW = 1024;  // rows of up to this many classes are a warp's
-
-int grid_of(int64_t rows, int rb) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rb - 1) / rb, (int64_t)device_sm_count() * 8));
-}
-
+// Calls f<G, T, POW>: the threads of a row, its type and what serves for the second exponential.
 template <class F>
 int with(const ow_distill_t* a, F&& f) {
-  auto type = [&](auto t) {
-    return a->classes <= WARP_ROW ? f(std::integral_constant<int, 32>(), t) : f(std::integral_constant<int, THREADS>(), t);
+  const bool hard = a->labels && a->weight < 1.0, soft = a->weight > 0.0;
+  const int pow = !hard || !soft || a->temperature == 1.0 ? 1 : a->temperature == 2.0 ? 2 : a->temperature == 4.0 ? 4 : 0;
+  auto power = [&](auto g, auto t) -> int {
+    switch (pow) {
+      case 1: return f(g, t, std::integral_constant<int, 1>());
+      case 2: return f(g, t, std::integral_constant<int, 2>());
+      case 4: return f(g, t, std::integral_constant<int, 4>());
+      default: return f(g, t, std::integral_constant<int, 0>());
+    }
+  };
+  auto type = [&](auto t) -> int {
+    if (a->classes <= 1024 && a->top <= 256) return power(std::integral_constant<int, 32>(), t);
+    return power(std::integral_constant<int, 224>(), t);
   };
   switch (a->dtype) {
     case OW_DTYPE_F32: return type(float());
     case OW_DTYPE_BF16: return type(__nv_bfloat16());
     default: return type(__half());
   }
+}
+
+template <class K>
+int launch_rows(K kern, const char* name, int G, size_t smem, const Args& k, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) {
+      set_error("ow_distill: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
+      return OW_ERR_CUDA;
+    }
+  }
+  const int rb = rows_of(G);
+  const int64_t grid = std::min<int64_t>((k.rows + rb - 1) / rb, (int64_t)device_sm_count() * 8);
+  launch(kern, (int)grid, block_of(G), smem, st, k);
+  OW_CHECK_LAUNCH(name);
+  return OW_OK;
 }
 
 }  // namespace
@@ -446,11 +702,10 @@ int ow_distill_fwd(const ow_distill_t* a, void* stream) {
     k.hard = k.soft + a->rows;
   }
   const cudaStream_t st = (cudaStream_t)stream;
-  with(a, [&](auto G, auto t) -> int {
-    launch(distill_fwd_kernel<G.value, decltype(t)>, grid_of(k.rows, THREADS / G.value), THREADS, 0, st, k);
-    return OW_OK;
-  });
-  OW_CHECK_LAUNCH("distill_fwd_kernel");
+  OW_RETURN_IF(with(a, [&](auto G, auto t, auto pow) -> int {
+    return launch_rows(distill_fwd_kernel<G.value, decltype(t), pow.value>, "distill_fwd_kernel", G.value,
+                       (size_t)rows_of(G.value) * 2 * k.K * sizeof(float), k, st);
+  }));
   if (a->reduction != OW_REDUCE_NONE) {
     launch(distill_sum_kernel, 1, 1024, 0, st, k, a->reduction == OW_REDUCE_MEAN, a->loss, a->factors);
     OW_CHECK_LAUNCH("distill_sum_kernel");
@@ -472,20 +727,11 @@ int ow_distill_bwd(const ow_distill_t* a, const ow_distill_grads_t* g, void* str
   k.coef = a->reduction == OW_REDUCE_NONE ? nullptr : a->factors;
   k.dz = g->dlogits;
   const cudaStream_t st = (cudaStream_t)stream;
-  return with(a, [&](auto G, auto t) -> int {
-    constexpr int RB = THREADS / G.value;
-    auto kern = distill_bwd_kernel<G.value, decltype(t)>;
-    const size_t smem = (size_t)RB * 2 * k.K * sizeof(float);  // at most 64 KB
-    if (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) {
-        set_error("ow_distill: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-        return OW_ERR_CUDA;
-      }
-    }
-    launch(kern, grid_of(k.rows, RB), THREADS, smem, st, k);
-    OW_CHECK_LAUNCH("distill_bwd_kernel");
-    return OW_OK;
+  k.slots = 2;
+  while (k.slots < 2 * k.K) k.slots *= 2;
+  return with(a, [&](auto G, auto t, auto pow) -> int {
+    return launch_rows(distill_bwd_kernel<G.value, decltype(t), pow.value>, "distill_bwd_kernel", G.value,
+                       (size_t)rows_of(G.value) * (3 * k.K + k.slots) * sizeof(float), k, st);
   });
 }
 
