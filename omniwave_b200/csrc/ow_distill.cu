@@ -206,10 +206,7 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
   f2 st = sm100::f2pack(run.st, 0.f), s1 = sm100::f2pack(run.s1, 0.f);
   const uint4* u = reinterpret_cast<const uint4*>(z + lay.lead);
   const f2 k2 = both(kt), k1 = both(LOG2E);
-  for (int i = lane; i < lay.units; i += N * G) {
-    uint4 v[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = i + n * G < lay.units ? __ldg(u + i + n * G) : least<T>();
+  auto step = [&](const uint4 (&v)[N]) {
     f2 x[P];
     widen<T>(larger<T>(larger<T>(v[0], v[1]), larger<T>(v[2], v[3])), x);
     float m = run.m;
@@ -236,6 +233,19 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
         if constexpr (POW == 0) s1 = sm100::add2(s1, ex2(sm100::fma2(x[j], k1, p1)));
       }
     }
+  };
+  int i = lane;
+  for (; i + (N - 1) * G < lay.units; i += N * G) {
+    uint4 v[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = __ldg(u + i + n * G);
+    step(v);
+  }
+  if (i < lay.units) {
+    uint4 v[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = i + n * G < lay.units ? __ldg(u + i + n * G) : least<T>();
+    step(v);
   }
   const float2 a = sm100::f2unpack(st), b = sm100::f2unpack(s1);
   run.st = a.x + a.y;

@@ -125,6 +125,9 @@ Mat mat_x(const ow_ffn_t* a) { return Mat{a->x, a->rows, a->in_features, a->ldx}
 Mat mat_g(const ow_ffn_t* a) { return Mat{a->gate_weight, a->hidden, a->in_features, a->ldg}; }
 Mat mat_u(const ow_ffn_t* a) { return Mat{a->up_weight, a->hidden, a->in_features, a->ldu}; }
 
+Mat mat_d(const ow_ffn_t* a) { return Mat{a->down_weight, a->out_features, a->hidden, a->ldd}; }
+Mat mat_dy(const ow_ffn_t* a, const ow_ffn_grads_t* g) { return Mat{g->dout, a->rows, a->out_features, a->out_features}; }
+
 bool in_units(const ow_ffn_t* a) {
   return a->in_features % 8 == 0 && tma_rows(a->x, a->ldx) && tma_rows(a->gate_weight, a->ldg) && tma_rows(a->up_weight, a->ldu);
 }
@@ -158,12 +161,13 @@ Plan plan_gate(const ow_ffn_t* a) { return plan_gemm(a->rows, 2 * a->hidden, blo
 
 // Everything a backward call needs, carved from its workspace.
 struct BwdWs {
-  void *dh, *dg, *du;
+  bool fused;        // dg and du come from dh's product itself
+  void *dh, *dg, *du;  // dh where they do not
   float* bias;       // [2][chunks][hidden]
   int chunks;
   int64_t chunk;
-  Plan px, pw;
-  DualWs x, w;
+  Plan ph, px, pw;
+  DualWs h, x, w;
   void* down;        // the projection back's own workspace
   size_t down_bytes;
 };
@@ -175,14 +179,22 @@ BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
   const int64_t M = a->rows, ld = up8(a->hidden);
   const int F = a->hidden, K = a->in_features;
   if (wants_gate(g)) {
-    b.dh = ws.take((size_t)M * F * 2);
+    // Where dh's product is split over k (few tiles), its sum is complete in another kernel only.
+    b.ph = plan_gemm(M, F, blocks_of(a->out_features));
+    b.fused = b.ph.splits == 1;
     b.dg = ws.take((size_t)M * ld * 2);
     b.du = ws.take((size_t)M * ld * 2);
-    // chunks of rows: a few blocks an SM, at least 8 rows each
-    const int64_t col_blocks = (F + 255) / 256;
-    b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
-    b.chunk = (M + b.chunks - 1) / b.chunks;
-    b.chunks = (int)((M + b.chunk - 1) / b.chunk);
+    if (b.fused) {
+      b.h = dual_take<GRAD>(mat_dy(a, g), mat_d(a), Second{}, M, F, b.ph, ws);
+      b.chunks = (int)((M + 31) / 32);
+    } else {
+      b.dh = ws.take((size_t)M * F * 2);
+      // chunks of rows: a few blocks an SM, at least 8 rows each
+      const int64_t col_blocks = (F + 255) / 256;
+      b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
+      b.chunk = (M + b.chunks - 1) / b.chunks;
+      b.chunks = (int)((M + b.chunk - 1) / b.chunk);
+    }
     if (g->dgate_bias || g->dup_bias) b.bias = (float*)ws.take((size_t)b.chunks * 2 * F * 4);
     const Mat dg{nullptr, M, F, ld};
     if (g->dx) {
@@ -195,10 +207,8 @@ BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
     }
   }
   const ow_linear_t d = down(a);
-  const ow_linear_grads_t dgr{g->dout, b.dh, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
-  // sized as if dh were wanted where it is: its address is not known when only the size is asked for
-  ow_linear_grads_t sized = dgr;
-  if (wants_gate(g)) sized.dx = (void*)16;
+  // sized with an address for dh where it is wanted: its own is not known when only the size is asked for
+  const ow_linear_grads_t sized{g->dout, wants_gate(g) && !b.fused ? (void*)16 : nullptr, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
   b.down_bytes = ow_linear_workspace_size(&d, &sized);
   b.down = ws.take(b.down_bytes);
   return b;
@@ -295,7 +305,7 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
   const int64_t M = a->rows, ld = up8(F);
   Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
   const BwdWs b = bwd_take(a, g, ws);
-  if (gate || g->ddown_weight || g->ddown_bias) {
+  if (b.dh || g->ddown_weight || g->ddown_bias) {
     ow_linear_t d = down(a);
     d.workspace = b.down;
     d.workspace_bytes = b.down_bytes;
@@ -303,19 +313,28 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
     OW_RETURN_IF(ow_linear_bwd(&d, &dgr, stream));
   }
   if (!gate) return OW_OK;
-  const GradArgs k{b.dh, a->g, a->u, b.dg, b.du, b.bias, M, ld, b.chunk, F, F % 8 == 0};
-  const dim3 grid((F + 255) / 256, b.chunks);
-  auto go = [&](auto act) {
-    if (bf) launch(gate_grad_kernel<decltype(act)::value, true>, grid, 256, 0, st, k);
-    else launch(gate_grad_kernel<decltype(act)::value, false>, grid, 256, 0, st, k);
-  };
-  switch (a->activation) {
-    case OW_ACT_NONE: go(std::integral_constant<int, OW_ACT_NONE>()); break;
-    case OW_ACT_RELU: go(std::integral_constant<int, OW_ACT_RELU>()); break;
-    case OW_ACT_SILU: go(std::integral_constant<int, OW_ACT_SILU>()); break;
-    default: go(std::integral_constant<int, OW_ACT_GELU>());
+  if (b.fused) {
+    Epi e{};
+    e.bf16 = bf; e.act = a->activation;
+    e.out = b.dg; e.ldo = ld; e.vo = 1;
+    Second s{};
+    s.c = b.du; s.g = a->g; s.u = a->u; s.part = b.bias;
+    OW_RETURN_IF((gemm_dual<GRAD, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)));
+  } else {
+    const GradArgs k{b.dh, a->g, a->u, b.dg, b.du, b.bias, M, ld, b.chunk, F, F % 8 == 0};
+    const dim3 grid((F + 255) / 256, b.chunks);
+    auto go = [&](auto act) {
+      if (bf) launch(gate_grad_kernel<decltype(act)::value, true>, grid, 256, 0, st, k);
+      else launch(gate_grad_kernel<decltype(act)::value, false>, grid, 256, 0, st, k);
+    };
+    switch (a->activation) {
+      case OW_ACT_NONE: go(std::integral_constant<int, OW_ACT_NONE>()); break;
+      case OW_ACT_RELU: go(std::integral_constant<int, OW_ACT_RELU>()); break;
+      case OW_ACT_SILU: go(std::integral_constant<int, OW_ACT_SILU>()); break;
+      default: go(std::integral_constant<int, OW_ACT_GELU>());
+    }
+    OW_CHECK_LAUNCH("gate_grad_kernel");
   }
-  OW_CHECK_LAUNCH("gate_grad_kernel");
   for (int i = 0; i < 2; ++i) {
     void* db = i ? g->dup_bias : g->dgate_bias;
     if (!db) continue;

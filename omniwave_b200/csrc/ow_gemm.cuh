@@ -28,20 +28,21 @@ constexpr int PATCH = 12;
 // products of the same A, a tile holding half as many columns of each, whose
 // epilogue joins them: act(A B1^T + b1) (A B2^T + b2).  CAT_K: the sum of two
 // products, the second's k blocks behind the first's.  CAT_M: two products with the
-// same B, the second's tiles behind the first's.
-enum Kind { PLAIN, GATE, CAT_K, CAT_M };
+// same B, the second's tiles behind the first's.  GRAD: one product d, whose epilogue
+// reads what GATE kept, g and u, and writes d u act'(g) and d act(g).
+enum Kind { PLAIN, GATE, CAT_K, CAT_M, GRAD };
 
 // BN columns of a tile; CG CTAs share it (2: 256 rows, BN / 2 rows of B each).
-template <int BN, int CG>
+template <int BN, int CG, int KIND = PLAIN>
 struct GC {
   static constexpr int B_ROWS = BN / CG;
-  static constexpr int CW = BN == 256 ? 64 : 32;   // columns of an epilogue warp
+  // GATE: a warp has 32 columns of either product
+  static constexpr int CW = KIND == GATE ? 64 : BN == 256 ? 64 : 32;   // columns of an epilogue warp
   static constexpr int NBLK = CW / 32;
   static constexpr int ACTIVE = 4 * (BN / CW);     // epilogue warps at work
-  static constexpr int GATE_ACTIVE = 4 * (BN / 64);  // the same with GATE: 32 columns of either product, two blocks of staging
-  static_assert(GATE_ACTIVE * 2 * BLOCK_ST <= ACTIVE * NBLK * BLOCK_ST, "GATE's staging");
-  static constexpr int STG_W = NBLK * BLOCK_ST;
-  static constexpr int STAGES = BN == 256 ? 5 : BN == 128 ? 6 : 8;
+  // blocks of staging a warp: GATE three (g, u and h leave together), GRAD two (what comes in and goes out in its place)
+  static constexpr int STG_W = (KIND == GATE ? 3 : KIND == GRAD ? 2 : NBLK) * BLOCK_ST;
+  static constexpr int STAGES = BN == 256 ? (KIND == GATE ? 4 : 5) : BN == 128 ? (KIND == GATE || KIND == GRAD ? 5 : 6) : 8;
   static constexpr int B_ST = B_ROWS * 128;
   static constexpr int OFF_B = STAGES * A_ST;
   static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
@@ -87,6 +88,7 @@ struct GemmArgs {
   // CAT_K: k blocks, CAT_M: rows of tiles of the first product
   int half;
   void* out2;        // CAT_M: the second product
+  float* part;       // GRAD: [2][blocks of 32 rows][N] column sums of both results, or NULL
 };
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
@@ -299,6 +301,63 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.f;
 }
 
+// gelu of two, the polynomial's steps in pairs; and as max(z, 0) - |z| tail, whose
+// terms take one operation less.  Beyond the clamp the tail is 0.
+template <bool BF16>
+__device__ __forceinline__ void gelu2(float& y, float& z) {
+  const float a = fminf(fabsf(y), BF16 ? 13.5f : 100.f), b = fminf(fabsf(z), BF16 ? 13.5f : 100.f);
+  const uint64_t x = f2pack(a, b);
+  auto c = [](float v) { return f2pack(v, v); };
+  uint64_t q;
+  if constexpr (BF16) {
+    q = fma2(x, c(3.98267339e-8f), c(-2.39384553e-6f));
+    q = fma2(q, x, c(6.14833989e-5f));
+    q = fma2(q, x, c(-8.9382549e-4f));
+    q = fma2(q, x, c(8.29635281e-3f));
+    q = fma2(q, x, c(-5.3509552e-2f));
+    q = fma2(q, x, c(-0.458847046f));
+    q = fma2(q, x, c(-1.15114152f));
+    q = fma2(q, x, c(-1.00000072f));
+  } else {
+    q = fma2(x, c(-1.39922733e-7f), c(1.43002126e-6f));
+    q = fma2(q, x, c(3.0813193e-5f));
+    q = fma2(q, x, c(-7.80530798e-4f));
+    q = fma2(q, x, c(8.10782891e-3f));
+    q = fma2(q, x, c(-5.33918403e-2f));
+    q = fma2(q, x, c(-0.458847821f));
+    q = fma2(q, x, c(-1.15115714f));
+    q = fma2(q, x, c(-0.999998868f));
+  }
+  const float2 f = f2unpack(q);
+  y = fmaf(-a, ex2(f.x), y < 0.f ? 0.f : y);
+  z = fmaf(-b, ex2(f.y), z < 0.f ? 0.f : z);
+}
+
+// An activation and its slope at z, which share what is costly: gelu's tail is
+// act_slope's, and the value max(z, 0) - |z| tail.
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float& a, float& s) {
+  if constexpr (ACT == OW_ACT_SILU) {
+    const float g = sigmoid(z);
+    a = z * g;
+    s = fmaf(a, 1.f - g, g);
+  } else if constexpr (ACT == OW_ACT_GELU) {
+    const float e = ex2(z * z * -0.72134752f);
+    const float t = rcp(fmaf(fabsf(z), 0.35f, 1.f));
+    float tail = fmaf(t, 0.0471570618f, -0.194429092f);
+    tail = fmaf(tail, t, 0.226878741f);
+    tail = fmaf(tail, t, -0.00380232154f);
+    tail = fmaf(tail, t, 0.148624128f);
+    tail = fmaf(tail, t, 0.135697883f);
+    tail = fmaf(tail, t, 0.139873699f) * t * e;
+    a = fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);
+    s = fmaf(z * 0.39894228040143268f, e, z > 0.f ? 1.f - tail : tail);
+  } else {
+    a = act_fwd<ACT, false>(z);
+    s = act_slope<ACT>(z);
+  }
+}
+
 // z as it is kept for the backward: a finite value stays finite in f16 (an
 // infinite one would make silu' and gelu' NaN).
 __device__ __forceinline__ float keep_z(float z, int bf16) {
@@ -331,17 +390,22 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int c0, int
                : "memory");
 }
 
-// The lanes' rows of 32 16-bit values, staged and sent to rows m0.. and
-// columns n0.. of an array.  The caller waits for the copy before it writes
-// the staging again.
-__device__ __forceinline__ void put16(unsigned char* stg, const float (&v)[32], int bf16, const CUtensorMap* map, bool boxes,
-                                      void* out, int64_t ld, int64_t m0, int64_t M, int n0, int N) {
+__device__ __forceinline__ void stage16(unsigned char* stg, const float (&v)[32], int bf16) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     *reinterpret_cast<uint4*>(stg + stg_at(lane, u)) =
         make_uint4(pk(v[8 * u], v[8 * u + 1], bf16), pk(v[8 * u + 2], v[8 * u + 3], bf16),
                    pk(v[8 * u + 4], v[8 * u + 5], bf16), pk(v[8 * u + 6], v[8 * u + 7], bf16));
+}
+
+// The lanes' rows of 32 16-bit values, staged and sent to rows m0.. and
+// columns n0.. of an array.  The caller waits for the copy before it writes
+// the staging again.
+__device__ __forceinline__ void put16(unsigned char* stg, const float (&v)[32], int bf16, const CUtensorMap* map, bool boxes,
+                                      void* out, int64_t ld, int64_t m0, int64_t M, int n0, int N) {
+  const int lane = threadIdx.x & 31;
+  stage16(stg, v, bf16);
   if (boxes) {
     fence_proxy_async_smem();
     __syncwarp();
@@ -466,10 +530,201 @@ struct Maps2 : Maps {  // of the second product; c2 is GATE's second z and CAT_M
 template <int KIND>
 using MapsOf = std::conditional_t<KIND == PLAIN, Maps, Maps2>;
 
+// The accumulator is read: the next but one tile may have it.
+template <int CG>
+__device__ __forceinline__ void give_back(uint64_t* tfree) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    if constexpr (CG == 1) mbar_arrive(tfree);
+    else arrive_in(in_cta(tfree, 0));
+  }
+}
+
+// GATE's epilogue: a warp has 32 rows and 32 columns of both products.  With g and u
+// kept, the three results are staged side by side and leave together (one after the
+// other, each waiting for the staging, 25088 x 512 -> 1024 gelu took 74.5 us).
+template <int BN, int CG, bool BF16, int ACT>
+__device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
+                                              uint32_t tbase, uint64_t* tfull, uint64_t* tfree, unsigned char* stg,
+                                              volatile int* abort) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, group = warp >> 2;
+  const Epi& e = a.e;
+  int tl = 0;
+  for (int u = first; u < units; ++tl) {
+    const int acc = tl & 1;
+    const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
+    const int n0 = t.nt * (BN / 2) + group * 32;
+    const bool some = m0 < a.M && n0 < a.N;
+    if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
+    __syncwarp();
+    tc_fence_after();
+    float v[32], w[32];  // the gate, its factor
+    if (some) {
+      uint32_t c[2][32];
+      const uint32_t at = tbase + acc * BN + group * 32 + ((uint32_t)(q * 32) << 16);
+      tmem_ld32(at, c[0]);
+      tmem_ld32(at + BN / 2, c[1]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        v[i] = __uint_as_float(c[0][i]);
+        w[i] = __uint_as_float(c[1][i]);
+      }
+    }
+    give_back<CG>(tfree + acc);
+    if (lane == 0) bulk_wait_read();  // the staging is free once the last tile's copies have read it
+    __syncwarp();
+    if (some && a.raw) {
+      const int nv = t.nt * BN + group * 32, all = a.ntiles * BN;
+      put32(stg, v, &maps.out, true, nullptr, 0, m0, a.M, nv, all, t.split);
+      put32(stg, w, &maps.out, true, nullptr, 0, m0, a.M, nv + BN / 2, all, t.split);
+    } else if (some) {
+      if (e.bias) add_bias(v, e.bias, e.bias_dt, n0, a.N);
+      if (a.bias2) add_bias(w, a.bias2, a.bias2_dt, n0, a.N);
+      if (e.z) {
+        float k[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) k[i] = keep_z(v[i], BF16);
+        stage16(stg, k, BF16);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) k[i] = keep_z(w[i], BF16);
+        stage16(stg + BLOCK_ST, k, BF16);
+      }
+      if constexpr (ACT == OW_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) gelu2<BF16>(v[i], v[i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT, BF16>(v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= w[i];
+      stage16(stg + 2 * BLOCK_ST, v, BF16);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (e.z) {
+          tma_store_3d(&maps.z, n0, (int)m0, 0, stg);
+          tma_store_3d(&maps.c2, n0, (int)m0, 0, stg + BLOCK_ST);
+        }
+        tma_store_3d(&maps.out, n0, (int)m0, 0, stg + 2 * BLOCK_ST);
+        bulk_commit();
+      }
+    }
+    if ((u += step) < units) t = unit_of(a, u);
+  }
+  if (lane == 0) bulk_wait_read();  // the staging stays until it is read
+}
+
+// Column sums of the lanes' rows: lane l gets column l's.  Each step halves the
+// columns that a lane carries on.
+__device__ __forceinline__ float column_sum(float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
+}
+
+// GRAD's epilogue: g and u of a block of 32 rows and 32 columns come to the staging
+// by copies (the first block's while the products are at work), d u act'(g) and
+// d act(g) take their places there and leave.  A lane reads and writes its own row.
+template <int BN, int CG, bool BF16, int ACT>
+__device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
+                                              uint32_t tbase, uint64_t* tfull, uint64_t* tfree, uint64_t* here, unsigned char* stg,
+                                              volatile int* abort) {
+  using C = GC<BN, CG, GRAD>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, group = warp >> 2;
+  int tl = 0, fetched = 0;
+  for (int u = first; u < units; ++tl) {
+    const int acc = tl & 1;
+    const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
+    const int nb = t.nt * BN + group * C::CW;
+    const bool some = m0 < a.M && nb < a.N;
+    const int blocks = !some ? 0 : nb + 32 < a.N ? C::NBLK : 1;
+    auto fetch = [&](int j) {  // by lane 0
+      bulk_wait_read();        // the last block's copies have read the staging
+      mbar_arrive_expect_tx(here, 2 * BLOCK_ST);
+      tma_load_2d(stg, &maps.res, nb + 32 * j, (int)m0, here);
+      tma_load_2d(stg + BLOCK_ST, &maps.b2, nb + 32 * j, (int)m0, here);
+    };
+    if (lane == 0 && some) fetch(0);
+    __syncwarp();
+    if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
+    __syncwarp();
+    tc_fence_after();
+#pragma unroll
+    for (int j = 0; j < C::NBLK; ++j) {
+      if (j >= blocks) break;
+      const int n0 = nb + 32 * j;
+      if (j > 0) {
+        if (lane == 0) fetch(j);
+        __syncwarp();
+      }
+      uint32_t w[32];
+      tmem_ld32(tbase + acc * BN + group * C::CW + j * 32 + ((uint32_t)(q * 32) << 16), w);
+      tmem_ld_wait();
+      if (j + 1 == blocks) give_back<CG>(tfree + acc);
+      if (!wait_for(here, fetched++ & 1, abort)) break;
+      __syncwarp();
+      float dg[32], du[32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint4* pg = reinterpret_cast<uint4*>(stg + stg_at(lane, k));
+        uint4* pu = reinterpret_cast<uint4*>(stg + BLOCK_ST + stg_at(lane, k));
+        const uint4 rg = *pg, ru = *pu;
+        const uint32_t gq[4] = {rg.x, rg.y, rg.z, rg.w}, uq[4] = {ru.x, ru.y, ru.z, ru.w};
+        uint32_t og[4], ou[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 g = unpack2<BF16>(gq[i]), f = unpack2<BF16>(uq[i]);
+          const int c = 8 * k + 2 * i;
+          const float d0 = __uint_as_float(w[c]), d1 = __uint_as_float(w[c + 1]);
+          float a0, s0, a1, s1;
+          act_both<ACT>(g.x, a0, s0);
+          act_both<ACT>(g.y, a1, s1);
+          dg[c] = d0 * f.x * s0;
+          dg[c + 1] = d1 * f.y * s1;
+          du[c] = d0 * a0;
+          du[c + 1] = d1 * a1;
+          og[i] = pack2<BF16>(dg[c], dg[c + 1]);
+          ou[i] = pack2<BF16>(du[c], du[c + 1]);
+        }
+        *pg = make_uint4(og[0], og[1], og[2], og[3]);
+        *pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&maps.out, n0, (int)m0, 0, stg);
+        tma_store_3d(&maps.c2, n0, (int)m0, 0, stg + BLOCK_ST);
+        bulk_commit();
+      }
+      if (a.part) {
+        const float sg = column_sum(dg), su = column_sum(du);
+        const int64_t rows32 = (a.M + 31) / 32;
+        if (n0 + lane < a.N) {
+          a.part[(m0 / 32) * a.N + n0 + lane] = sg;
+          a.part[(rows32 + m0 / 32) * a.N + n0 + lane] = su;
+        }
+      }
+    }
+    if (blocks == 0) give_back<CG>(tfree + acc);
+    if ((u += step) < units) t = unit_of(a, u);
+  }
+  if (lane == 0) bulk_wait_read();
+}
+
 template <int BN, int CG, bool AMN, bool BMN, bool BF16, int ACT, int KIND = PLAIN>
 __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant__ MapsOf<KIND> maps, const GemmArgs a) {
-  using C = GC<BN, CG>;
-  constexpr int ACTIVE = KIND == GATE ? C::GATE_ACTIVE : C::ACTIVE;
+  using C = GC<BN, CG, KIND>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
@@ -489,7 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   if (warp == 0) {  // a lane a barrier
     for (int i = lane; i < C::NBAR; i += 32) {
       uint64_t* b = full + i;
-      mbar_init(b, b == tfree || b == tfree + 1 ? ACTIVE * CG : 1);
+      mbar_init(b, b == tfree || b == tfree + 1 ? C::ACTIVE * CG : 1);
     }
     fence_mbar_init();
     __syncwarp();
@@ -610,71 +865,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         if ((u += step) < units) t = unit_of(a, u);
       }
     }
-  } else if (KIND == GATE && warp < ACTIVE) {
-   if constexpr (KIND == GATE) {
-    unsigned char* stg = sm + C::OFF_STG + warp * 2 * BLOCK_ST;
-    const int q = warp & 3, group = warp >> 2;
-    const Epi& e = a.e;
-    int tl = 0;
-    for (int u = first; u < units; ++tl) {
-      const int acc = tl & 1;
-      const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
-      const int n0 = t.nt * (BN / 2) + group * 32;
-      const bool some = m0 < a.M && n0 < a.N;
-      if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
-      __syncwarp();
-      tc_fence_after();
-      float v[32], w[32];  // the gate, its factor
-      if (some) {
-        uint32_t c[2][32];
-        const uint32_t at = tbase + acc * BN + group * 32 + ((uint32_t)(q * 32) << 16);
-        tmem_ld32(at, c[0]);
-        tmem_ld32(at + BN / 2, c[1]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          v[i] = __uint_as_float(c[0][i]);
-          w[i] = __uint_as_float(c[1][i]);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 1) mbar_arrive(tfree + acc);
-        else arrive_in(in_cta(tfree + acc, 0));
-        bulk_wait_read();  // the staging is free once the last tile's copies have read it
-      }
-      __syncwarp();
-      if (some && a.raw) {
-        const int nv = t.nt * BN + group * 32, all = a.ntiles * BN;
-        put32(stg, v, &maps.out, true, nullptr, 0, m0, a.M, nv, all, t.split);
-        put32(stg, w, &maps.out, true, nullptr, 0, m0, a.M, nv + BN / 2, all, t.split);
-      } else if (some) {
-        if (e.bias) add_bias(v, e.bias, e.bias_dt, n0, a.N);
-        if (a.bias2) add_bias(w, a.bias2, a.bias2_dt, n0, a.N);
-        if (e.z) {
-          float k[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) k[i] = keep_z(v[i], BF16);
-          put16(stg, k, BF16, &maps.z, true, nullptr, 0, m0, a.M, n0, a.N);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) k[i] = keep_z(w[i], BF16);
-          put16(stg + BLOCK_ST, k, BF16, &maps.c2, true, nullptr, 0, m0, a.M, n0, a.N);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT, BF16>(v[i]) * w[i];
-        if (e.z) {
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-        }
-        put16(stg, v, BF16, &maps.out, true, nullptr, 0, m0, a.M, n0, a.N);
-      }
-      if ((u += step) < units) t = unit_of(a, u);
-    }
-    if (lane == 0) bulk_wait_read();
-   }
-  } else if (KIND != GATE && warp < ACTIVE) {
+  } else if (warp < C::ACTIVE) {
     unsigned char* stg = sm + C::OFF_STG + warp * C::STG_W;
+    if constexpr (KIND == GATE) gate_epilogue<BN, CG, BF16, ACT>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, stg, abort);
+    else if constexpr (KIND == GRAD) grad_epilogue<BN, CG, BF16, ACT>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, rbar + warp, stg, abort);
+    else {
     const int q = warp & 3, group = warp >> 2;
     const Epi& e = a.e;
     int tl = 0, fetched = 0;
@@ -780,6 +975,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       if ((u += step) < units) t = unit_of(a, u);
     }
     if (lane == 0) bulk_wait_read();  // the staging stays until it is read
+    }
   }
 
   __syncwarp();
@@ -1224,7 +1420,7 @@ int block_map(CUtensorMap* map, int dtype, const void* p, int64_t rows, int cols
 
 template <int BN, int CG, bool AMN, bool BMN, bool BF16, int ACT, int KIND = PLAIN>
 int run_gemm(const MapsOf<KIND>& maps, const GemmArgs& k, int grid, cudaStream_t st) {
-  using C = GC<BN, CG>;
+  using C = GC<BN, CG, KIND>;
   auto kern = gemm_kernel<BN, CG, AMN, BMN, BF16, ACT, KIND>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) {
@@ -1303,7 +1499,10 @@ struct Second {
   Mat a, b;           // CAT_K both, CAT_M a, GATE b
   const void* bias;   // GATE
   int bias_dt;
-  void* c;            // GATE: its z, beside e.z; CAT_M: its output
+  void* c;            // GATE: its z, beside e.z; CAT_M: its output; GRAD: d act(g)
+  const void* g;      // GRAD: rows of e.ldo, as the results'
+  const void* u;
+  float* part;        // GRAD: column sums, or NULL
 };
 struct DualWs {
   void *a, *b, *a2, *b2;
@@ -1319,8 +1518,8 @@ DualWs dual_take(const Mat& A, const Mat& B, const Second& s, int64_t M, int N, 
   auto copy = [&](const Mat& m) { return tma_rows(m.p, m.ld) ? nullptr : ws.take((size_t)m.rows * up8(m.cols) * 2); };
   w.a = copy(A);
   w.b = copy(B);
-  if (KIND != GATE) w.a2 = copy(s.a);
-  if (KIND != CAT_M) w.b2 = copy(s.b);
+  if (KIND == CAT_K || KIND == CAT_M) w.a2 = copy(s.a);
+  if (KIND == CAT_K || KIND == GATE) w.b2 = copy(s.b);
   w.part_ld = KIND == GATE ? gate_cols(N, p.bn) : (N + 3) / 4 * 4;
   if (p.splits > 1) w.part = (float*)ws.take((size_t)p.splits * (KIND == CAT_M ? 2 : 1) * M * w.part_ld * 4);
   return w;
@@ -1338,8 +1537,8 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
   const uint32_t arows = AMN ? KE : TM, brows = BMN ? KE : KIND == GATE ? p.bn / 2 : p.bn / p.cg;
   OW_RETURN_IF(map_of(&maps.a, A, bf16, arows));
   OW_RETURN_IF(map_of(&maps.b, B, bf16, brows));
-  if (KIND != GATE) OW_RETURN_IF(map_of(&maps.a2, s.a, bf16, arows));
-  if (KIND != CAT_M) OW_RETURN_IF(map_of(&maps.b2, s.b, bf16, brows));
+  if (KIND == CAT_K || KIND == CAT_M) OW_RETURN_IF(map_of(&maps.a2, s.a, bf16, arows));
+  if (KIND == CAT_K || KIND == GATE) OW_RETURN_IF(map_of(&maps.b2, s.b, bf16, brows));
   GemmArgs k{};
   k.M = M;
   k.N = N;
@@ -1370,6 +1569,12 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
       if (e.z) OW_RETURN_IF(block_map(&maps.z, t16, e.z, M, N, e.ldz, 1));
       if (e.z) OW_RETURN_IF(block_map(&maps.c2, t16, s.c, M, N, e.ldz, 1));
     }
+    if (KIND == GRAD) {
+      k.part = s.part;
+      OW_RETURN_IF(block_map(&maps.c2, t16, s.c, M, N, e.ldo, 1));
+      OW_RETURN_IF(block_map(&maps.res, t16, s.g, M, N, e.ldo, 0));
+      OW_RETURN_IF(block_map(&maps.b2, t16, s.u, M, N, e.ldo, 0));
+    }
     if (KIND == CAT_M) {
       k.out2 = s.c;
       if (e.vo) OW_RETURN_IF(block_map(&maps.c2, e.out32 ? OW_DTYPE_F32 : t16, s.c, M, N, e.ldo, 1));
@@ -1390,7 +1595,7 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
     if (p.bn == 64) return tile(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     return tile(std::integral_constant<int, 128>(), std::integral_constant<int, 1>());
   };
-  if constexpr (KIND == GATE) {
+  if constexpr (KIND == GATE || KIND == GRAD) {
     switch (e.act) {
       case OW_ACT_RELU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_RELU>())); break;
       case OW_ACT_SILU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_SILU>())); break;
