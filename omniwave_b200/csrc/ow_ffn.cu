@@ -335,11 +335,9 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
     }
     OW_CHECK_LAUNCH("gate_grad_kernel");
   }
-  for (int i = 0; i < 2; ++i) {
-    void* db = i ? g->dup_bias : g->dgate_bias;
-    if (!db) continue;
-    launch(dbias_kernel, (F + 31) / 32, 1024, 0, st, (const float*)b.bias + (size_t)i * b.chunks * F, b.chunks, F, db,
-           i ? a->up_bias_dtype : a->gate_bias_dtype);
+  if (b.bias) {
+    launch(dbias_kernel, dim3((F + 31) / 32, 2), 1024, 0, st, (const float*)b.bias, b.chunks, F, g->dgate_bias, a->gate_bias_dtype,
+           g->dup_bias, a->up_bias_dtype);
     OW_CHECK_LAUNCH("dbias_kernel");
   }
   const Mat dg{b.dg, M, F, ld}, du{b.du, M, F, ld};

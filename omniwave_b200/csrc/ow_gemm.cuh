@@ -88,7 +88,7 @@ struct GemmArgs {
   // CAT_K: k blocks, CAT_M: rows of tiles of the first product
   int half;
   void* out2;        // CAT_M: the second product
-  float* part;       // GRAD: [2][blocks of 32 rows][N] column sums of both results, or NULL
+  float* part;       // GRAD: [2][blocks of 32 rows][N] column sums of both rounded results, or NULL
 };
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
@@ -333,28 +333,37 @@ __device__ __forceinline__ void gelu2(float& y, float& z) {
   z = fmaf(-b, ex2(f.y), z < 0.f ? 0.f : z);
 }
 
-// An activation and its slope at z, which share what is costly: gelu's tail is
-// act_slope's, and the value max(z, 0) - |z| tail.
+// An activation and its slope at two z, which share what is costly, in pairs: gelu's
+// tail is act_slope's, and the value max(z, 0) - |z| tail.
 template <int ACT>
-__device__ __forceinline__ void act_both(float z, float& a, float& s) {
+__device__ __forceinline__ void act_both(float2 z, uint64_t& a, uint64_t& s) {
+  auto c = [](float v) { return f2pack(v, v); };
+  const uint64_t zz = f2pack(z.x, z.y);
   if constexpr (ACT == OW_ACT_SILU) {
-    const float g = sigmoid(z);
-    a = z * g;
-    s = fmaf(a, 1.f - g, g);
+    const float2 x = f2unpack(mul2(zz, c(-1.44269504f)));
+    const float2 y = f2unpack(add2(f2pack(ex2(x.x), ex2(x.y)), c(1.f)));
+    const uint64_t g = f2pack(rcp(y.x), rcp(y.y));
+    a = mul2(zz, g);
+    s = fma2(a, fma2(g, c(-1.f), c(1.f)), g);
   } else if constexpr (ACT == OW_ACT_GELU) {
-    const float e = ex2(z * z * -0.72134752f);
-    const float t = rcp(fmaf(fabsf(z), 0.35f, 1.f));
-    float tail = fmaf(t, 0.0471570618f, -0.194429092f);
-    tail = fmaf(tail, t, 0.226878741f);
-    tail = fmaf(tail, t, -0.00380232154f);
-    tail = fmaf(tail, t, 0.148624128f);
-    tail = fmaf(tail, t, 0.135697883f);
-    tail = fmaf(tail, t, 0.139873699f) * t * e;
-    a = fmaf(-fabsf(z), tail, z < 0.f ? 0.f : z);
-    s = fmaf(z * 0.39894228040143268f, e, z > 0.f ? 1.f - tail : tail);
+    const uint64_t m = f2pack(fabsf(z.x), fabsf(z.y));
+    const float2 x = f2unpack(mul2(mul2(zz, zz), c(-0.72134752f)));
+    const uint64_t e = f2pack(ex2(x.x), ex2(x.y));
+    const float2 y = f2unpack(fma2(m, c(0.35f), c(1.f)));
+    const uint64_t t = f2pack(rcp(y.x), rcp(y.y));
+    uint64_t tail = fma2(t, c(0.0471570618f), c(-0.194429092f));
+    tail = fma2(tail, t, c(0.226878741f));
+    tail = fma2(tail, t, c(-0.00380232154f));
+    tail = fma2(tail, t, c(0.148624128f));
+    tail = fma2(tail, t, c(0.135697883f));
+    tail = mul2(mul2(fma2(tail, t, c(0.139873699f)), t), e);
+    const uint64_t less = mul2(tail, c(-1.f));
+    a = fma2(m, less, f2pack(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y));
+    const float2 u = f2unpack(add2(less, c(1.f))), v = f2unpack(tail);
+    s = fma2(mul2(zz, c(0.39894228040143268f)), e, f2pack(z.x > 0.f ? u.x : v.x, z.y > 0.f ? u.y : v.y));
   } else {
-    a = act_fwd<ACT, false>(z);
-    s = act_slope<ACT>(z);
+    a = f2pack(act_fwd<ACT, false>(z.x), act_fwd<ACT, false>(z.y));
+    s = f2pack(act_slope<ACT>(z.x), act_slope<ACT>(z.y));
   }
 }
 
@@ -617,20 +626,28 @@ __device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs&
   if (lane == 0) bulk_wait_read();  // the staging stays until it is read
 }
 
-// Column sums of the lanes' rows: lane l gets column l's.  Each step halves the
-// columns that a lane carries on.
-__device__ __forceinline__ float column_sum(float (&v)[32]) {
+// Column sums of a staged block of 32 x 32 16-bit values, to 32 floats of ``out`` of
+// which ``cols`` are columns: ones times the block on the warp-wide MMA.  (By shuffles,
+// from the registers, it took as many instructions as gelu and its slope.)
+template <bool BF16>
+__device__ __forceinline__ void column_sums(const unsigned char* stg, float* out, int cols) {
   const int lane = threadIdx.x & 31;
+  const uint32_t one = BF16 ? 0x3F803F80u : 0x3C003C00u, at = smem_u32(stg);
+  const uint32_t ones[4] = {one, one, one, one};
+  float2 mine = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-    }
+  for (int u = 0; u < 4; ++u) {  // 8 columns
+    uint32_t b[4];
+    ldsm_x4_trans(at + stg_at(lane, u), b[0], b[1], b[2], b[3]);
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16816<BF16>(c, ones, b[0], b[1]);
+    mma16816<BF16>(c, ones, b[2], b[3]);
+    if (lane >> 2 == u) mine = make_float2(c[0], c[1]);
   }
-  return v[0];
+  const int n = (lane >> 2) * 8 + (lane & 3) * 2;  // every row of the product is the sums
+  if (lane >= 16) return;
+  if (n < cols) out[n] = mine.x;
+  if (n + 1 < cols) out[n + 1] = mine.y;
 }
 
 // GRAD's epilogue: g and u of a block of 32 rows and 32 columns come to the staging
@@ -674,7 +691,6 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
       if (j + 1 == blocks) give_back<CG>(tfree + acc);
       if (!wait_for(here, fetched++ & 1, abort)) break;
       __syncwarp();
-      float dg[32], du[32];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint4* pg = reinterpret_cast<uint4*>(stg + stg_at(lane, k));
@@ -684,18 +700,13 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
         uint32_t og[4], ou[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 g = unpack2<BF16>(gq[i]), f = unpack2<BF16>(uq[i]);
-          const int c = 8 * k + 2 * i;
-          const float d0 = __uint_as_float(w[c]), d1 = __uint_as_float(w[c + 1]);
-          float a0, s0, a1, s1;
-          act_both<ACT>(g.x, a0, s0);
-          act_both<ACT>(g.y, a1, s1);
-          dg[c] = d0 * f.x * s0;
-          dg[c + 1] = d1 * f.y * s1;
-          du[c] = d0 * a0;
-          du[c + 1] = d1 * a1;
-          og[i] = pack2<BF16>(dg[c], dg[c + 1]);
-          ou[i] = pack2<BF16>(du[c], du[c + 1]);
+          const float2 f = unpack2<BF16>(uq[i]);
+          const uint64_t d = (uint64_t)w[8 * k + 2 * i] | (uint64_t)w[8 * k + 2 * i + 1] << 32;
+          uint64_t v, slope;
+          act_both<ACT>(unpack2<BF16>(gq[i]), v, slope);
+          const float2 dg = f2unpack(mul2(mul2(d, f2pack(f.x, f.y)), slope)), du = f2unpack(mul2(d, v));
+          og[i] = pack2<BF16>(dg.x, dg.y);
+          ou[i] = pack2<BF16>(du.x, du.y);
         }
         *pg = make_uint4(og[0], og[1], og[2], og[3]);
         *pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
@@ -708,12 +719,9 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
         bulk_commit();
       }
       if (a.part) {
-        const float sg = column_sum(dg), su = column_sum(du);
-        const int64_t rows32 = (a.M + 31) / 32;
-        if (n0 + lane < a.N) {
-          a.part[(m0 / 32) * a.N + n0 + lane] = sg;
-          a.part[(rows32 + m0 / 32) * a.N + n0 + lane] = su;
-        }
+        float* to = a.part + m0 / 32 * a.N + n0;
+        column_sums<BF16>(stg, to, a.N - n0);
+        column_sums<BF16>(stg + BLOCK_ST, to + (a.M + 31) / 32 * a.N, a.N - n0);
       }
     }
     if (blocks == 0) give_back<CG>(tfree + acc);
@@ -1264,8 +1272,16 @@ __global__ void __launch_bounds__(UNIT_WARPS * 32) linear_units_kernel(const Row
   cluster_sync();  // a block's sums stay until the first has read them
 }
 
-__global__ void __launch_bounds__(1024) dbias_kernel(const float* __restrict__ part, int chunks, int N, void* out, int dt) {
+// blockIdx.y: the second of two arrays of partial sums.
+__global__ void __launch_bounds__(1024) dbias_kernel(const float* __restrict__ part, int chunks, int N, void* out, int dt, void* out2 = nullptr,
+                                                     int dt2 = 0) {
   __shared__ float sh[32][33];
+  if (blockIdx.y) {
+    part += (int64_t)chunks * N;
+    out = out2;
+    dt = dt2;
+  }
+  if (!out) return;
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5, c = blockIdx.x * 32 + cx;
   float t[4] = {0.f, 0.f, 0.f, 0.f};  // four loads in flight: a chain of them is what this kernel takes
   if (c < N)

@@ -281,7 +281,7 @@ int ow_linear_bwd(const ow_linear_t* a, const ow_linear_grads_t* g, void* stream
     }
     OW_CHECK_LAUNCH("dz_kernel");
     if (g->dbias) {
-      launch(dbias_kernel, (N + 31) / 32, 1024, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype);
+      launch(dbias_kernel, (N + 31) / 32, 1024, 0, st, (const float*)b.bias, b.chunks, N, g->dbias, a->bias_dtype, nullptr, 0);
       OW_CHECK_LAUNCH("dbias_kernel");
     }
   }

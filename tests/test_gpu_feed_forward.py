@@ -6,7 +6,8 @@ matrix product of 16-bit operands sums exact products in f32, in any order, with
 f32; a 16-bit result is off by half(t) of itself.  The activations are within 8 u
 (|z| + 1) of theirs, gelu's bf16 tail within 4e-4 of itself; slopes change by at
 most 0.8 |dz| (silu'' <= 0.5, gelu'' <= 0.8), values by 1.13 |dz|.  The backward
-holds g and u in 16 bits; dh may be rounded to 16 bits before the gate's formula.
+holds g and u in 16 bits; dh may be rounded to 16 bits before the gate's formula,
+and the biases' gradients are sums of dg and du that may have been.
 """
 
 from __future__ import annotations
@@ -98,8 +99,8 @@ def _define(x, wg, wu, wd, bg, bu, bd, r, dy, act, t):
     a, s = _act(g16, act, t)
     dh = (dy @ wd).round(t)
     dg, du = dh * u16 * s, dh * a
-    out["bg"], out["bu"], out["bd"] = dg.sum0(), du.sum0(), dy.sum0()
     dg, du = dg.round(t), du.round(t)
+    out["bg"], out["bu"], out["bd"] = dg.sum0(), du.sum0(), dy.sum0()  # of dg and du as they are rounded, or before
     out["x"] = dg @ wg + du @ wu
     out["wg"], out["wu"], out["wd"] = dg.t() @ x, du.t() @ x, dy.t() @ h
     return out
