@@ -96,7 +96,22 @@ __device__ __forceinline__ f2 both(float v) { return sm100::f2pack(v, v); }
 template <typename T>
 constexpr int PER = 16 / sizeof(T);  // elements of a 16-byte vector
 
-// A vector's elements as pairs of floats.
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& r, float (&o)[PER<T>]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = sm100::unpack2<std::is_same_v<T, __nv_bfloat16>>(w[i]);
+      o[2 * i] = f.x;
+      o[2 * i + 1] = f.y;
+    }
+  }
+}
+// The same as pairs.
 template <typename T>
 __device__ __forceinline__ void widen(const uint4& r, f2 (&o)[PER<T> / 2]) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -180,19 +195,26 @@ struct Run {
 __device__ __forceinline__ float pivot(float m) { return m == -INFINITY ? 0.f : m; }
 // What a sum around m is worth around the pivot p: a sum that has seen no logit yet is 0.
 __device__ __forceinline__ float moved(float m, float p, float k) { return m == -INFINITY ? 0.f : ex2((m - p) * k); }
-__device__ __forceinline__ Run join(const Run& a, const Run& b, float kt) {
-  Run r;
-  r.m = fmaxf(a.m, b.m);
+// The states of a warp's lanes as one: each sum is moved once, to the largest maximum.
+__device__ __forceinline__ Run join(Run r, float kt) {
+  const float mine = r.m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
   const float p = pivot(r.m);
-  r.st = a.st * moved(a.m, p, kt) + b.st * moved(b.m, p, kt);
-  r.s1 = a.s1 * moved(a.m, p, LOG2E) + b.s1 * moved(b.m, p, LOG2E);
+  r.st *= moved(mine, p, kt);
+  r.s1 *= moved(mine, p, LOG2E);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    r.st += __shfl_xor_sync(0xffffffffu, r.st, o);
+    r.s1 += __shfl_xor_sync(0xffffffffu, r.s1, o);
+  }
   return r;
 }
 
 // The softmax state of a thread's share of a row, every G-th unit from ``lane`` on.
 template <typename T, int G, int POW>
 __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float kt) {
-  constexpr int N = 4, P = PER<T> / 2;  // vectors under way at once
+  constexpr int N = 4;  // vectors under way at once
   const Lay<T> lay(z, V);
   Run run{-INFINITY, 0.f, 0.f};
   auto single = [&](int i) {
@@ -203,34 +225,35 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
   };
   for (int i = lane; i < lay.lead; i += G) single(i);
   for (int i = lay.rest() + lane; i < V; i += G) single(i);
-  f2 st = sm100::f2pack(run.st, 0.f), s1 = sm100::f2pack(run.s1, 0.f);
+  float st[2] = {run.st, 0.f}, s1[2] = {run.s1, 0.f};  // two chains of sums
   const uint4* u = reinterpret_cast<const uint4*>(z + lay.lead);
-  const f2 k2 = both(kt), k1 = both(LOG2E);
   auto step = [&](const uint4 (&v)[N]) {
-    f2 x[P];
+    float x[PER<T>];
     widen<T>(larger<T>(larger<T>(v[0], v[1]), larger<T>(v[2], v[3])), x);
     float m = run.m;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const float2 f = sm100::f2unpack(x[j]);
-      m = fmaxf(m, fmaxf(f.x, f.y));
-    }
+    for (int j = 0; j < PER<T>; ++j) m = fmaxf(m, x[j]);
     const float p = pivot(m);
     if (m > run.m) {
-      st = sm100::mul2(st, both(moved(run.m, p, kt)));
-      if constexpr (POW != 1) s1 = sm100::mul2(s1, both(moved(run.m, p, LOG2E)));
+      const float ft = moved(run.m, p, kt), f1 = POW != 1 ? moved(run.m, p, LOG2E) : 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        st[c] *= ft;
+        if constexpr (POW != 1) s1[c] *= f1;
+      }
       run.m = m;
     }
-    const f2 pt = both(-p * kt), p1 = both(-p * LOG2E);
+    const float pt = -p * kt, p1 = -p * LOG2E;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       widen<T>(v[n], x);
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        const f2 e = ex2(sm100::fma2(x[j], k2, pt));
-        st = sm100::add2(st, e);
-        if constexpr (POW >= 2) s1 = sm100::fma2(power1<POW>(e), e, s1);
-        if constexpr (POW == 0) s1 = sm100::add2(s1, ex2(sm100::fma2(x[j], k1, p1)));
+      for (int j = 0; j < PER<T>; ++j) {
+        const float e = ex2(fmaf(x[j], kt, pt));
+        st[j & 1] += e;
+        if constexpr (POW == 2) s1[j & 1] = fmaf(e, e, s1[j & 1]);
+        if constexpr (POW == 4) s1[j & 1] = fmaf(e * e, e * e, s1[j & 1]);
+        if constexpr (POW == 0) s1[j & 1] += ex2(fmaf(x[j], LOG2E, p1));
       }
     }
   };
@@ -247,9 +270,8 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
     for (int n = 0; n < N; ++n) v[n] = i + n * G < lay.units ? __ldg(u + i + n * G) : least<T>();
     step(v);
   }
-  const float2 a = sm100::f2unpack(st), b = sm100::f2unpack(s1);
-  run.st = a.x + a.y;
-  run.s1 = POW == 1 ? run.st : b.x + b.y;
+  run.st = st[0] + st[1];
+  run.s1 = POW == 1 ? run.st : s1[0] + s1[1];
   return run;
 }
 
@@ -359,10 +381,7 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
       const T* z = (const T*)a.z + row * a.ld;
       Run run = softmax_share<T, 32, POW>(z, a.V, lane, a.kt);
       const Said said = listen(a, z, row, lane, sx, sx + a.K);
-#pragma unroll
-      for (int o = 16; o; o >>= 1)
-        run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
-                            __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+      run = join(run, a.kt);
       if (lane == 0) conclude(a, row, run, said);
       __syncwarp();  // before the next row's entries overwrite these
     }
@@ -375,10 +394,7 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
       Said said;
       if (warp < W) {
         Run run = softmax_share<T, G, POW>(z, a.V, threadIdx.x, a.kt);
-#pragma unroll
-        for (int o = 16; o; o >>= 1)
-          run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
-                              __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+        run = join(run, a.kt);
         if (lane == 0) sh[turn][warp] = run;
       } else {
         said = listen(a, z, row, lane, dyn, dyn + a.K);
@@ -386,10 +402,7 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
       __syncthreads();
       if (warp == W) {
         Run run = lane < W ? sh[turn][lane] : Run{-INFINITY, 0.f, 0.f};
-#pragma unroll
-        for (int o = 16; o; o >>= 1)
-          run = join(run, Run{__shfl_xor_sync(0xffffffffu, run.m, o), __shfl_xor_sync(0xffffffffu, run.st, o),
-                              __shfl_xor_sync(0xffffffffu, run.s1, o)}, a.kt);
+        run = join(run, a.kt);
         if (lane == 0) conclude(a, row, run, said);
       }
     }
@@ -401,6 +414,7 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const Args a, int mean, float* loss, float* coef) {
   __shared__ double sh[4][32];
   double v[4] = {0, 0, 0, 0};  // soft, its rows, hard, its rows
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < a.rows; i += 1024) {
     v[0] += a.soft[i];
     v[1] += a.top[i] != INFINITY;
@@ -655,8 +669,11 @@ int with(const ow_distill_t* a, F&& f) {
     }
   };
   auto type = [&](auto t) -> int {
-    if (a->classes <= 1024 && a->top <= 256) return power(std::integral_constant<int, 32>(), t);
-    return power(std::integral_constant<int, 224>(), t);
+    // A warp a row where rows are many and not long: 16384 x 2000 bf16 forward 37 us and backward 31 (a block a row
+    // 95 and 87), 4096 x 8000 26 and 23 (34 and 32); 1024 x 8000 12 and 13 (11 and 11), 128 x 1500 7.2 and 7.2
+    // (5.7 and 6.2).  Its entries have to leave room for those of the block's other rows.
+    const bool warps = a->top <= 256 && (a->classes <= 256 || (a->classes <= 8192 && a->rows >= 6 * (int64_t)device_sm_count()));
+    return warps ? power(std::integral_constant<int, 32>(), t) : power(std::integral_constant<int, 224>(), t);
   };
   switch (a->dtype) {
     case OW_DTYPE_F32: return type(float());
