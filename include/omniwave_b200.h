@@ -613,11 +613,11 @@ OW_API int ow_linear_bwd(const ow_linear_t* args, const ow_linear_grads_t* grads
  * with row stride ldd, residual [rows, out_features] with row stride ldr, all of
  * ``dtype`` (bf16 or f16) with unit column stride; biases f32, bf16 or f16, or
  * NULL; out [rows, out_features] contiguous.  Sums and activation are f32.  h
- * [rows, ldh], ldh = hidden rounded up to 8, gets h rounded to ``dtype``; g and u
- * (both NULL, or [rows, ldh]) g and u, for the backward.
+ * [rows, ldh], ldh = hidden rounded up to 8, gets h rounded to ``dtype``; act and
+ * slope (both NULL, or [rows, ldh]) act(g) and u act'(g), for the backward.
  *
  * Backward, from dout: NULL outputs are not computed; dgate_weight and dup_weight
- * come together, with one dtype.  h is needed for ddown_weight only, g, u and
+ * come together, with one dtype.  h is needed for ddown_weight only, act, slope and
  * down_weight for all gradients but the projection back's.  dg and du are rounded
  * to ``dtype``, and where dh's product is split so is dh; dgate_bias and dup_bias
  * are f32 sums of dg and du, rounded where dh is not.  All sums are taken in a fixed
@@ -645,8 +645,8 @@ typedef struct ow_ffn_t {
   int64_t ldr;
   void* out;
   void* h;
-  void* g;
-  void* u;
+  void* act;
+  void* slope;
   void* workspace;             /* ow_ffn_workspace_size() bytes */
   size_t workspace_bytes;
 } ow_ffn_t;

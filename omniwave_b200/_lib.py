@@ -172,7 +172,7 @@ class Ffn(ctypes.Structure):
         ("up_weight", _vp), ("ldu", ctypes.c_int64), ("down_weight", _vp), ("ldd", ctypes.c_int64),
         ("gate_bias", _vp), ("gate_bias_dtype", _c_i32), ("up_bias", _vp), ("up_bias_dtype", _c_i32),
         ("down_bias", _vp), ("down_bias_dtype", _c_i32), ("residual", _vp), ("ldr", ctypes.c_int64),
-        ("out", _vp), ("h", _vp), ("g", _vp), ("u", _vp),
+        ("out", _vp), ("h", _vp), ("act", _vp), ("slope", _vp),
         ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 

@@ -580,7 +580,7 @@ struct FfnCall {
 };
 
 struct FfnOut {
-  Tensor y, h, g, u;  // g and u for the backward
+  Tensor y, h, act, slope;  // the last two for the backward
 };
 
 FfnOut ffn_forward(const FfnCall& k, const Tensor& res, bool keep, at::IntArrayRef shape) {
@@ -591,8 +591,8 @@ FfnOut ffn_forward(const FfnCall& k, const Tensor& res, bool keep, at::IntArrayR
   if (m == 0) return o;
   o.h = at::empty({m, f}, k.x.options());
   if (keep) {
-    o.g = at::empty({m, f}, k.x.options());
-    o.u = at::empty({m, f}, k.x.options());
+    o.act = at::empty({m, f}, k.x.options());
+    o.slope = at::empty({m, f}, k.x.options());
   }
   ow_ffn_t a = k.args();
   if (res.defined()) {
@@ -601,8 +601,8 @@ FfnOut ffn_forward(const FfnCall& k, const Tensor& res, bool keep, at::IntArrayR
   }
   a.out = ptr(o.y);
   a.h = ptr(o.h);
-  a.g = ptr(o.g);
-  a.u = ptr(o.u);
+  a.act = ptr(o.act);
+  a.slope = ptr(o.slope);
   const Tensor ws = k.workspace(&a, nullptr);
   check_status(ow_ffn_fwd(&a, stream_of(k.x)), "ow_ffn_fwd");
   return o;
@@ -620,7 +620,7 @@ struct FfnFn : torch::autograd::Function<FfnFn> {
     // the projection back's own gradients take h alone
     const bool keep = needs(x) || needs(wg) || needs(wu) || needs(k.bg) || needs(k.bu);
     FfnOut o = ffn_forward(k, as_rows(cast(res, t)), keep, out_shape(x, wd.size(0)));
-    ctx->save_for_backward({k.x, k.wg, k.wu, k.wd, k.bg, k.bu, k.bd, o.h, o.g, o.u});
+    ctx->save_for_backward({k.x, k.wg, k.wu, k.wd, k.bg, k.bu, k.bd, o.h, o.act, o.slope});
     ctx->saved_data["act"] = act;
     ctx->saved_data["x_shape"] = x.sizes().vec();
     std::vector<int64_t> types;
@@ -665,8 +665,8 @@ struct FfnFn : torch::autograd::Function<FfnFn> {
     } else {
       ow_ffn_t a = k.args();
       a.h = ptr(s[7]);
-      a.g = ptr(s[8]);
-      a.u = ptr(s[9]);
+      a.act = ptr(s[8]);
+      a.slope = ptr(s[9]);
       auto dt = [](const Tensor& t) { return t.defined() ? code(t.scalar_type()) : 0; };
       const ow_ffn_grads_t gr{ptr(g), ptr(d[0]), ptr(d[1]), dt(d[1]), ptr(d[2]), dt(d[2]), ptr(d[3]), dt(d[3]), ptr(d[4]), ptr(d[5]), ptr(d[6])};
       const Tensor ws = k.workspace(&a, &gr);

@@ -29,7 +29,7 @@ constexpr int PATCH = 12;
 // epilogue joins them: act(A B1^T + b1) (A B2^T + b2).  CAT_K: the sum of two
 // products, the second's k blocks behind the first's.  CAT_M: two products with the
 // same B, the second's tiles behind the first's.  GRAD: one product d, whose epilogue
-// reads what GATE kept, g and u, and writes d u act'(g) and d act(g).
+// reads what GATE kept, act(g) and u act'(g), and writes d times either.
 enum Kind { PLAIN, GATE, CAT_K, CAT_M, GRAD };
 
 // BN columns of a tile; CG CTAs share it (2: 256 rows, BN / 2 rows of B each).
@@ -40,14 +40,15 @@ struct GC {
   static constexpr int CW = KIND == GATE ? 64 : BN == 256 ? 64 : 32;   // columns of an epilogue warp
   static constexpr int NBLK = CW / 32;
   static constexpr int ACTIVE = 4 * (BN / CW);     // epilogue warps at work
-  // blocks of staging a warp: GATE three (g, u and h leave together), GRAD two (what comes in and goes out in its place)
-  static constexpr int STG_W = (KIND == GATE ? 3 : KIND == GRAD ? 2 : NBLK) * BLOCK_ST;
-  static constexpr int STAGES = BN == 256 ? (KIND == GATE ? 4 : 5) : BN == 128 ? (KIND == GATE || KIND == GRAD ? 5 : 6) : 8;
+  // blocks of staging a warp: GATE three (its results leave together), GRAD two for each of its blocks (what comes in
+  // and goes out in its place)
+  static constexpr int STG_W = (KIND == GATE ? 3 : KIND == GRAD ? 2 * NBLK : NBLK) * BLOCK_ST;
+  static constexpr int STAGES = BN == 256 ? (KIND == GATE ? 4 : KIND == GRAD ? 3 : 5) : BN == 128 ? (KIND == GATE || KIND == GRAD ? 5 : 6) : 8;
   static constexpr int B_ST = B_ROWS * 128;
   static constexpr int OFF_B = STAGES * A_ST;
   static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
   static constexpr int OFF_BAR = OFF_STG + ACTIVE * STG_W;
-  static constexpr int NBAR = 2 * STAGES + 4 + 1 + EPI_WARPS;  // full, empty, tfull[2], tfree[2], probe, residual
+  static constexpr int NBAR = 2 * STAGES + 4 + 1 + 2 * EPI_WARPS;  // full, empty, tfull[2], tfree[2], probe, residual[2]
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
   static_assert(SMEM <= 232448, "shared memory budget");
@@ -301,38 +302,6 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.f;
 }
 
-// gelu of two, the polynomial's steps in pairs; and as max(z, 0) - |z| tail, whose
-// terms take one operation less.  Beyond the clamp the tail is 0.
-template <bool BF16>
-__device__ __forceinline__ void gelu2(float& y, float& z) {
-  const float a = fminf(fabsf(y), BF16 ? 13.5f : 100.f), b = fminf(fabsf(z), BF16 ? 13.5f : 100.f);
-  const uint64_t x = f2pack(a, b);
-  auto c = [](float v) { return f2pack(v, v); };
-  uint64_t q;
-  if constexpr (BF16) {
-    q = fma2(x, c(3.98267339e-8f), c(-2.39384553e-6f));
-    q = fma2(q, x, c(6.14833989e-5f));
-    q = fma2(q, x, c(-8.9382549e-4f));
-    q = fma2(q, x, c(8.29635281e-3f));
-    q = fma2(q, x, c(-5.3509552e-2f));
-    q = fma2(q, x, c(-0.458847046f));
-    q = fma2(q, x, c(-1.15114152f));
-    q = fma2(q, x, c(-1.00000072f));
-  } else {
-    q = fma2(x, c(-1.39922733e-7f), c(1.43002126e-6f));
-    q = fma2(q, x, c(3.0813193e-5f));
-    q = fma2(q, x, c(-7.80530798e-4f));
-    q = fma2(q, x, c(8.10782891e-3f));
-    q = fma2(q, x, c(-5.33918403e-2f));
-    q = fma2(q, x, c(-0.458847821f));
-    q = fma2(q, x, c(-1.15115714f));
-    q = fma2(q, x, c(-0.999998868f));
-  }
-  const float2 f = f2unpack(q);
-  y = fmaf(-a, ex2(f.x), y < 0.f ? 0.f : y);
-  z = fmaf(-b, ex2(f.y), z < 0.f ? 0.f : z);
-}
-
 // An activation and its slope at two z, which share what is costly, in pairs: gelu's
 // tail is act_slope's, and the value max(z, 0) - |z| tail.
 template <int ACT>
@@ -533,7 +502,7 @@ __device__ __forceinline__ Unit unit_of(const GemmArgs& a, int u) {
 struct Maps {
   CUtensorMap a, b, out, z, res;
 };
-struct Maps2 : Maps {  // of the second product; c2 is GATE's second z and CAT_M's second output
+struct Maps2 : Maps {  // of the second product; c2 is GATE's second z, CAT_M's and GRAD's second output, GRAD's b2 act(g)
   CUtensorMap a2, b2, c2;
 };
 template <int KIND>
@@ -550,9 +519,12 @@ __device__ __forceinline__ void give_back(uint64_t* tfree) {
   }
 }
 
-// GATE's epilogue: a warp has 32 rows and 32 columns of both products.  With g and u
-// kept, the three results are staged side by side and leave together (one after the
-// other, each waiting for the staging, 25088 x 512 -> 1024 gelu took 74.5 us).
+// GATE's epilogue: a warp has 32 rows and 32 columns of both products.  For the
+// backward it keeps what that multiplies dh with, act(g) and u act'(g), rounded once
+// each, rather than g and u: the slope costs less here, next to the activation, and
+// the backward's epilogue is left with two products.  The three results are staged side
+// by side and leave together (one after the other, each waiting for the staging,
+// 25088 x 512 -> 1024 gelu took 74.5 us, and 61 so, with g and u).
 template <int BN, int CG, bool BF16, int ACT>
 __device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
                                               uint32_t tbase, uint64_t* tfull, uint64_t* tfree, unsigned char* stg,
@@ -591,25 +563,29 @@ __device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs&
     } else if (some) {
       if (e.bias) add_bias(v, e.bias, e.bias_dt, n0, a.N);
       if (a.bias2) add_bias(w, a.bias2, a.bias2_dt, n0, a.N);
-      if (e.z) {
-        float k[32];
+      auto block = [&](auto keep) {
+        constexpr bool KEEP = decltype(keep)::value;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) k[i] = keep_z(v[i], BF16);
-        stage16(stg, k, BF16);
+        for (int k = 0; k < 4; ++k) {
+          uint32_t o[3][4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) k[i] = keep_z(w[i], BF16);
-        stage16(stg + BLOCK_ST, k, BF16);
-      }
-      if constexpr (ACT == OW_ACT_GELU) {
+          for (int i = 0; i < 4; ++i) {
+            const int j = 8 * k + 2 * i;
+            uint64_t x, y;
+            act_both<ACT>(make_float2(v[j], v[j + 1]), x, y);
+            const uint64_t f = f2pack(w[j], w[j + 1]);
+            const float2 act = f2unpack(x), slope = f2unpack(mul2(y, f)), h = f2unpack(mul2(x, f));
+            o[0][i] = pack2<BF16>(keep_z(act.x, BF16), keep_z(act.y, BF16));
+            o[1][i] = pack2<BF16>(keep_z(slope.x, BF16), keep_z(slope.y, BF16));
+            o[2][i] = pack2<BF16>(h.x, h.y);
+          }
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) gelu2<BF16>(v[i], v[i + 1]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = act_fwd<ACT, BF16>(v[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= w[i];
-      stage16(stg + 2 * BLOCK_ST, v, BF16);
+          for (int i = KEEP ? 0 : 2; i < 3; ++i)
+            *reinterpret_cast<uint4*>(stg + i * BLOCK_ST + stg_at(lane, k)) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        }
+      };
+      if (e.z) block(std::true_type());
+      else block(std::false_type());
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -650,30 +626,39 @@ __device__ __forceinline__ void column_sums(const unsigned char* stg, float* out
   if (n + 1 < cols) out[n + 1] = mine.y;
 }
 
-// GRAD's epilogue: g and u of a block of 32 rows and 32 columns come to the staging
-// by copies (the first block's while the products are at work), d u act'(g) and
-// d act(g) take their places there and leave.  A lane reads and writes its own row.
-template <int BN, int CG, bool BF16, int ACT>
+// GRAD's epilogue: u act'(g) and act(g) of a block of 32 rows and 32 columns come to
+// the staging by copies, their products with d take their places there and leave.  A
+// lane reads and writes its own row.  Each of a warp's blocks has its own staging, and a
+// tile's are asked for while the tile before it is worked on (one after the other, in
+// one, 25088 x 512 -> 1024 took 62 us).
+template <int BN, int CG, bool BF16>
 __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
-                                              uint32_t tbase, uint64_t* tfull, uint64_t* tfree, uint64_t* here, unsigned char* stg,
+                                              uint32_t tbase, uint64_t* tfull, uint64_t* tfree, uint64_t* here, unsigned char* stg0,
                                               volatile int* abort) {
   using C = GC<BN, CG, GRAD>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, group = warp >> 2;
-  int tl = 0, fetched = 0;
+  auto row_of = [&](const Unit& t) { return (t.mt * CG + (int)rank) * TM + q * 32; };
+  auto col_of = [&](const Unit& t) { return t.nt * BN + group * C::CW; };
+  auto blocks_of = [&](const Unit& t) { return row_of(t) >= a.M || col_of(t) >= a.N ? 0 : col_of(t) + 32 < a.N ? C::NBLK : 1; };
+  auto fetch = [&](const Unit& t, int j) {  // by lane 0, once the copies that left the block's staging have read it
+    unsigned char* stg = stg0 + 2 * j * BLOCK_ST;
+    uint64_t* bar = here + j * EPI_WARPS;
+    mbar_arrive_expect_tx(bar, 2 * BLOCK_ST);
+    tma_load_2d(stg, &maps.res, col_of(t) + 32 * j, row_of(t), bar);
+    tma_load_2d(stg + BLOCK_ST, &maps.b2, col_of(t) + 32 * j, row_of(t), bar);
+  };
+  if (lane == 0)
+    for (int j = 0; j < blocks_of(t); ++j) fetch(t, j);
+  int tl = 0;
+  uint32_t phases = 0;  // of the blocks' barriers
   for (int u = first; u < units; ++tl) {
-    const int acc = tl & 1;
-    const int64_t m0 = (int64_t)(t.mt * CG + (int)rank) * TM + q * 32;
-    const int nb = t.nt * BN + group * C::CW;
-    const bool some = m0 < a.M && nb < a.N;
-    const int blocks = !some ? 0 : nb + 32 < a.N ? C::NBLK : 1;
-    auto fetch = [&](int j) {  // by lane 0
-      bulk_wait_read();        // the last block's copies have read the staging
-      mbar_arrive_expect_tx(here, 2 * BLOCK_ST);
-      tma_load_2d(stg, &maps.res, nb + 32 * j, (int)m0, here);
-      tma_load_2d(stg + BLOCK_ST, &maps.b2, nb + 32 * j, (int)m0, here);
-    };
-    if (lane == 0 && some) fetch(0);
-    __syncwarp();
+    const int acc = tl & 1, blocks = blocks_of(t);
+    const int64_t m0 = row_of(t);
+    const int nb = col_of(t);
+    Unit next = t;
+    const bool more = (u += step) < units;
+    if (more) next = unit_of(a, u);
+    const int then = more ? blocks_of(next) : 0;
     if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
     __syncwarp();
     tc_fence_after();
@@ -681,36 +666,29 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
     for (int j = 0; j < C::NBLK; ++j) {
       if (j >= blocks) break;
       const int n0 = nb + 32 * j;
-      if (j > 0) {
-        if (lane == 0) fetch(j);
-        __syncwarp();
-      }
+      unsigned char* stg = stg0 + 2 * j * BLOCK_ST;
       uint32_t w[32];
       tmem_ld32(tbase + acc * BN + group * C::CW + j * 32 + ((uint32_t)(q * 32) << 16), w);
       tmem_ld_wait();
       if (j + 1 == blocks) give_back<CG>(tfree + acc);
-      if (!wait_for(here, fetched++ & 1, abort)) break;
+      if (!wait_for(here + j * EPI_WARPS, phases >> j & 1, abort)) break;
+      phases ^= 1u << j;
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint4* pg = reinterpret_cast<uint4*>(stg + stg_at(lane, k));
-        uint4* pu = reinterpret_cast<uint4*>(stg + BLOCK_ST + stg_at(lane, k));
-        const uint4 rg = *pg, ru = *pu;
-        const uint32_t gq[4] = {rg.x, rg.y, rg.z, rg.w}, uq[4] = {ru.x, ru.y, ru.z, ru.w};
-        uint32_t og[4], ou[4];
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = unpack2<BF16>(uq[i]);
-          const uint64_t d = (uint64_t)w[8 * k + 2 * i] | (uint64_t)w[8 * k + 2 * i + 1] << 32;
-          uint64_t v, slope;
-          act_both<ACT>(unpack2<BF16>(gq[i]), v, slope);
-          const float2 dg = f2unpack(mul2(mul2(d, f2pack(f.x, f.y)), slope)), du = f2unpack(mul2(d, v));
-          og[i] = pack2<BF16>(dg.x, dg.y);
-          ou[i] = pack2<BF16>(du.x, du.y);
+        for (int h = 0; h < 2; ++h) {
+          uint4* at = reinterpret_cast<uint4*>(stg + h * BLOCK_ST + stg_at(lane, k));
+          const uint4 r = *at;
+          const uint32_t f[4] = {r.x, r.y, r.z, r.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = unpack2<BF16>(f[i]);
+            o[i] = pack2<BF16>(__uint_as_float(w[8 * k + 2 * i]) * c.x, __uint_as_float(w[8 * k + 2 * i + 1]) * c.y);
+          }
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        *pg = make_uint4(og[0], og[1], og[2], og[3]);
-        *pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -723,9 +701,22 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
         column_sums<BF16>(stg, to, a.N - n0);
         column_sums<BF16>(stg + BLOCK_ST, to + (a.M + 31) / 32 * a.N, a.N - n0);
       }
+      // the staging of the block before this one has been read by now, or soon
+      if (j > 0 && lane == 0 && then > j - 1) {
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        fetch(next, j - 1);
+      }
+      __syncwarp();
     }
     if (blocks == 0) give_back<CG>(tfree + acc);
-    if ((u += step) < units) t = unit_of(a, u);
+    if (lane == 0) {
+      // what is not asked for yet: the last block's, and all where this tile had none
+      const int from = blocks == 0 ? 0 : blocks - 1;
+      if (then > from) bulk_wait_read();
+      for (int j = from; j < then; ++j) fetch(next, j);
+    }
+    __syncwarp();
+    t = next;
   }
   if (lane == 0) bulk_wait_read();
 }
@@ -740,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tfree = tfull + 2;
   uint64_t* probe = tfree + 2;
-  uint64_t* rbar = probe + 1;  // [EPI_WARPS] a warp's residual has landed
+  uint64_t* rbar = probe + 1;  // [EPI_WARPS] a warp's residual has landed; [2][EPI_WARPS] what GRAD's two blocks take
   uint32_t* tmem = reinterpret_cast<uint32_t*>(full + C::NBAR);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -876,7 +867,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   } else if (warp < C::ACTIVE) {
     unsigned char* stg = sm + C::OFF_STG + warp * C::STG_W;
     if constexpr (KIND == GATE) gate_epilogue<BN, CG, BF16, ACT>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, stg, abort);
-    else if constexpr (KIND == GRAD) grad_epilogue<BN, CG, BF16, ACT>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, rbar + warp, stg, abort);
+    else if constexpr (KIND == GRAD) grad_epilogue<BN, CG, BF16>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, rbar + warp, stg, abort);
     else {
     const int q = warp & 3, group = warp >> 2;
     const Epi& e = a.e;
@@ -1033,16 +1024,23 @@ __global__ void __launch_bounds__(256) gemm_sum_kernel(const float* __restrict__
 struct Gate {
   const void* bias2;
   int bias2_dt;
-  void* z2;          // beside e.z
+  void* z2;          // u act'(g), beside e.z: act(g)
 };
+__device__ __forceinline__ float act_slope(float z, int act) {
+  return act == OW_ACT_RELU   ? act_slope<OW_ACT_RELU>(z)
+         : act == OW_ACT_SILU ? act_slope<OW_ACT_SILU>(z)
+         : act == OW_ACT_GELU ? act_slope<OW_ACT_GELU>(z)
+                              : 1.f;
+}
 __device__ __forceinline__ void finish_gate(const Epi& e, const Gate& g, float v, float w, int64_t m, int n, int bf) {
   if (e.bias) v += ld_any(e.bias, e.bias_dt, n);
   if (g.bias2) w += ld_any(g.bias2, g.bias2_dt, n);
+  const float a = act_fwd(v, e.act, bf);
   if (e.z) {
-    st16(e.z, m * e.ldz + n, bf, keep_z(v, bf));
-    st16(g.z2, m * e.ldz + n, bf, keep_z(w, bf));
+    st16(e.z, m * e.ldz + n, bf, keep_z(a, bf));
+    st16(g.z2, m * e.ldz + n, bf, keep_z(w * act_slope(v, e.act), bf));
   }
-  st16(e.out, m * e.ldo + n, bf, act_fwd(v, e.act, bf) * w);
+  st16(e.out, m * e.ldo + n, bf, a * w);
 }
 
 // The same for GATE's partials, whose rows hold tiles of ``bn`` columns, half of them of either product.
@@ -1515,9 +1513,9 @@ struct Second {
   Mat a, b;           // CAT_K both, CAT_M a, GATE b
   const void* bias;   // GATE
   int bias_dt;
-  void* c;            // GATE: its z, beside e.z; CAT_M: its output; GRAD: d act(g)
-  const void* g;      // GRAD: rows of e.ldo, as the results'
-  const void* u;
+  void* c;            // GATE: its z, beside e.z; CAT_M: its output; GRAD: d act(g), e.out being d u act'(g)
+  const void* kept;   // GRAD: act(g) and u act'(g), rows of e.ldo, as the results'
+  const void* kept2;
   float* part;        // GRAD: column sums, or NULL
 };
 struct DualWs {
@@ -1588,8 +1586,8 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
     if (KIND == GRAD) {
       k.part = s.part;
       OW_RETURN_IF(block_map(&maps.c2, t16, s.c, M, N, e.ldo, 1));
-      OW_RETURN_IF(block_map(&maps.res, t16, s.g, M, N, e.ldo, 0));
-      OW_RETURN_IF(block_map(&maps.b2, t16, s.u, M, N, e.ldo, 0));
+      OW_RETURN_IF(block_map(&maps.res, t16, s.kept2, M, N, e.ldo, 0));
+      OW_RETURN_IF(block_map(&maps.b2, t16, s.kept, M, N, e.ldo, 0));
     }
     if (KIND == CAT_M) {
       k.out2 = s.c;
@@ -1611,7 +1609,7 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
     if (p.bn == 64) return tile(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     return tile(std::integral_constant<int, 128>(), std::integral_constant<int, 1>());
   };
-  if constexpr (KIND == GATE || KIND == GRAD) {
+  if constexpr (KIND == GATE) {
     switch (e.act) {
       case OW_ACT_RELU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_RELU>())); break;
       case OW_ACT_SILU: OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_SILU>())); break;

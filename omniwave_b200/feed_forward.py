@@ -42,7 +42,8 @@ def gated_feed_forward(x: Tensor, gate_weight: Tensor, up_weight: Tensor, down_w
     serve as they are), the biases ``[F]``, ``[F]`` and ``[N]``, ``residual``
     ``[..., N]``; ``activation`` is ``"silu"``, ``"gelu"`` (by erf), ``"relu"`` or
     ``"none"``.  Types, errors and derivatives as for ``linear.linear``.  The backward
-    holds both projections and their gated product in the compute type.
+    holds the gated product, the activation and its slope times the other projection,
+    each ``[..., F]`` in the compute type.
     """
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:

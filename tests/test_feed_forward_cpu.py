@@ -81,11 +81,11 @@ BAD = [
     (dict(gate_bias_dtype=1), 1, "bias must be"),
     (dict(up_bias_dtype=1), 1, "bias must be"),
     (dict(down_bias_dtype=1), 1, "bias must be"),
-    (dict(g=None), 1, "both or neither"),
+    (dict(act=None), 1, "both or neither"),
     (dict(x=17), 1, "not aligned"),
     (dict(up_weight=17), 1, "not aligned"),
     (dict(h=18), 1, "not aligned"),
-    (dict(u=18), 1, "not aligned"),
+    (dict(slope=18), 1, "not aligned"),
     (dict(gate_bias=18), 1, "not aligned"),
 ]
 
@@ -100,7 +100,7 @@ def test_c_forward_refuses_before_any_cuda_call(over, status, msg):
 
 @pytest.mark.parametrize("over,grads,status,msg", [(o, {}, s, m) for o, s, m in BAD] + [
     (dict(rows=0), {}, 1, "no rows"),
-    (dict(g=None, u=None), {}, 1, "pointer is NULL"),
+    (dict(act=None, slope=None), {}, 1, "pointer is NULL"),
     (dict(x=None), {}, 1, "pointer is NULL"),
     (dict(h=None), {}, 1, "pointer is NULL"),
     (dict(down_weight=None), {}, 1, "pointer is NULL"),

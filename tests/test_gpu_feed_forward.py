@@ -6,7 +6,8 @@ matrix product of 16-bit operands sums exact products in f32, in any order, with
 f32; a 16-bit result is off by half(t) of itself.  The activations are within 8 u
 (|z| + 1) of theirs, gelu's bf16 tail within 4e-4 of itself; slopes change by at
 most 0.8 |dz| (silu'' <= 0.5, gelu'' <= 0.8), values by 1.13 |dz|.  The backward
-holds g and u in 16 bits; dh may be rounded to 16 bits before the gate's formula,
+holds act(g) and u act'(g) in 16 bits, which is no further off than from g and u in
+16 bits (|act(g)| <= |g|); dh may be rounded to 16 bits before the gate's formula,
 and the biases' gradients are sums of dg and du that may have been.
 """
 
