@@ -302,37 +302,50 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.f;
 }
 
-// An activation and its slope at two z, which share what is costly, in pairs: gelu's
-// tail is act_slope's, and the value max(z, 0) - |z| tail.
-template <int ACT>
-__device__ __forceinline__ void act_both(float2 z, uint64_t& a, uint64_t& s) {
-  auto c = [](float v) { return f2pack(v, v); };
-  const uint64_t zz = f2pack(z.x, z.y);
+// The larger of z and 0, NaN where z is.
+__device__ __forceinline__ float max0(float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
+}
+
+// An activation at z and, where it is used, its slope.  gelu is max(z, 0) - |z| tail
+// with the tail of ``gelu``, an operation less than z Phi, and the slope takes Phi from
+// the same tail; beyond the clamp the tail is 0.
+template <int ACT, bool BF16>
+__device__ __forceinline__ void act_both(float z, float& a, float& s) {
   if constexpr (ACT == OW_ACT_SILU) {
-    const float2 x = f2unpack(mul2(zz, c(-1.44269504f)));
-    const float2 y = f2unpack(add2(f2pack(ex2(x.x), ex2(x.y)), c(1.f)));
-    const uint64_t g = f2pack(rcp(y.x), rcp(y.y));
-    a = mul2(zz, g);
-    s = fma2(a, fma2(g, c(-1.f), c(1.f)), g);
+    const float g = sigmoid(z);
+    a = z * g;
+    s = fmaf(a, 1.f - g, g);
   } else if constexpr (ACT == OW_ACT_GELU) {
-    const uint64_t m = f2pack(fabsf(z.x), fabsf(z.y));
-    const float2 x = f2unpack(mul2(mul2(zz, zz), c(-0.72134752f)));
-    const uint64_t e = f2pack(ex2(x.x), ex2(x.y));
-    const float2 y = f2unpack(fma2(m, c(0.35f), c(1.f)));
-    const uint64_t t = f2pack(rcp(y.x), rcp(y.y));
-    uint64_t tail = fma2(t, c(0.0471570618f), c(-0.194429092f));
-    tail = fma2(tail, t, c(0.226878741f));
-    tail = fma2(tail, t, c(-0.00380232154f));
-    tail = fma2(tail, t, c(0.148624128f));
-    tail = fma2(tail, t, c(0.135697883f));
-    tail = mul2(mul2(fma2(tail, t, c(0.139873699f)), t), e);
-    const uint64_t less = mul2(tail, c(-1.f));
-    a = fma2(m, less, f2pack(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y));
-    const float2 u = f2unpack(add2(less, c(1.f))), v = f2unpack(tail);
-    s = fma2(mul2(zz, c(0.39894228040143268f)), e, f2pack(z.x > 0.f ? u.x : v.x, z.y > 0.f ? u.y : v.y));
+    const float x = fminf(fabsf(z), BF16 ? 13.5f : 100.f);
+    float q;
+    if constexpr (BF16) {
+      q = fmaf(x, 3.98267339e-8f, -2.39384553e-6f);
+      q = fmaf(q, x, 6.14833989e-5f);
+      q = fmaf(q, x, -8.9382549e-4f);
+      q = fmaf(q, x, 8.29635281e-3f);
+      q = fmaf(q, x, -5.3509552e-2f);
+      q = fmaf(q, x, -0.458847046f);
+      q = fmaf(q, x, -1.15114152f);
+      q = fmaf(q, x, -1.00000072f);
+    } else {
+      q = fmaf(x, -1.39922733e-7f, 1.43002126e-6f);
+      q = fmaf(q, x, 3.0813193e-5f);
+      q = fmaf(q, x, -7.80530798e-4f);
+      q = fmaf(q, x, 8.10782891e-3f);
+      q = fmaf(q, x, -5.33918403e-2f);
+      q = fmaf(q, x, -0.458847821f);
+      q = fmaf(q, x, -1.15115714f);
+      q = fmaf(q, x, -0.999998868f);
+    }
+    const float tail = ex2(q);
+    a = fmaf(-x, tail, max0(z));
+    s = fmaf(z * 0.39894228040143268f, ex2(z * z * -0.72134752f), z > 0.f ? 1.f - tail : tail);
   } else {
-    a = f2pack(act_fwd<ACT, false>(z.x), act_fwd<ACT, false>(z.y));
-    s = f2pack(act_slope<ACT>(z.x), act_slope<ACT>(z.y));
+    a = act_fwd<ACT, false>(z);
+    s = act_slope<ACT>(z);
   }
 }
 
@@ -450,17 +463,18 @@ __device__ __forceinline__ void stage_res(unsigned char* stg, const Epi& e, int6
   __syncwarp();
 }
 
-__device__ __forceinline__ void add_bias(float (&v)[32], const void* bias, int bias_dt, int n0, int N) {
-  if (n0 + 32 <= N && bias_dt == OW_DTYPE_F32 && ((uintptr_t)bias & 15) == 0) {
+template <int C>
+__device__ __forceinline__ void add_bias(float (&v)[C], const void* bias, int bias_dt, int n0, int N) {
+  if (n0 + C <= N && bias_dt == OW_DTYPE_F32 && ((uintptr_t)bias & 15) == 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < C / 4; ++i) {
       const float4 b = __ldg(reinterpret_cast<const float4*>((const float*)bias + n0) + i);
       v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
     }
-  } else if (n0 + 32 <= N && bias_dt != OW_DTYPE_F32 && ((uintptr_t)bias & 15) == 0) {
+  } else if (n0 + C <= N && bias_dt != OW_DTYPE_F32 && ((uintptr_t)bias & 15) == 0) {
     const int bf = bias_dt == OW_DTYPE_BF16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < C / 8; ++i) {
       const uint4 b = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)bias + n0) + i);
       const uint32_t q[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -472,7 +486,7 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const void* bias, int b
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < C; ++i)
       if (n0 + i < N) v[i] += ld_any(bias, bias_dt, n0 + i);
   }
 }
@@ -540,52 +554,63 @@ __device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs&
     if (!wait_for(tfull + acc, (tl >> 1) & 1, abort)) break;
     __syncwarp();
     tc_fence_after();
-    float v[32], w[32];  // the gate, its factor
-    if (some) {
-      uint32_t c[2][32];
-      const uint32_t at = tbase + acc * BN + group * 32 + ((uint32_t)(q * 32) << 16);
-      tmem_ld32(at, c[0]);
-      tmem_ld32(at + BN / 2, c[1]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        v[i] = __uint_as_float(c[0][i]);
-        w[i] = __uint_as_float(c[1][i]);
-      }
-    }
-    give_back<CG>(tfree + acc);
+    const uint32_t at = tbase + acc * BN + group * 32 + ((uint32_t)(q * 32) << 16);
     if (lane == 0) bulk_wait_read();  // the staging is free once the last tile's copies have read it
     __syncwarp();
-    if (some && a.raw) {
+    if (!some) {
+      give_back<CG>(tfree + acc);
+    } else if (a.raw) {
       const int nv = t.nt * BN + group * 32, all = a.ntiles * BN;
-      put32(stg, v, &maps.out, true, nullptr, 0, m0, a.M, nv, all, t.split);
-      put32(stg, w, &maps.out, true, nullptr, 0, m0, a.M, nv + BN / 2, all, t.split);
-    } else if (some) {
-      if (e.bias) add_bias(v, e.bias, e.bias_dt, n0, a.N);
-      if (a.bias2) add_bias(w, a.bias2, a.bias2_dt, n0, a.N);
-      auto block = [&](auto keep) {
-        constexpr bool KEEP = decltype(keep)::value;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t o[3][4];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t c[32];
+        tmem_ld32(at + h * (BN / 2), c);
+        tmem_ld_wait();
+        if (h == 1) give_back<CG>(tfree + acc);
+        float v[32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = 8 * k + 2 * i;
-            uint64_t x, y;
-            act_both<ACT>(make_float2(v[j], v[j + 1]), x, y);
-            const uint64_t f = f2pack(w[j], w[j + 1]);
-            const float2 act = f2unpack(x), slope = f2unpack(mul2(y, f)), h = f2unpack(mul2(x, f));
-            o[0][i] = pack2<BF16>(keep_z(act.x, BF16), keep_z(act.y, BF16));
-            o[1][i] = pack2<BF16>(keep_z(slope.x, BF16), keep_z(slope.y, BF16));
-            o[2][i] = pack2<BF16>(h.x, h.y);
-          }
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(c[i]);
+        put32(stg, v, &maps.out, true, nullptr, 0, m0, a.M, nv + h * (BN / 2), all, t.split);
+      }
+    } else {
 #pragma unroll
-          for (int i = KEEP ? 0 : 2; i < 3; ++i)
-            *reinterpret_cast<uint4*>(stg + i * BLOCK_ST + stg_at(lane, k)) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+      for (int h = 0; h < 2; ++h) {  // 16 columns at a time, which the registers hold beside the arithmetic
+        uint32_t c[2][16];
+        tmem_ld16(at + 16 * h, c[0]);
+        tmem_ld16(at + BN / 2 + 16 * h, c[1]);
+        tmem_ld_wait();
+        if (h == 1) give_back<CG>(tfree + acc);
+        float v[16], w[16];  // the gate, its factor
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          v[i] = __uint_as_float(c[0][i]);
+          w[i] = __uint_as_float(c[1][i]);
         }
-      };
-      if (e.z) block(std::true_type());
-      else block(std::false_type());
+        if (e.bias) add_bias(v, e.bias, e.bias_dt, n0 + 16 * h, a.N);
+        if (a.bias2) add_bias(w, a.bias2, a.bias2_dt, n0 + 16 * h, a.N);
+        auto block = [&](auto keep) {
+          constexpr bool KEEP = decltype(keep)::value;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t o[3][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = 8 * k + 2 * i;
+              float a0, s0, a1, s1;
+              act_both<ACT, BF16>(v[j], a0, s0);
+              act_both<ACT, BF16>(v[j + 1], a1, s1);
+              o[0][i] = pack2<BF16>(keep_z(a0, BF16), keep_z(a1, BF16));
+              o[1][i] = pack2<BF16>(keep_z(s0 * w[j], BF16), keep_z(s1 * w[j + 1], BF16));
+              o[2][i] = pack2<BF16>(a0 * w[j], a1 * w[j + 1]);
+            }
+#pragma unroll
+            for (int i = KEEP ? 0 : 2; i < 3; ++i)
+              *reinterpret_cast<uint4*>(stg + i * BLOCK_ST + stg_at(lane, 2 * h + k)) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+          }
+        };
+        if (e.z) block(std::true_type());
+        else block(std::false_type());
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
