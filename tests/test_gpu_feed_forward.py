@@ -357,6 +357,59 @@ def test_captured_and_on_another_stream(cuda_device):
         assert all(torch.equal(p, q) for p, q in zip(outs, once()))
 
 
+def test_a_wait_that_gives_up_is_reported(cuda_device):
+    from omniwave_b200 import _lib
+
+    a, dy = _inputs(cuda_device, 300, 128, 96, 64, BF, seed=7)
+    leaves = {key: v.detach().requires_grad_() for key, v in a.items()}
+
+    def once():
+        y = _run(leaves, "silu")
+        return (y.detach(), *torch.autograd.grad(y, list(leaves.values()), dy))
+
+    want = once()
+    lib = _lib.load()
+    try:
+        assert lib.ow_debug_wait_probe(1_000_000) == 0
+        once()
+        torch.cuda.synchronize()
+    finally:
+        lib.ow_debug_wait_probe(0)
+    assert _lib.device_fault(0, reset=True) == 1
+    assert all(torch.equal(p, q) for p, q in zip(once(), want))
+
+
+def test_two_threads(cuda_device):
+    """Calls from two threads on streams of their own, forward and backward."""
+    import threading
+
+    cases = [_inputs(cuda_device, m, 128, 200, 64, BF, seed=m) for m in (40, 700)]
+
+    def once(a, dy):
+        leaves = {key: v.detach().requires_grad_() for key, v in a.items()}
+        y = _run(leaves, "gelu")
+        return (y.detach(), *torch.autograd.grad(y, list(leaves.values()), dy))
+
+    want = [once(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = once(*cases[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 class _Net(torch.nn.Module):
     """norm -> feed-forward -> residual, twice, and a head: the operators as a model has them."""
 

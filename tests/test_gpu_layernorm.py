@@ -272,3 +272,58 @@ def test_captured_and_on_another_stream(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(outs, once()))
+
+
+def test_past_two_to_the_31_elements(cuda_device):
+    n, c = 2_200_000, 1000  # 4.4 GB in 16 bits
+    x = torch.empty(n, c, dtype=BF, device=cuda_device)
+    x[:] = torch.randn(c, device=cuda_device).to(BF)
+    x[-40:] = torch.randn(40, c, device=cuda_device).to(BF)
+    w, b = torch.randn(c, device=cuda_device), torch.randn(c, device=cuda_device)
+    leaf = x.requires_grad_()
+    y = norm.layer_norm(leaf, w, b)
+    pick = torch.tensor([0, 1, n // 2, *range(n - 41, n)], device=cuda_device)
+    dn = torch.zeros_like(x)
+    dn[pick] = torch.randn(len(pick), c, device=cuda_device).to(BF)
+    (dx,) = torch.autograd.grad(y, leaf, dn)
+    want, tol = _define(x.detach()[pick], w, b, dn[pick], 1e-5)
+    _ok(y.detach()[pick], want["n"], tol["n"], "n")
+    _ok(dx[pick], want["dx"], tol["dx"], "dx")
+    rest = torch.ones(n, dtype=torch.bool, device=cuda_device)
+    rest[pick] = False
+    assert not dx[rest][:: 1000].any()
+
+
+def test_two_captured_graphs_and_a_wait_that_gives_up(cuda_device):
+    """Two graphs replayed in turn do not share what they work in; a wait that runs out is reported, and the next call is right."""
+    from omniwave_b200 import _lib
+
+    x, w, b, dn = _inputs(cuda_device, (4000, 1024), BF, F32, seed=10)
+    dn = dn.to(BF)
+
+    def once(t):
+        leaves = [v.detach().requires_grad_() for v in (t, w, b)]
+        n = norm.layer_norm(*leaves)
+        return (n.detach(), *torch.autograd.grad(n, leaves, dn))
+
+    want = [once(x), once(x * 2)]
+    graphs, outs = [], []
+    y = x * 2
+    for t in (x, y):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(once(t))
+        graphs.append(g)
+    for i in (0, 1, 0):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs[i], want[i]))
+    lib = _lib.load()
+    try:
+        assert lib.ow_debug_wait_probe(1_000_000) == 0
+        once(x)
+        torch.cuda.synchronize()
+    finally:
+        lib.ow_debug_wait_probe(0)
+    assert _lib.device_fault(0, reset=True) == 1
+    assert all(torch.equal(p, q) for p, q in zip(once(x), want[0]))

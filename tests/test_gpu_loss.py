@@ -320,3 +320,31 @@ def test_captured_and_on_another_stream(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(outs, once()))
+
+
+def test_padding_by_zero_class_and_by_lowest_value(cuda_device):
+    """Entries padded with class 0 at -inf, or at the type's lowest value, take nothing off class 0."""
+    for v, k in ((200, 40), (9000, 300)):
+        z, top, cls, y = _inputs(cuda_device, 20, v, k, BF, HF, seed=13, ragged=False)
+        for fill in (float("-inf"), torch.finfo(HF).min):
+            t, c = top.clone(), cls.clone()
+            t[:, k // 3:], c[:, k // 3:] = fill, 0
+            short = _both(z, top[:, :k // 3], cls[:, :k // 3], y, 2.0, 0.5, "none", "short")
+            leaf = z.detach().requires_grad_()
+            rows = loss.distill_loss(leaf, t, c, y, temperature=2.0, weight=0.5, reduction="none")
+            (g,) = torch.autograd.grad(rows, leaf, torch.ones_like(rows))
+            want, tol, dz, edz = _define(z, top[:, :k // 3], cls[:, :k // 3], y, 2.0, 0.5, "none")
+            assert ((rows.detach().double() - want).abs() <= tol + U * want.abs()).all()
+            assert ((g.double() - dz).abs() <= edz).all()
+            assert torch.allclose(rows.detach(), short[0], rtol=1e-5)
+
+
+def test_all_entries_one_class(cuda_device):
+    """1024 entries of one class: p is spread over them, so sum p (log p - log q) is the class's -log q less p's entropy."""
+    for v in (30, 3000):
+        z, _, _, y = _inputs(cuda_device, 5, v, 3, F32, seed=14, ragged=False)
+        cls, t = torch.full((5, 1024), 7, device=cuda_device), torch.randn(5, 1024, device=cuda_device)
+        rows, g = _both(z, t, cls, y, 1.0, 1.0, "none", "one class")
+        entropy = -(t.softmax(1) * t.log_softmax(1)).sum(1)
+        one = loss.distill_loss(z, t[:, :1], cls[:, :1], y, weight=1.0, reduction="none")
+        assert torch.allclose(rows + entropy, one, rtol=1e-5, atol=1e-5)
