@@ -1019,8 +1019,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
 }
 
 // Adds the split-k partials of [M, N] (row stride ld) in order and finishes.
+// blockIdx.y: the second of CAT_M's results, whose partials are ``second`` floats on.
 __global__ void __launch_bounds__(256) gemm_sum_kernel(const float* __restrict__ part, int splits, int64_t stride, int64_t ld,
-                                                       int64_t M, int N, const Epi e) {
+                                                       int64_t M, int N, Epi e, void* out2, int64_t second) {
+  if (blockIdx.y) {
+    part += second;
+    e.out = out2;
+  }
   const int64_t nv = (N + 3) / 4, total = M * nv;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t m = i / nv;
@@ -1527,7 +1532,7 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   if (p.splits > 1) {
     const int64_t total = M * ((N + 3) / 4);
     const int g2 = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);
-    launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, M * w.part_ld, w.part_ld, M, N, e);
+    launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, M * w.part_ld, w.part_ld, M, N, e, nullptr, 0);
     OW_CHECK_LAUNCH("gemm_sum_kernel");
   }
   return OW_OK;
@@ -1651,13 +1656,9 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
       launch(gate_sum_kernel, blocks(M * N), 256, 0, st, (const float*)w.part, p.splits, stride, w.part_ld, p.bn, M, N, e,
              Gate{s.bias, s.bias_dt, s.c});
     } else {
-      const int64_t step = stride * (KIND == CAT_M ? 2 : 1);
-      launch(gemm_sum_kernel, blocks(M * ((N + 3) / 4)), 256, 0, st, (const float*)w.part, p.splits, step, w.part_ld, M, N, e);
-      if (KIND == CAT_M) {
-        Epi e2 = e;
-        e2.out = s.c;
-        launch(gemm_sum_kernel, blocks(M * ((N + 3) / 4)), 256, 0, st, (const float*)w.part + stride, p.splits, step, w.part_ld, M, N, e2);
-      }
+      const int both = KIND == CAT_M ? 2 : 1;
+      launch(gemm_sum_kernel, dim3(blocks(M * ((N + 3) / 4)), both), 256, 0, st, (const float*)w.part, p.splits, stride * both, w.part_ld,
+             M, N, e, s.c, stride);
     }
     OW_CHECK_LAUNCH("gemm_sum_kernel");
   }
