@@ -25,6 +25,11 @@
 //
 // A row is a warp's, or a block's, of which the last warp has the teacher's entries
 // while the others have the logits: its loads depend on one another.
+//
+// Measured (B200, device time in a CUDA graph): 4096 x 32000 bf16, T = 2, 64 entries,
+// forward 65 us (4.1 TB/s; issue slots, half of them taken, and rows that end together)
+// and backward 85 (6.2 TB/s, HBM); 1531 x 40009 f16 forward 30; 128 x 1000 5.7 and 6.2.
+// Asking for a row's vectors ahead, across rows too, cost a fourth of the blocks and 6 us.
 #include <algorithm>
 #include <type_traits>
 

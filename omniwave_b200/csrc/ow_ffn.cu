@@ -13,7 +13,14 @@
 // h, dg and du are held in 16 bits because the tensor core takes no other; act(g) and
 // u act'(g), which the backward multiplies dh with, for their traffic.  Each is rounded
 // once, and so dWg is off by what three roundings make, its own among them: 0.0029 of
-// its norm in bf16, where its own makes 0.0017.
+// its norm in bf16, where its own makes 0.0017.  gate's and up's bias gradients are f32
+// sums of dg and du as they are rounded.
+//
+// Bound and measured (B200, device time in a CUDA graph): the tensor pipe under the
+// power cap for 16384 x 4096 x 8192, forward 2120 to 2280 us, with the backward 7.6 to
+// 8.1 ms (1230 to 1310 TFLOP/s); with k of 512 the epilogues (25088 x 512 x 1024 gelu,
+// biases and residual 78 and 286 us); 12544 x 1024 x 2048 f16 silu forward 127 us; one
+// token 1024 -> 2048 -> 1024 6.8 us, 12.6 MB at 1.9 TB/s in two launches.
 #include "ow_gemm.cuh"
 
 namespace ow {
@@ -321,7 +328,11 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
     e.out = b.dg; e.ldo = ld; e.vo = 1;
     Second s{};
     s.c = b.du; s.kept = a->act; s.kept2 = a->slope; s.part = b.bias;
-    OW_RETURN_IF((gemm_dual<GRAD, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)));
+    // Up to 8 blocks of k a tile's epilogue takes longer than its products (25088 x 512 -> 1024 52 us, and 62 with the
+    // other; with 16 blocks, 12544 x 1024 -> 2048, 83 and 74).
+    const bool brief = blocks_of(a->out_features) <= 8;
+    OW_RETURN_IF((brief ? gemm_dual<GRAD, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)
+                        : gemm_dual<GRAD_LONG, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)));
   } else {
     const GradArgs k{b.dh, a->act, a->slope, b.dg, b.du, b.bias, M, ld, b.chunk, F, F % 8 == 0};
     launch(bf ? gate_grad_kernel<true> : gate_grad_kernel<false>, dim3((F + 255) / 256, b.chunks), 256, 0, st, k);

@@ -29,8 +29,10 @@ constexpr int PATCH = 12;
 // epilogue joins them: act(A B1^T + b1) (A B2^T + b2).  CAT_K: the sum of two
 // products, the second's k blocks behind the first's.  CAT_M: two products with the
 // same B, the second's tiles behind the first's.  GRAD: one product d, whose epilogue
-// reads what GATE kept, act(g) and u act'(g), and writes d times either.
-enum Kind { PLAIN, GATE, CAT_K, CAT_M, GRAD };
+// reads what GATE kept, act(g) and u act'(g), and writes d times either; GRAD_LONG is
+// the same for long k, with more of shared memory for the operands.
+enum Kind { PLAIN, GATE, CAT_K, CAT_M, GRAD, GRAD_LONG };
+constexpr bool is_grad(int kind) { return kind == GRAD || kind == GRAD_LONG; }
 
 // BN columns of a tile; CG CTAs share it (2: 256 rows, BN / 2 rows of B each).
 template <int BN, int CG, int KIND = PLAIN>
@@ -40,10 +42,11 @@ struct GC {
   static constexpr int CW = KIND == GATE ? 64 : BN == 256 ? 64 : 32;   // columns of an epilogue warp
   static constexpr int NBLK = CW / 32;
   static constexpr int ACTIVE = 4 * (BN / CW);     // epilogue warps at work
-  // blocks of staging a warp: GATE three (its results leave together), GRAD two for each of its blocks (what comes in
-  // and goes out in its place)
-  static constexpr int STG_W = (KIND == GATE ? 3 : KIND == GRAD ? 2 * NBLK : NBLK) * BLOCK_ST;
-  static constexpr int STAGES = BN == 256 ? (KIND == GATE ? 4 : KIND == GRAD ? 3 : 5) : BN == 128 ? (KIND == GATE || KIND == GRAD ? 5 : 6) : 8;
+  // blocks of staging a warp: GATE three (its results leave together), GRAD two (what comes in and goes out in its
+  // place) for each of its blocks, GRAD_LONG for all
+  static constexpr int SETS = KIND == GRAD ? NBLK : 1;
+  static constexpr int STG_W = (KIND == GATE ? 3 : is_grad(KIND) ? 2 * SETS : NBLK) * BLOCK_ST;
+  static constexpr int STAGES = BN == 256 ? (KIND == GATE ? 4 : KIND == GRAD ? 3 : 5) : BN == 128 ? (KIND == GATE || is_grad(KIND) ? 5 : 6) : 8;
   static constexpr int B_ST = B_ROWS * 128;
   static constexpr int OFF_B = STAGES * A_ST;
   static constexpr int OFF_STG = OFF_B + STAGES * B_ST;
@@ -537,8 +540,12 @@ __device__ __forceinline__ void give_back(uint64_t* tfree) {
 // backward it keeps what that multiplies dh with, act(g) and u act'(g), rounded once
 // each, rather than g and u: the slope costs less here, next to the activation, and
 // the backward's epilogue is left with two products.  The three results are staged side
-// by side and leave together (one after the other, each waiting for the staging,
-// 25088 x 512 -> 1024 gelu took 74.5 us, and 61 so, with g and u).
+// by side and leave together, 16 columns at a time, which the registers hold beside the
+// arithmetic.  With k of 512 the arithmetic of an epilogue is what a tile takes: 25088 x
+// 512 -> 1024 gelu, with biases, 70 us and 43 with nothing kept, where the products
+// alone take 32 (all 32 columns at once, spilling, 81; each result waiting for the one
+// before it, 74 with gelu alone; written through the load and store units in the place
+// of TMA, 78).
 template <int BN, int CG, bool BF16, int ACT>
 __device__ __forceinline__ void gate_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
                                               uint32_t tbase, uint64_t* tfull, uint64_t* tfree, unsigned char* stg,
@@ -653,29 +660,33 @@ __device__ __forceinline__ void column_sums(const unsigned char* stg, float* out
 
 // GRAD's epilogue: u act'(g) and act(g) of a block of 32 rows and 32 columns come to
 // the staging by copies, their products with d take their places there and leave.  A
-// lane reads and writes its own row.  Each of a warp's blocks has its own staging, and a
-// tile's are asked for while the tile before it is worked on (one after the other, in
-// one, 25088 x 512 -> 1024 took 62 us).
-template <int BN, int CG, bool BF16>
+// lane reads and writes its own row.  With short k a tile's time is the epilogue's: each
+// of a warp's blocks has its own staging, and a tile's are asked for while the tile
+// before it is worked on (25088 x 512 -> 1024 52 us, where its traffic takes 36; all in
+// one staging 62; 8 warps with blocks of 64 columns 76; by the load and store units, with
+// gelu, 109 and TMA 76).  That leaves three stages for the operands, which long k does
+// not bear (16384 x 4096 -> 8192 1227 us, and 834 to 960 with five and one staging).
+template <int BN, int CG, bool BF16, int KIND>
 __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs& a, Unit t, uint32_t rank, int first, int step, int units,
                                               uint32_t tbase, uint64_t* tfull, uint64_t* tfree, uint64_t* here, unsigned char* stg0,
                                               volatile int* abort) {
-  using C = GC<BN, CG, GRAD>;
+  using C = GC<BN, CG, KIND>;
+  constexpr int SETS = C::SETS;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, group = warp >> 2;
   auto row_of = [&](const Unit& t) { return (t.mt * CG + (int)rank) * TM + q * 32; };
   auto col_of = [&](const Unit& t) { return t.nt * BN + group * C::CW; };
   auto blocks_of = [&](const Unit& t) { return row_of(t) >= a.M || col_of(t) >= a.N ? 0 : col_of(t) + 32 < a.N ? C::NBLK : 1; };
   auto fetch = [&](const Unit& t, int j) {  // by lane 0, once the copies that left the block's staging have read it
-    unsigned char* stg = stg0 + 2 * j * BLOCK_ST;
-    uint64_t* bar = here + j * EPI_WARPS;
+    unsigned char* stg = stg0 + 2 * (j % SETS) * BLOCK_ST;
+    uint64_t* bar = here + (j % SETS) * EPI_WARPS;
     mbar_arrive_expect_tx(bar, 2 * BLOCK_ST);
     tma_load_2d(stg, &maps.res, col_of(t) + 32 * j, row_of(t), bar);
     tma_load_2d(stg + BLOCK_ST, &maps.b2, col_of(t) + 32 * j, row_of(t), bar);
   };
   if (lane == 0)
-    for (int j = 0; j < blocks_of(t); ++j) fetch(t, j);
+    for (int j = 0; j < min(SETS, blocks_of(t)); ++j) fetch(t, j);
   int tl = 0;
-  uint32_t phases = 0;  // of the blocks' barriers
+  uint32_t phases = 0;  // of the stagings' barriers
   for (int u = first; u < units; ++tl) {
     const int acc = tl & 1, blocks = blocks_of(t);
     const int64_t m0 = row_of(t);
@@ -691,13 +702,13 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
     for (int j = 0; j < C::NBLK; ++j) {
       if (j >= blocks) break;
       const int n0 = nb + 32 * j;
-      unsigned char* stg = stg0 + 2 * j * BLOCK_ST;
+      unsigned char* stg = stg0 + 2 * (j % SETS) * BLOCK_ST;
       uint32_t w[32];
       tmem_ld32(tbase + acc * BN + group * C::CW + j * 32 + ((uint32_t)(q * 32) << 16), w);
       tmem_ld_wait();
       if (j + 1 == blocks) give_back<CG>(tfree + acc);
-      if (!wait_for(here + j * EPI_WARPS, phases >> j & 1, abort)) break;
-      phases ^= 1u << j;
+      if (!wait_for(here + (j % SETS) * EPI_WARPS, phases >> (j % SETS) & 1, abort)) break;
+      phases ^= 1u << (j % SETS);
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -726,19 +737,24 @@ __device__ __forceinline__ void grad_epilogue(const Maps2& maps, const GemmArgs&
         column_sums<BF16>(stg, to, a.N - n0);
         column_sums<BF16>(stg + BLOCK_ST, to + (a.M + 31) / 32 * a.N, a.N - n0);
       }
-      // the staging of the block before this one has been read by now, or soon
-      if (j > 0 && lane == 0 && then > j - 1) {
-        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        fetch(next, j - 1);
+      if constexpr (SETS > 1) {
+        // the staging of the block before this one has been read by now, or soon
+        if (j > 0 && lane == 0 && then > j - 1) {
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          fetch(next, j - 1);
+        }
+      } else if (lane == 0 && j + 1 < blocks) {
+        bulk_wait_read();
+        fetch(t, j + 1);
       }
       __syncwarp();
     }
     if (blocks == 0) give_back<CG>(tfree + acc);
     if (lane == 0) {
       // what is not asked for yet: the last block's, and all where this tile had none
-      const int from = blocks == 0 ? 0 : blocks - 1;
-      if (then > from) bulk_wait_read();
-      for (int j = from; j < then; ++j) fetch(next, j);
+      const int from = SETS == 1 || blocks == 0 ? 0 : blocks - 1, to = min(SETS, then);
+      if (to > from) bulk_wait_read();
+      for (int j = from; j < to; ++j) fetch(next, j);
     }
     __syncwarp();
     t = next;
@@ -892,7 +908,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   } else if (warp < C::ACTIVE) {
     unsigned char* stg = sm + C::OFF_STG + warp * C::STG_W;
     if constexpr (KIND == GATE) gate_epilogue<BN, CG, BF16, ACT>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, stg, abort);
-    else if constexpr (KIND == GRAD) grad_epilogue<BN, CG, BF16>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, rbar + warp, stg, abort);
+    else if constexpr (is_grad(KIND)) grad_epilogue<BN, CG, BF16, KIND>(maps, a, t, rank, first, step, units, tbase, tfull, tfree, rbar + warp, stg, abort);
     else {
     const int q = warp & 3, group = warp >> 2;
     const Epi& e = a.e;
@@ -1613,7 +1629,7 @@ int gemm_dual(Mat A, Mat B, Second s, int64_t M, int N, int64_t K, const Plan& p
       if (e.z) OW_RETURN_IF(block_map(&maps.z, t16, e.z, M, N, e.ldz, 1));
       if (e.z) OW_RETURN_IF(block_map(&maps.c2, t16, s.c, M, N, e.ldz, 1));
     }
-    if (KIND == GRAD) {
+    if (is_grad(KIND)) {
       k.part = s.part;
       OW_RETURN_IF(block_map(&maps.c2, t16, s.c, M, N, e.ldo, 1));
       OW_RETURN_IF(block_map(&maps.res, t16, s.kept2, M, N, e.ldo, 0));
