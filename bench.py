@@ -102,8 +102,8 @@ def _kernel_flops(name: str, b: int, h: int, w: int, c: int, d: int) -> float:
 _KERNEL_SRC = {"tc_bwd_kernel": "ow_tc_bwd.cu", "tc_pack_kernel": "ow_tc_bwd.cu", "tcf_kernel": "ow_tcf.cu",
                "tc_fwd_kernel": "ow_tc.cu", "tc_fwd_gather_kernel": "ow_tcf.cu"}
 _TRAFFIC = {
-    ("tc_bwd_kernel", "56x56x128/radix1", 128): (2 * (543.642368e6 + 95.328768e6), "193297c62c2ff48268c6fdac3b25b0efc23d60fc296045182fdeb114a282b42b"),
-    ("tc_bwd_kernel", "56x56x128/radix2", 128): (2 * (541.888000e6 + 93.432576e6), "193297c62c2ff48268c6fdac3b25b0efc23d60fc296045182fdeb114a282b42b"),
+    ("tc_bwd_kernel", "56x56x128/radix1", 128): (2 * (541.665280e6 + 94.068480e6), "7782aa9e1a43f15bc35f8140e2be93189578a1af94896019ec75baf82ee1ced2"),
+    ("tc_bwd_kernel", "56x56x128/radix2", 128): (2 * (543.121408e6 + 95.214592e6), "7782aa9e1a43f15bc35f8140e2be93189578a1af94896019ec75baf82ee1ced2"),
 }
 
 
