@@ -23,7 +23,7 @@
 // Bound and measured (B200, device time in a CUDA graph): HBM.  401408 x 128, f32 in
 // and bf16 out, forward 53 us (5.8 TB/s) and with the backward 142 (82 of it the
 // backward's, 6.2 TB/s); 50176 x 1024 bf16 41 and 102 us (5.0 TB/s, the backward 62);
-// 12544 x 4096 38 and 100.  Rows of single channels are bound by instructions: 50176 x
+// 12544 x 4096 38 and 99.  Rows of single channels are bound by instructions: 50176 x
 // 777 bf16 72 and 157 us.  One token of 1024 2.1 us.  Without the ring (every row
 // straight from global memory, 8 channels a thread) these were 58 and 244, 64 and 236,
 // 74 and 270, 174 and 594 us.

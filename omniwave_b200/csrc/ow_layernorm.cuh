@@ -357,10 +357,13 @@ constexpr int LONG = 8192;  // channels a row may have in the register kernels
 template <class F>
 int split_stream(int C, F&& f) {
 #define OW_SPLIT(G, E) return f(std::integral_constant<int, G>(), std::integral_constant<int, E>())
-  if (C % 8) {  // by single channels, in fewer splits: what they cost is not idle threads
+  if (C % 8) {  // by single channels, in fewer splits; a thread's idle channels cost it their instructions
     if (C <= 64) OW_SPLIT(8, 8);
     if (C <= 256) OW_SPLIT(16, 16);
+    if (C <= 512) OW_SPLIT(32, 16);
     if (C <= 1024) OW_SPLIT(32, 32);
+    if (C <= 2048) OW_SPLIT(64, 32);
+    if (C <= 4096) OW_SPLIT(128, 32);
     OW_SPLIT(256, 32);
   }
   if (C <= 32) OW_SPLIT(4, 8);
@@ -441,7 +444,7 @@ int run_stream(const Args& k, int* grid, cudaStream_t st, F&& kernel_of) {
     };
     constexpr int g = G.value, e = E.value;
     if (k.C % 8 == 0) return k.C == g * e ? types(std::integral_constant<int, 16>()) : types(std::integral_constant<int, 8>());
-    if constexpr ((g == 8 && e == 8) || (g == 16 && e == 16) || (g == 32 && e == 32) || (g == 256 && e == 32))
+    if constexpr ((g == 8 && e == 8) || (g == 16 && e == 16) || (g == 32 && e == 16) || (g >= 32 && e == 32))
       return types(std::integral_constant<int, 1>());
     return OW_ERR_INVALID;  // not a split of such rows
   });

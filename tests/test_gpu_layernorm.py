@@ -134,6 +134,21 @@ def test_larger(cuda_device, shape, t):
     assert all(torch.equal(p, q) for p, q in zip(first, second))  # bit for bit
 
 
+@pytest.mark.parametrize("shape", [(100_001, 25), (50_000, 56), (40_003, 70), (20_001, 131), (9001, 311), (10_000, 400), (4001, 777),
+                                   (3001, 888), (2600, 1000), (1701, 1501), (1301, 2000), (1001, 3001), (901, 3504), (501, 5001),
+                                   (403, 7016)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("t,out", [(F32, F32), (F32, HF), (BF, BF), (HF, HF)], ids=["f32", "f32-f16", "bf16", "f16"])
+def test_many_rows(cuda_device, shape, t, out):
+    """Rows enough for the streaming kernels: whole vectors, part of a split, single channels, a last unit that is not whole."""
+    x, w, b, dn = _inputs(cuda_device, shape, t, F32, seed=11)
+    first = _both(x, w, b, dn, str(shape), out=out)
+    assert all(torch.equal(p, q) for p, q in zip(first, _both(x, w, b, dn, str(shape), out=out)))
+    # the bytes around the arrays' ends are nobody's business: a view that ends inside a larger array
+    flat = torch.full((x.numel() + 64,), float("nan"), dtype=t, device=cuda_device)
+    inner = flat[:x.numel()].view(shape).copy_(x)
+    assert torch.equal(norm.layer_norm(inner, w, b, out_dtype=out), norm.layer_norm(x, w, b, out_dtype=out))
+
+
 def test_rows_far_from_zero(cuda_device):
     """The variance survives a mean a thousand times the deviation, and one channel a thousand times the others."""
     for c in (64, 777, 1024):
