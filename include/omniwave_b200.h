@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define OW_ABI_VERSION 7
+#define OW_ABI_VERSION 8
 
 #if defined(__GNUC__)
 #define OW_API __attribute__((visibility("default")))
@@ -688,7 +688,7 @@ OW_API int ow_ffn_bwd(const ow_ffn_t* args, const ow_ffn_grads_t* grads, void* s
  * times that of hard.  weight 0 leaves soft out, 1 hard.
  *
  * All in f32, sums over rows in f64, in a fixed order.  The forward leaves in
- * stats [3 rows] and factors [2] (not with NONE) what the backward takes, which
+ * stats [5 rows] and factors [2] (not with NONE) what the backward takes, which
  * writes dlogits [rows, classes] of logits' dtype from dloss ([rows] with NONE,
  * else [1]).
  */

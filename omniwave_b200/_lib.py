@@ -16,7 +16,7 @@ import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libomniwave_b200.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DTYPE_CODE = {
     torch.float32: 0,

@@ -754,7 +754,7 @@ std::tuple<Tensor, Tensor, Tensor> distill_forward(const DistillCall& k, at::Int
   const int64_t rows = k.logits.size(0);
   if (rows == 0) return {at::zeros(shape, f32), Tensor(), Tensor()};
   const c10::cuda::CUDAGuard guard(k.logits.device());
-  const Tensor loss = at::empty(shape, f32), stats = at::empty({3, rows}, f32);
+  const Tensor loss = at::empty(shape, f32), stats = at::empty({5, rows}, f32);
   Tensor factors;
   if (k.reduction != OW_REDUCE_NONE) factors = at::empty({2}, f32);
   ow_distill_t a = k.args(stats, factors);

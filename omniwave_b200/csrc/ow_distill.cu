@@ -7,10 +7,13 @@
 //   loss = weight soft + (1 - weight) hard            (mean, sum or row by row)
 //   dz   = a T (q_T - sum_j p_j [c_j]) + b (q_1 - [label])
 // with a and b the factors of soft and hard in the loss times its gradient.
-// All in f32, exponentials to the base of 2: with k = log2(e), the row's largest
-// logit m and mk = m k,
-//   s = sum 2^(z k - mk),   log q = (z k - mk - log2 s) / k
-// where z k - mk is one rounding and the rounding of mk drops out.
+// All in f32, exponentials to the base of 2: with k = log2(e) and the row's largest
+// logit m,
+//   s = sum 2^((z - m) k),   log q = ((z - m) k - log2 s) / k
+// where z - m comes first: a softmax does not hang on what its logits have in common,
+// and z k - m k would lose as many of its bits as that has, and overflow where z is its
+// type's lowest value (a class masked so is 2^-inf = 0).  A row's own terms, which the
+// sums leave out, are in 64 bits.
 //
 // The forward reads z once, with a running maximum that is looked at once for
 // four vectors; the backward reads it again and writes dz, first as if there were
@@ -27,8 +30,10 @@
 // while the others have the logits: its loads depend on one another.
 //
 // Measured (B200, device time in a CUDA graph): 4096 x 32000 bf16, T = 2, 64 entries,
-// forward 65 us (4.1 TB/s; issue slots, half of them taken, and rows that end together)
-// and backward 85 (6.2 TB/s, HBM); 1531 x 40009 f16 forward 30; 128 x 1000 5.7 and 6.2.
+// forward 67 us (3.9 TB/s; issue slots, half of them taken, and rows that end together; 65
+// with one multiply-add, z k - m k, in the place of distance and product) and backward 86
+// (6.2 TB/s, HBM); T = 3 94 and 106; 2048 x 32000 f32, any T, 54 to 57 and 94 to 97; 1531 x
+// 40009 f16 forward 30; 128 x 1000 5.7 and 6.2.
 // Asking for a row's vectors ahead, across rows too, cost a fourth of the blocks and 6 us.
 #include <algorithm>
 #include <type_traits>
@@ -40,7 +45,8 @@
 namespace ow {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LN2 = 0.6931471805599453;
 constexpr int MOST_TOP = 1024;  // a lane's entries are 32 at most
 
 struct Args {
@@ -56,11 +62,16 @@ struct Args {
   float kt;              // log2(e) / T
   float temp;
   float weight;
-  float* lse_t;          // [rows] log2 of the sum of 2^(z kt); only where not NULL
-  float* lse_1;          // the same for T = 1
-  float* top;            // the same of the teacher's entries; +inf: the row has none
+  // What a row's forward leaves: its largest logit m and 1 over the sums of 2^((z - m) kt) and of 2^((z - m) k), apart,
+  // since a logarithm of a sum in one float with m would take the rounding of m to every probability.  A scale's sign
+  // bit says that the row lacks its term, NaN that an index or an entry makes the term NaN.
+  float* pivot;          // [rows]
+  float* scale_t;
+  float* scale_1;
+  float* top_pivot;      // [rows] the same of the teacher's entries: the largest t, 1 over the sum of 2^((t - it) kt)
+  float* top_scale;
   float* soft;           // [rows] or NULL
-  float* hard;           // [rows] or NULL, NaN-free 0 and top / lse_1 tell whether the row has one
+  float* hard;
   float* loss;           // [rows] or NULL
   // backward
   const float* dloss;
@@ -200,6 +211,9 @@ struct Run {
 __device__ __forceinline__ float pivot(float m) { return m == -INFINITY ? 0.f : m; }
 // What a sum around m is worth around the pivot p: a sum that has seen no logit yet is 0.
 __device__ __forceinline__ float moved(float m, float p, float k) { return m == -INFINITY ? 0.f : ex2((m - p) * k); }
+// 2^((v - p) k).  The distance first: it is at most 0 where p is the largest, so that no logit, a type's lowest
+// value among them, can overflow on the way, and it does not lose what v k and p k have in common.
+__device__ __forceinline__ float above(float v, float p, float k) { return ex2((v - p) * k); }
 // The states of a warp's lanes as one: each sum is moved once, to the largest maximum.
 __device__ __forceinline__ Run join(Run r, float kt) {
   const float mine = r.m;
@@ -224,13 +238,13 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
   Run run{-INFINITY, 0.f, 0.f};
   auto single = [&](int i) {
     const float v = widen(z[i]), m = fmaxf(run.m, v), p = pivot(m);
-    run.st = run.st * moved(run.m, p, kt) + ex2(fmaf(v, kt, -p * kt));
-    run.s1 = run.s1 * moved(run.m, p, LOG2E) + ex2(fmaf(v, LOG2E, -p * LOG2E));
+    run.st = run.st * moved(run.m, p, kt) + above(v, p, kt);
+    run.s1 = run.s1 * moved(run.m, p, LOG2E) + above(v, p, LOG2E);
     run.m = m;
   };
   for (int i = lane; i < lay.lead; i += G) single(i);
   for (int i = lay.rest() + lane; i < V; i += G) single(i);
-  float st[2] = {run.st, 0.f}, s1[2] = {run.s1, 0.f};  // two chains of sums
+  f2 st[2] = {sm100::f2pack(run.st, 0.f), 0}, s1[2] = {sm100::f2pack(run.s1, 0.f), 0};  // four chains of sums
   const uint4* u = reinterpret_cast<const uint4*>(z + lay.lead);
   auto step = [&](const uint4 (&v)[N]) {
     float x[PER<T>];
@@ -243,22 +257,24 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
       const float ft = moved(run.m, p, kt), f1 = POW != 1 ? moved(run.m, p, LOG2E) : 0.f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        st[c] *= ft;
-        if constexpr (POW != 1) s1[c] *= f1;
+        st[c] = sm100::mul2(st[c], both(ft));
+        if constexpr (POW != 1) s1[c] = sm100::mul2(s1[c], both(f1));
       }
       run.m = m;
     }
-    const float pt = -p * kt, p1 = -p * LOG2E;
+    const f2 less = both(-p);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      widen<T>(v[n], x);
+      f2 d[PER<T> / 2];
+      widen<T>(v[n], d);
 #pragma unroll
-      for (int j = 0; j < PER<T>; ++j) {
-        const float e = ex2(fmaf(x[j], kt, pt));
-        st[j & 1] += e;
-        if constexpr (POW == 2) s1[j & 1] = fmaf(e, e, s1[j & 1]);
-        if constexpr (POW == 4) s1[j & 1] = fmaf(e * e, e * e, s1[j & 1]);
-        if constexpr (POW == 0) s1[j & 1] += ex2(fmaf(x[j], LOG2E, p1));
+      for (int j = 0; j < PER<T> / 2; ++j) {
+        d[j] = sm100::add2(d[j], less);
+        const f2 e = ex2(sm100::mul2(d[j], both(kt)));
+        st[j & 1] = sm100::add2(st[j & 1], e);
+        if constexpr (POW == 2) s1[j & 1] = sm100::fma2(e, e, s1[j & 1]);
+        if constexpr (POW == 4) s1[j & 1] = sm100::fma2(sm100::mul2(e, e), sm100::mul2(e, e), s1[j & 1]);
+        if constexpr (POW == 0) s1[j & 1] = sm100::add2(s1[j & 1], ex2(sm100::mul2(d[j], both(LOG2E))));
       }
     }
   };
@@ -275,10 +291,18 @@ __device__ __forceinline__ Run softmax_share(const T* z, int V, int lane, float 
     for (int n = 0; n < N; ++n) v[n] = i + n * G < lay.units ? __ldg(u + i + n * G) : least<T>();
     step(v);
   }
-  run.st = st[0] + st[1];
-  run.s1 = POW == 1 ? run.st : s1[0] + s1[1];
+  auto whole = [](const f2 (&v)[2]) {
+    const float2 f = sm100::f2unpack(sm100::add2(v[0], v[1]));
+    return f.x + f.y;
+  };
+  run.st = whole(st);
+  run.s1 = POW == 1 ? run.st : whole(s1);
   return run;
 }
+
+// A scale as it is left for the backward, and whether its row has the term.
+__device__ __forceinline__ float leave(float s, bool has) { return __uint_as_float((__float_as_uint(s) & 0x7FFFFFFFu) | (has ? 0u : 0x80000000u)); }
+__device__ __forceinline__ bool has_term(float s) { return __float_as_int(s) >= 0; }
 
 template <typename F>
 __device__ __forceinline__ F warp_sum(F v) {
@@ -293,21 +317,23 @@ constexpr int rows_of(int G) { return G == 32 ? 8 : 1; }
 
 // ---------------------------------------------------------------- forward
 // What a row's entries and label have to say without its logits' sums, by one warp:
-//   soft / (T^2 ln 2) = own + log2 of the sum of 2^(z kt)
-// in 64 bits, because large logits of the entries and the sum's take each other away.
+//   soft / (T^2 ln 2) = own + (m - r) kt + log2 of the sum of 2^((z - m) kt)
+// with r the largest of the entries' logits, in 64 bits: what is common to them and m is taken off before the product.
 struct Said {
   double own;
-  float top;             // +inf no entries, NaN not to be used
+  float r;
+  float top_pivot, top_scale;
   float label;           // the label's logit
+  int has_soft;          // 1, 0: no entries, or -1: not to be used
   int has_label;         // 1, 0, or -1: not a class
 };
 template <typename T>
 __device__ __forceinline__ Said listen(const Args& a, const T* z, int64_t row, int lane, float* sx, float* sz) {
-  Said s{0., INFINITY, 0.f, 0};
+  Said s{0., 0.f, 0.f, 0.f, 0.f, 0, 0};
   const int64_t at = row * a.K;
   int64_t label = -1;
   if (a.label && a.weight < 1.f) label = ld_index(a.label, a.label8, row);
-  float tm = -INFINITY;
+  float tm = -INFINITY, r = -INFINITY;
   bool bad = false;
   if (a.weight > 0.f) {
 #pragma unroll 4
@@ -319,6 +345,7 @@ __device__ __forceinline__ Said listen(const Args& a, const T* z, int64_t row, i
       sx[j] = on ? t : -INFINITY;
       sz[j] = in ? widen(z[c]) : 0.f;
       if (on) tm = fmaxf(tm, t);
+      if (in) r = fmaxf(r, sz[j]);
     }
   }
   if (label >= 0) {
@@ -328,47 +355,49 @@ __device__ __forceinline__ Said listen(const Args& a, const T* z, int64_t row, i
   if (a.weight <= 0.f) return s;
   __syncwarp();
 #pragma unroll
-  for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+  for (int o = 16; o; o >>= 1) {
+    tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, o));
+  }
   if (__any_sync(0xffffffffu, bad)) {
-    s.own = s.top = NAN;
+    s.has_soft = -1;
     return s;
   }
   if (tm == -INFINITY) return s;
-  const float tk = tm * a.kt;
-  float sd = 0.f;           // sum of e (x - tk)
-  double ts = 0., sq = 0.;  // of e, e z
+  s.has_soft = 1;
+  s.r = pivot(r);
+  float sd = 0.f;           // sum of e d
+  double ts = 0., sq = 0.;  // of e, e (z - r)
   for (int j = lane; j < a.K; j += 32) {
-    const float d = fmaf(sx[j], a.kt, -tk), e = ex2(d);
+    const float d = (sx[j] - tm) * a.kt, e = ex2(d);
     if (e > 0.f) {  // a probability of 0 has no part, whatever the student says
       ts += e;
       sd = fmaf(e, d, sd);
-      sq = fma((double)e, (double)sz[j], sq);
+      sq = fma((double)e, (double)sz[j] - s.r, sq);
     }
   }
   ts = warp_sum(ts);
   sd = warp_sum(sd);
   sq = warp_sum(sq);
-  const float log_s = log2f((float)ts);
-  s.own = (sd - sq * a.kt) / ts - log_s;
-  s.top = tk + log_s;
+  s.own = (sd - sq * a.kt) / ts - log2f((float)ts);
+  s.top_pivot = tm;
+  s.top_scale = 1.f / (float)ts;
   return s;
 }
 
 // Writes down a row's results.
-__device__ __forceinline__ void conclude(const Args& a, int64_t row, const Run& run, const Said& s) {
-  const float p = pivot(run.m), mt = p * a.kt, m1 = p * LOG2E;
-  const float log_t = log2f(run.st), log_1 = log2f(run.s1);
-  float soft = 0.f, hard = 0.f, lse_1 = INFINITY;
-  if (s.top != INFINITY) soft = LN2 * a.temp * a.temp * (float)(s.own + ((double)mt + log_t));
-  if (s.has_label > 0) {
-    hard = LN2 * (log_1 - fmaf(s.label, LOG2E, -m1));
-    lse_1 = m1 + log_1;
-  } else if (s.has_label < 0) {
-    hard = lse_1 = NAN;
-  }
-  a.lse_t[row] = mt + log_t;
-  a.lse_1[row] = lse_1;
-  a.top[row] = s.top;
+__device__ __forceinline__ void conclude(const Args& a, int64_t row, Run run, const Said& s) {
+  const float p = pivot(run.m);
+  float soft = 0.f, hard = 0.f;
+  if (s.has_soft > 0) soft = (float)(LN2 * a.temp * a.temp * (s.own + (((double)p - s.r) * a.kt + log2f(run.st))));
+  if (s.has_label > 0) hard = (float)((double)p - s.label + LN2 * log2f(run.s1));
+  if (s.has_soft < 0) soft = run.st = NAN;
+  if (s.has_label < 0) hard = run.s1 = NAN;
+  a.pivot[row] = p;
+  a.scale_t[row] = leave(1.f / run.st, s.has_soft != 0);
+  a.scale_1[row] = leave(1.f / run.s1, s.has_label != 0);
+  a.top_pivot[row] = s.top_pivot;
+  a.top_scale[row] = s.top_scale;
   if (a.soft) {
     a.soft[row] = soft;
     a.hard[row] = hard;
@@ -422,9 +451,9 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const Args a, int mea
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < a.rows; i += 1024) {
     v[0] += a.soft[i];
-    v[1] += a.top[i] != INFINITY;
+    v[1] += has_term(a.scale_t[i]);
     v[2] += a.hard[i];
-    v[3] += a.lse_1[i] != INFINITY;
+    v[3] += has_term(a.scale_1[i]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -447,28 +476,33 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const Args a, int mea
 
 // ---------------------------------------------------------------- backward
 // A row's gradient but for its entries and its label:
-//   ks 2^(z kt - lse_t) + kh 2^(z k - lse_1),   e (ks + c e^(POW - 1)) where POW says so
+//   qs 2^((z - m) kt) + qh 2^((z - m) k),   e (qs + c e^(POW - 1)) where POW says so
+// with qs and qh the factors ks and kh of the two probabilities times their scales.
 template <int POW>
 struct Slope {
-  float kt, ks, kh, lse_t, lse_1, c;
-  bool none;  // a row that learns from nothing
-  __device__ __forceinline__ Slope(const Args& a, int64_t row, float top) : kt(a.kt), ks(0.f), kh(0.f), c(0.f) {
-    lse_t = a.lse_t[row];
-    lse_1 = a.lse_1[row];
-    const float g = a.dloss[a.dloss_rows ? row : 0];
-    if (top != INFINITY) ks = top == top ? g * (a.coef ? a.coef[0] : a.weight) * a.temp : NAN;
-    if (lse_1 != INFINITY) kh = lse_1 == lse_1 ? g * (a.coef ? a.coef[1] : 1.f - a.weight) : NAN;
-    none = top == INFINITY && lse_1 == INFINITY;
-    if constexpr (POW == 1) c = ks + kh;
-    if constexpr (POW >= 2) c = lse_1 == INFINITY ? 0.f : kh * ex2(fmaf((float)POW, lse_t, -lse_1));
-    if (lse_1 == INFINITY) lse_1 = 0.f;
+  float kt, ks, kh, qs, qh, c;
+  f2 less;
+  bool soft, none;  // has a teacher; learns from nothing
+  __device__ __forceinline__ Slope(const Args& a, int64_t row) : kt(a.kt), ks(0.f), kh(0.f), qs(0.f), qh(0.f), less(both(-a.pivot[row])) {
+    const float scale_t = a.scale_t[row], scale_1 = a.scale_1[row], g = a.dloss[a.dloss_rows ? row : 0];
+    soft = has_term(scale_t);
+    none = !soft && !has_term(scale_1);
+    if (soft) {
+      ks = g * (a.coef ? a.coef[0] : a.weight) * a.temp;
+      qs = ks * scale_t;
+    }
+    if (has_term(scale_1)) {
+      kh = g * (a.coef ? a.coef[1] : 1.f - a.weight);
+      qh = kh * scale_1;
+    }
+    c = POW == 1 ? qs + qh : qh;
   }
   __device__ __forceinline__ f2 operator()(f2 v) const {
-    const f2 e = ex2(sm100::fma2(v, both(kt), both(-lse_t)));
+    const f2 d = sm100::add2(v, less), e = ex2(sm100::mul2(d, both(kt)));
     if constexpr (POW == 1) return sm100::mul2(e, both(c));
-    if constexpr (POW >= 2) return sm100::mul2(e, sm100::fma2(both(c), power1<POW>(e), both(ks)));
-    const f2 f = ex2(sm100::fma2(v, both(LOG2E), both(-lse_1)));
-    return sm100::fma2(e, both(ks), kh != 0.f ? sm100::mul2(f, both(kh)) : 0);
+    if constexpr (POW >= 2) return sm100::mul2(e, sm100::fma2(both(c), power1<POW>(e), both(qs)));
+    const f2 f = ex2(sm100::mul2(d, both(LOG2E)));
+    return sm100::fma2(e, both(qs), qh != 0.f ? sm100::mul2(f, both(qh)) : 0);
   }
   __device__ __forceinline__ float operator()(float v) const { return sm100::f2unpack((*this)(both(v))).x; }
 };
@@ -510,7 +544,7 @@ struct Amends {
 };
 // ``mem``: [K] classes, [K] probabilities, [K] values, [slots] of a table of classes.
 template <typename T, int POW>
-__device__ __forceinline__ Amends amends(const Args& a, const T* z, int64_t row, float top, int lane, const Slope<POW>& slope, float* mem) {
+__device__ __forceinline__ Amends amends(const Args& a, const T* z, int64_t row, int lane, const Slope<POW>& slope, float* mem) {
   int* sc = reinterpret_cast<int*>(mem);
   float *sp = mem + a.K, *sv = sp + a.K;
   int* table = reinterpret_cast<int*>(sv + a.K);
@@ -522,14 +556,15 @@ __device__ __forceinline__ Amends amends(const Args& a, const T* z, int64_t row,
       m.value = slope(widen(z[y])) - slope.kh;
     }
   }
-  if (top == INFINITY) return m;
+  if (!slope.soft) return m;
   for (int i = lane; i < a.slots; i += 32) table[i] = -1;
+  const float tm = a.top_pivot[row], by = a.top_scale[row];
 #pragma unroll 4
   for (int j = lane; j < a.K; j += 32) {
     const int64_t c = ld_index(a.cls, a.cls8, row * a.K + j);
     const float t = ld_teacher(a, row * a.K + j);
     const bool in = c >= 0 && c < a.V;
-    const float p = in ? ex2(fmaf(t, a.kt, -top)) : 0.f;
+    const float p = in ? above(t, tm, a.kt) * by : 0.f;
     sc[j] = p > 0.f ? (int)c : -1;  // what has no probability takes nothing off
     sp[j] = p;
     sv[j] = in ? slope(widen(z[c])) : 0.f;
@@ -584,9 +619,8 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
     for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.rows; row += (int64_t)gridDim.x * 8) {
       const T* z = (const T*)a.z + row * a.ld;
       T* dz = (T*)a.dz + row * a.V;
-      const float top = a.top[row];
-      const Slope<POW> slope(a, row, top);
-      const Amends m = amends<T>(a, z, row, top, lane, slope, mem);
+      const Slope<POW> slope(a, row);
+      const Amends m = amends<T>(a, z, row, lane, slope, mem);
       slope_share<T, 32>(z, dz, a.V, lane, slope);
       __syncwarp();
       amend(a, dz, m, lane, mem);
@@ -597,11 +631,10 @@ __global__ void __launch_bounds__(block_of(G), G == 32 ? 4 : 1024 / block_of(G))
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
       const T* z = (const T*)a.z + row * a.ld;
       T* dz = (T*)a.dz + row * a.V;
-      const float top = a.top[row];
-      const Slope<POW> slope(a, row, top);
+      const Slope<POW> slope(a, row);
       Amends m{};
       if (warp < W) slope_share<T, G>(z, dz, a.V, threadIdx.x, slope);
-      else m = amends<T>(a, z, row, top, lane, slope, dyn);
+      else m = amends<T>(a, z, row, lane, slope, dyn);
       __syncthreads();
       if (warp == W) {
         amend(a, dz, m, lane, dyn);
@@ -654,9 +687,11 @@ Args base(const ow_distill_t* a) {
     k.kt = LOG2E;
     k.temp = 1.f;
   }
-  k.lse_t = a->stats;
-  k.lse_1 = a->stats + a->rows;
-  k.top = a->stats + 2 * a->rows;
+  k.pivot = a->stats;
+  k.scale_t = a->stats + a->rows;
+  k.scale_1 = a->stats + 2 * a->rows;
+  k.top_pivot = a->stats + 3 * a->rows;
+  k.top_scale = a->stats + 4 * a->rows;
   return k;
 }
 
