@@ -147,8 +147,9 @@ class TrainStep:
 
     ``cuda_graph=True`` (single process only) captures the whole step --
     forward, backward, finite check, optimizer and EMA -- into one CUDA
-    graph after ``graph_warmup`` eager steps; later steps copy the batch
-    into the graph's input buffers and replay it.
+    graph after ``graph_warmup`` eager steps; later steps copy the batch,
+    of the captured shapes (others raise ``ValueError``), into the graph's
+    input buffers and replay it.
     """
 
     def __init__(
@@ -268,6 +269,17 @@ class TrainStep:
                 for p, old in zip(self._params, snapshot):
                     p.copy_(torch.where(keep, old, p))
 
+    def _check_captured(self, batch: tuple[Tensor, ...]) -> None:
+        """A captured step takes its own batch's shapes, and its teacher's types: ``copy_`` would spread one entry
+        (or sample) over all that were captured, and round or wrap what does not fit."""
+        if self._static is None:
+            return
+        for i, (name, held, t) in enumerate(zip(("images", "labels", "top_logits", "top_classes"), self._static[0], batch)):
+            if t.shape != held.shape:
+                raise ValueError(f"the step was captured with {name} {tuple(held.shape)}, got {tuple(t.shape)}")
+            if i >= 2 and t.dtype != held.dtype:
+                raise ValueError(f"the step was captured with {name} in {held.dtype}, got {t.dtype}")
+
     def step(self, images: Tensor, labels: Tensor, teacher: tuple[Tensor, Tensor] | None = None) -> Tensor:
         """Forward, backward (gradients all-reduced by DDP), optimizer step.
 
@@ -277,6 +289,7 @@ class TrainStep:
         batch = (images, labels, *(teacher or ()))
         if self._static is not None and len(self._static[0]) != len(batch):
             raise ValueError("the step was captured " + ("without" if teacher else "with") + " a teacher")
+        self._check_captured(batch)
         self._nsteps += 1
         if self._graph_warmup < 0:
             return self._body(*batch)
