@@ -123,9 +123,9 @@ __device__ __forceinline__ float lds1(uint32_t at) {
   }
 }
 
-// A thread's share of a row in shared memory, in pairs; 0 beside the channels.
+// A thread's share of a row in shared memory, in pairs; 0 beside the channels, or ``beside`` where they come singly.
 template <typename T, int V, int G, int E, bool FULL>
-__device__ __forceinline__ void take2(uint32_t row, int C, int lane, bool live, f2 (&o)[E / 2]) {
+__device__ __forceinline__ void take2(uint32_t row, int C, int lane, bool live, f2 (&o)[E / 2], float beside = 0.f) {
   if constexpr (V == 8) {
 #pragma unroll
     for (int j = 0; j < E / 8; ++j) {
@@ -146,7 +146,7 @@ __device__ __forceinline__ void take2(uint32_t row, int C, int lane, bool live, 
   } else {
     float v[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = live && e * G + lane < C ? lds1<T>(row + (e * G + lane) * (int)sizeof(T)) : 0.f;
+    for (int e = 0; e < E; ++e) v[e] = live && e * G + lane < C ? lds1<T>(row + (e * G + lane) * (int)sizeof(T)) : beside;
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) o[i] = sm100::f2pack(v[2 * i], v[2 * i + 1]);
   }
@@ -251,7 +251,8 @@ struct Span {
 };
 
 // A team's walk over its chunks, with the ring in front of it.  Rows are counted in
-// 32 bits (there are fewer than 2^31 - 2^20, and no step is longer than 2^20).
+// 32 bits: there are fewer than 2^31, and a step is no longer than a third of them, or than
+// the 2^15 rows of one pass of all teams (stream_of).
 template <typename XT, typename NT, int V, int G, bool TWO>
 struct Walk {
   static constexpr int TEAM = team_of(G), TEAMS = STREAM_T / TEAM, XS = sizeof(XT), NS = sizeof(NT);

@@ -32,12 +32,15 @@ __global__ void __launch_bounds__(STREAM_T, bwd_an_sm(E)) layernorm_stream_bwd_k
       const bool live = p + sub < rows;
       const int64_t row = walk.row + p + sub;
       f2 x[P], g[P], s0 = 0, s1 = 0;
-      take2<XT, V, G, E, FULL>(px + (p + sub) * a.C * (int)sizeof(XT), a.C, lane, live, x);
+      take2<XT, V, G, E, FULL>(px + (p + sub) * a.C * (int)sizeof(XT), a.C, lane, live, x, mean);
       take2<NT, V, G, E, FULL>(pn + (p + sub) * a.C * (int)sizeof(NT), a.C, lane, live, g);
       const f2 less = both(-mean), by = both(rstd);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        x[i] = sm100::mul2(sm100::add2(x[i], less), by);  // x^; beside the channels g is 0
+        // x^.  Beside the channels and behind the rows, where g is 0, it has to be 0 too: a mean times a deviation's
+        // inverse may overflow, and 0 times that is NaN.
+        const bool in = FULL || V == 1 || channel<8, G>(2 * i & ~7, lane) < a.C;
+        x[i] = sm100::mul2(sm100::add2(x[i], less), in ? by : 0);
         dw[i] = sm100::fma2(g[i], x[i], dw[i]);
         db[i] = sm100::add2(db[i], g[i]);
         g[i] = sm100::mul2(g[i], w[i]);                                               // u
@@ -46,7 +49,8 @@ __global__ void __launch_bounds__(STREAM_T, bwd_an_sm(E)) layernorm_stream_bwd_k
       }
       const float rs = rstd;
       const uint32_t then = (p + PASS < rows ? walk.row + p + PASS : walk.row + walk.step) + sub;
-      if (then < walk.rows) {  // (past a chunk's end the loads are of another's rows, and not used)
+      mean = rstd = 0.f;  // of what is no row (only the last chunk ends inside a pass)
+      if (then < walk.rows) {
         mean = a.mean[then];
         rstd = a.rstd[then];
       }
