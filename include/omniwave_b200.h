@@ -619,9 +619,9 @@ OW_API int ow_linear_bwd(const ow_linear_t* args, const ow_linear_grads_t* grads
  * Backward, from dout: NULL outputs are not computed; dgate_weight and dup_weight
  * come together, with one dtype.  h is needed for ddown_weight only, act, slope and
  * down_weight for all gradients but the projection back's.  dg and du are rounded
- * to ``dtype``, and where dh's product is split so is dh; dgate_bias and dup_bias
- * are f32 sums of dg and du, rounded where dh is not.  All sums are taken in a fixed
- * order.
+ * to ``dtype``, dh is not; dgate_bias and dup_bias are f32 sums of dg and du, rounded
+ * unless dh's product is split.  In f16, act and slope end at its largest value.  All
+ * sums are taken in a fixed order.
  */
 typedef struct ow_ffn_t {
   int64_t rows;

@@ -13,8 +13,10 @@
 // h, dg and du are held in 16 bits because the tensor core takes no other; act(g) and
 // u act'(g), which the backward multiplies dh with, for their traffic.  Each is rounded
 // once, and so dWg is off by what three roundings make, its own among them: 0.0029 of
-// its norm in bf16, where its own makes 0.0017.  gate's and up's bias gradients are f32
-// sums of dg and du as they are rounded.
+// its norm in bf16, where its own makes 0.0017.  dh is rounded
+// nowhere.  gate's and up's bias gradients are f32 sums of dg and du, as they are
+// rounded where dh's product is whole (its epilogue sums what it has staged) and before
+// that where it is split.
 //
 // Bound and measured (B200, device time in a CUDA graph): the tensor pipe under the
 // power cap for 16384 x 4096 x 8192, forward 2120 to 2280 us, with the backward 7.6 to
@@ -27,18 +29,18 @@ namespace ow {
 namespace {
 
 struct GradArgs {
-  const void* dh;    // [M, N] contiguous
+  const float* dh;   // [splits][M, ldh] partial sums of dh
   const void* act;   // [M, ld] act(g)
   const void* slope; // [M, ld] u act'(g)
   void* dg;          // [M, ld]
   void* du;          // [M, ld]
   float* part;       // [chunks][2][N] column sums of dg and of du, or NULL
-  int64_t M, ld, chunk;
-  int N, vec;
+  int64_t M, ld, ldh, chunk;
+  int N, splits;
 };
 
-// dg and du, rounded to the 16-bit type, and their f32 column sums for the biases.
-// A block does 256 columns of a chunk of rows.
+// dg and du from the partial sums of dh, which stays in f32, rounded to the 16-bit type,
+// and their f32 column sums for the biases.  A block does 256 columns of a chunk of rows.
 template <bool BF16>
 __global__ void __launch_bounds__(256) gate_grad_kernel(const GradArgs a) {
   __shared__ float sh[8][264];
@@ -48,19 +50,26 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const GradArgs a) {
   float s[2][8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) s[0][k] = s[1][k] = 0.f;
-  const bool whole = a.vec && n + 8 <= a.N;
+  const bool whole = n + 8 <= a.N;
   for (int64_t m = blockIdx.y * a.chunk + ty; m < m1; m += 8) {
     if (n >= a.N) continue;
     float d[8], g[8], u[8];
+    const float* part = a.dh + m * a.ldh + n;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) d[k] = 0.f;
     if (whole) {
-      const uint4 dv = *reinterpret_cast<const uint4*>((const uint16_t*)a.dh + m * a.N + n);
+#pragma unroll 4
+      for (int i = 0; i < a.splits; ++i, part += a.M * a.ldh) {
+        const float4 p = *reinterpret_cast<const float4*>(part), q = *reinterpret_cast<const float4*>(part + 4);
+        d[0] += p.x; d[1] += p.y; d[2] += p.z; d[3] += p.w;
+        d[4] += q.x; d[5] += q.y; d[6] += q.z; d[7] += q.w;
+      }
       const uint4 gv = *reinterpret_cast<const uint4*>((const uint16_t*)a.act + m * a.ld + n);
       const uint4 uv = *reinterpret_cast<const uint4*>((const uint16_t*)a.slope + m * a.ld + n);
-      const uint32_t dq[4] = {dv.x, dv.y, dv.z, dv.w}, gq[4] = {gv.x, gv.y, gv.z, gv.w}, uq[4] = {uv.x, uv.y, uv.z, uv.w};
+      const uint32_t gq[4] = {gv.x, gv.y, gv.z, gv.w}, uq[4] = {uv.x, uv.y, uv.z, uv.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 f = unpack2<BF16>(dq[k]), i = unpack2<BF16>(gq[k]), j = unpack2<BF16>(uq[k]);
-        d[2 * k] = f.x; d[2 * k + 1] = f.y;
+        const float2 i = unpack2<BF16>(gq[k]), j = unpack2<BF16>(uq[k]);
         g[2 * k] = i.x; g[2 * k + 1] = i.y;
         u[2 * k] = j.x; u[2 * k + 1] = j.y;
       }
@@ -68,7 +77,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const GradArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const bool in = n + k < a.N;
-        d[k] = in ? ld16(a.dh, m * a.N + n + k, BF16) : 0.f;
+        for (int i = 0; in && i < a.splits; ++i) d[k] += part[i * a.M * a.ldh + k];
         g[k] = in ? ld16(a.act, m * a.ld + n + k, BF16) : 0.f;
         u[k] = in ? ld16(a.slope, m * a.ld + n + k, BF16) : 0.f;
       }
@@ -171,12 +180,13 @@ Plan plan_gate(const ow_ffn_t* a) { return plan_gemm(a->rows, 2 * a->hidden, blo
 // Everything a backward call needs, carved from its workspace.
 struct BwdWs {
   bool fused;        // dg and du come from dh's product itself
-  void *dh, *dg, *du;  // dh where they do not
+  void *dg, *du;
   float* bias;       // [2][chunks][hidden]
   int chunks;
   int64_t chunk;
   Plan ph, px, pw;
   DualWs h, x, w;
+  GemmWs hs;         // dh's product where it is split
   void* down;        // the projection back's own workspace
   size_t down_bytes;
 };
@@ -188,7 +198,7 @@ BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
   const int64_t M = a->rows, ld = up8(a->hidden);
   const int F = a->hidden, K = a->in_features;
   if (wants_gate(g)) {
-    // Where dh's product is split over k (few tiles), its sum is complete in another kernel only.
+    // Where dh's product is split over k (few tiles), its sum is complete in another kernel only, which then makes dg and du.
     b.ph = plan_gemm(M, F, blocks_of(a->out_features));
     b.fused = b.ph.splits == 1;
     b.dg = ws.take((size_t)M * ld * 2);
@@ -197,7 +207,7 @@ BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
       b.h = dual_take<GRAD>(mat_dy(a, g), mat_d(a), Second{}, M, F, b.ph, ws);
       b.chunks = (int)((M + 31) / 32);
     } else {
-      b.dh = ws.take((size_t)M * F * 2);
+      b.hs = gemm_take(mat_dy(a, g), mat_d(a), M, F, b.ph, ws);
       // chunks of rows: a few blocks an SM, at least 8 rows each
       const int64_t col_blocks = (F + 255) / 256;
       b.chunks = (int)std::max<int64_t>(1, std::min<int64_t>((M + 7) / 8, (int64_t)device_sm_count() * 8 / col_blocks));
@@ -216,9 +226,8 @@ BwdWs bwd_take(const ow_ffn_t* a, const ow_ffn_grads_t* g, Carver& ws) {
     }
   }
   const ow_linear_t d = down(a);
-  // sized with an address for dh where it is wanted: its own is not known when only the size is asked for
-  const ow_linear_grads_t sized{g->dout, wants_gate(g) && !b.fused ? (void*)16 : nullptr, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
-  b.down_bytes = ow_linear_workspace_size(&d, &sized);
+  const ow_linear_grads_t dgr{g->dout, nullptr, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
+  b.down_bytes = ow_linear_workspace_size(&d, &dgr);
   b.down = ws.take(b.down_bytes);
   return b;
 }
@@ -314,11 +323,11 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
   const int64_t M = a->rows, ld = up8(F);
   Carver ws((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255));
   const BwdWs b = bwd_take(a, g, ws);
-  if (b.dh || g->ddown_weight || g->ddown_bias) {
+  if (g->ddown_weight || g->ddown_bias) {
     ow_linear_t d = down(a);
     d.workspace = b.down;
     d.workspace_bytes = b.down_bytes;
-    const ow_linear_grads_t dgr{g->dout, b.dh, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
+    const ow_linear_grads_t dgr{g->dout, nullptr, g->ddown_weight, g->ddown_dtype, g->ddown_bias};
     OW_RETURN_IF(ow_linear_bwd(&d, &dgr, stream));
   }
   if (!gate) return OW_OK;
@@ -334,7 +343,8 @@ int ow_ffn_bwd(const ow_ffn_t* a, const ow_ffn_grads_t* g, void* stream) {
     OW_RETURN_IF((brief ? gemm_dual<GRAD, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)
                         : gemm_dual<GRAD_LONG, false, true>(mat_dy(a, g), mat_d(a), s, M, F, a->out_features, b.ph, b.h, e, bf, st)));
   } else {
-    const GradArgs k{b.dh, a->act, a->slope, b.dg, b.du, b.bias, M, ld, b.chunk, F, F % 8 == 0};
+    OW_RETURN_IF((gemm<false, true>(mat_dy(a, g), mat_d(a), M, F, a->out_features, b.ph, b.hs, Epi{}, bf, st, true)));
+    const GradArgs k{b.hs.part, a->act, a->slope, b.dg, b.du, b.bias, M, ld, b.hs.part_ld, b.chunk, F, b.ph.splits};
     launch(bf ? gate_grad_kernel<true> : gate_grad_kernel<false>, dim3((F + 255) / 256, b.chunks), 256, 0, st, k);
     OW_CHECK_LAUNCH("gate_grad_kernel");
   }

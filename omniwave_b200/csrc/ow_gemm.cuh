@@ -1491,9 +1491,11 @@ int run_gemm(const MapsOf<KIND>& maps, const GemmArgs& k, int grid, cudaStream_t
 }
 
 // D[M, N] = sum_k A B with the epilogue ``e``.  AMN/BMN: the operand's rows
-// run along M or N and its row index is k.
+// run along M or N and its row index is k.  ``parts``: the f32 partials of a split
+// product stay as they are, and there is no epilogue.
 template <bool AMN, bool BMN>
-int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs& w, const Epi& e, bool bf16, cudaStream_t st) {
+int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs& w, const Epi& e, bool bf16, cudaStream_t st,
+         bool parts = false) {
   if (w.a) OW_RETURN_IF(pad_rows(A, w.a, st));
   if (w.b) OW_RETURN_IF(pad_rows(B, w.b, st));
   Maps maps{};
@@ -1545,7 +1547,7 @@ int gemm(Mat A, Mat B, int64_t M, int N, int64_t K, const Plan& p, const GemmWs&
   } else {
     OW_RETURN_IF(go(std::integral_constant<int, OW_ACT_NONE>()));
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 && !parts) {
     const int64_t total = M * ((N + 3) / 4);
     const int g2 = (int)std::min<int64_t>((total + 255) / 256, (int64_t)device_sm_count() * 16);
     launch(gemm_sum_kernel, g2, 256, 0, st, (const float*)w.part, p.splits, M * w.part_ld, w.part_ld, M, N, e, nullptr, 0);

@@ -43,7 +43,8 @@ def gated_feed_forward(x: Tensor, gate_weight: Tensor, up_weight: Tensor, down_w
     ``[..., N]``; ``activation`` is ``"silu"``, ``"gelu"`` (by erf), ``"relu"`` or
     ``"none"``.  Types, errors and derivatives as for ``linear.linear``.  The backward
     holds the gated product, the activation and its slope times the other projection,
-    each ``[..., F]`` in the compute type.
+    each ``[..., F]`` in the compute type; in float16 the last two end at its largest
+    value, 65504.
     """
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:
