@@ -709,10 +709,12 @@ int with(const ow_distill_t* a, F&& f) {
     }
   };
   auto type = [&](auto t) -> int {
-    // A warp a row where rows are many and not long: 16384 x 2000 bf16 forward 37 us and backward 31 (a block a row
-    // 95 and 87), 4096 x 8000 26 and 23 (34 and 32); 1024 x 8000 12 and 13 (11 and 11), 128 x 1500 7.2 and 7.2
-    // (5.7 and 6.2).  Its entries have to leave room for those of the block's other rows.
-    const bool warps = a->top <= 256 && (a->classes <= 256 || (a->classes <= 8192 && a->rows >= 6 * (int64_t)device_sm_count()));
+    // A warp a row where rows are many and not long, forward and backward of bf16, T = 2, 32 entries: 16384 x 2000 70 us
+    // (a block a row 188), 4096 x 8000 50 (69), 2048 x 8000 36 (38; f32 54 and 51), 1024 x 2000 18 (20); but 1024 x 8000
+    // 25 (23), 4096 x 16000 87 (98; f32 160 and 144), 128 x 1000 15 (13).  Its entries have to leave room for those of the
+    // block's other rows.
+    const int64_t rows = a->rows, sms = device_sm_count();
+    const bool warps = a->top <= 256 && (a->classes <= 256 || (a->classes <= 8192 && rows >= (a->classes <= 4096 ? 6 : 14) * sms));
     return warps ? power(std::integral_constant<int, 32>(), t) : power(std::integral_constant<int, 224>(), t);
   };
   switch (a->dtype) {
@@ -722,15 +724,9 @@ int with(const ow_distill_t* a, F&& f) {
   }
 }
 
+// ``smem``: at most 40 KB, of eight rows with 256 entries each (one with 1024: 20 KB).
 template <class K>
 int launch_rows(K kern, const char* name, int G, size_t smem, const Args& k, cudaStream_t st) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) {
-      set_error("ow_distill: cannot reserve %zu bytes of shared memory: %s", smem, cudaGetErrorString(e));
-      return OW_ERR_CUDA;
-    }
-  }
   const int rb = rows_of(G);
   const int64_t grid = std::min<int64_t>((k.rows + rb - 1) / rb, (int64_t)device_sm_count() * 8);
   launch(kern, (int)grid, block_of(G), smem, st, k);

@@ -240,30 +240,32 @@ __device__ __forceinline__ float sigmoid(float z) { return rcp(1.f + ex2(z * -1.
 // quotient, the epilogue is slower (25088 x 512 x 1024 with bias and kept z 56 and
 // 47 us, here 41).
 template <bool BF16>
-__device__ __forceinline__ float gelu(float z) {
+__device__ __forceinline__ float gelu_tail(float x) {  // x = |z|
   float q;
   if constexpr (BF16) {
-    const float a = fminf(fabsf(z), 13.5f);
-    q = fmaf(a, 3.98267339e-8f, -2.39384553e-6f);
-    q = fmaf(q, a, 6.14833989e-5f);
-    q = fmaf(q, a, -8.9382549e-4f);
-    q = fmaf(q, a, 8.29635281e-3f);
-    q = fmaf(q, a, -5.3509552e-2f);
-    q = fmaf(q, a, -0.458847046f);
-    q = fmaf(q, a, -1.15114152f);
-    q = fmaf(q, a, -1.00000072f);
+    q = fmaf(x, 3.98267339e-8f, -2.39384553e-6f);
+    q = fmaf(q, x, 6.14833989e-5f);
+    q = fmaf(q, x, -8.9382549e-4f);
+    q = fmaf(q, x, 8.29635281e-3f);
+    q = fmaf(q, x, -5.3509552e-2f);
+    q = fmaf(q, x, -0.458847046f);
+    q = fmaf(q, x, -1.15114152f);
+    q = fmaf(q, x, -1.00000072f);
   } else {
-    const float a = fabsf(z);
-    q = fmaf(a, -1.39922733e-7f, 1.43002126e-6f);
-    q = fmaf(q, a, 3.0813193e-5f);
-    q = fmaf(q, a, -7.80530798e-4f);
-    q = fmaf(q, a, 8.10782891e-3f);
-    q = fmaf(q, a, -5.33918403e-2f);
-    q = fmaf(q, a, -0.458847821f);
-    q = fmaf(q, a, -1.15115714f);
-    q = fmaf(q, a, -0.999998868f);
+    q = fmaf(x, -1.39922733e-7f, 1.43002126e-6f);
+    q = fmaf(q, x, 3.0813193e-5f);
+    q = fmaf(q, x, -7.80530798e-4f);
+    q = fmaf(q, x, 8.10782891e-3f);
+    q = fmaf(q, x, -5.33918403e-2f);
+    q = fmaf(q, x, -0.458847821f);
+    q = fmaf(q, x, -1.15115714f);
+    q = fmaf(q, x, -0.999998868f);
   }
-  const float tail = ex2(q);
+  return ex2(q);
+}
+template <bool BF16>
+__device__ __forceinline__ float gelu(float z) {
+  const float x = fabsf(z), tail = gelu_tail<BF16>(BF16 ? fminf(x, 13.5f) : x);
   return z * (z > 0.f ? 1.f - tail : tail);
 }
 template <int ACT, bool BF16>
@@ -322,28 +324,7 @@ __device__ __forceinline__ void act_both(float z, float& a, float& s) {
     a = z * g;
     s = fmaf(a, 1.f - g, g);
   } else if constexpr (ACT == OW_ACT_GELU) {
-    const float x = fminf(fabsf(z), BF16 ? 13.5f : 100.f);
-    float q;
-    if constexpr (BF16) {
-      q = fmaf(x, 3.98267339e-8f, -2.39384553e-6f);
-      q = fmaf(q, x, 6.14833989e-5f);
-      q = fmaf(q, x, -8.9382549e-4f);
-      q = fmaf(q, x, 8.29635281e-3f);
-      q = fmaf(q, x, -5.3509552e-2f);
-      q = fmaf(q, x, -0.458847046f);
-      q = fmaf(q, x, -1.15114152f);
-      q = fmaf(q, x, -1.00000072f);
-    } else {
-      q = fmaf(x, -1.39922733e-7f, 1.43002126e-6f);
-      q = fmaf(q, x, 3.0813193e-5f);
-      q = fmaf(q, x, -7.80530798e-4f);
-      q = fmaf(q, x, 8.10782891e-3f);
-      q = fmaf(q, x, -5.33918403e-2f);
-      q = fmaf(q, x, -0.458847821f);
-      q = fmaf(q, x, -1.15115714f);
-      q = fmaf(q, x, -0.999998868f);
-    }
-    const float tail = ex2(q);
+    const float x = fminf(fabsf(z), BF16 ? 13.5f : 100.f), tail = gelu_tail<BF16>(x);
     a = fmaf(-x, tail, max0(z));
     s = fmaf(z * 0.39894228040143268f, ex2(z * z * -0.72134752f), z > 0.f ? 1.f - tail : tail);
   } else {
