@@ -33,7 +33,7 @@
 // forward 67 us (3.9 TB/s; issue slots, half of them taken, and rows that end together; 65
 // with one multiply-add, z k - m k, in the place of distance and product) and backward 86
 // (6.2 TB/s, HBM); T = 3 94 and 106; 2048 x 32000 f32, any T, 54 to 57 and 94 to 97; 1531 x
-// 40009 f16 forward 30; 128 x 1000 5.7 and 6.2.
+// 40009 f16 forward 35; 128 x 1000 6.7 and 5.7.
 // Asking for a row's vectors ahead, across rows too, cost a fourth of the blocks and 6 us.
 #include <algorithm>
 #include <type_traits>
