@@ -102,8 +102,8 @@ def _kernel_flops(name: str, b: int, h: int, w: int, c: int, d: int) -> float:
 _KERNEL_SRC = {"tc_bwd_kernel": "ow_tc_bwd.cu", "tc_pack_kernel": "ow_tc_bwd.cu", "tcf_kernel": "ow_tcf.cu",
                "tc_fwd_kernel": "ow_tc.cu", "tc_fwd_gather_kernel": "ow_tcf.cu"}
 _TRAFFIC = {
-    ("tc_bwd_kernel", "56x56x128/radix1", 128): (2 * (542.262016e6 + 93.747200e6), "cb11faa60cdf459a49a979ba186b9baaaa779a1caef2e6a6ca1520864263ad80"),
-    ("tc_bwd_kernel", "56x56x128/radix2", 128): (2 * (542.140416e6 + 93.632256e6), "cb11faa60cdf459a49a979ba186b9baaaa779a1caef2e6a6ca1520864263ad80"),
+    ("tc_bwd_kernel", "56x56x128/radix1", 128): (2 * (541.011456e6 + 93.765632e6), "8cf2970959473e197a35ed78bbfd28f680216e52b2489a7faf24bad6944a620b"),
+    ("tc_bwd_kernel", "56x56x128/radix2", 128): (2 * (540.616960e6 + 93.639936e6), "8cf2970959473e197a35ed78bbfd28f680216e52b2489a7faf24bad6944a620b"),
 }
 
 
